@@ -19,10 +19,11 @@ ROCM = os.environ.get('ROCM_PATH', '/opt/rocm')
 HIPCC = os.path.join(ROCM, 'bin', 'hipcc')
 ARCH = 'gfx950'
 
-SOURCES = ['lt_decode.hip', 'lt_results.hip', 'lt_capi.cpp', 'lt_packer.cpp', 'lt_comm.cpp', 'lt_lookup.cpp']
+SOURCES = ['lt_decode.hip', 'lt_results.hip', 'lt_logits.hip', 'lt_capi.cpp', 'lt_packer.cpp', 'lt_comm.cpp', 'lt_lookup.cpp']
 HEADERS = ['lt_common.h', 'lt_internal.h', 'lt_error.h', 'lt_handles.h', 'lt_host.h', os.path.join('..', '..', 'include', 'lattice_decode.h'),
            os.path.join('..', '..', 'include', 'lattice_pack.h'),
-           os.path.join('..', '..', 'include', 'lattice_lookup.h')]
+           os.path.join('..', '..', 'include', 'lattice_lookup.h'),
+           os.path.join('..', '..', 'include', 'lattice_logits.h')]
 
 PYOBJ_SRC = os.path.join(CSRC, 'lt_pyobj.c')
 # named for the interpreter ABI it is built against (EXT_SUFFIX, e.g.
@@ -32,6 +33,11 @@ PYOBJ = os.path.join(LIBDIR, '_ltpy' + (sysconfig.get_config_var('EXT_SUFFIX') o
 
 COMMON_FLAGS = ['-O3', '-std=c++17', '-fPIC', '-ffp-contract=off', '-fno-fast-math',
                 '-Wall', '-Wno-unused-result', '-I' + os.path.join(HERE, '..', 'include')]
+
+# Without packed float32 instructions (hipcc makes them of ordinary float code
+# at -O3; some of their forms are unreliable on this hardware).  The decoders'
+# sources compile to none of them either way.
+SOURCE_FLAGS = {'lt_logits.hip': ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']}
 
 
 def _stale(target, deps):
@@ -74,7 +80,7 @@ def build(force=False, verbose=True, defines=(), out=None):
         # (objects named after the library too: experiment builds can run in parallel)
         obj = os.path.join(LIBDIR, os.path.splitext(os.path.basename(lib))[0] + '_' + os.path.splitext(src)[0] + '.o')
         extra = os.environ.get('LT_EXTRA_FLAGS', '').split() if out is not None else []   # experiment builds only
-        cmd = [HIPCC, '--offload-arch=' + ARCH] + COMMON_FLAGS + extra + ['-D' + d for d in defines] + [
+        cmd = [HIPCC, '--offload-arch=' + ARCH] + COMMON_FLAGS + SOURCE_FLAGS.get(src, []) + extra + ['-D' + d for d in defines] + [
             '-c', os.path.join(CSRC, src), '-o', obj]
         if verbose:
             print(' '.join(cmd), file=sys.stderr)

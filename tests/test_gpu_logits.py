@@ -1,0 +1,517 @@
+"""The operators over logits on the GPU against tests/logits_plain.py (64 bits,
+CPU), with its bounds: the k best and whole numbers exactly, the rest within
+the rounding of float32 sums and of the output's type."""
+
+import math
+
+import pytest
+import torch
+
+import logits_plain as plain
+from lattice_based_tagger_amd import logits
+
+pytestmark = pytest.mark.gpu
+
+INF = math.inf
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+LOWEST = {t: torch.finfo(t).min for t in TYPES}
+
+
+def rand(shape, dtype, seed, scale=3.0, pad=0):
+    """Random logits on the GPU; with ``pad``, a view of rows of a wider pitch
+    whose padding is NaN."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(tuple(shape[:-1]) + (shape[-1] + pad,), generator=g) * scale
+    if pad:
+        x[..., shape[-1]:] = math.nan
+    return x.to(dtype).cuda()[..., :shape[-1]]
+
+
+def same(a, b):
+    """Equal values, a NaN equal to a NaN."""
+    a, b = a.double().cpu(), b.double().cpu()
+    return a.shape == b.shape and bool(((a == b) | (a.isnan() & b.isnan())).all())
+
+
+def near(got, want, tol):
+    got = got.double().cpu()
+    off = (got - want).abs()
+    fine = (off <= tol) | (got == want) | (got.isnan() & want.isnan())
+    assert fine.all(), 'off by %s where %s is allowed' % (off[~fine][:5].tolist(), tol.expand_as(off)[~fine][:5].tolist())
+
+
+# ---- top_logits -------------------------------------------------------------
+
+def check_top(x, k, temperature=1.0):
+    got = logits.top_logits(x, k, temperature=temperature)
+    values, ids, lse = plain.top_logits(x, k, temperature)
+    assert got.values.dtype == x.dtype and got.ids.dtype == torch.int64 and got.lse.dtype == torch.float32
+    assert torch.equal(got.ids.cpu(), ids)
+    assert same(got.values, values)
+    near(got.lse, lse, plain.lse_tolerance(torch.where(lse.isfinite(), lse, 0.0), x.shape[-1]))
+    return got
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('rows, vocab, k, pad', [
+    (1, 1, 1, 0), (3, 2, 2, 1), (70, 41, 5, 0), (300, 41, 41, 0), (5, 63, 7, 2), (5, 64, 64, 0), (5, 65, 16, 0),
+    (9, 127, 100, 0), (9, 128, 3, 0), (9, 129, 129, 0), (4, 257, 256, 3), (33, 1000, 10, 0), (6, 2047, 64, 1),
+    (6, 2048, 256, 0), (6, 2049, 1, 0), (3, 8191, 17, 0), (2, 8200, 256, 5), (1, 32000, 16, 0), (2, 50261, 64, 3),
+    (1, 131072, 256, 0), (40, 33000, 50, 0), (600, 300, 30, 0), (1, 300001, 33, 0)])
+def test_top(dtype, rows, vocab, k, pad):
+    check_top(rand((rows, vocab), dtype, rows * 7 + vocab, pad=pad), k, temperature=0.7 if pad else 1.0)
+
+
+@pytest.mark.parametrize('vocab', [50, 1500, 9000, 70000])
+@pytest.mark.parametrize('kind', ['constant', 'ascending', 'descending', 'two', 'masked', 'all masked', 'lowest',
+                                  'nan', 'all nan', 'inf', 'zeros', 'integers', 'late', 'stripes'])
+def test_top_orders(vocab, kind):
+    """Rows where ties, masks or the order of the values could go wrong."""
+    for dtype in (torch.float32, torch.bfloat16):
+        x = rand((2, vocab), dtype, 5)
+        v = torch.arange(vocab, device='cuda')
+        if kind == 'constant':
+            x[:] = 1.5
+        elif kind == 'ascending':
+            x = x.sort(-1).values
+        elif kind == 'descending':
+            x = x.sort(-1, descending=True).values
+        elif kind == 'two':
+            x[:] = (v % 3 == 0).to(dtype)
+        elif kind == 'masked':
+            x[:, (v % (vocab // 10)) != 3] = -INF
+        elif kind == 'all masked':
+            x[0] = -INF
+        elif kind == 'lowest':
+            x[0] = LOWEST[dtype]
+            x[1, ::2] = LOWEST[dtype]
+        elif kind == 'nan':
+            x[:, ::7] = math.nan
+        elif kind == 'all nan':
+            x[0] = math.nan
+        elif kind == 'inf':
+            x[0, 17] = INF
+            x[1, 40:44] = INF
+            x[1, 3] = -INF
+        elif kind == 'zeros':
+            x[:] = 0.0
+            x[:, ::2] = -0.0
+        elif kind == 'integers':
+            x = x.round()
+        elif kind == 'late':
+            x[:, vocab - 20:] += 50
+        elif kind == 'stripes':
+            x[:, 8:16] += 60                       # the best all in one thread's first vector
+            x[:, vocab // 2:vocab // 2 + 40] += 40
+        for k in (1, 5, 33):
+            check_top(x, k)
+
+
+def test_top_views():
+    x = rand((4, 6, 777), torch.bfloat16, 3)
+    check_top(x[:, :-1], 9)
+    check_top(x[:, 1:, 5:700], 9)
+    check_top(x.transpose(0, 1), 9)
+    check_top(x[1, 2].expand(5, 777), 9)
+    check_top(x[0, 0], 9)
+    got = logits.top_logits(x[:, :0], 9)
+    assert got.values.shape == (4, 0, 9) and got.lse.shape == (4, 0)
+
+
+def test_top_many_rows():
+    """More rows than blocks are ever resident, of a tag set and of a small vocabulary."""
+    check_top(rand((20011, 13), torch.float32, 1), 13)
+    check_top(rand((9001, 200), torch.bfloat16, 2), 20)
+
+
+# ---- distillation -----------------------------------------------------------
+
+def teacher(z, k, dtype, seed, tail, temperature, empty=0.0):
+    t = (z.float() + rand(z.shape, torch.float32, seed, 1.5)).to(dtype)
+    top, ids = t.topk(k, -1)
+    lse = torch.logsumexp(t.double() / temperature, -1).float() if tail else None
+    g = torch.Generator().manual_seed(seed)
+    ids[(torch.rand(z.shape[:-1], generator=g) < empty).cuda()] = -1
+    return ids, top, lse
+
+
+def check_distill(z, ids, top, lse=None, temperature=1.0, weight=None):
+    """Autograd and the one-pass call, against the plain form."""
+    rows = z.shape[:-1]
+    vocab = z.shape[-1]
+    if weight is None:
+        weight = torch.rand(rows, generator=torch.Generator().manual_seed(9)).cuda()
+    flat = lambda t, n: None if t is None else t.reshape(-1, n) if n else t.reshape(-1)
+    loss, grad, loss_tol, grad_tol = plain.distill(flat(z, vocab), flat(ids, ids.shape[-1]), flat(top, ids.shape[-1]),
+                                                   flat(lse, 0), temperature, flat(weight, 0))
+    grad_tol = grad_tol + plain.type_tolerance(grad, z.dtype)
+    x = z.detach().requires_grad_()
+    got = logits.distill_loss(x, ids, top, top_lse=lse, temperature=temperature)
+    assert got.shape == rows and got.dtype == torch.float32
+    near(got.detach().reshape(-1), loss, loss_tol)
+    g, = torch.autograd.grad(got, x, weight)
+    assert g.shape == z.shape and g.dtype == z.dtype
+    near(g.reshape(-1, vocab), grad, grad_tol)
+    got2, g2 = logits.distill_loss_grad(z, ids, top, weight, top_lse=lse, temperature=temperature)
+    near(got2.reshape(-1), loss, loss_tol)
+    near(g2.reshape(-1, vocab), grad, grad_tol)
+    return got.detach(), g
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('tail', [False, True])
+@pytest.mark.parametrize('rows, vocab, k, pad, temperature', [
+    (1, 1, 1, 0, 1.0), (3, 2, 1, 1, 1.0), (70, 41, 5, 0, 1.0), (300, 13, 13, 0, 2.0), (5, 64, 9, 0, 1.0),
+    (5, 65, 65, 3, 0.5), (9, 128, 128, 0, 1.0), (9, 129, 30, 0, 1.0), (7, 1000, 256, 0, 1.0), (4, 2048, 1, 5, 3.0),
+    (4, 2049, 64, 0, 1.0), (3, 8192, 32, 0, 1.0), (2, 8197, 33, 2, 0.7), (2, 32000, 16, 0, 1.0),
+    (2, 50261, 32, 0, 2.0), (1, 131072, 64, 0, 1.0)])
+def test_distill(dtype, tail, rows, vocab, k, pad, temperature):
+    z = rand((rows, vocab), dtype, rows * 11 + vocab, pad=pad)
+    ids, top, lse = teacher(z, k, dtype, vocab, tail, temperature, empty=0.2 if rows > 4 else 0.0)
+    check_distill(z, ids, top, lse, temperature)
+
+
+@pytest.mark.parametrize('tail', [False, True])
+def test_distill_beyond_a_window_of_bits(tail):
+    z = rand((2, 600007), torch.bfloat16, 4)
+    ids, top, lse = teacher(z, 20, torch.bfloat16, 5, tail, 1.0)
+    ids[0, :4] = torch.tensor([0, 262143, 262144, 600006])
+    check_distill(z, ids, top, lse)
+
+
+@pytest.mark.parametrize('vocab', [30, 1200, 20000])
+def test_distill_masks(vocab):
+    """Padding, masked entries and masked logits, of the teacher and the student."""
+    z = rand((9, vocab), torch.float32, 6)
+    ids, top, lse = teacher(z, 8, torch.float32, 7, True, 1.0)
+    ids[0] = -1                                        # no entry
+    ids[1, 3:] = -1                                    # few entries
+    ids[2, 5] = vocab                                  # an id outside
+    ids[3, 0] = 2 ** 40
+    top[4] = -INF                                      # entries without weight
+    top[5, 2:] = -INF
+    z[6, ::2] = -INF                                   # masked in the student, the teacher's entries not
+    z[6].scatter_(0, ids[6], 0.0)
+    keep = z[7].gather(0, ids[7])                      # nothing but the entries is left
+    z[7] = -INF
+    z[7].scatter_(0, ids[7], keep)
+    z[8] = torch.finfo(torch.float32).min
+    z[8, 5] = 1.0
+    z[8].scatter_(0, ids[8], 0.5)
+    for use in (None, lse):
+        loss, grad = check_distill(z, ids, top, use)
+        assert not loss[0].item() and not grad[0].any()
+    assert torch.isfinite(loss).all() and torch.isfinite(grad).all()
+
+
+def test_distill_repeated_ids():
+    z = rand((5, 500), torch.float32, 8)
+    ids, top, lse = teacher(z, 12, torch.float32, 9, True, 1.0)
+    ids[:, 6:] = ids[:, :6]
+    top = top - 1.0                                    # the mass of both copies within the whole
+    a = check_distill(z, ids, top, None)
+    b = check_distill(z, ids, top, lse)
+    for _ in range(3):                                 # the same sums every time
+        assert torch.equal(check_distill(z, ids, top, None)[1], a[1])
+        assert torch.equal(check_distill(z, ids, top, lse)[1], b[1])
+
+
+def test_distill_impossible_entry():
+    """A teacher's entry that the student masks: an infinite loss, a finite gradient."""
+    z = rand((2, 300), torch.float32, 10)
+    ids, top, lse = teacher(z, 4, torch.float32, 11, False, 1.0)
+    z[0, ids[0, 1]] = -INF
+    loss, grad = logits.distill_loss_grad(z, ids, top, 1.0)
+    assert loss[0].item() == INF and math.isfinite(loss[1].item())
+    assert torch.isfinite(grad).all() and grad[0, ids[0, 1]] < 0
+
+
+def test_distill_types_and_views():
+    z = rand((3, 5, 1001), torch.bfloat16, 12)
+    view = z[:, :-1]
+    ids, top, lse = teacher(view, 6, torch.float32, 13, True, 1.0)
+    weight = torch.rand(3, 4).cuda()
+    a = check_distill(view, ids, top, lse, weight=weight)
+    b = check_distill(view, ids.int(), top, lse, weight=weight)
+    assert torch.equal(a[1], b[1])
+    check_distill(view, ids, top.half(), None, weight=weight.t().contiguous().t())
+    wide = rand((4, 999), torch.float16, 14, pad=25)
+    ids, top, _ = teacher(wide, 6, torch.float16, 15, False, 1.0)
+    check_distill(wide, ids, top)
+    one = z[0, 0]
+    check_distill(one.expand(3, 1001), *teacher(one.expand(3, 1001), 6, torch.float32, 16, True, 1.0))
+    ids, top, lse = teacher(one[None], 6, torch.float32, 16, True, 1.0)
+    check_distill(one, ids[0], top[0], lse[0], weight=torch.tensor(0.5).cuda())
+
+
+def test_distill_weights():
+    """Gradients of sums, means and numbers; of a broadcast input."""
+    z = rand((6, 400), torch.float32, 17)
+    ids, top, lse = teacher(z, 5, torch.float32, 18, True, 1.0)
+    for reduce, w in ((lambda t: t.sum(), 1.0), (lambda t: t.mean(), 1 / 6), (lambda t: (t * 0.5).sum(), 0.5)):
+        x = z.clone().requires_grad_()
+        reduce(logits.distill_loss(x, ids, top, top_lse=lse)).backward()
+        _, want = logits.distill_loss_grad(z, ids, top, w, top_lse=lse)
+        assert (x.grad - want).abs().max() <= 2.0 ** -23 * want.abs().max()
+    x = z[:1].clone().requires_grad_()
+    logits.distill_loss(x.expand(6, 400), ids, top).sum().backward()
+    _, each = logits.distill_loss_grad(z[:1].expand(6, 400), ids, top, 1.0)
+    assert x.grad.shape == (1, 400)
+    # six gradients added: 5 roundings of at most their sum
+    assert (x.grad[0] - each.sum(0)).abs().max() <= 10 * 2.0 ** -24 * each.abs().sum(0).max()
+    loss, grad = logits.distill_loss_grad(z[:0], ids[:0], top[:0], 1.0)
+    assert loss.shape == (0,) and grad.shape == (0, 400)
+
+
+def test_distill_gradient_against_differences():
+    """Central differences of the loss itself: h = 0.05 leaves h^2/6 |L'''| (at
+    most 4.2e-4, |L'''| <= 1) and the loss's rounding, 2 delta / h."""
+    z = rand((1, 10), torch.float32, 19, 1.0)
+    ids, top, lse = teacher(z, 3, torch.float32, 20, True, 1.0)
+    _, grad = logits.distill_loss_grad(z, ids, top, 1.0, top_lse=lse)
+    step = 0.05 * torch.eye(10, device='cuda')
+    both = torch.cat([z + step, z - step])
+    loss = logits.distill_loss(both, ids.expand(20, 3), top.expand(20, 3), top_lse=lse.expand(20))
+    diff = (loss[:10] - loss[10:]) / 0.1
+    assert (diff - grad[0]).abs().max() <= 4.2e-4 + 2 * (2 * plain.delta(10) + 2.0 ** -22) / 0.05
+
+
+# ---- verification -----------------------------------------------------------
+
+def drafted(batch, drafts, vocab, dtype, seed, certain=False, noise=0.7, pad=0):
+    target = rand((batch, drafts + 1, vocab), dtype, seed, pad=pad)
+    g = torch.Generator().manual_seed(seed + 1)
+    draft = None
+    if certain:
+        ids = target[:, :drafts].float().argmax(-1)
+        ids = torch.where((torch.rand(batch, drafts, generator=g) < 0.8).cuda(), ids,
+                          torch.randint(vocab, (batch, drafts), generator=g).cuda())
+    else:
+        draft = torch.zeros(batch, drafts, vocab + pad, dtype=dtype, device='cuda')[..., :vocab]
+        draft[:] = (target[:, :drafts].float() + rand((batch, drafts, vocab), torch.float32, seed + 2, noise)).to(dtype)
+        p = torch.softmax(draft.float(), -1).reshape(batch * drafts, vocab).cpu()
+        ids = torch.multinomial(p, 1, generator=g).view(batch, drafts).cuda() if batch * drafts else \
+            torch.zeros(batch, drafts, dtype=torch.int64, device='cuda')
+    return dict(target=target, draft_ids=ids, accept_u=torch.rand(batch, drafts, generator=g).cuda(),
+                sample_u=torch.rand(batch, generator=g).cuda(), draft=draft)
+
+
+def check_verify(**a):
+    got = logits.verify_draft(**a)
+    tokens, accepted = plain.verify(a['target'], a['draft_ids'], a['accept_u'], a['sample_u'], a.get('draft'),
+                                    a.get('lengths'), a.get('temperature', 1.0))
+    assert got.tokens.dtype == torch.int64 and got.accepted.dtype == torch.int64
+    assert torch.equal(got.accepted.cpu(), accepted)
+    assert torch.equal(got.tokens.cpu(), tokens)
+    return got
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('certain', [False, True])
+@pytest.mark.parametrize('batch, drafts, vocab, pad, temperature', [
+    (1, 0, 5, 0, 1.0), (1, 1, 1, 0, 1.0), (5, 3, 2, 0, 1.0), (40, 4, 41, 0, 1.0), (7, 2, 64, 1, 0.8),
+    (9, 5, 1000, 0, 1.0), (3, 8, 4097, 3, 1.5), (1, 4, 32000, 0, 1.0), (4, 3, 50261, 0, 0.6), (2, 2, 131072, 0, 1.0),
+    (300, 3, 700, 0, 1.0), (2, 20, 300, 0, 1.0)])
+def test_verify(dtype, certain, batch, drafts, vocab, pad, temperature):
+    a = drafted(batch, drafts, vocab, dtype, batch * 13 + vocab, certain, pad=pad)
+    check_verify(temperature=temperature, **a)
+
+
+@pytest.mark.parametrize('certain', [False, True])
+def test_verify_lengths(certain):
+    """Drafts of 0 tokens and more; what lies behind them is not read."""
+    a = drafted(30, 4, 900, torch.bfloat16, 30, certain)
+    n = torch.arange(30, dtype=torch.int32) % 5
+    for b in range(30):
+        a['target'][b, n[b] + 1:] = math.nan
+        a['draft_ids'][b, n[b]:] = 2 ** 50
+        a['accept_u'][b, n[b]:] = math.nan
+        if a['draft'] is not None:
+            a['draft'][b, n[b]:] = math.nan
+    got = check_verify(lengths=n.cuda(), **a)
+    assert (got.accepted.cpu() <= n).all()
+
+
+def test_verify_edges():
+    """Random numbers at their ends, ids outside, masked targets, equal
+    distributions, a row without any token."""
+    a = drafted(12, 2, 600, torch.float32, 31)
+    a['accept_u'][0] = 0.0
+    a['accept_u'][1] = 1 - 2.0 ** -24
+    a['sample_u'][:3] = torch.tensor([0.0, 1 - 2.0 ** -24, 0.0])
+    a['draft_ids'][2, 0] = -1
+    a['draft_ids'][3, 1] = 600
+    a['target'][4, :, 5:] = -INF                        # only five tokens are allowed
+    a['target'][5, :, ::2] = -INF
+    a['draft'][6] = a['target'][6, :2]                  # the same: all is accepted
+    a['accept_u'][6] = 1 - 2.0 ** -24
+    a['target'][7, 0] = -INF                            # nothing to draw
+    a['target'][8, :] = torch.finfo(torch.float32).min  # all alike
+    a['draft'][9, 0] = -INF
+    a['draft'][9, 0, a['draft_ids'][9, 0]] = 0.0        # a certain drafter, by its logits
+    a['target'][10, 0, 1:] = -INF                       # one token is left
+    a['sample_u'][10] = 1 - 2.0 ** -24
+    got = check_verify(**a)
+    assert got.accepted[6] == 2 and got.accepted[7] == 0 and got.tokens[7, 0] == -1
+    a = drafted(12, 2, 600, torch.float32, 32, certain=True)
+    a['accept_u'][0] = 0.0
+    a['draft_ids'][1, 0] = -5
+    a['target'][2, 0] = -INF
+    a['target'][2, 0, a['draft_ids'][2, 0]] = 0.0       # p = 1 at the certain token
+    a['accept_u'][2] = 1 - 2.0 ** -24
+    a['target'][3, 0, a['draft_ids'][3, 0]] = -INF
+    check_verify(**a)
+
+
+def test_verify_views_and_ids():
+    wide = drafted(6, 5, 333, torch.bfloat16, 33)
+    a = {k: v[:, :3] if k in ('draft_ids', 'accept_u', 'draft') else v[:, :4] if k == 'target' else v
+         for k, v in wide.items()}
+    got = check_verify(**a)
+    again = logits.verify_draft(**{**a, 'draft_ids': a['draft_ids'].int()})
+    assert torch.equal(got.tokens, again.tokens)
+    none = logits.verify_draft(a['target'][:0], a['draft_ids'][:0], a['accept_u'][:0], a['sample_u'][:0])
+    assert none.tokens.shape == (0, 4) and none.accepted.shape == (0,)
+
+
+# ---- streams, graphs, use together -------------------------------------------
+
+def calls(seed):
+    """One call of every operator on fixed tensors: (function, what to refill)."""
+    z = rand((6, 5000), torch.bfloat16, seed)
+    ids, top, lse = teacher(z, 8, torch.bfloat16, seed + 1, True, 1.0)
+    w = torch.rand(6).cuda()
+    a = drafted(4, 3, 5000, torch.bfloat16, seed + 2)
+    def run():
+        return [*logits.top_logits(z, 7), logits.distill_loss(z, ids, top, top_lse=lse),
+                *logits.distill_loss_grad(z, ids, top, w, top_lse=lse), *logits.verify_draft(**a)]
+    return run, (z, a['target'], a['draft'])
+
+
+def test_other_stream():
+    run, _ = calls(40)
+    want = run()
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        got = run()
+    s.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_two_streams_at_once():
+    one, _ = calls(41)
+    two, _ = calls(42)
+    want1, want2 = one(), two()
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    got1, got2 = [], []
+    for _ in range(5):
+        with torch.cuda.stream(s1):
+            got1.append(one())
+        with torch.cuda.stream(s2):
+            got2.append(two())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for got in got1 for a, b in zip(want1, got))
+    assert all(torch.equal(a, b) for got in got2 for a, b in zip(want2, got))
+
+
+def test_captured():
+    """Two graphs of the same calls, replayed with new logits and the program's
+    own work between the replays."""
+    run, fill = calls(43)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        run()
+    torch.cuda.current_stream().wait_stream(s)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = run()
+        graphs.append((g, out))
+    for i in range(4):
+        for t, new in zip(fill, [rand(t.shape, t.dtype, 50 + 3 * i + j) for j, t in enumerate(fill)]):
+            t.copy_(new)
+        want = run()
+        torch.cuda.synchronize()
+        for g, out in graphs if i % 2 else graphs[::-1]:
+            g.replay()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(want, out))
+
+
+def test_captured_training_step():
+    """Forward and backward in a graph, replayed; every replay against the eager gradient."""
+    z = rand((5, 3001), torch.float32, 60).requires_grad_()
+    ids, top, lse = teacher(z.detach(), 8, torch.float32, 61, True, 1.0)
+    w = torch.rand(5).cuda()
+    def step():
+        return torch.autograd.grad(logits.distill_loss(z, ids, top, top_lse=lse), z, w)[0]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for i in range(3):
+        with torch.no_grad():
+            z.copy_(rand((5, 3001), torch.float32, 70 + i))
+        want = step()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+def test_teach_draft_verify():
+    """As they are used together: a teacher's top logits are kept, a student is
+    fitted to them, and its drafts are verified against the teacher."""
+    vocab, dim = 500, 64
+    states = rand((256, dim), torch.float32, 80, 1.0)
+    head = rand((dim, vocab), torch.float32, 81, 0.6)
+    w = torch.zeros(dim, vocab, device='cuda').requires_grad_()
+    top = logits.top_logits((states @ head).bfloat16(), 16)
+    losses = []
+    for _ in range(20):
+        loss = logits.distill_loss(states @ w, top.ids, top.values, top_lse=top.lse).mean()
+        grad, = torch.autograd.grad(loss, w)
+        assert torch.isfinite(grad).all()
+        # by the chain rule from the one-pass gradient; products of 256 terms in float32
+        _, gz = logits.distill_loss_grad(states @ w, top.ids, top.values, 1 / 256, top_lse=top.lse)
+        want = states.double().t() @ gz.double()
+        bound = (states.double().abs().t() @ gz.double().abs()) * 260 * 2.0 ** -24 + 1e-9
+        assert ((grad.double() - want).abs() <= bound).all()
+        with torch.no_grad():
+            w -= 2.0 * grad
+        losses.append(float(loss.detach()))
+    assert all(math.isfinite(x) for x in losses)
+    target = (states @ head).view(64, 4, vocab)
+    draft = (states @ w.detach()).view(64, 4, vocab)[:, :3]
+    g = torch.Generator(device='cuda').manual_seed(5)
+    ids = torch.multinomial(torch.softmax(draft.reshape(192, vocab), -1), 1, generator=g).view(64, 3)
+    check_verify(target=target, draft_ids=ids, accept_u=torch.rand(64, 3, generator=g, device='cuda'),
+                 sample_u=torch.rand(64, generator=g, device='cuda'), draft=draft)
+
+
+def test_decoded_paths_teach():
+    """The k best paths of a lattice decode as a teacher's entries, other
+    scorers' scores of the same paths as the student's logits."""
+    from golden_io import load
+    from lattice_based_tagger_amd import (BeamScoreFunctions, RegularizationScore, beam_search_batch, evaluate_batch)
+    cases = [c for c in load('base') if not any('error' in e for e in c.expected.values())][:12]
+    teach = cases[0].funcs
+    student = BeamScoreFunctions(RegularizationScore(-0.3, 0.1, -0.1))
+    k = 8
+    paths = beam_search_batch([(c.bindex, c.chars) for c in cases], teach, beam_size=k, max_len=cases[0].max_len)
+    paths = [m for m in paths if len(m) == k]
+    assert paths
+    scores = torch.tensor([[float(s.score) for s in m] for m in paths], device='cuda')
+    z = torch.tensor(evaluate_batch([s for m in paths for s in m], student), device='cuda',
+                     dtype=torch.float32).view(len(paths), k)
+    best = logits.top_logits(scores, k)
+    assert torch.equal(best.ids.cpu(), torch.arange(k).expand(len(paths), k))      # the decoder's order
+    check_distill(z, best.ids, best.values, None)
