@@ -1,9 +1,9 @@
 # Sanitizer builds of the library's host code (ADVICE / VERDICT r1: ASan, UBSan,
 # TSan over lt_lookup.cpp, lt_packer.cpp and the host half of lt_capi.cpp /
 # lt_comm.cpp).  The host sources are compiled by g++ with the sanitizer; the
-# device sources (lt_decode.hip, lt_results.hip, lt_logits.hip) by hipcc for gfx950 without
-# one (GPU sanitizers are not available on the pool).  The CPU test suite then
-# runs against the instrumented library (LT_LIBRARY) with the sanitizer runtime
+# device sources (lt_decode.hip, lt_results.hip, lt_top.hip, lt_distill.hip,
+# lt_verify.hip) by hipcc for gfx950 without one (GPU sanitizers are not
+# available on the pool).  The CPU test suite then runs against the instrumented library (LT_LIBRARY) with the sanitizer runtime
 # preloaded into the interpreter:
 #
 #   make check-asan     # AddressSanitizer + UndefinedBehaviorSanitizer
@@ -20,7 +20,8 @@ OUT := build/san
 HOST := lt_capi lt_packer lt_comm lt_lookup
 # without packed float32 instructions, as in _build.py
 NOPK := -Xclang -target-feature -Xclang -packed-fp32-ops
-DEV := lt_decode lt_results lt_logits
+LOGITS := lt_top lt_distill lt_verify
+DEV := lt_decode lt_results $(LOGITS)
 HDRS := $(wildcard $(CSRC)/*.h) $(wildcard include/*.h)
 SANFLAGS_COMMON := -O1 -g -std=c++17 -fPIC -ffp-contract=off -fno-omit-frame-pointer -Wall \
   -D__HIP_PLATFORM_AMD__ -I$(ROCM)/include -Iinclude
@@ -41,7 +42,7 @@ lib:
 
 $(OUT)/dev/%.o: $(CSRC)/%.hip $(HDRS)
 	@mkdir -p $(dir $@)
-	$(HIPCC) --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off $(if $(findstring lt_logits,$<),$(NOPK)) -Iinclude -c $< -o $@
+	$(HIPCC) --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off $(if $(filter $*,$(LOGITS)),$(NOPK)) -Iinclude -c $< -o $@
 
 $(OUT)/asan/%.o: $(CSRC)/%.cpp $(HDRS)
 	@mkdir -p $(dir $@)

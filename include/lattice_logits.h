@@ -36,6 +36,7 @@ extern "C" {
 #define LT_F16 1
 #define LT_BF16 2
 
+#define LT_MAX_VOCAB (1 << 30)
 #define LT_MAX_TOP 256     /* largest k of lt_top_logits, entries of a teacher's row */
 
 /* Rows of logits: row r starts at element (r / inner) * stride_outer +
@@ -50,7 +51,7 @@ typedef struct {
   int64_t inner;          /* >= 1 */
   int64_t stride_outer;   /* in elements */
   int64_t stride_inner;
-  int64_t vocab;          /* 1 .. 2^31 - 1 */
+  int64_t vocab;          /* 1 .. LT_MAX_VOCAB */
 } lt_rows;
 
 /* Path of the HIP runtime library this library is bound to. */
@@ -58,8 +59,8 @@ const char* lt_hip_library(void);
 
 /* ---- the k best logits of a row --------------------------------------------
  * ids[r*k + j], j = 0..k-1: the k largest logits of row r, largest first, ties
- * to the lowest index; a NaN counts as -inf in this order.  values: those
- * logits, in the rows' type.  lse[r] = log sum_v exp(x_v / temperature): -inf
+ * to the lowest index; a NaN counts as -inf in this order, -0 as 0.  values:
+ * those logits, in the rows' type.  lse[r] = log sum_v exp(x_v / temperature): -inf
  * for a row of -inf, NaN if the row holds a NaN (and no +inf).
  * 1 <= k <= min(vocab, LT_MAX_TOP). */
 int64_t lt_top_logits_workspace(const lt_rows* x, int32_t k);

@@ -19,8 +19,9 @@ ROCM = os.environ.get('ROCM_PATH', '/opt/rocm')
 HIPCC = os.path.join(ROCM, 'bin', 'hipcc')
 ARCH = 'gfx950'
 
-SOURCES = ['lt_decode.hip', 'lt_results.hip', 'lt_logits.hip', 'lt_capi.cpp', 'lt_packer.cpp', 'lt_comm.cpp', 'lt_lookup.cpp']
-HEADERS = ['lt_common.h', 'lt_internal.h', 'lt_error.h', 'lt_handles.h', 'lt_host.h', os.path.join('..', '..', 'include', 'lattice_decode.h'),
+SOURCES = ['lt_decode.hip', 'lt_results.hip', 'lt_top.hip', 'lt_distill.hip', 'lt_verify.hip',
+           'lt_capi.cpp', 'lt_packer.cpp', 'lt_comm.cpp', 'lt_lookup.cpp']
+HEADERS = ['lt_common.h', 'lt_logits.h', 'lt_internal.h', 'lt_error.h', 'lt_handles.h', 'lt_host.h', os.path.join('..', '..', 'include', 'lattice_decode.h'),
            os.path.join('..', '..', 'include', 'lattice_pack.h'),
            os.path.join('..', '..', 'include', 'lattice_lookup.h'),
            os.path.join('..', '..', 'include', 'lattice_logits.h')]
@@ -37,7 +38,8 @@ COMMON_FLAGS = ['-O3', '-std=c++17', '-fPIC', '-ffp-contract=off', '-fno-fast-ma
 # Without packed float32 instructions (hipcc makes them of ordinary float code
 # at -O3; some of their forms are unreliable on this hardware).  The decoders'
 # sources compile to none of them either way.
-SOURCE_FLAGS = {'lt_logits.hip': ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']}
+NO_PACKED = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
+SOURCE_FLAGS = {src: NO_PACKED for src in ('lt_top.hip', 'lt_distill.hip', 'lt_verify.hip')}
 
 
 def _stale(target, deps):

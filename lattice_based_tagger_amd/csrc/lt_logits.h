@@ -1,0 +1,221 @@
+// lt_logits.h -- what the operators over logits share (lt_top.hip,
+// lt_distill.hip, lt_verify.hip): element types, rows, block reductions, and
+// the host's checks and launches.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "../../include/lattice_logits.h"
+#include "lt_error.h"
+
+namespace {
+
+constexpr int MAXK = LT_MAX_TOP;
+constexpr float LOWEST = -3.4028234663852886e38f;
+
+struct Rows {
+  const void* data;
+  int64_t inner, stride_outer, stride_inner;
+  int32_t vocab;
+  __device__ __forceinline__ int64_t at(int64_t r) const {
+    return inner == 1 ? r * stride_outer : (r / inner) * stride_outer + (r % inner) * stride_inner;
+  }
+};
+
+struct F32 {
+  using raw = float;
+  static __device__ __forceinline__ float get(raw v) { return v; }
+  static __device__ __forceinline__ raw put(float v) { return v; }
+};
+struct F16 {
+  using raw = uint16_t;
+  static __device__ __forceinline__ float get(raw v) { return (float)__builtin_bit_cast(_Float16, v); }
+  static __device__ __forceinline__ raw put(float v) { return __builtin_bit_cast(raw, (_Float16)v); }
+};
+struct BF16 {
+  using raw = uint16_t;
+  static __device__ __forceinline__ float get(raw v) { return __builtin_bit_cast(float, (uint32_t)v << 16); }
+  // to the nearest, ties to even; a NaN stays one
+  static __device__ __forceinline__ raw put(float v) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    if (v != v) return (raw)((b >> 16) | 0x40);
+    return (raw)((b + 0x7fff + ((b >> 16) & 1)) >> 16);
+  }
+};
+
+// 16 bytes of a row, at any address its type allows (the loads and stores are
+// single ones: global memory takes them unaligned).
+struct __attribute__((packed, aligned(2))) Bytes16 {
+  uint32_t w[4];
+};
+
+// The E = 16 / sizeof(raw) logits of a vector.
+template <class T>
+struct Vec {
+  static constexpr int E = 16 / sizeof(typename T::raw);
+  Bytes16 b;
+  __device__ __forceinline__ void load(const typename T::raw* p) { b = *(const Bytes16*)p; }
+  __device__ __forceinline__ void store(typename T::raw* p) const { *(Bytes16*)p = b; }
+  __device__ __forceinline__ float get(int i) const;
+  // n < E logits, `fill` behind them
+  __device__ __forceinline__ void load_part(const typename T::raw* p, int n, typename T::raw fill) {
+    if constexpr (E == 4) {
+      for (int i = 0; i < 4; ++i) b.w[i] = __builtin_bit_cast(uint32_t, i < n ? p[i] : fill);
+    } else {
+      for (int i = 0; i < 4; ++i)
+        b.w[i] = (uint32_t)(2 * i < n ? p[2 * i] : fill) | (uint32_t)(2 * i + 1 < n ? p[2 * i + 1] : fill) << 16;
+    }
+  }
+};
+template <>
+__device__ __forceinline__ float Vec<F32>::get(int i) const {
+  return __builtin_bit_cast(float, b.w[i]);
+}
+template <>
+__device__ __forceinline__ float Vec<F16>::get(int i) const {
+  return F16::get((uint16_t)(b.w[i >> 1] >> (i & 1) * 16));
+}
+template <>
+__device__ __forceinline__ float Vec<BF16>::get(int i) const {
+  return __builtin_bit_cast(float, i & 1 ? b.w[i >> 1] & 0xffff0000u : b.w[i >> 1] << 16);
+}
+
+// The larger of two, of three; a NaN gives way to a number.
+__device__ __forceinline__ float max2(float a, float b) {
+  float r;
+  asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+template <class T>
+__device__ __forceinline__ float max_of(const Vec<T>& v) {
+  if constexpr (Vec<T>::E == 4) return max2(max3(v.get(0), v.get(1), v.get(2)), v.get(3));
+  else return max3(max3(max3(v.get(0), v.get(1), v.get(2)), v.get(3), v.get(4)), max2(v.get(5), v.get(6)), v.get(7));
+}
+
+// 2^x of the hardware: within an ulp, 0 below the normal numbers.
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ float any_float(const void* p, int64_t i, int dtype) {
+  if (dtype == LT_F32) return ((const float*)p)[i];
+  return dtype == LT_F16 ? F16::get(((const uint16_t*)p)[i]) : BF16::get(((const uint16_t*)p)[i]);
+}
+
+__device__ __forceinline__ int64_t any_id(const void* p, int64_t i, int bytes) {
+  return bytes == 8 ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
+}
+
+// ---- reductions of a block -------------------------------------------------
+struct Max {
+  template <class T>
+  static __device__ __forceinline__ T of(T a, T b) { return a > b ? a : b; }
+};
+struct Sum {
+  template <class T>
+  static __device__ __forceinline__ T of(T a, T b) { return a + b; }
+};
+
+// Every thread gets the result.  sh: NT / 64 entries, free for reuse on return.
+template <int NT, class Op, class T>
+__device__ __forceinline__ T block_reduce(T v, T* sh) {
+  for (int o = 32; o; o >>= 1) v = Op::of(v, __shfl_xor(v, o, 64));
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = sh[0];
+  for (int w = 1; w < NT / 64; ++w) v = Op::of(v, sh[w]);
+  __syncthreads();
+  return v;
+}
+
+// sum of exp2((x - m) c) over what a thread has seen; m is LOWEST at first, so
+// that a -inf logit adds 0 and a row of the type's lowest value adds 1 each.
+struct Running {
+  float m = LOWEST, s = 0.f;
+  __device__ __forceinline__ void add(float x, float c) {
+    if (x > m) {
+      s *= exp2f((m - x) * c);
+      m = x;
+    }
+    s += exp2f((x - m) * c);
+  }
+};
+
+// A logit as a whole number in the order of the values (NaN as -inf, -0 as 0).
+__device__ __forceinline__ uint32_t order_of(float x) {
+  x = x != x ? -INFINITY : x + 0.f;
+  const uint32_t b = __builtin_bit_cast(uint32_t, x);
+  return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float of_order(uint32_t o) {
+  return __builtin_bit_cast(float, o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu));
+}
+
+// The order above the complement of the index: no two keys of a row are alike,
+// and of equal logits the first has the larger.
+__device__ __forceinline__ uint64_t order_key(float x, uint32_t id) { return ((uint64_t)order_of(x) << 32) | (uint32_t)~id; }
+
+// ---- host ------------------------------------------------------------------
+#define BAD(...) return lt::set_error(LT_EINVAL, __VA_ARGS__)
+
+inline int dtype_bytes(int d) { return d == LT_F32 ? 4 : 2; }
+
+inline bool rows_ok(const lt_rows* x, const char* what, lt_status* st) {
+  *st = LT_OK;
+  if (!x) *st = lt::set_error(LT_EINVAL, "%s: NULL", what);
+  else if (x->dtype < LT_F32 || x->dtype > LT_BF16) *st = lt::set_error(LT_EINVAL, "%s: dtype %d", what, x->dtype);
+  else if (x->rows < 0 || x->inner < 1) *st = lt::set_error(LT_EINVAL, "%s: rows %lld, inner %lld", what, (long long)x->rows, (long long)x->inner);
+  else if (x->vocab < 1 || x->vocab > LT_MAX_VOCAB) *st = lt::set_error(LT_EINVAL, "%s: vocab %lld", what, (long long)x->vocab);
+  else if (x->rows > 0 && (!x->data || (uintptr_t)x->data % dtype_bytes(x->dtype)))
+    *st = lt::set_error(LT_EINVAL, "%s: data is NULL or not aligned to its type", what);
+  return *st == LT_OK;
+}
+
+inline bool temperature_ok(double t) { return t >= 1e-6 && t <= 1e6; }
+
+inline Rows rows_of(const lt_rows* x) {
+  Rows r;
+  r.data = x->data;
+  r.inner = x->inner;
+  r.stride_outer = x->stride_outer;
+  r.stride_inner = x->stride_inner;
+  r.vocab = (int32_t)x->vocab;
+  return r;
+}
+
+// The call's device is current for as long as this lives.
+struct OnDevice {
+  int was = -1;
+  hipError_t err;
+  explicit OnDevice(int device) {
+    err = hipGetDevice(&was);
+    if (err == hipSuccess && was != device) err = hipSetDevice(device);
+    else if (err == hipSuccess) was = -1;
+  }
+  ~OnDevice() {
+    if (was >= 0) (void)hipSetDevice(was);
+  }
+};
+
+template <class P>
+lt_status launch(void (*kernel)(P), int64_t blocks, int threads, P& p, void* stream, const char* what) {
+  void* args[] = {&p};
+  const hipError_t e = hipLaunchKernel((const void*)kernel, dim3((uint32_t)blocks), dim3(threads), args, 0, (hipStream_t)stream);
+  if (e != hipSuccess) return lt::set_error(LT_EHIP, "%s: %s", what, hipGetErrorString(e));
+  return LT_OK;
+}
+
+#define BY_TYPE(dtype, kernel) ((dtype) == LT_F32 ? kernel<F32> : (dtype) == LT_F16 ? kernel<F16> : kernel<BF16>)
+#define ON_DEVICE(d)                                                                                   \
+  OnDevice on(d);                                                                                      \
+  if (on.err != hipSuccess) return lt::set_error(LT_EHIP, "device %d: %s", (int)(d), hipGetErrorString(on.err))
+
+constexpr int64_t MAX_BLOCKS = 1 << 20;
+
+constexpr double LOG2E = 1.4426950408889634;
+
+}  // namespace

@@ -15,8 +15,8 @@ logits over a vocabulary or a tag set:
                             accept, from given random numbers, and the token
                             that follows them.
 
-The kernels are HIP (``csrc/lt_logits.hip``, C-ABI
-``include/lattice_logits.h``, in ``liblt.so``); there is no other path.  They
+The kernels are HIP (``csrc/lt_top.hip``, ``lt_distill.hip``,
+``lt_verify.hip``; C-ABI ``include/lattice_logits.h``, in ``liblt.so``); there is no other path.  They
 run on the tensors' device, on its current stream, and may be captured into a
 graph.  This module is the only one of the package that imports ``torch``:
 import ``torch`` (or this module) before anything of the package decodes, so
@@ -37,7 +37,8 @@ import torch
 
 from . import _capi
 
-MAX_TOP = 256              # lattice_logits.h LT_MAX_TOP
+MAX_VOCAB = 1 << 30      # lattice_logits.h LT_MAX_VOCAB
+MAX_TOP = 256              # LT_MAX_TOP
 MAX_DRAFTS = 256           # LT_MAX_DRAFTS
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _STATS = 4                 # LT_DISTILL_STATS
@@ -120,8 +121,8 @@ def _logits(x, what):
         raise TypeError('%s must be a torch.Tensor, not %s' % (what, type(x).__name__))
     if x.dtype not in _DTYPES:
         raise TypeError('%s must be float32, float16 or bfloat16, not %s' % (what, x.dtype))
-    if x.dim() < 1 or x.shape[-1] < 1 or x.shape[-1] > 0x7fffffff:
-        raise ValueError('%s must be [..., vocab] with 1 <= vocab < 2^31, not %s' % (what, tuple(x.shape)))
+    if x.dim() < 1 or x.shape[-1] < 1 or x.shape[-1] > MAX_VOCAB:
+        raise ValueError('%s must be [..., vocab] with 1 <= vocab <= 2^30, not %s' % (what, tuple(x.shape)))
     if x.shape[-1] > 1 and x.stride(-1) != 1:
         raise ValueError('%s: the elements of a row must be adjacent (stride 1, not %d)' % (what, x.stride(-1)))
 

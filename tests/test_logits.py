@@ -90,7 +90,7 @@ def _desc(**kw):
 
 
 @pytest.mark.parametrize('kw', [dict(dtype=3), dict(dtype=-1), dict(rows=-1), dict(inner=0), dict(vocab=0),
-                                dict(vocab=1 << 31), dict(data=None), dict(data=4098)])
+                                dict(vocab=(1 << 30) + 1), dict(data=None), dict(data=4098)])
 def test_c_entries_refuse_rows(kw):
     lib = logits._load()
     x = _desc(**kw)
