@@ -16,6 +16,7 @@ struct Teacher {
 };
 
 struct DistillParams {
+  int64_t block0;         // of this launch
   Rows z;
   Teacher t;
   int64_t rows;
@@ -75,7 +76,8 @@ __global__ __launch_bounds__(NT) void lt_distill_fwd(DistillParams p) {
   __shared__ TeacherRow t;
   __shared__ uint32_t bits[WINDOW / 32];
   __shared__ float shf[NW];
-  for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+  {
+    const int64_t r = p.block0 + blockIdx.x;
     const raw* z = (const raw*)p.z.data + p.z.at(r);
     double psum, prest;
     teacher_row(p.t, r, p.z.vocab, p.inv_t, t, psum, prest);
@@ -124,7 +126,8 @@ template <class T>
 __global__ __launch_bounds__(NT) void lt_distill_bwd(DistillParams p) {
   using raw = typename T::raw;
   __shared__ TeacherRow t;
-  for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+  {
+    const int64_t r = p.block0 + blockIdx.x;
     const raw* z = (const raw*)p.z.data + p.z.at(r);
     raw* g = (raw*)p.grad.data + p.grad.at(r);
     double psum, prest;
@@ -195,7 +198,7 @@ lt_status lt_distill_forward(const lt_rows* z, const lt_teacher* t, double tempe
   DistillParams p = distill_params(z, t, temperature);
   p.loss = loss;
   p.stats = stats;
-  return launch(BY_TYPE(z->dtype, lt_distill_fwd), z->rows < MAX_BLOCKS ? z->rows : MAX_BLOCKS, NT, p, stream, "lt_distill_forward");
+  return launch(BY_TYPE(z->dtype, lt_distill_fwd), z->rows, NT, p, stream, "lt_distill_forward");
 }
 
 lt_status lt_distill_backward(const lt_rows* z, const lt_teacher* t, double temperature, const float* stats,
@@ -210,7 +213,7 @@ lt_status lt_distill_backward(const lt_rows* z, const lt_teacher* t, double temp
   p.weight = weight;
   p.weight_stride = weight_stride;
   p.grad = rows_of(grad);
-  return launch(BY_TYPE(z->dtype, lt_distill_bwd), z->rows < MAX_BLOCKS ? z->rows : MAX_BLOCKS, NT, p, stream, "lt_distill_backward");
+  return launch(BY_TYPE(z->dtype, lt_distill_bwd), z->rows, NT, p, stream, "lt_distill_backward");
 }
 
 lt_status lt_distill_fused(const lt_rows* z, const lt_teacher* t, double temperature, const float* weight,

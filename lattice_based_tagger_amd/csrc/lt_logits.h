@@ -58,13 +58,25 @@ struct Vec {
   __device__ __forceinline__ void load(const typename T::raw* p) { b = *(const Bytes16*)p; }
   __device__ __forceinline__ void store(typename T::raw* p) const { *(Bytes16*)p = b; }
   __device__ __forceinline__ float get(int i) const;
-  // n < E logits, `fill` behind them
+  // What is computed from the logits ahead of this is not kept for later.
+  __device__ __forceinline__ void keep() { asm volatile("" : "+v"(b.w[0]), "+v"(b.w[1]), "+v"(b.w[2]), "+v"(b.w[3])); }
+  // n < E logits, `fill` behind them (a rolled loop: few registers, taken once a row)
   __device__ __forceinline__ void load_part(const typename T::raw* p, int n, typename T::raw fill) {
-    if constexpr (E == 4) {
-      for (int i = 0; i < 4; ++i) b.w[i] = __builtin_bit_cast(uint32_t, i < n ? p[i] : fill);
-    } else {
-      for (int i = 0; i < 4; ++i)
-        b.w[i] = (uint32_t)(2 * i < n ? p[2 * i] : fill) | (uint32_t)(2 * i + 1 < n ? p[2 * i + 1] : fill) << 16;
+    b.w[0] = b.w[1] = b.w[2] = b.w[3] = 0;
+#pragma nounroll
+    for (int i = E - 1; i >= 0; --i) {
+      const typename T::raw v = i < n ? p[i] : fill;
+      if constexpr (E == 4) {
+        b.w[3] = b.w[2];
+        b.w[2] = b.w[1];
+        b.w[1] = b.w[0];
+        b.w[0] = __builtin_bit_cast(uint32_t, v);
+      } else {
+        b.w[3] = b.w[3] << 16 | b.w[2] >> 16;
+        b.w[2] = b.w[2] << 16 | b.w[1] >> 16;
+        b.w[1] = b.w[1] << 16 | b.w[0] >> 16;
+        b.w[0] = b.w[0] << 16 | v;
+      }
     }
   }
 };
@@ -120,10 +132,58 @@ struct Sum {
   static __device__ __forceinline__ T of(T a, T b) { return a + b; }
 };
 
+// v of another lane by a data-parallel-primitives control word, `other` where
+// there is none (in steps of 32 bits).
+template <int CTRL, int ROWS, class T>
+__device__ __forceinline__ T dpp(T v, T other) {
+  constexpr int N = sizeof(T) / 4;
+  struct Words { int w[N]; };
+  Words a = __builtin_bit_cast(Words, v), o = __builtin_bit_cast(Words, other);
+#pragma unroll
+  for (int i = 0; i < N; ++i) a.w[i] = __builtin_amdgcn_update_dpp(o.w[i], a.w[i], CTRL, ROWS, 0xf, false);
+  return __builtin_bit_cast(T, a);
+}
+
+// Op over the lanes up to each one (0 .. lane), `none` being Op's neutral value.
+template <class Op, class T>
+__device__ __forceinline__ T wave_scan(T v, T none) {
+  v = Op::of(v, dpp<0x111, 0xf>(v, none));      // the row's lane - 1, - 2, - 4, - 8
+  v = Op::of(v, dpp<0x112, 0xf>(v, none));
+  v = Op::of(v, dpp<0x114, 0xf>(v, none));
+  v = Op::of(v, dpp<0x118, 0xf>(v, none));
+  v = Op::of(v, dpp<0x142, 0xa>(v, none));      // lane 15 of the row before, into rows 1 and 3
+  v = Op::of(v, dpp<0x143, 0xc>(v, none));      // lane 31, into rows 2 and 3
+  return v;
+}
+
+template <class T>
+__device__ __forceinline__ T lane_value(T v, int lane) {
+  constexpr int N = sizeof(T) / 4;
+  struct Words { int w[N]; };
+  Words a = __builtin_bit_cast(Words, v);
+#pragma unroll
+  for (int i = 0; i < N; ++i) a.w[i] = __builtin_amdgcn_readlane(a.w[i], lane);
+  return __builtin_bit_cast(T, a);
+}
+
+template <class Op, class T>
+__device__ __forceinline__ T wave_reduce(T v, T none) {
+  return lane_value(wave_scan<Op>(v, none), 63);
+}
+
+template <class Op, class T>
+__device__ __forceinline__ T neutral();
+template <> __device__ __forceinline__ float neutral<Max, float>() { return -INFINITY; }
+template <> __device__ __forceinline__ double neutral<Max, double>() { return -INFINITY; }
+template <> __device__ __forceinline__ uint64_t neutral<Max, uint64_t>() { return 0; }
+template <> __device__ __forceinline__ float neutral<Sum, float>() { return 0.f; }
+template <> __device__ __forceinline__ double neutral<Sum, double>() { return 0.; }
+
 // Every thread gets the result.  sh: NT / 64 entries, free for reuse on return.
 template <int NT, class Op, class T>
 __device__ __forceinline__ T block_reduce(T v, T* sh) {
-  for (int o = 32; o; o >>= 1) v = Op::of(v, __shfl_xor(v, o, 64));
+  v = wave_reduce<Op>(v, neutral<Op, T>());
+  if (NT == 64) return v;
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
   __syncthreads();
   v = sh[0];
@@ -201,11 +261,17 @@ struct OnDevice {
   }
 };
 
+// `blocks` blocks, in as many launches as the grid's limit (2^32 threads) takes:
+// block 0 of a launch is p.block0.
 template <class P>
-lt_status launch(void (*kernel)(P), int64_t blocks, int threads, P& p, void* stream, const char* what) {
-  void* args[] = {&p};
-  const hipError_t e = hipLaunchKernel((const void*)kernel, dim3((uint32_t)blocks), dim3(threads), args, 0, (hipStream_t)stream);
-  if (e != hipSuccess) return lt::set_error(LT_EHIP, "%s: %s", what, hipGetErrorString(e));
+lt_status launch(void (*kernel)(P), int64_t blocks, int threads, P p, void* stream, const char* what) {
+  const int64_t most = (int64_t)1 << 21;
+  for (p.block0 = 0; p.block0 < blocks; p.block0 += most) {
+    const int64_t n = blocks - p.block0 < most ? blocks - p.block0 : most;
+    void* args[] = {&p};
+    const hipError_t e = hipLaunchKernel((const void*)kernel, dim3((uint32_t)n), dim3(threads), args, 0, (hipStream_t)stream);
+    if (e != hipSuccess) return lt::set_error(LT_EHIP, "%s: %s", what, hipGetErrorString(e));
+  }
   return LT_OK;
 }
 
@@ -213,8 +279,6 @@ lt_status launch(void (*kernel)(P), int64_t blocks, int threads, P& p, void* str
 #define ON_DEVICE(d)                                                                                   \
   OnDevice on(d);                                                                                      \
   if (on.err != hipSuccess) return lt::set_error(LT_EHIP, "device %d: %s", (int)(d), hipGetErrorString(on.err))
-
-constexpr int64_t MAX_BLOCKS = 1 << 20;
 
 constexpr double LOG2E = 1.4426950408889634;
 

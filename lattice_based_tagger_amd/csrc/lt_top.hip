@@ -5,10 +5,17 @@
 #include "lt_logits.h"
 
 namespace {
+#ifndef XTH
+#define XTH 512
+#endif
+#ifndef XP
+#define XP 192
+#endif
 
 struct TopParams {
   Rows x;
   int64_t rows;
+  int64_t block0;         // of this launch
   int32_t k;
   int32_t splits;         // blocks of a row
   int32_t chunk;          // logits of a block (a multiple of 8), the last one's fewer
@@ -26,25 +33,139 @@ __device__ __forceinline__ float log_sum(float m, float s, float c) {
   return m == INFINITY ? m : (float)((double)m * (c * 0.6931471805599453) + log((double)s));
 }
 
-// The keys of buf[0 .. n), n <= C, each by its rank (the number of larger
-// ones): afterwards buf[0 .. min(n, k)) holds the best in order.
+// The key of lane ^ X: by the data-parallel primitives where they can, else by
+// the LDS crossbar.
+template <int X>
+__device__ __forceinline__ uint64_t from_lane_xor(uint64_t v) {
+  constexpr int CTRL = X == 1 ? 0xb1 : X == 2 ? 0x4e : X == 3 ? 0x1b : X == 7 ? 0x141 : X == 8 ? 0x128 : X == 15 ? 0x140 : 0;
+  if constexpr (CTRL) {
+    return dpp<CTRL, 0xf>(v, v);
+  } else if constexpr (X < 32) {
+    const uint32_t lo = __builtin_amdgcn_ds_swizzle((int)(uint32_t)v, X << 10 | 0x1f);
+    const uint32_t hi = __builtin_amdgcn_ds_swizzle((int)(uint32_t)(v >> 32), X << 10 | 0x1f);
+    return (uint64_t)hi << 32 | lo;
+  } else {
+    return __shfl_xor(v, X, 64);
+  }
+}
+// The larger of the two keys to the lane whose bit BIT is 0.
+template <int X, int BIT>
+__device__ __forceinline__ void exchange(uint64_t& key) {
+  const uint64_t other = from_lane_xor<X>(key);
+  key = (key > other) == ((threadIdx.x & BIT) == 0) ? key : other;
+}
+
+// A wave's 64 keys, largest in lane 0: a bitonic sort, every merge's first
+// exchange with the mirrored lane, so that all go the same way.
+__device__ __forceinline__ uint64_t sort_wave(uint64_t key) {
+  exchange<1, 1>(key);
+  exchange<3, 2>(key), exchange<1, 1>(key);
+  exchange<7, 4>(key), exchange<2, 2>(key), exchange<1, 1>(key);
+  exchange<15, 8>(key), exchange<4, 4>(key), exchange<2, 2>(key), exchange<1, 1>(key);
+  exchange<31, 16>(key), exchange<8, 8>(key), exchange<4, 4>(key), exchange<2, 2>(key), exchange<1, 1>(key);
+  exchange<63, 32>(key), exchange<16, 16>(key), exchange<8, 8>(key), exchange<4, 4>(key), exchange<2, 2>(key), exchange<1, 1>(key);
+  return key;
+}
+
+// The best min(n, k) of the keys buf[0 .. n), n <= C, in order: sorted 64 at a
+// time, then each by its rank, its place in its own 64 and how many of every
+// other 64 are larger (a search of seven steps).
 template <int NT, int C>
-__device__ __forceinline__ void rank_keys(uint64_t* buf, int n, int k) {
+__device__ __forceinline__ void sort_keys(uint64_t* buf, int n, int k) {
+  const int tid = threadIdx.x, lane = tid & 63;
   uint64_t key[C / NT];
+#pragma unroll
+  for (int i = 0; i < C / NT; ++i) {
+    key[i] = 0;
+    if (i * NT + (tid & ~63) < n) {
+      key[i] = sort_wave(i * NT + tid < n ? buf[i * NT + tid] : 0);
+      if (n > 64 || NT == 64) buf[i * NT + tid] = key[i];
+    }
+  }
+  __syncthreads();
   int rank[C / NT];
 #pragma unroll
   for (int i = 0; i < C / NT; ++i) {
-    const int at = i * NT + threadIdx.x;
-    rank[i] = at < n ? 0 : k;
-    key[i] = at < n ? buf[at] : ~0ull;
-    if (i * NT + (int)(threadIdx.x & ~63u) < n)
-      for (int j = 0; j < n; ++j) rank[i] += buf[j] > key[i];
+    rank[i] = lane;
+    if (n > 64 && i * NT + (tid & ~63) < n)
+#pragma unroll 2
+      for (int l = 0; l < n; l += 64) {
+        const uint64_t* o = buf + l;
+        int at = 0;
+#pragma unroll
+        for (int step = 32; step; step /= 2) at += o[at + step - 1] > key[i] ? step : 0;
+        at += o[at] > key[i];
+        rank[i] += l == i * NT + (tid & ~63) ? 0 : at;
+      }
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < C / NT; ++i)
-    if (rank[i] < k) buf[rank[i]] = key[i];
+    if (key[i] && rank[i] < k) buf[rank[i]] = key[i];
   __syncthreads();
+}
+
+// Keeps the k largest of the keys buf[0 .. n), k < n <= C, in any order, and
+// returns a key that they reach and the others do not: the k-th is found eight bits at a time, from the leading bit in which the keys
+// differ, by counting the keys of every value of the eight.  hist: 256 counts,
+// cnt: one more, sh: NT / 64 keys.
+template <int NT, int C>
+__device__ __forceinline__ uint64_t cut_keys(uint64_t* buf, int n, int k, int* hist, int* cnt, uint64_t* sh) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  uint64_t key[C / NT], hi = 0, lo = ~0ull;
+#pragma unroll
+  for (int i = 0; i < C / NT; ++i) {
+    key[i] = i * NT + tid < n ? buf[i * NT + tid] : 0;
+    hi = key[i] > hi ? key[i] : hi;
+    if (key[i]) lo = key[i] < lo ? key[i] : lo;
+  }
+  hi = block_reduce<NT, Max>(hi, sh);
+  lo = ~block_reduce<NT, Max>(~lo, sh);
+  uint64_t at_least = lo;                 // the k-th key's leading bits, as a key
+  int need = k;
+  uint64_t width = ~0ull;                 // the keys still in question: less than this above it
+  for (int shift = max(0, 56 - __clzll(hi - lo)); ; shift = max(0, shift - 8)) {
+    for (int i = tid; i < 256; i += NT) hist[i] = 0;
+    if (tid == 0) *cnt = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < C / NT; ++i) {
+      const uint64_t over = key[i] - at_least;
+      if (key[i] >= at_least && over < width) atomicAdd(&hist[over >> shift], 1);
+    }
+    __syncthreads();
+    const int4 h = ((const int4*)hist)[lane];
+    int above = h.x + h.y + h.z + h.w;
+    const int upto = wave_scan<Sum>(above, 0);
+    above += lane_value(upto, 63) - upto;         // keys from this lane's four values up
+    const int l = 63 - __clzll(__ballot(above >= need));
+    int d = l * 4, left = lane_value(above, l);      // keys of value d and up
+    const int c0 = lane_value(h.x, l), c1 = lane_value(h.y, l), c2 = lane_value(h.z, l), c3 = lane_value(h.w, l);
+    int here = c0;
+    if (left - here >= need) left -= here, ++d, here = c1;
+    if (d == l * 4 + 1 && left - here >= need) left -= here, ++d, here = c2;
+    if (d == l * 4 + 2 && left - here >= need) left -= here, ++d, here = c3;
+    at_least += (uint64_t)d << shift;
+    need -= left - here;
+    width = 1ull << shift;
+    __syncthreads();
+    if (here == need || shift == 0) break;
+  }
+#pragma unroll
+  for (int i = 0; i < C / NT; ++i)
+    if (key[i] >= at_least) buf[atomicAdd(cnt, 1)] = key[i];
+  __syncthreads();
+  return at_least;
+}
+
+// The k best of the keys buf[0 .. n), in order.
+template <int NT, int C>
+__device__ __forceinline__ void best_keys(uint64_t* buf, int n, int k, int* hist, int* cnt, uint64_t* sh) {
+    if (n > XTH && n > k) {
+    cut_keys<NT, C>(buf, n, k, hist, cnt, sh);
+    n = k;
+  }
+  sort_keys<NT, C>(buf, n, k);
 }
 
 // The k best of x[v0 .. v1) one after another, k passes: rows with a NaN.
@@ -65,179 +186,263 @@ __device__ void best_by_passes(const typename T::raw* x, int v0, int v1, int k, 
 
 // One pass over a row (or a chunk of it).  A step takes U vectors of 16 bytes
 // a thread.  From the first step's largest logit of every thread comes a
-// bound tau that at least k logits reach; what is above it goes into an LDS
-// buffer, a few more than k of a row's logits, which are then ranked.
+// bound tau that at least k logits reach; a vector with a logit above it goes
+// on a list in LDS (its number: a few instructions of a wave, where sorting
+// out single logits here took half of the time).  When the list is long, and
+// at the end, the vectors' logits above tau become keys, the k largest of
+// which are kept and raise tau.
 // - Equal logits: those at tau itself are left out; if fewer than k lie above
 //   it, the first of them fill up (a scan that ends when enough are found),
 //   which also serves rows masked with -inf.
-// - A step that overflows the buffer (logits that rise along the row) is
-//   taken again from the registers, one logit of a thread at a time, ranking
-//   when the buffer is full, which raises tau to the k-th best so far.
-template <class T, int NT, int U, int C>
+// - What overflows the list or the keys (logits that rise along the row) is
+//   taken again, one logit of a thread at a time, cutting the keys to k when
+//   they are full.
+// (keep() has the logits unpacked anew for each use: held as floats between
+// the uses they took 118 registers and half the waves.)
+template <class T, int NT, int U, int C, int CL>
 __global__ __launch_bounds__(NT) void lt_top_k(TopParams p) {
   using raw = typename T::raw;
   constexpr int E = Vec<T>::E, W = NT / 64, STEP = NT * U * E;
   __shared__ __attribute__((aligned(16))) uint64_t buf[C];
+  __shared__ __attribute__((aligned(16))) int hist[256];
+  __shared__ uint32_t list[CL];
   __shared__ uint64_t sh64[W];
   __shared__ float shf[W];
-  __shared__ int cnt;
+  __shared__ uint32_t sh_th[W];
+  __shared__ int sh_reach[W];
+  __shared__ int cnt, cnt2, listed;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int per_wave = (p.k + W - 1) / W + 1;
-  for (int64_t blk = blockIdx.x; blk < p.rows * p.splits; blk += gridDim.x) {
-    const int64_t r = p.splits == 1 ? blk : blk / p.splits;
-    const int split = p.splits == 1 ? 0 : (int)(blk % p.splits);
-    const raw* x = (const raw*)p.x.data + p.x.at(r);
-    const int v0 = split * p.chunk, v1 = min(p.x.vocab, v0 + p.chunk);
-    const int k = min(p.k, v1 - v0);
-    float m = LOWEST, s = 0.f, tau = -INFINITY;
-    if (tid == 0) cnt = 0;
-    __syncthreads();
-    int before = 0;                        // the buffer's entries ahead of this step
-    for (int base = v0; base < v1; base += STEP) {
-      Vec<T> v[U];
-      float vm[U];
-      if (base + STEP <= v1) {
+  const int64_t blk = p.block0 + blockIdx.x;
+  const int64_t r = p.splits == 1 ? blk : blk / p.splits;
+  const int split = p.splits == 1 ? 0 : (int)(blk % p.splits);
+  const raw* x = (const raw*)p.x.data + p.x.at(r);
+  const int v0 = split * p.chunk, v1 = min(p.x.vocab, v0 + p.chunk);
+  const int k = min(p.k, v1 - v0);
+  const int per_wave = (k + W - 1) / W + 1;
+  float m = LOWEST, s = 0.f, tau = -INFINITY;
+  int n = 0;                             // keys
+  if (tid == 0) cnt = listed = 0;
+  __syncthreads();
+
+  // Above tau; or equal to it, and ahead of the last that a cut kept (in a
+  // list, whose vectors lie in any order: of later steps none is ahead).
+  uint32_t tie = 0xffffffffu;
+  auto counts = [&](float f, int id) { return f > tau || (f == tau && ~(uint32_t)id > tie); };
+  auto cut = [&]() {
+    const uint64_t least = cut_keys<NT, C>(buf, n, k, hist, &cnt2, sh64);
+    tau = of_order((uint32_t)(least >> 32));
+    tie = max((uint32_t)least, 1u) - 1;
+    n = k;
+  };
+
+  // The logits of nv vectors -- list[i], or first + i -- that count become keys.
+  auto expand = [&](const uint32_t* of, int first, int nv) {
+#pragma nounroll
+    for (int i0 = 0; i0 < nv; i0 += NT) {
+      const int i = i0 + tid;
+      const int at = i < nv ? v0 + (of ? (int)of[i] : first + i) * E : v1;
+      Vec<T> v;
+      if (at + E <= v1) v.load(x + at);
+      else v.load_part(x + at, max(0, v1 - at), T::put(-INFINITY));
+      int mine = 0;
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u].load(x + base + (u * NT + tid) * E);
-      } else {
+      for (int e = 0; e < E; ++e) mine += at + e < v1 && counts(v.get(e), at + e);
+      if (__any(mine)) {
+        const int upto = wave_scan<Sum>(mine, 0);
+        int pos = 0;
+        if (lane == 63) pos = atomicAdd(&cnt, upto);
+        pos = __builtin_amdgcn_readlane(pos, 63) + upto - mine;
+        v.keep();
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int at = base + (u * NT + tid) * E;
-          if (at + E <= v1) v[u].load(x + at);
-          else v[u].load_part(x + at, max(0, v1 - at), T::put(-INFINITY));
+        for (int e = 0; e < E; ++e) {
+          const float f = v.get(e);
+          if (at + e < v1 && counts(f, at + e)) {
+            if (pos < C) buf[pos] = order_key(f, (uint32_t)(at + e));
+            ++pos;
+          }
         }
       }
-      float t = -INFINITY;
+      __syncthreads();
+      const int was = n;
+      n = cnt;
+      __syncthreads();
+      if (n > C) {
+        n = was;
+        if (n > C - NT) cut();             // (room for a logit of every thread)
+        if (tid == 0) cnt = n;
+        __syncthreads();
+#pragma nounroll
+        for (int e = 0; e < E; ++e) {
+          const float f = at + e < v1 ? T::get(x[at + e]) : -INFINITY;
+          if (at + e < v1 && counts(f, at + e)) buf[atomicAdd(&cnt, 1)] = order_key(f, (uint32_t)(at + e));
+          __syncthreads();
+          n = cnt;
+          __syncthreads();
+          if (n > C - NT) {
+            cut();
+            if (tid == 0) cnt = k;
+            __syncthreads();
+          }
+        }
+      }
+    }
+  };
+  // The best k so far: fewer of the logits to come lie above the last of them.
+  auto tighten = [&]() {
+    if (n > k) cut();
+    tie = 0xffffffffu;
+    if (tid == 0) {
+      cnt = n;
+      listed = 0;
+    }
+    __syncthreads();
+  };
+
+  int have = 0;                          // vectors on the list
+  for (int base = v0; base < v1; base += STEP) {
+    Vec<T> v[U];
+    float vm[U];
+    if (base + STEP <= v1) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u].load(x + base + (u * NT + tid) * E);
+    } else {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        vm[u] = max_of(v[u]);
-        t = max2(t, vm[u]);
+        const int at = base + (u * NT + tid) * E;
+        if (at + E <= v1) v[u].load(x + at);
+        else v[u].load_part(x + at, max(0, v1 - at), T::put(-INFINITY));
       }
-      if ((t - m) * p.c > 32.f) {
-        s *= exp2_((m - t) * p.c);
-        m = t;
-      }
-      float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int e = 0; e < E; e += 2) {
-          s0 += exp2_((v[u].get(e) - m) * p.c);
-          s1 += exp2_((v[u].get(e + 1) - m) * p.c);
-        }
-      s += s0 + s1;
-      if (base == v0) {
-        // the per_wave-th largest of a wave's threads (from its leading 18
-        // bits down): over all waves at least k logits reach the least of them
-        const uint32_t o = order_of(t);
-        uint32_t th = 0;
-        for (int bit = 31; bit >= 14; --bit) {
-          const uint32_t cand = th | 1u << bit;
-          if (__popcll(__ballot(o >= cand)) >= per_wave) th = cand;
-        }
-        tau = th <= order_of(-INFINITY) ? -INFINITY : of_order(th);
-        if (W > 1) {
-          if (lane == 0) shf[wave] = tau;
-          __syncthreads();
-          for (int w = 0; w < W; ++w) tau = fminf(tau, shf[w]);
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (vm[u] > tau) {
-#pragma unroll
-          for (int e = 0; e < E; ++e) {
-            const float f = v[u].get(e);
-            if (f > tau) {
-              const int at = atomicAdd(&cnt, 1);
-              if (at < C) buf[at] = order_key(f, (uint32_t)(base + (u * NT + tid) * E + e));
-            }
-          }
-        }
-      __syncthreads();
-      int n = cnt;
-      if (n > C) {
-        uint64_t above = (uint64_t)order_of(tau) << 32 | 0xffffffffu;
-        __syncthreads();
-        if (tid == 0) cnt = before;
-        __syncthreads();
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          for (int e = 0; e < E; ++e) {
-            float f = 0;
-#pragma unroll
-            for (int i = 0; i < E; ++i) f = i == e ? v[u].get(i) : f;
-            const int at = base + (u * NT + tid) * E + e;
-            const uint64_t key = order_key(f, (uint32_t)at);
-            if (at < v1 && key > above) buf[atomicAdd(&cnt, 1)] = key;
-            __syncthreads();
-            n = cnt;
-            __syncthreads();
-            if (n > C - NT) {
-              rank_keys<NT, C>(buf, n, k);
-              above = buf[k - 1];
-              tau = of_order((uint32_t)(above >> 32));
-              n = k;
-              if (tid == 0) cnt = k;
-              __syncthreads();
-            }
-          }
-      }
-      before = n;
-      // (a later step's first push may run ahead of this step's slowest read)
-      if (base + STEP < v1) __syncthreads();
     }
-    const float top = block_reduce<NT, Max>(m, shf);
-    const float sum = block_reduce<NT, Sum>(s * exp2_((m - top) * p.c), shf);
-    int n = before;
-    if (sum != sum) {
-      best_by_passes<T, NT>(x, v0, v1, k, buf, sh64);
-    } else {
-      for (int base = v0; n < k; base += NT) {
-        // the first logits that equal tau: in order, a thread a logit
-        const int at = base + tid;
-        const bool hit = at < v1 && T::get(x[min(at, v1 - 1)]) == tau;
-        const uint64_t b = __ballot(hit);
-        if (lane == 0) sh64[wave] = b;
+    float t = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      vm[u] = max_of(v[u]);
+      t = max2(t, vm[u]);
+      v[u].keep();
+    }
+    if ((t - m) * p.c > 32.f) {
+      s *= exp2_((m - t) * p.c);
+      m = t;
+    }
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        s0 += exp2_((v[u].get(e) - m) * p.c);
+        s1 += exp2_((v[u].get(e + 1) - m) * p.c);
+      }
+    s += s0 + s1;
+    if (base == v0) {
+      // the per_wave-th largest of a wave's threads (from its leading 18 bits
+      // down), and of the waves' the largest that k threads of the block reach
+      const uint32_t o = order_of(t);
+      uint32_t th = 0;
+      for (int bit = 31; bit >= 14; --bit) {
+        const uint32_t cand = th | 1u << bit;
+        if (__popcll(__ballot(o >= cand)) >= per_wave) th = cand;
+      }
+      if (W > 1) {
+        if (lane == 0) {
+          sh_th[wave] = th;
+          sh_reach[wave] = 0;
+        }
         __syncthreads();
-        int pos = n + __popcll(b & ((1ull << lane) - 1)), all = 0;
+#pragma nounroll
         for (int w = 0; w < W; ++w) {
-          const int c = __popcll(sh64[w]);
-          if (w < wave) pos += c;
-          all += c;
+          const int c = __popcll(__ballot(o >= sh_th[w]));
+          if (lane == w) atomicAdd(&sh_reach[w], c);
         }
-        if (hit && pos < k) buf[pos] = order_key(tau, (uint32_t)at);
-        n = min(k, n + all);
         __syncthreads();
-        if (base + NT >= v1) break;        // (never short of k: at least k logits reach tau)
+        th = 0;
+#pragma nounroll
+        for (int w = 0; w < W; ++w)
+          if (sh_reach[w] > k && sh_th[w] > th) th = sh_th[w];
       }
-      rank_keys<NT, C>(buf, n, k);
+      tau = th <= order_of(-INFINITY) ? -INFINITY : of_order(th);
     }
-    if (p.splits == 1) {
-      if (tid == 0) p.lse[r] = log_sum(top, sum, p.c);
-      for (int j = tid; j < k; j += NT) {
-        const uint32_t id = ~(uint32_t)buf[j];
-        p.ids[r * k + j] = id;
-        // (the key holds a NaN as -inf)
-        ((raw*)p.values)[r * k + j] = sum != sum ? x[id] : T::put(of_order((uint32_t)(buf[j] >> 32)));
+    if (__any(t > tau)) {
+      uint64_t b[U];
+      int all = 0, pos = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        b[u] = __ballot(vm[u] > tau);
+        all += __popcll(b[u]);
       }
-    } else {
-      if (tid == 0) p.part_sums[blk] = make_float2(top, sum);
-      for (int j = tid; j < p.k; j += NT) p.part_keys[blk * p.k + j] = j < k ? buf[j] : 0;
+      if (lane == 0) pos = atomicAdd(&listed, all);
+      pos = __builtin_amdgcn_readfirstlane(pos);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int at = pos + __builtin_amdgcn_mbcnt_hi((uint32_t)(b[u] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b[u], 0));
+        if (vm[u] > tau && at < CL) list[at] = (uint32_t)((base - v0) / E + u * NT + tid);
+        pos += __popcll(b[u]);
+      }
     }
     __syncthreads();
+    const int was = have;
+    have = listed;
+    if (have > CL) {
+      __syncthreads();
+      expand(list, 0, was);
+      expand(nullptr, (base - v0) / E, min(NT * U, (v1 - base + E - 1) / E));
+      tighten();
+      have = 0;
+    } else if (base + STEP < v1) {
+      __syncthreads();                   // (a push of the next step may run ahead of the slowest read of `listed`)
+      if (n + have > k + k / 2 + XP) {
+        expand(list, 0, have);
+        tighten();
+        have = 0;
+      }
+    }
+  }
+  expand(list, 0, have);
+  const float top = block_reduce<NT, Max>(m, shf);
+  const float sum = block_reduce<NT, Sum>(s * exp2_((m - top) * p.c), shf);
+  if (sum != sum) {
+    best_by_passes<T, NT>(x, v0, v1, k, buf, sh64);
+  } else {
+    for (int base = v0; n < k; base += NT) {
+      // the first logits that equal tau: in order, a thread a logit
+      const int at = base + tid;
+      const bool hit = at < v1 && T::get(x[min(at, v1 - 1)]) == tau;
+      const uint64_t b = __ballot(hit);
+      if (lane == 0) sh64[wave] = b;
+      __syncthreads();
+      int pos = n + __popcll(b & ((1ull << lane) - 1)), all = 0;
+      for (int w = 0; w < W; ++w) {
+        const int c = __popcll(sh64[w]);
+        if (w < wave) pos += c;
+        all += c;
+      }
+      if (hit && pos < k) buf[pos] = order_key(tau, (uint32_t)at);
+      n = min(k, n + all);
+      __syncthreads();
+      if (base + NT >= v1) break;        // (never short of k: at least k logits reach tau)
+    }
+    best_keys<NT, C>(buf, n, k, hist, &cnt2, sh64);
+  }
+  if (p.splits == 1) {
+    if (tid == 0) p.lse[r] = log_sum(top, sum, p.c);
+    for (int j = tid; j < k; j += NT) {
+      const uint32_t id = ~(uint32_t)buf[j];
+      p.ids[r * k + j] = id;
+      // (the key holds a NaN as -inf)
+      ((raw*)p.values)[r * k + j] = sum != sum ? x[id] : T::put(of_order((uint32_t)(buf[j] >> 32)));
+    }
+  } else {
+    if (tid == 0) p.part_sums[blk] = make_float2(top, sum);
+    for (int j = tid; j < p.k; j += NT) p.part_keys[blk * p.k + j] = j < k ? buf[j] : 0;
   }
 }
 
 template <class T>
 lt_status launch_top(TopParams& p, void* stream) {
-  const int64_t rows = p.rows < MAX_BLOCKS ? p.rows : MAX_BLOCKS;
-  p.splits = 1;
+    p.splits = 1;
   p.chunk = (p.x.vocab + 7) / 8 * 8;
-  if (p.k > 192 ? p.x.vocab > 2048 : p.x.vocab > 16384)
-    return launch(lt_top_k<T, 1024, 4, 2048>, rows, 1024, p, stream, "lt_top_logits");
-  if (p.k > 62 || p.x.vocab > 2048) return launch(lt_top_k<T, 256, 4, 2048>, rows, 256, p, stream, "lt_top_logits");
-  return launch(lt_top_k<T, 64, 4, 512>, rows, 64, p, stream, "lt_top_logits");
+  if (p.k > 192 || p.x.vocab > 8192) return launch(lt_top_k<T, 512, 4, 1024, 1024>, p.rows * p.splits, 512, p, stream, "lt_top_logits");
+  if (p.k > 62 || p.x.vocab > 2048) return launch(lt_top_k<T, 256, 4, 1024, 512>, p.rows * p.splits, 256, p, stream, "lt_top_logits");
+  return launch(lt_top_k<T, 64, 4, 256, 128>, p.rows * p.splits, 64, p, stream, "lt_top_logits");
 }
 
 }  // namespace

@@ -9,6 +9,7 @@ constexpr int NW = NT / 64;               // its waves
 
 // ---- verification ----------------------------------------------------------
 struct VerifyParams {
+  int64_t block0;         // of this launch
   Rows target, draft;     // draft.data NULL: certain tokens
   const void* ids;
   const float* accept_u;
@@ -47,7 +48,8 @@ __global__ __launch_bounds__(NT) void lt_verify(VerifyParams p) {
   __shared__ int sh_last;
   const int V = p.target.vocab;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  for (int64_t b = blockIdx.x; b < p.batch; b += gridDim.x) {
+  {
+    const int64_t b = p.block0 + blockIdx.x;
     int n = p.lengths ? p.lengths[b] : p.drafts;
     n = max(0, min(n, p.drafts));
     const raw *x = nullptr, *y = nullptr;
@@ -160,7 +162,7 @@ lt_status lt_verify_draft(const lt_draft* d, double temperature, int64_t* tokens
   p.inv_t = 1 / temperature;
   p.tokens = tokens;
   p.accepted = accepted;
-  return launch(BY_TYPE(d->target->dtype, lt_verify), d->batch < MAX_BLOCKS ? d->batch : MAX_BLOCKS, NT, p, stream, "lt_verify_draft");
+  return launch(BY_TYPE(d->target->dtype, lt_verify), d->batch, NT, p, stream, "lt_verify_draft");
 }
 
 }  // extern "C"
