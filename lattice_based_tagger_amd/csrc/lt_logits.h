@@ -179,11 +179,29 @@ template <> __device__ __forceinline__ uint64_t neutral<Max, uint64_t>() { retur
 template <> __device__ __forceinline__ float neutral<Sum, float>() { return 0.f; }
 template <> __device__ __forceinline__ double neutral<Sum, double>() { return 0.; }
 
+// A barrier of a group of NT threads: of a block, or of one wave of several
+// that work on rows of their own.
+template <int NT>
+__device__ __forceinline__ void sync() {
+  if constexpr (NT == 64) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  } else {
+    __syncthreads();
+  }
+}
+
+// A thread's number in its group, the group's in its block.
+template <int NT>
+__device__ __forceinline__ int thread_of() { return NT == 64 ? threadIdx.x & 63 : threadIdx.x; }
+template <int NT>
+__device__ __forceinline__ int group_of() { return NT == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0; }
+
 // Every thread gets the result.  sh: NT / 64 entries, free for reuse on return.
 template <int NT, class Op, class T>
 __device__ __forceinline__ T block_reduce(T v, T* sh) {
   v = wave_reduce<Op>(v, neutral<Op, T>());
-  if (NT == 64) return v;
+  if constexpr (NT == 64) return v;
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
   __syncthreads();
   v = sh[0];
@@ -218,6 +236,28 @@ __device__ __forceinline__ float of_order(uint32_t o) {
 // The order above the complement of the index: no two keys of a row are alike,
 // and of equal logits the first has the larger.
 __device__ __forceinline__ uint64_t order_key(float x, uint32_t id) { return ((uint64_t)order_of(x) << 32) | (uint32_t)~id; }
+
+// ---- rows of a few logits ----------------------------------------------------
+// A wave takes 64 rows, a thread one of them, from LDS: the logits come in
+// together (each row's own addresses, 64 of the rows' logits at a time) and lie
+// in words of 4 bytes at an odd pitch, so that the threads' reads of one column
+// fall on different banks.
+constexpr int FEW = 64;                    // logits of such a row, at most
+
+__host__ __device__ inline int few_pitch(int vocab) { return vocab | 1; }
+
+// f(row of the 64, v, its place among all) for every logit, 64 at a time
+template <class F>
+__device__ __forceinline__ void each_of_rows(int rows, int vocab, F f) {
+  const int lane = threadIdx.x & 63, dr = 64 / vocab, dv = 64 - dr * vocab;
+  int r = lane / vocab, v = lane - r * vocab;
+  for (int i = lane; i < rows * vocab; i += 64) {
+    f(r, v, i);
+    r += dr;
+    v += dv;
+    if (v >= vocab) v -= vocab, ++r;
+  }
+}
 
 // ---- host ------------------------------------------------------------------
 #define BAD(...) return lt::set_error(LT_EINVAL, __VA_ARGS__)
@@ -264,12 +304,12 @@ struct OnDevice {
 // `blocks` blocks, in as many launches as the grid's limit (2^32 threads) takes:
 // block 0 of a launch is p.block0.
 template <class P>
-lt_status launch(void (*kernel)(P), int64_t blocks, int threads, P p, void* stream, const char* what) {
+lt_status launch(void (*kernel)(P), int64_t blocks, int threads, P p, void* stream, const char* what, int lds = 0) {
   const int64_t most = (int64_t)1 << 21;
   for (p.block0 = 0; p.block0 < blocks; p.block0 += most) {
     const int64_t n = blocks - p.block0 < most ? blocks - p.block0 : most;
     void* args[] = {&p};
-    const hipError_t e = hipLaunchKernel((const void*)kernel, dim3((uint32_t)n), dim3(threads), args, 0, (hipStream_t)stream);
+    const hipError_t e = hipLaunchKernel((const void*)kernel, dim3((uint32_t)n), dim3(threads), args, lds, (hipStream_t)stream);
     if (e != hipSuccess) return lt::set_error(LT_EHIP, "%s: %s", what, hipGetErrorString(e));
   }
   return LT_OK;

@@ -72,7 +72,7 @@ __device__ __forceinline__ uint64_t sort_wave(uint64_t key) {
 // other 64 are larger (a search of seven steps).
 template <int NT, int C>
 __device__ __forceinline__ void sort_keys(uint64_t* buf, int n, int k) {
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int tid = thread_of<NT>(), lane = tid & 63;
   uint64_t key[C / NT];
 #pragma unroll
   for (int i = 0; i < C / NT; ++i) {
@@ -82,7 +82,7 @@ __device__ __forceinline__ void sort_keys(uint64_t* buf, int n, int k) {
       if (n > 64 || NT == 64) buf[i * NT + tid] = key[i];
     }
   }
-  __syncthreads();
+  sync<NT>();
   int rank[C / NT];
 #pragma unroll
   for (int i = 0; i < C / NT; ++i) {
@@ -98,11 +98,11 @@ __device__ __forceinline__ void sort_keys(uint64_t* buf, int n, int k) {
         rank[i] += l == i * NT + (tid & ~63) ? 0 : at;
       }
   }
-  __syncthreads();
+  sync<NT>();
 #pragma unroll
   for (int i = 0; i < C / NT; ++i)
     if (key[i] && rank[i] < k) buf[rank[i]] = key[i];
-  __syncthreads();
+  sync<NT>();
 }
 
 // Keeps the k largest of the keys buf[0 .. n), k < n <= C, in any order, and
@@ -111,7 +111,7 @@ __device__ __forceinline__ void sort_keys(uint64_t* buf, int n, int k) {
 // cnt: one more, sh: NT / 64 keys.
 template <int NT, int C>
 __device__ __forceinline__ uint64_t cut_keys(uint64_t* buf, int n, int k, int* hist, int* cnt, uint64_t* sh) {
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int tid = thread_of<NT>(), lane = tid & 63;
   uint64_t key[C / NT], hi = 0, lo = ~0ull;
 #pragma unroll
   for (int i = 0; i < C / NT; ++i) {
@@ -127,13 +127,13 @@ __device__ __forceinline__ uint64_t cut_keys(uint64_t* buf, int n, int k, int* h
   for (int shift = max(0, 56 - __clzll(hi - lo)); ; shift = max(0, shift - 8)) {
     for (int i = tid; i < 256; i += NT) hist[i] = 0;
     if (tid == 0) *cnt = 0;
-    __syncthreads();
+    sync<NT>();
 #pragma unroll
     for (int i = 0; i < C / NT; ++i) {
       const uint64_t over = key[i] - at_least;
       if (key[i] >= at_least && over < width) atomicAdd(&hist[over >> shift], 1);
     }
-    __syncthreads();
+    sync<NT>();
     const int4 h = ((const int4*)hist)[lane];
     int above = h.x + h.y + h.z + h.w;
     const int upto = wave_scan<Sum>(above, 0);
@@ -148,13 +148,13 @@ __device__ __forceinline__ uint64_t cut_keys(uint64_t* buf, int n, int k, int* h
     at_least += (uint64_t)d << shift;
     need -= left - here;
     width = 1ull << shift;
-    __syncthreads();
+    sync<NT>();
     if (here == need || shift == 0) break;
   }
 #pragma unroll
   for (int i = 0; i < C / NT; ++i)
     if (key[i] >= at_least) buf[atomicAdd(cnt, 1)] = key[i];
-  __syncthreads();
+  sync<NT>();
   return at_least;
 }
 
@@ -174,14 +174,14 @@ __device__ void best_by_passes(const typename T::raw* x, int v0, int v1, int k, 
   uint64_t below = ~0ull;
   for (int j = 0; j < k; ++j) {
     uint64_t best = 0;
-    for (int v = v0 + threadIdx.x; v < v1; v += NT) {
+    for (int v = v0 + thread_of<NT>(); v < v1; v += NT) {
       const uint64_t key = order_key(T::get(x[v]), (uint32_t)v);
       if (key < below && key > best) best = key;
     }
     below = block_reduce<NT, Max>(best, sh);
-    if (threadIdx.x == 0) out[j] = below;
+    if (thread_of<NT>() == 0) out[j] = below;
   }
-  __syncthreads();
+  sync<NT>();
 }
 
 // One pass over a row (or a chunk of it).  A step takes U vectors of 16 bytes
@@ -199,20 +199,28 @@ __device__ void best_by_passes(const typename T::raw* x, int v0, int v1, int k, 
 //   they are full.
 // (keep() has the logits unpacked anew for each use: held as floats between
 // the uses they took 118 registers and half the waves.)
+template <int NT, int C, int CL>
+struct TopShared {
+  uint64_t buf[C];
+  uint64_t sh64[NT / 64];
+  int hist[256];
+  uint32_t list[CL];
+  float shf[NT / 64];
+  uint32_t th[NT / 64];
+  int reach[NT / 64];
+  int cnt, cnt2, listed;
+};
+
 template <class T, int NT, int U, int C, int CL>
-__global__ __launch_bounds__(NT) void lt_top_k(TopParams p) {
+__global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
   using raw = typename T::raw;
-  constexpr int E = Vec<T>::E, W = NT / 64, STEP = NT * U * E;
-  __shared__ __attribute__((aligned(16))) uint64_t buf[C];
-  __shared__ __attribute__((aligned(16))) int hist[256];
-  __shared__ uint32_t list[CL];
-  __shared__ uint64_t sh64[W];
-  __shared__ float shf[W];
-  __shared__ uint32_t sh_th[W];
-  __shared__ int sh_reach[W];
-  __shared__ int cnt, cnt2, listed;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t blk = p.block0 + blockIdx.x;
+  constexpr int E = Vec<T>::E, W = NT / 64, STEP = NT * U * E, GROUPS = NT == 64 ? 4 : 1;
+  __shared__ __attribute__((aligned(16))) TopShared<NT, C, CL> shared[GROUPS];
+  TopShared<NT, C, CL>& sh = shared[group_of<NT>()];
+  uint64_t* const buf = sh.buf;
+  const int tid = thread_of<NT>(), lane = tid & 63, wave = tid >> 6;
+  const int64_t blk = (p.block0 + blockIdx.x) * GROUPS + group_of<NT>();
+  if (blk >= p.rows * p.splits) return;  // (a wave as a whole)
   const int64_t r = p.splits == 1 ? blk : blk / p.splits;
   const int split = p.splits == 1 ? 0 : (int)(blk % p.splits);
   const raw* x = (const raw*)p.x.data + p.x.at(r);
@@ -221,15 +229,15 @@ __global__ __launch_bounds__(NT) void lt_top_k(TopParams p) {
   const int per_wave = (k + W - 1) / W + 1;
   float m = LOWEST, s = 0.f, tau = -INFINITY;
   int n = 0;                             // keys
-  if (tid == 0) cnt = listed = 0;
-  __syncthreads();
+  if (tid == 0) sh.cnt = sh.listed = 0;
+  sync<NT>();
 
   // Above tau; or equal to it, and ahead of the last that a cut kept (in a
   // list, whose vectors lie in any order: of later steps none is ahead).
   uint32_t tie = 0xffffffffu;
   auto counts = [&](float f, int id) { return f > tau || (f == tau && ~(uint32_t)id > tie); };
   auto cut = [&]() {
-    const uint64_t least = cut_keys<NT, C>(buf, n, k, hist, &cnt2, sh64);
+    const uint64_t least = cut_keys<NT, C>(buf, n, k, sh.hist, &sh.cnt2, sh.sh64);
     tau = of_order((uint32_t)(least >> 32));
     tie = max((uint32_t)least, 1u) - 1;
     n = k;
@@ -250,7 +258,7 @@ __global__ __launch_bounds__(NT) void lt_top_k(TopParams p) {
       if (__any(mine)) {
         const int upto = wave_scan<Sum>(mine, 0);
         int pos = 0;
-        if (lane == 63) pos = atomicAdd(&cnt, upto);
+        if (lane == 63) pos = atomicAdd(&sh.cnt, upto);
         pos = __builtin_amdgcn_readlane(pos, 63) + upto - mine;
         v.keep();
 #pragma unroll
@@ -262,26 +270,26 @@ __global__ __launch_bounds__(NT) void lt_top_k(TopParams p) {
           }
         }
       }
-      __syncthreads();
+      sync<NT>();
       const int was = n;
-      n = cnt;
-      __syncthreads();
+      n = sh.cnt;
+      sync<NT>();
       if (n > C) {
         n = was;
         if (n > C - NT) cut();             // (room for a logit of every thread)
-        if (tid == 0) cnt = n;
-        __syncthreads();
+        if (tid == 0) sh.cnt = n;
+        sync<NT>();
 #pragma nounroll
         for (int e = 0; e < E; ++e) {
           const float f = at + e < v1 ? T::get(x[at + e]) : -INFINITY;
-          if (at + e < v1 && counts(f, at + e)) buf[atomicAdd(&cnt, 1)] = order_key(f, (uint32_t)(at + e));
-          __syncthreads();
-          n = cnt;
-          __syncthreads();
+          if (at + e < v1 && counts(f, at + e)) buf[atomicAdd(&sh.cnt, 1)] = order_key(f, (uint32_t)(at + e));
+          sync<NT>();
+          n = sh.cnt;
+          sync<NT>();
           if (n > C - NT) {
             cut();
-            if (tid == 0) cnt = k;
-            __syncthreads();
+            if (tid == 0) sh.cnt = k;
+            sync<NT>();
           }
         }
       }
@@ -292,10 +300,10 @@ __global__ __launch_bounds__(NT) void lt_top_k(TopParams p) {
     if (n > k) cut();
     tie = 0xffffffffu;
     if (tid == 0) {
-      cnt = n;
-      listed = 0;
+      sh.cnt = n;
+      sh.listed = 0;
     }
-    __syncthreads();
+    sync<NT>();
   };
 
   int have = 0;                          // vectors on the list
@@ -344,20 +352,20 @@ __global__ __launch_bounds__(NT) void lt_top_k(TopParams p) {
       }
       if (W > 1) {
         if (lane == 0) {
-          sh_th[wave] = th;
-          sh_reach[wave] = 0;
+          sh.th[wave] = th;
+          sh.reach[wave] = 0;
         }
-        __syncthreads();
+        sync<NT>();
 #pragma nounroll
         for (int w = 0; w < W; ++w) {
-          const int c = __popcll(__ballot(o >= sh_th[w]));
-          if (lane == w) atomicAdd(&sh_reach[w], c);
+          const int c = __popcll(__ballot(o >= sh.th[w]));
+          if (lane == w) atomicAdd(&sh.reach[w], c);
         }
-        __syncthreads();
+        sync<NT>();
         th = 0;
 #pragma nounroll
         for (int w = 0; w < W; ++w)
-          if (sh_reach[w] > k && sh_th[w] > th) th = sh_th[w];
+          if (sh.reach[w] > k && sh.th[w] > th) th = sh.th[w];
       }
       tau = th <= order_of(-INFINITY) ? -INFINITY : of_order(th);
     }
@@ -369,58 +377,58 @@ __global__ __launch_bounds__(NT) void lt_top_k(TopParams p) {
         b[u] = __ballot(vm[u] > tau);
         all += __popcll(b[u]);
       }
-      if (lane == 0) pos = atomicAdd(&listed, all);
+      if (lane == 0) pos = atomicAdd(&sh.listed, all);
       pos = __builtin_amdgcn_readfirstlane(pos);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int at = pos + __builtin_amdgcn_mbcnt_hi((uint32_t)(b[u] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b[u], 0));
-        if (vm[u] > tau && at < CL) list[at] = (uint32_t)((base - v0) / E + u * NT + tid);
+        if (vm[u] > tau && at < CL) sh.list[at] = (uint32_t)((base - v0) / E + u * NT + tid);
         pos += __popcll(b[u]);
       }
     }
-    __syncthreads();
+    sync<NT>();
     const int was = have;
-    have = listed;
+    have = sh.listed;
     if (have > CL) {
-      __syncthreads();
-      expand(list, 0, was);
+      sync<NT>();
+      expand(sh.list, 0, was);
       expand(nullptr, (base - v0) / E, min(NT * U, (v1 - base + E - 1) / E));
       tighten();
       have = 0;
     } else if (base + STEP < v1) {
-      __syncthreads();                   // (a push of the next step may run ahead of the slowest read of `listed`)
+      sync<NT>();                   // (a push of the next step may run ahead of the slowest read of `listed`)
       if (n + have > k + k / 2 + XP) {
-        expand(list, 0, have);
+        expand(sh.list, 0, have);
         tighten();
         have = 0;
       }
     }
   }
-  expand(list, 0, have);
-  const float top = block_reduce<NT, Max>(m, shf);
-  const float sum = block_reduce<NT, Sum>(s * exp2_((m - top) * p.c), shf);
+  expand(sh.list, 0, have);
+  const float top = block_reduce<NT, Max>(m, sh.shf);
+  const float sum = block_reduce<NT, Sum>(s * exp2_((m - top) * p.c), sh.shf);
   if (sum != sum) {
-    best_by_passes<T, NT>(x, v0, v1, k, buf, sh64);
+    best_by_passes<T, NT>(x, v0, v1, k, buf, sh.sh64);
   } else {
     for (int base = v0; n < k; base += NT) {
       // the first logits that equal tau: in order, a thread a logit
       const int at = base + tid;
       const bool hit = at < v1 && T::get(x[min(at, v1 - 1)]) == tau;
       const uint64_t b = __ballot(hit);
-      if (lane == 0) sh64[wave] = b;
-      __syncthreads();
+      if (lane == 0) sh.sh64[wave] = b;
+      sync<NT>();
       int pos = n + __popcll(b & ((1ull << lane) - 1)), all = 0;
       for (int w = 0; w < W; ++w) {
-        const int c = __popcll(sh64[w]);
+        const int c = __popcll(sh.sh64[w]);
         if (w < wave) pos += c;
         all += c;
       }
       if (hit && pos < k) buf[pos] = order_key(tau, (uint32_t)at);
       n = min(k, n + all);
-      __syncthreads();
+      sync<NT>();
       if (base + NT >= v1) break;        // (never short of k: at least k logits reach tau)
     }
-    best_keys<NT, C>(buf, n, k, hist, &cnt2, sh64);
+    best_keys<NT, C>(buf, n, k, sh.hist, &sh.cnt2, sh.sh64);
   }
   if (p.splits == 1) {
     if (tid == 0) p.lse[r] = log_sum(top, sum, p.c);
@@ -436,13 +444,74 @@ __global__ __launch_bounds__(NT) void lt_top_k(TopParams p) {
   }
 }
 
+// Rows of at most FEW logits and k <= K: a thread keeps its row's k best in
+// registers, inserting each logit (64 rows of 41 logits, k 5: about 20
+// instructions of a wave a row, where a wave a row takes 600).
+template <class T, int K>
+__global__ __launch_bounds__(64) void lt_top_few(TopParams p) {
+  using raw = typename T::raw;
+  extern __shared__ float few[];           // [64][few_pitch(vocab)], then [64][k] results
+  const int lane = threadIdx.x, vocab = p.x.vocab, pitch = few_pitch(vocab);
+  const int64_t r0 = (p.block0 + blockIdx.x) * 64;
+  const int rows = (int)min((int64_t)64, p.rows - r0);
+  each_of_rows(rows, vocab, [&](int r, int v, int) {
+    few[r * pitch + v] = T::get(((const raw*)p.x.data + p.x.at(r0 + r))[v]);
+  });
+  __syncthreads();
+  const float* x = few + min(lane, rows - 1) * pitch;
+  uint32_t best[K];
+  int id[K];
+#pragma unroll
+  for (int j = 0; j < K; ++j) best[j] = 0, id[j] = 0;
+  float m = LOWEST;
+  for (int v = 0; v < vocab; ++v) {
+    const float f = x[v];
+    m = max2(m, f);
+    const uint32_t o = order_of(f);
+    // (behind an equal one, which came earlier)
+#pragma unroll
+    for (int j = K - 1; j >= 0; --j) {
+      const bool here = o > best[j], ahead = j > 0 && o > best[j > 0 ? j - 1 : 0];
+      best[j] = ahead ? best[j > 0 ? j - 1 : 0] : here ? o : best[j];
+      id[j] = ahead ? id[j > 0 ? j - 1 : 0] : here ? v : id[j];
+    }
+  }
+  float s = 0.f;
+  for (int v = 0; v < vocab; ++v) s += exp2_((x[v] - m) * p.c);
+  if (lane < rows) p.lse[r0 + lane] = log_sum(m, s, p.c);
+  // results by way of LDS, so that the rows' are written together
+  raw* val = (raw*)(few + 64 * pitch);
+  uint8_t* at = (uint8_t*)(val + 64 * p.k);
+#pragma unroll
+  for (int j = 0; j < K; ++j)
+    if (j < p.k) {
+      val[lane * p.k + j] = T::put(x[id[j]]);
+      at[lane * p.k + j] = (uint8_t)id[j];
+    }
+  __syncthreads();
+  for (int i = lane; i < rows * p.k; i += 64) {
+    ((raw*)p.values)[r0 * p.k + i] = val[i];
+    p.ids[r0 * p.k + i] = at[i];
+  }
+}
+
 template <class T>
 lt_status launch_top(TopParams& p, void* stream) {
-    p.splits = 1;
+    // Few logits a row, few of them wanted, and rows enough: a thread a row.
+  // (131072 x 41 float32, k 5: 23 us, a wave a row 158 us; 4096 x 128, k 16 the
+  // other way round: 65 and 19.)
+  if (p.x.vocab <= FEW && p.k <= 8 && p.rows >= 4096) {
+    const int64_t blocks = (p.rows + 63) / 64;
+    const int lds = 64 * (few_pitch(p.x.vocab) * 4 + p.k * (int)(sizeof(typename T::raw) + 1));
+    if (p.k == 1) return launch(lt_top_few<T, 1>, blocks, 64, p, stream, "lt_top_logits", lds);
+    if (p.k <= 5) return launch(lt_top_few<T, 5>, blocks, 64, p, stream, "lt_top_logits", lds);
+    return launch(lt_top_few<T, 8>, blocks, 64, p, stream, "lt_top_logits", lds);
+  }
+  p.splits = 1;
   p.chunk = (p.x.vocab + 7) / 8 * 8;
   if (p.k > 192 || p.x.vocab > 8192) return launch(lt_top_k<T, 512, 4, 1024, 1024>, p.rows * p.splits, 512, p, stream, "lt_top_logits");
   if (p.k > 62 || p.x.vocab > 2048) return launch(lt_top_k<T, 256, 4, 1024, 512>, p.rows * p.splits, 256, p, stream, "lt_top_logits");
-  return launch(lt_top_k<T, 64, 4, 256, 128>, p.rows * p.splits, 64, p, stream, "lt_top_logits");
+  return launch(lt_top_k<T, 64, 4, 256, 128>, (p.rows + 3) / 4, 256, p, stream, "lt_top_logits");
 }
 
 }  // namespace

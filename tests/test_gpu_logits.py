@@ -124,6 +124,24 @@ def test_top_many_rows():
     check_top(rand((9001, 200), torch.bfloat16, 2), 20)
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('vocab, k, pad', [(1, 1, 0), (2, 2, 0), (5, 1, 3), (41, 5, 0), (64, 3, 0), (64, 8, 1),
+                                           (63, 9, 0), (65, 5, 0), (128, 16, 0)])
+def test_top_few_logits(dtype, vocab, k, pad):
+    """Many rows of a few logits, ties and masks among them."""
+    x = rand((16411, vocab), dtype, vocab, pad=pad)
+    x[::3] = x[::3].round()
+    x[5::7, ::2] = -INF
+    x[11] = -INF
+    x[12] = math.nan
+    x[13, -1] = math.nan
+    x[14, 0] = INF
+    x[15] = LOWEST[dtype]
+    x[16] = -0.0
+    x[16, vocab // 2:] = 0.0
+    check_top(x, k)
+
+
 # ---- distillation -----------------------------------------------------------
 
 def teacher(z, k, dtype, seed, tail, temperature, empty=0.0):
