@@ -495,6 +495,44 @@ __global__ __launch_bounds__(64) void lt_top_few(TopParams p) {
   }
 }
 
+// Rows of at most SMALL logits: a wave takes one and sorts all of it.
+constexpr int SMALL = 256;
+
+template <class T>
+__global__ __launch_bounds__(256) void lt_top_small(TopParams p) {
+  using raw = typename T::raw;
+  __shared__ uint64_t keys[4][SMALL];
+  const int lane = threadIdx.x & 63, vocab = p.x.vocab;
+  uint64_t* const buf = keys[group_of<64>()];
+  const int64_t r = (p.block0 + blockIdx.x) * 4 + group_of<64>();
+  if (r >= p.rows) return;                 // (a wave as a whole)
+  const raw* x = (const raw*)p.x.data + p.x.at(r);
+  float f[SMALL / 64], m = LOWEST, s = 0.f;
+#pragma unroll
+  for (int i = 0; i < SMALL / 64; ++i) f[i] = i * 64 + lane < vocab ? T::get(x[i * 64 + lane]) : -INFINITY;
+#pragma unroll
+  for (int i = 0; i < SMALL / 64; ++i) m = max2(m, f[i]);
+  m = wave_reduce<Max>(m, LOWEST);
+#pragma unroll
+  for (int i = 0; i < SMALL / 64; ++i) {
+    s += exp2_((f[i] - m) * p.c);
+    if (i * 64 + lane < vocab) buf[i * 64 + lane] = order_key(f[i], (uint32_t)(i * 64 + lane));
+  }
+  s = wave_reduce<Sum>(s, 0.f);
+  sync<64>();
+  sort_keys<64, SMALL>(buf, vocab, p.k);
+  if (lane == 0) p.lse[r] = log_sum(m, s, p.c);
+#pragma unroll
+  for (int i = 0; i < SMALL / 64; ++i) {
+    const int j = i * 64 + lane;
+    if (j < p.k) {
+      const uint32_t id = ~(uint32_t)buf[j];
+      p.ids[r * p.k + j] = id;
+      ((raw*)p.values)[r * p.k + j] = s != s ? x[id] : T::put(of_order((uint32_t)(buf[j] >> 32)));
+    }
+  }
+}
+
 template <class T>
 lt_status launch_top(TopParams& p, void* stream) {
     // Few logits a row, few of them wanted, and rows enough: a thread a row.
@@ -507,6 +545,10 @@ lt_status launch_top(TopParams& p, void* stream) {
     if (p.k <= 5) return launch(lt_top_few<T, 5>, blocks, 64, p, stream, "lt_top_logits", lds);
     return launch(lt_top_few<T, 8>, blocks, 64, p, stream, "lt_top_logits", lds);
   }
+#ifndef XSM
+#define XSM SMALL
+#endif
+  if (p.x.vocab <= XSM) return launch(lt_top_small<T>, (p.rows + 3) / 4, 256, p, stream, "lt_top_logits");
   p.splits = 1;
   p.chunk = (p.x.vocab + 7) / 8 * 8;
   if (p.k > 192 || p.x.vocab > 8192) return launch(lt_top_k<T, 512, 4, 1024, 1024>, p.rows * p.splits, 512, p, stream, "lt_top_logits");
