@@ -50,6 +50,9 @@ struct __attribute__((packed, aligned(2))) Bytes16 {
   uint32_t w[4];
 };
 
+__device__ __forceinline__ uint32_t twice(float v) { return __builtin_bit_cast(uint32_t, v); }
+__device__ __forceinline__ uint32_t twice(uint16_t v) { return (uint32_t)v << 16 | v; }
+
 // The E = 16 / sizeof(raw) logits of a vector.
 template <class T>
 struct Vec {
@@ -60,6 +63,12 @@ struct Vec {
   __device__ __forceinline__ float get(int i) const;
   // What is computed from the logits ahead of this is not kept for later.
   __device__ __forceinline__ void keep() { asm volatile("" : "+v"(b.w[0]), "+v"(b.w[1]), "+v"(b.w[2]), "+v"(b.w[3])); }
+  // The vector at `at` of a row's logits [.., end), `fill` behind them.
+  __device__ __forceinline__ void load(const typename T::raw* x, int at, int end, typename T::raw fill) {
+    if (at + E <= end) load(x + at);
+    else if (at < end) load_part(x + at, end - at, fill);
+    else b.w[0] = b.w[1] = b.w[2] = b.w[3] = twice(fill);
+  }
   // n < E logits, `fill` behind them (a rolled loop: few registers, taken once a row)
   __device__ __forceinline__ void load_part(const typename T::raw* p, int n, typename T::raw fill) {
     b.w[0] = b.w[1] = b.w[2] = b.w[3] = 0;

@@ -5,12 +5,6 @@
 #include "lt_logits.h"
 
 namespace {
-#ifndef XTH
-#define XTH 512
-#endif
-#ifndef XP
-#define XP 192
-#endif
 
 struct TopParams {
   Rows x;
@@ -30,7 +24,7 @@ struct TopParams {
 // The sum behind a log-sum-exp: that of exp2((x - m) c), m any logit at most 32
 // (in the exponent) below the largest seen.
 __device__ __forceinline__ float log_sum(float m, float s, float c) {
-  return m == INFINITY ? m : (float)((double)m * (c * 0.6931471805599453) + log((double)s));
+  return m == INFINITY ? m : (float)((double)m * (c * 0.6931471805599453) + (double)__builtin_amdgcn_logf(s) * 0.6931471805599453);
 }
 
 // The key of lane ^ X: by the data-parallel primitives where they can, else by
@@ -158,16 +152,6 @@ __device__ __forceinline__ uint64_t cut_keys(uint64_t* buf, int n, int k, int* h
   return at_least;
 }
 
-// The k best of the keys buf[0 .. n), in order.
-template <int NT, int C>
-__device__ __forceinline__ void best_keys(uint64_t* buf, int n, int k, int* hist, int* cnt, uint64_t* sh) {
-    if (n > XTH && n > k) {
-    cut_keys<NT, C>(buf, n, k, hist, cnt, sh);
-    n = k;
-  }
-  sort_keys<NT, C>(buf, n, k);
-}
-
 // The k best of x[v0 .. v1) one after another, k passes: rows with a NaN.
 template <class T, int NT>
 __device__ void best_by_passes(const typename T::raw* x, int v0, int v1, int k, uint64_t* out, uint64_t* sh) {
@@ -250,8 +234,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
       const int i = i0 + tid;
       const int at = i < nv ? v0 + (of ? (int)of[i] : first + i) * E : v1;
       Vec<T> v;
-      if (at + E <= v1) v.load(x + at);
-      else v.load_part(x + at, max(0, v1 - at), T::put(-INFINITY));
+      v.load(x, at, v1, T::put(-INFINITY));
       int mine = 0;
 #pragma unroll
       for (int e = 0; e < E; ++e) mine += at + e < v1 && counts(v.get(e), at + e);
@@ -276,34 +259,19 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
       sync<NT>();
       if (n > C) {
         n = was;
-        if (n > C - NT) cut();             // (room for a logit of every thread)
-        if (tid == 0) sh.cnt = n;
-        sync<NT>();
 #pragma nounroll
         for (int e = 0; e < E; ++e) {
+          if (n > C - NT) cut();           // (room for a logit of every thread)
+          if (tid == 0) sh.cnt = n;
+          sync<NT>();
           const float f = at + e < v1 ? T::get(x[at + e]) : -INFINITY;
           if (at + e < v1 && counts(f, at + e)) buf[atomicAdd(&sh.cnt, 1)] = order_key(f, (uint32_t)(at + e));
           sync<NT>();
           n = sh.cnt;
           sync<NT>();
-          if (n > C - NT) {
-            cut();
-            if (tid == 0) sh.cnt = k;
-            sync<NT>();
-          }
         }
       }
     }
-  };
-  // The best k so far: fewer of the logits to come lie above the last of them.
-  auto tighten = [&]() {
-    if (n > k) cut();
-    tie = 0xffffffffu;
-    if (tid == 0) {
-      sh.cnt = n;
-      sh.listed = 0;
-    }
-    sync<NT>();
   };
 
   int have = 0;                          // vectors on the list
@@ -315,11 +283,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
       for (int u = 0; u < U; ++u) v[u].load(x + base + (u * NT + tid) * E);
     } else {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int at = base + (u * NT + tid) * E;
-        if (at + E <= v1) v[u].load(x + at);
-        else v[u].load_part(x + at, max(0, v1 - at), T::put(-INFINITY));
-      }
+      for (int u = 0; u < U; ++u) v[u].load(x, base + (u * NT + tid) * E, v1, T::put(-INFINITY));
     }
     float t = -INFINITY;
 #pragma unroll
@@ -389,22 +353,23 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
     sync<NT>();
     const int was = have;
     have = sh.listed;
-    if (have > CL) {
-      sync<NT>();
-      expand(sh.list, 0, was);
-      expand(nullptr, (base - v0) / E, min(NT * U, (v1 - base + E - 1) / E));
-      tighten();
+    sync<NT>();                          // (a push of the next step may run ahead of the slowest read of `listed`)
+    const bool last = base + STEP >= v1, over = have > CL;
+    if (last || over || n + have > k + k / 2 + 192) {
+#pragma nounroll
+      for (int pass = 0; pass <= (int)over; ++pass)
+        expand(pass ? nullptr : sh.list, (base - v0) / E, pass ? min(NT * U, (v1 - base + E - 1) / E) : over ? was : have);
+      // the best k so far: fewer of the logits to come lie above the last of them
+      if (n > k && (!last || n > 512)) cut();
+      tie = 0xffffffffu;
       have = 0;
-    } else if (base + STEP < v1) {
-      sync<NT>();                   // (a push of the next step may run ahead of the slowest read of `listed`)
-      if (n + have > k + k / 2 + XP) {
-        expand(sh.list, 0, have);
-        tighten();
-        have = 0;
+      if (tid == 0) {
+        sh.cnt = n;
+        sh.listed = 0;
       }
+      sync<NT>();
     }
   }
-  expand(sh.list, 0, have);
   const float top = block_reduce<NT, Max>(m, sh.shf);
   const float sum = block_reduce<NT, Sum>(s * exp2_((m - top) * p.c), sh.shf);
   if (sum != sum) {
@@ -428,7 +393,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
       sync<NT>();
       if (base + NT >= v1) break;        // (never short of k: at least k logits reach tau)
     }
-    best_keys<NT, C>(buf, n, k, sh.hist, &sh.cnt2, sh.sh64);
+    sort_keys<NT, C>(buf, n, k);
   }
   if (p.splits == 1) {
     if (tid == 0) p.lse[r] = log_sum(top, sum, p.c);
@@ -545,15 +510,13 @@ lt_status launch_top(TopParams& p, void* stream) {
     if (p.k <= 5) return launch(lt_top_few<T, 5>, blocks, 64, p, stream, "lt_top_logits", lds);
     return launch(lt_top_few<T, 8>, blocks, 64, p, stream, "lt_top_logits", lds);
   }
-#ifndef XSM
-#define XSM SMALL
-#endif
-  if (p.x.vocab <= XSM) return launch(lt_top_small<T>, (p.rows + 3) / 4, 256, p, stream, "lt_top_logits");
+  if (p.x.vocab <= SMALL) return launch(lt_top_small<T>, (p.rows + 3) / 4, 256, p, stream, "lt_top_logits");
   p.splits = 1;
   p.chunk = (p.x.vocab + 7) / 8 * 8;
   if (p.k > 192 || p.x.vocab > 8192) return launch(lt_top_k<T, 512, 4, 1024, 1024>, p.rows * p.splits, 512, p, stream, "lt_top_logits");
   if (p.k > 62 || p.x.vocab > 2048) return launch(lt_top_k<T, 256, 4, 1024, 512>, p.rows * p.splits, 256, p, stream, "lt_top_logits");
-  return launch(lt_top_k<T, 64, 4, 256, 128>, (p.rows + 3) / 4, 256, p, stream, "lt_top_logits");
+  if (p.x.vocab > 1024) return launch(lt_top_k<T, 64, 4, 256, 128>, (p.rows + 3) / 4, 256, p, stream, "lt_top_logits");
+  return launch(lt_top_k<T, 64, 2, 256, 128>, (p.rows + 3) / 4, 256, p, stream, "lt_top_logits");
 }
 
 }  // namespace
