@@ -6,6 +6,8 @@
 
 namespace {
 
+constexpr int JOIN = 1024;                 // keys of a row's chunks, at most
+
 struct TopParams {
   Rows x;
   int64_t rows;
@@ -210,7 +212,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
   const raw* x = (const raw*)p.x.data + p.x.at(r);
   const int v0 = split * p.chunk, v1 = min(p.x.vocab, v0 + p.chunk);
   const int k = min(p.k, v1 - v0);
-  const int per_wave = (k + W - 1) / W + 1;
+  const int per_wave = W == 1 ? min(63, k + 2 + k / 16) : (k + W - 1) / W + 1;
   float m = LOWEST, s = 0.f, tau = -INFINITY;
   int n = 0;                             // keys
   if (tid == 0) sh.cnt = sh.listed = 0;
@@ -307,7 +309,8 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
     s += s0 + s1;
     if (base == v0) {
       // the per_wave-th largest of a wave's threads (from its leading 18 bits
-      // down), and of the waves' the largest that k threads of the block reach
+      // down), and of the waves' the largest that k threads of the block are
+      // above (the least where ties leave none: k threads reach that)
       const uint32_t o = order_of(t);
       uint32_t th = 0;
       for (int bit = 31; bit >= 14; --bit) {
@@ -320,16 +323,17 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
           sh.reach[wave] = 0;
         }
         sync<NT>();
-#pragma nounroll
+        const uint32_t theirs = lane < W ? sh.th[lane] : 0;
+        int reach = 0;
+#pragma unroll
         for (int w = 0; w < W; ++w) {
-          const int c = __popcll(__ballot(o >= sh.th[w]));
-          if (lane == w) atomicAdd(&sh.reach[w], c);
+          const int c = __popcll(__ballot(o > (uint32_t)__builtin_amdgcn_readlane(theirs, w)));
+          reach = lane == w ? c : reach;
         }
+        if (lane < W) atomicAdd(&sh.reach[lane], reach);
         sync<NT>();
-        th = 0;
-#pragma nounroll
-        for (int w = 0; w < W; ++w)
-          if (sh.reach[w] > k && sh.th[w] > th) th = sh.th[w];
+        th = wave_reduce<Max>(lane < W && sh.reach[lane] >= k ? theirs : 0u, 0u);
+        if (!th) th = ~wave_reduce<Max>(lane < W ? ~theirs : 0u, 0u);
       }
       tau = th <= order_of(-INFINITY) ? -INFINITY : of_order(th);
     }
@@ -375,23 +379,33 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
   if (sum != sum) {
     best_by_passes<T, NT>(x, v0, v1, k, buf, sh.sh64);
   } else {
-    for (int base = v0; n < k; base += NT) {
-      // the first logits that equal tau: in order, a thread a logit
-      const int at = base + tid;
-      const bool hit = at < v1 && T::get(x[min(at, v1 - 1)]) == tau;
-      const uint64_t b = __ballot(hit);
-      if (lane == 0) sh.sh64[wave] = b;
+    for (int base = v0; n < k && base < v1; base += NT * E) {
+      // the first logits that equal tau: in order, a vector a thread (never
+      // short of k: at least k logits reach tau)
+      const int at = base + tid * E;
+      Vec<T> v;
+      v.load(x, at, v1, T::put(-INFINITY));
+      int mine = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) mine += at + e < v1 && v.get(e) == tau;
+      const int upto = wave_scan<Sum>(mine, 0);
+      if (lane == 63) sh.reach[wave] = upto;
       sync<NT>();
-      int pos = n + __popcll(b & ((1ull << lane) - 1)), all = 0;
+      int pos = n + upto - mine, all = 0;
+#pragma unroll
       for (int w = 0; w < W; ++w) {
-        const int c = __popcll(sh.sh64[w]);
+        const int c = sh.reach[w];
         if (w < wave) pos += c;
         all += c;
       }
-      if (hit && pos < k) buf[pos] = order_key(tau, (uint32_t)at);
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (at + e < v1 && v.get(e) == tau) {
+          if (pos < k) buf[pos] = order_key(tau, (uint32_t)(at + e));
+          ++pos;
+        }
       n = min(k, n + all);
       sync<NT>();
-      if (base + NT >= v1) break;        // (never short of k: at least k logits reach tau)
     }
     sort_keys<NT, C>(buf, n, k);
   }
@@ -406,6 +420,37 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
   } else {
     if (tid == 0) p.part_sums[blk] = make_float2(top, sum);
     for (int j = tid; j < p.k; j += NT) p.part_keys[blk * p.k + j] = j < k ? buf[j] : 0;
+  }
+}
+
+// The k best of a row's chunks' lists, and its sum.
+template <class T>
+__global__ __launch_bounds__(256) void lt_top_join(TopParams p) {
+  constexpr int NT = 256, C = JOIN;
+  __shared__ __attribute__((aligned(16))) TopShared<NT, C, 1> sh;
+  const int tid = threadIdx.x;
+  const int64_t r = p.block0 + blockIdx.x;
+  const int n = p.splits * p.k;
+  for (int i = tid; i < n; i += NT) sh.buf[i] = p.part_keys[r * n + i];
+  float m = LOWEST, s = 0.f;
+  for (int i = 0; i < p.splits; ++i) m = max2(m, p.part_sums[r * p.splits + i].x);
+  for (int i = 0; i < p.splits; ++i) {
+    const float2 part = p.part_sums[r * p.splits + i];
+    s += part.y * exp2_((part.x - m) * p.c);
+  }
+  __syncthreads();
+  int left = n;
+  if (n > 256) {
+    cut_keys<NT, C>(sh.buf, n, p.k, sh.hist, &sh.cnt2, sh.sh64);
+    left = p.k;
+  }
+  sort_keys<NT, C>(sh.buf, left, p.k);
+  if (tid == 0) p.lse[r] = log_sum(m, s, p.c);
+  const typename T::raw* x = (const typename T::raw*)p.x.data + p.x.at(r);
+  for (int j = tid; j < p.k; j += NT) {
+    const uint32_t id = ~(uint32_t)sh.buf[j];
+    p.ids[r * p.k + j] = id;
+    ((typename T::raw*)p.values)[r * p.k + j] = s != s ? x[id] : T::put(of_order((uint32_t)(sh.buf[j] >> 32)));
   }
 }
 
@@ -498,6 +543,26 @@ __global__ __launch_bounds__(256) void lt_top_small(TopParams p) {
   }
 }
 
+// Chunks of a row: one where the rows fill the card or a row is a few steps of
+// a block; else a step or more each.  (131072 bf16, k 20, one row: 22 us whole,
+// 17 us in 8 chunks and joined; 64 rows: 27 and 18 us.)
+void split_rows(TopParams& p, int dtype) {
+  const int step = 512 * 4 * (dtype == LT_F32 ? 4 : 8);
+  int64_t n = 1;
+  if (p.x.vocab > 2 * step && p.rows < 256) {
+    n = (p.x.vocab + step - 1) / step;
+    n = n < 512 / p.rows ? n : 512 / p.rows;
+    n = n < JOIN / p.k ? n : JOIN / p.k;
+  }
+  const int64_t steps = (p.x.vocab + n * step - 1) / (n * step);
+  p.chunk = (int32_t)(n == 1 ? (int64_t)1 << 30 : steps * step);
+  p.splits = (int32_t)(((int64_t)p.x.vocab + p.chunk - 1) / p.chunk);
+}
+
+int64_t top_workspace(const TopParams& p) {
+  return p.splits == 1 ? 0 : p.rows * p.splits * (int64_t)(p.k * sizeof(uint64_t) + sizeof(float2));
+}
+
 template <class T>
 lt_status launch_top(TopParams& p, void* stream) {
     // Few logits a row, few of them wanted, and rows enough: a thread a row.
@@ -511,8 +576,12 @@ lt_status launch_top(TopParams& p, void* stream) {
     return launch(lt_top_few<T, 8>, blocks, 64, p, stream, "lt_top_logits", lds);
   }
   if (p.x.vocab <= SMALL) return launch(lt_top_small<T>, (p.rows + 3) / 4, 256, p, stream, "lt_top_logits");
-  p.splits = 1;
-  p.chunk = (p.x.vocab + 7) / 8 * 8;
+  if (p.splits > 1) {
+    const lt_status st = launch(lt_top_k<T, 512, 4, 1024, 1024>, p.rows * p.splits, 512, p, stream, "lt_top_logits");
+    return st != LT_OK ? st : launch(lt_top_join<T>, p.rows, 256, p, stream, "lt_top_logits");
+  }
+  if (p.k > 62 && p.x.vocab <= 2048)
+    return launch(lt_top_k<T, 256, 8 / Vec<T>::E, 2048, 256 * 8 / Vec<T>::E>, p.rows * p.splits, 256, p, stream, "lt_top_logits");
   if (p.k > 192 || p.x.vocab > 8192) return launch(lt_top_k<T, 512, 4, 1024, 1024>, p.rows * p.splits, 512, p, stream, "lt_top_logits");
   if (p.k > 62 || p.x.vocab > 2048) return launch(lt_top_k<T, 256, 4, 1024, 512>, p.rows * p.splits, 256, p, stream, "lt_top_logits");
   if (p.x.vocab > 1024) return launch(lt_top_k<T, 64, 4, 256, 128>, (p.rows + 3) / 4, 256, p, stream, "lt_top_logits");
@@ -531,17 +600,24 @@ const char* lt_hip_library(void) {
   return path;
 }
 
-int64_t lt_top_logits_workspace(const lt_rows*, int32_t) { return 0; }
+int64_t lt_top_logits_workspace(const lt_rows* x, int32_t k) {
+  if (!x || x->rows < 1 || x->vocab < 1 || x->vocab > LT_MAX_VOCAB || k < 1 || k > MAXK) return 0;
+  TopParams p{};
+  p.x = rows_of(x);
+  p.rows = x->rows;
+  p.k = k;
+  split_rows(p, x->dtype);
+  return top_workspace(p);
+}
 
 lt_status lt_top_logits(const lt_rows* x, int32_t k, double temperature, void* values, int64_t* ids, float* lse,
-                        void*, int64_t, void* stream) {
+                        void* workspace, int64_t workspace_bytes, void* stream) {
   lt_status st;
   if (!rows_ok(x, "logits", &st)) return st;
   if (k < 1 || k > MAXK || k > x->vocab) BAD("k %d (1 .. min(vocab, %d))", k, MAXK);
   if (!temperature_ok(temperature)) BAD("temperature %g (1e-6 .. 1e6)", temperature);
   if (x->rows == 0) return LT_OK;
   if (!values || !ids || !lse) BAD("output: NULL");
-  ON_DEVICE(x->device);
   TopParams p{};
   p.x = rows_of(x);
   p.rows = x->rows;
@@ -550,6 +626,13 @@ lt_status lt_top_logits(const lt_rows* x, int32_t k, double temperature, void* v
   p.values = values;
   p.ids = ids;
   p.lse = lse;
+  split_rows(p, x->dtype);
+  const int64_t need = top_workspace(p);
+  if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
+    BAD("workspace: %lld bytes, 16 B aligned, are needed", (long long)need);
+  p.part_keys = (uint64_t*)workspace;
+  p.part_sums = (float2*)((char*)workspace + p.rows * p.splits * (int64_t)p.k * sizeof(uint64_t));
+  ON_DEVICE(x->device);
   return x->dtype == LT_F32 ? launch_top<F32>(p, stream) : x->dtype == LT_F16 ? launch_top<F16>(p, stream) : launch_top<BF16>(p, stream);
 }
 

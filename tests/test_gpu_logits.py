@@ -57,12 +57,13 @@ def check_top(x, k, temperature=1.0):
     (1, 1, 1, 0), (3, 2, 2, 1), (70, 41, 5, 0), (300, 41, 41, 0), (5, 63, 7, 2), (5, 64, 64, 0), (5, 65, 16, 0),
     (9, 127, 100, 0), (9, 128, 3, 0), (9, 129, 129, 0), (4, 257, 256, 3), (33, 1000, 10, 0), (6, 2047, 64, 1),
     (6, 2048, 256, 0), (6, 2049, 1, 0), (3, 8191, 17, 0), (2, 8200, 256, 5), (1, 32000, 16, 0), (2, 50261, 64, 3),
-    (1, 131072, 256, 0), (40, 33000, 50, 0), (600, 300, 30, 0), (1, 300001, 33, 0)])
+    (1, 131072, 256, 0), (40, 33000, 50, 0), (600, 300, 30, 0), (1, 300001, 33, 0), (3, 40000, 200, 1),
+    (100, 33001, 3, 0), (2, 1000003, 5, 0)])
 def test_top(dtype, rows, vocab, k, pad):
     check_top(rand((rows, vocab), dtype, rows * 7 + vocab, pad=pad), k, temperature=0.7 if pad else 1.0)
 
 
-@pytest.mark.parametrize('vocab', [50, 1500, 9000, 70000])
+@pytest.mark.parametrize('vocab', [50, 700, 1500, 9000, 70000])
 @pytest.mark.parametrize('kind', ['constant', 'ascending', 'descending', 'two', 'masked', 'all masked', 'lowest',
                                   'nan', 'all nan', 'inf', 'zeros', 'integers', 'late', 'stripes'])
 def test_top_orders(vocab, kind):

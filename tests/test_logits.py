@@ -122,6 +122,18 @@ def test_c_entries_refuse(call):
     assert call(logits._load(), _desc(), logits._Teacher(4096, 4096, None, 1, 8, 0)) == -1
 
 
+def test_c_entry_refuses_a_short_workspace():
+    lib = logits._load()
+    x = _desc(rows=3, vocab=200000, stride_outer=200000)
+    need = lib.lt_top_logits_workspace(C.byref(x), 20)
+    assert need > 0
+    for at, size in ((None, need), (4096, need - 1), (4100, need)):
+        assert lib.lt_top_logits(C.byref(x), 20, 1.0, 4096, 4096, 4096, at, size, None) == -1
+        assert b'workspace' in _capi.load().lt_last_error()
+    assert lib.lt_top_logits_workspace(C.byref(_desc(rows=1000, vocab=200000)), 20) == 0
+    assert lib.lt_top_logits_workspace(None, 20) == 0
+
+
 @pytest.mark.parametrize('entries, ids_bytes, dtype', [(0, 8, 0), (257, 8, 0), (1, 2, 0), (1, 8, 3)])
 def test_c_entries_refuse_a_teacher(entries, ids_bytes, dtype):
     x, t = _desc(), logits._Teacher(4096, 4096, None, entries, ids_bytes, dtype)
