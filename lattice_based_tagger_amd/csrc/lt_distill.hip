@@ -4,10 +4,6 @@
 
 namespace {
 
-constexpr int NT = 256;                   // threads of a block
-constexpr int NW = NT / 64;               // its waves
-
-// ---- distillation ----------------------------------------------------------
 struct Teacher {
   const void* ids;
   const void* top;
@@ -22,131 +18,362 @@ struct DistillParams {
   int64_t rows;
   double inv_t;           // 1 / temperature
   float c;                // log2(e) / temperature
+  int32_t splits;         // blocks of a row
+  int32_t chunk;          // logits of a block (a multiple of 8), the last one's fewer
   float* loss;
-  float* stats;
+  float* stats;           // [rows][LT_DISTILL_STATS]: m, the gradient's factors of exp2((z - m) c)
+  float4* part;           // splits > 1: [rows][splits] reference, sums within and outside the entries
   const float* weight;
   int64_t weight_stride;
   Rows grad;
 };
 
-// A teacher's row in LDS: id[j] (-1: no entry) and p[j].
-struct TeacherRow {
-  int32_t id[MAXK];
-  double p[MAXK];
-  double sh[NW];
+// What a block (or a wave with a row of its own) keeps in LDS: the entries, and
+// a bit for each logit of a window that says whether it is one.
+template <int NT, int WINDOW>
+struct DistillShared {
+  int id[MAXK];
+  float mass[MAXK];
+  uint32_t bits[WINDOW / 32];
+  double sh[NT / 64];
+  float shf[NT / 64];
 };
 
-// Fills it; returns sum p (0: a row without entries) and p_rest, in 64 bits:
-// p_rest is what is left of 1.
-__device__ __forceinline__ void teacher_row(const Teacher& t, int64_t r, int32_t vocab, double inv_t, TeacherRow& o,
-                                            double& psum, double& prest) {
-  double m = -INFINITY;
-  for (int j = threadIdx.x; j < t.entries; j += NT) {
-    const int64_t id = any_id(t.ids, r * t.entries + j, t.ids_bytes);
-    const bool there = id >= 0 && id < vocab;
-    const double v = there ? any_float(t.top, r * t.entries + j, t.top_dtype) * inv_t : -INFINITY;
-    o.id[j] = there ? (int32_t)id : -1;
-    o.p[j] = v;
-    m = v > m || v != v ? v : m;
+// A thread's entries of the teacher's row, j = i * NT + thread: logits that are
+// no entry have id -1 and p 0.  All in 64 bits: what is left of 1 is used.
+template <int NT>
+struct Entries {
+  static constexpr int N = MAXK / NT > 1 ? MAXK / NT : 1;
+  int id[N];
+  double p[N], logp[N];
+  double sum, rest;       // of the row
+};
+
+template <int NT>
+__device__ __forceinline__ void load_entries(const Teacher& t, int64_t r, int vocab, double inv_t, Entries<NT>& o,
+                                             double* sh) {
+  double m = -INFINITY, s = 0;
+#pragma unroll
+  for (int i = 0; i < Entries<NT>::N; ++i) {
+    const int j = i * NT + thread_of<NT>();
+    o.id[i] = -1;
+    o.logp[i] = -INFINITY;
+    if (j < t.entries) {
+      const int64_t id = any_id(t.ids, r * t.entries + j, t.ids_bytes);
+      if (id >= 0 && id < vocab) {
+        o.id[i] = (int)id;
+        o.logp[i] = any_float(t.top, r * t.entries + j, t.top_dtype) * inv_t;
+      }
+    }
+    m = o.logp[i] > m || o.logp[i] != o.logp[i] ? o.logp[i] : m;
   }
-  double ref = t.top_lse ? (double)t.top_lse[r] : block_reduce<NT, Max>(m, o.sh);
+  double ref = t.top_lse ? (double)t.top_lse[r] : block_reduce<NT, Max>(m, sh);
   if (!t.top_lse && ref == -INFINITY) ref = 0;
-  double s = 0;
-  for (int j = threadIdx.x; j < t.entries; j += NT) {
-    const double e = o.id[j] < 0 ? 0.0 : exp(o.p[j] - ref);
-    o.p[j] = e;
-    s += e;
+#pragma unroll
+  for (int i = 0; i < Entries<NT>::N; ++i) {
+    o.logp[i] -= ref;
+    o.p[i] = o.id[i] < 0 ? 0.0 : exp(o.logp[i]);
+    s += o.p[i];
   }
-  psum = block_reduce<NT, Sum>(s, o.sh);
-  prest = 0;
+  o.sum = block_reduce<NT, Sum>(s, sh);
+  o.rest = 0;
   if (t.top_lse) {
-    prest = psum < 1 ? 1 - psum : 0;
-  } else if (psum > 0) {
-    for (int j = threadIdx.x; j < t.entries; j += NT) o.p[j] /= psum;
-    psum = 1;
-  }
-  __syncthreads();
-}
-
-constexpr int WINDOW = 1 << 18;           // logits whose membership bits are held at a time
-
-template <class T>
-__global__ __launch_bounds__(NT) void lt_distill_fwd(DistillParams p) {
-  using raw = typename T::raw;
-  __shared__ TeacherRow t;
-  __shared__ uint32_t bits[WINDOW / 32];
-  __shared__ float shf[NW];
-  {
-    const int64_t r = p.block0 + blockIdx.x;
-    const raw* z = (const raw*)p.z.data + p.z.at(r);
-    double psum, prest;
-    teacher_row(p.t, r, p.z.vocab, p.inv_t, t, psum, prest);
-    Running all, rest;
-    for (int64_t w0 = 0; w0 < p.z.vocab; w0 += WINDOW) {
-      const int n = (int)min((int64_t)WINDOW, p.z.vocab - w0);
-      for (int i = threadIdx.x; i < (n + 31) / 32; i += NT) bits[i] = 0;
-      __syncthreads();
-      for (int j = threadIdx.x; j < p.t.entries; j += NT) {
-        const int64_t v = t.id[j] - w0;
-        if (t.id[j] >= 0 && v >= 0 && v < n) atomicOr(&bits[v >> 5], 1u << (v & 31));
-      }
-      __syncthreads();
-      for (int i = threadIdx.x; i < n; i += NT) {
-        const float x = T::get(z[w0 + i]);
-        all.add(x, p.c);
-        if (!(bits[i >> 5] >> (i & 31) & 1)) rest.add(x, p.c);
-      }
-      __syncthreads();
+    if (o.sum < 1) o.rest = 1 - o.sum;
+  } else if (o.sum != 0) {
+    const double logs = log(o.sum), inv = 1 / o.sum;
+#pragma unroll
+    for (int i = 0; i < Entries<NT>::N; ++i) {
+      o.logp[i] -= logs;
+      o.p[i] *= inv;
     }
-    const float m = block_reduce<NT, Max>(all.m, shf);
-    const float s = block_reduce<NT, Sum>(all.s * exp2f((all.m - m) * p.c), shf);
-    const float sr = block_reduce<NT, Sum>(rest.s * exp2f((rest.m - m) * p.c), shf);
-    const double logs = log((double)s);
-    double loss = 0;
-    for (int j = threadIdx.x; j < p.t.entries; j += NT) {
-      const double pj = t.p[j];
-      if (t.id[j] >= 0 && pj != 0) loss += pj * (log(pj) - ((double)T::get(z[t.id[j]]) - m) * p.inv_t + logs);
-    }
-    loss = block_reduce<NT, Sum>(loss, t.sh);
-    if (threadIdx.x == 0) {
-      const double qrest = (double)sr / s;
-      if (!(qrest > 0)) prest = 0;
-      if (prest > 0) loss += prest * (log(prest) - log(qrest));
-      p.loss[r] = (float)loss;
-      const double whole = psum + prest;
-      float* st = p.stats + r * LT_DISTILL_STATS;
-      st[0] = m;
-      st[1] = s > 0 ? (float)(whole * p.inv_t / s) : 0.f;
-      st[2] = s > 0 ? (float)((whole - (prest > 0 ? prest / qrest : 0)) * p.inv_t / s) : 0.f;
-    }
+    o.sum = o.sum > 0 ? 1 : o.sum;         // (a NaN stays)
   }
 }
 
-template <class T>
-__global__ __launch_bounds__(NT) void lt_distill_bwd(DistillParams p) {
-  using raw = typename T::raw;
-  __shared__ TeacherRow t;
-  {
-    const int64_t r = p.block0 + blockIdx.x;
-    const raw* z = (const raw*)p.z.data + p.z.at(r);
-    raw* g = (raw*)p.grad.data + p.grad.at(r);
-    double psum, prest;
-    teacher_row(p.t, r, p.z.vocab, p.inv_t, t, psum, prest);
-    const float* st = p.stats + r * LT_DISTILL_STATS;
-    const float m = st[0], w = p.weight[r * p.weight_stride];
-    const float in = st[1] * w, out = st[2] * w;
-    for (int64_t v = threadIdx.x; v < p.z.vocab; v += NT) g[v] = T::put(exp2f((T::get(z[v]) - m) * p.c) * out);
-    __syncthreads();
-    for (int j = threadIdx.x; j < p.t.entries; j += NT) {
-      const int id = t.id[j];
-      if (id < 0) continue;
-      double pj = 0;                       // of every entry with this id
-      for (int i = 0; i < p.t.entries; ++i)
-        if (t.id[i] == id) pj += t.p[i];
-      g[id] = T::put(exp2f((T::get(z[id]) - m) * p.c) * in - (float)(pj * p.inv_t) * w);
+// sums of exp2((z - m) c) of a thread: within the entries (TAIL) and of all else
+struct Sums {
+  float m = LOWEST, in = 0.f, out = 0.f;
+};
+
+// One pass over z[v0 .. v1).
+template <class T, int NT, int U, int WINDOW, bool TAIL>
+__device__ __forceinline__ Sums sum_row(const typename T::raw* z, int v0, int v1, float c, const Entries<NT>& t,
+                                        DistillShared<NT, WINDOW>& sh) {
+  constexpr int E = Vec<T>::E, STEP = NT * U * E;
+  static_assert(WINDOW % STEP == 0 || WINDOW >= STEP, "a step lies in a window");
+  const int tid = thread_of<NT>();
+  Sums o;
+  for (int w0 = v0; w0 < v1; w0 += WINDOW) {
+    const int w1 = min(v1, w0 + WINDOW);
+    if (TAIL) {
+      for (int i = tid; i < (w1 - w0 + 31) / 32; i += NT) sh.bits[i] = 0;
+      sync<NT>();
+#pragma unroll
+      for (int i = 0; i < Entries<NT>::N; ++i) {
+        const int at = t.id[i] - w0;
+        if (t.id[i] >= w0 && t.id[i] < w1) atomicOr(&sh.bits[at >> 5], 1u << (at & 31));
+      }
+      sync<NT>();
     }
-    __syncthreads();
+    for (int base = w0; base < w1; base += STEP) {
+      Vec<T> v[U];
+      if (base + STEP <= w1) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u].load(z + base + (u * NT + tid) * E);
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u].load(z, base + (u * NT + tid) * E, w1, T::put(-INFINITY));
+      }
+      uint32_t in[U];
+      float t = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (TAIL) {
+          const int at = min(base + (u * NT + tid) * E, w1 - 1) - w0;
+          in[u] = (sh.bits[at >> 5] >> (at & 31 & ~(E - 1))) & ((1u << E) - 1);
+        }
+        t = max2(t, max_of(v[u]));
+        v[u].keep();
+      }
+      if ((t - o.m) * c > 32.f) {
+        const float f = exp2_((o.m - t) * c);
+        o.in *= f;
+        o.out *= f;
+        o.m = t;
+      }
+      float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (TAIL && __any(in[u])) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const float f = exp2_((v[u].get(e) - o.m) * c);
+            const bool entry = in[u] >> e & 1;
+            o.in += entry ? f : 0.f;
+            s0 += entry ? 0.f : f;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; e += 2) {
+            s0 += exp2_((v[u].get(e) - o.m) * c);
+            s1 += exp2_((v[u].get(e + 1) - o.m) * c);
+          }
+        }
+      }
+      o.out += s0 + s1;
+    }
+    if (TAIL) sync<NT>();
   }
+  return o;
+}
+
+// The sums of a group's threads, or of a row's chunks.
+template <int NT>
+__device__ __forceinline__ Sums join(Sums o, float c, float* shf) {
+  const float m = block_reduce<NT, Max>(o.m, shf), f = exp2_((o.m - m) * c);
+  o.in = block_reduce<NT, Sum>(o.in * f, shf);
+  o.out = block_reduce<NT, Sum>(o.out * f, shf);
+  o.m = m;
+  return o;
+}
+
+// Loss and the gradient's factors of a row from its sums.  (z: the row.)
+template <class T, int NT>
+__device__ __forceinline__ float3 finish_row(const Entries<NT>& t, const typename T::raw* z, Sums o, double inv_t,
+                                             double* sh, float& loss) {
+  const double s = (double)o.in + o.out, logs = log(s);
+  double l = 0;
+#pragma unroll
+  for (int i = 0; i < Entries<NT>::N; ++i)
+    if (t.id[i] >= 0 && t.p[i] != 0) l += t.p[i] * (t.logp[i] - ((double)T::get(z[t.id[i]]) - o.m) * inv_t + logs);
+  l = block_reduce<NT, Sum>(l, sh);
+  const double qrest = o.out / s;
+  const double rest = t.rest > 0 && qrest > 0 ? t.rest : 0;
+  if (rest > 0) l += rest * (log(rest) - log(qrest));
+  loss = (float)l;
+  const double whole = t.sum + rest;
+  if (!(s > 0)) return make_float3(o.m, 0.f, 0.f);
+  return make_float3(o.m, (float)(whole * inv_t / s), (float)((whole - (rest > 0 ? rest / qrest : 0)) * inv_t / s));
+}
+
+// The gradient of z[v0 .. v1): st from finish_row, w the row's weight.  The
+// entries' own are written behind a barrier over what the others were given.
+template <class T, int NT, int U, int WINDOW>
+__device__ __forceinline__ void grad_row(const typename T::raw* z, typename T::raw* g, int v0, int v1, float c,
+                                         float3 st, float w, double inv_t, const Entries<NT>& t,
+                                         DistillShared<NT, WINDOW>& sh, int entries) {
+  constexpr int E = Vec<T>::E, STEP = NT * U * E;
+  const int tid = thread_of<NT>();
+  const float out = st.z * w;
+  for (int base = v0; base < v1; base += STEP) {
+    Vec<T> v[U];
+    if (base + STEP <= v1) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u].load(z + base + (u * NT + tid) * E);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u].load(z, base + (u * NT + tid) * E, v1, T::put(-INFINITY));
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float f[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[e] = exp2_((v[u].get(e) - st.x) * c) * out;
+      v[u].put(f);
+      const int at = base + (u * NT + tid) * E;
+      if (at + E <= v1) v[u].store(g + at);
+      else if (at < v1) v[u].store_part(g + at, v1 - at);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < Entries<NT>::N; ++i) {
+    const int j = i * NT + tid;
+    if (j < MAXK) {
+      sh.id[j] = t.id[i];
+      sh.mass[j] = (float)(t.p[i] * inv_t);
+    }
+  }
+  sync<NT>();
+  if (NT == 64) __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+#pragma unroll
+  for (int i = 0; i < Entries<NT>::N; ++i) {
+    const int id = t.id[i];
+    if (id < v0 || id >= v1) continue;
+    int alike = 0;                         // entries with this id, itself among them
+    for (int j = 0; j < entries; j += 4) {
+      const int4 o = *(const int4*)&sh.id[j];
+      alike += (o.x == id) + (o.y == id) + (o.z == id) + (o.w == id);
+    }
+    float mass = (float)(t.p[i] * inv_t);
+    if (alike > 1) {
+      mass = 0;
+      for (int j = 0; j < entries; ++j) mass += sh.id[j] == id ? sh.mass[j] : 0.f;
+    }
+    g[id] = T::put((exp2_((T::get(z[id]) - st.x) * c) * st.y - mass) * w);
+  }
+}
+
+// Logits of a row and threads that take it: a wave, four of them a block, up to
+// 2048; else a block.
+#define GROUP_HEAD                                                                                        \
+  constexpr int GROUPS = NT == 64 ? 4 : 1;                                                                \
+  __shared__ __attribute__((aligned(16))) DistillShared<NT, WINDOW> shared[GROUPS];                       \
+  DistillShared<NT, WINDOW>& sh = shared[group_of<NT>()];                                                 \
+  const int64_t blk = (p.block0 + blockIdx.x) * GROUPS + group_of<NT>();                                  \
+  if (blk >= p.rows * p.splits) return; /* (a wave as a whole) */                                         \
+  const int64_t r = p.splits == 1 ? blk : blk / p.splits;                                                 \
+  const int v0 = p.splits == 1 ? 0 : (int)(blk % p.splits) * p.chunk;                                     \
+  const int v1 = p.splits == 1 ? p.z.vocab : min(p.z.vocab, v0 + p.chunk);                                \
+  const typename T::raw* z = (const typename T::raw*)p.z.data + p.z.at(r);                                \
+  Entries<NT> t;                                                                                          \
+  load_entries<NT>(p.t, r, p.z.vocab, p.inv_t, t, sh.sh)
+
+template <class T, int NT, int U, int WINDOW, bool TAIL>
+__global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_distill_sums(DistillParams p) {
+  GROUP_HEAD;
+  const Sums o = join<NT>(sum_row<T, NT, U, WINDOW, TAIL>(z, v0, v1, p.c, t, sh), p.c, sh.shf);
+  if (p.splits > 1) {
+    if (thread_of<NT>() == 0) p.part[blk] = make_float4(o.m, o.in, o.out, 0.f);
+    return;
+  }
+  float loss;
+  const float3 st = finish_row<T, NT>(t, z, o, p.inv_t, sh.sh, loss);
+  if (thread_of<NT>() == 0) {
+    p.loss[r] = loss;
+    *(float4*)(p.stats + r * LT_DISTILL_STATS) = make_float4(st.x, st.y, st.z, 0.f);
+  }
+}
+
+// A row's chunks joined.
+template <class T>
+__global__ __launch_bounds__(256) void lt_distill_join(DistillParams p) {
+  constexpr int NT = 256;
+  __shared__ DistillShared<NT, 32> sh;
+  const int64_t r = p.block0 + blockIdx.x;
+  Entries<NT> t;
+  load_entries<NT>(p.t, r, p.z.vocab, p.inv_t, t, sh.sh);
+  Sums o;
+  if ((int)threadIdx.x < p.splits) {       // (at most NT chunks)
+    const float4 part = p.part[r * p.splits + threadIdx.x];
+    o.m = part.x;
+    o.in = part.y;
+    o.out = part.z;
+  }
+  o = join<NT>(o, p.c, sh.shf);
+  float loss;
+  const float3 st = finish_row<T, NT>(t, (const typename T::raw*)p.z.data + p.z.at(r), o, p.inv_t, sh.sh, loss);
+  if (threadIdx.x == 0) {
+    p.loss[r] = loss;
+    *(float4*)(p.stats + r * LT_DISTILL_STATS) = make_float4(st.x, st.y, st.z, 0.f);
+  }
+}
+
+template <class T, int NT, int U, int WINDOW>
+__global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_distill_grad(DistillParams p) {
+  GROUP_HEAD;
+  const float4 st = *(const float4*)(p.stats + r * LT_DISTILL_STATS);
+  grad_row<T, NT, U, WINDOW>(z, (typename T::raw*)p.grad.data + p.grad.at(r), v0, v1, p.c,
+                             make_float3(st.x, st.y, st.z), p.weight[r * p.weight_stride], p.inv_t, t, sh, p.t.entries);
+}
+
+// Both: the second pass finds the row in the caches (a card's blocks hold 512
+// rows at a time, 128 MB of 131072 bf16).
+template <class T, int NT, int U, int WINDOW, bool TAIL>
+__global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_distill_both(DistillParams p) {
+  GROUP_HEAD;
+  const Sums o = join<NT>(sum_row<T, NT, U, WINDOW, TAIL>(z, v0, v1, p.c, t, sh), p.c, sh.shf);
+  float loss;
+  const float3 st = finish_row<T, NT>(t, z, o, p.inv_t, sh.sh, loss);
+  if (thread_of<NT>() == 0) p.loss[r] = loss;
+  grad_row<T, NT, U, WINDOW>(z, (typename T::raw*)p.grad.data + p.grad.at(r), v0, v1, p.c, st,
+                             p.weight[r * p.weight_stride], p.inv_t, t, sh, p.t.entries);
+}
+
+// ---- host ------------------------------------------------------------------
+enum Pass { SUMS, GRAD, BOTH };
+
+// Chunks of a row: one where the rows fill the card or a row is a few steps of
+// a block.
+void split_rows(DistillParams& p, int dtype) {
+  const int step = 512 * 4 * (dtype == LT_F32 ? 4 : 8);
+  int64_t n = 1;
+  if (p.z.vocab > 16384 && p.rows < 256) {
+    n = (p.z.vocab + step - 1) / step;
+    n = n < 512 / p.rows ? n : 512 / p.rows;
+    n = n < 256 ? n : 256;
+  }
+  const int64_t steps = (p.z.vocab + n * step - 1) / (n * step);
+  p.chunk = (int32_t)(n == 1 ? (int64_t)1 << 30 : steps * step);
+  p.splits = (int32_t)(((int64_t)p.z.vocab + p.chunk - 1) / p.chunk);
+}
+
+int64_t parts_bytes(const DistillParams& p) { return p.splits == 1 ? 0 : p.rows * p.splits * (int64_t)sizeof(float4); }
+
+template <class T, int NT, int U, int WINDOW>
+lt_status launch_group(const DistillParams& p, Pass pass, void* stream, const char* what) {
+  const int64_t blocks = NT == 64 ? (p.rows + 3) / 4 : p.rows * p.splits;
+  const int threads = NT == 64 ? 256 : NT;
+  if (pass == GRAD) return launch(lt_distill_grad<T, NT, U, WINDOW>, blocks, threads, p, stream, what);
+  if (pass == SUMS)
+    return p.t.top_lse ? launch(lt_distill_sums<T, NT, U, WINDOW, true>, blocks, threads, p, stream, what)
+                       : launch(lt_distill_sums<T, NT, U, WINDOW, false>, blocks, threads, p, stream, what);
+  return p.t.top_lse ? launch(lt_distill_both<T, NT, U, WINDOW, true>, blocks, threads, p, stream, what)
+                     : launch(lt_distill_both<T, NT, U, WINDOW, false>, blocks, threads, p, stream, what);
+}
+
+template <class T>
+lt_status launch_pass(const DistillParams& p, Pass pass, void* stream, const char* what) {
+  if (p.z.vocab <= 2048) return launch_group<T, 64, 16 / Vec<T>::E, 2048>(p, pass, stream, what);
+  if (p.z.vocab <= 16384) return launch_group<T, 256, 4, 16384>(p, pass, stream, what);
+  const lt_status st = launch_group<T, 512, 4, 1 << 18>(p, pass, stream, what);
+  if (st != LT_OK || pass != SUMS || p.splits == 1) return st;
+  return launch(lt_distill_join<T>, p.rows, 256, p, stream, what);
+}
+
+lt_status launch_pass(const DistillParams& p, int dtype, Pass pass, void* stream, const char* what) {
+  return dtype == LT_F32   ? launch_pass<F32>(p, pass, stream, what)
+         : dtype == LT_F16 ? launch_pass<F16>(p, pass, stream, what)
+                           : launch_pass<BF16>(p, pass, stream, what);
 }
 
 lt_status distill_check(const lt_rows* z, const lt_teacher* t, double temperature) {
@@ -178,7 +405,12 @@ DistillParams distill_params(const lt_rows* z, const lt_teacher* t, double tempe
   p.rows = z->rows;
   p.inv_t = 1 / temperature;
   p.c = (float)(LOG2E / temperature);
+  split_rows(p, z->dtype);
   return p;
+}
+
+bool workspace_ok(const DistillParams& p, const void* at, int64_t bytes) {
+  return p.splits == 1 || (at && (uintptr_t)at % 16 == 0 && bytes >= p.rows * LT_DISTILL_STATS * (int64_t)sizeof(float) + parts_bytes(p));
 }
 
 }  // namespace
@@ -186,19 +418,26 @@ DistillParams distill_params(const lt_rows* z, const lt_teacher* t, double tempe
 extern "C" {
 
 int64_t lt_distill_workspace(const lt_rows* z, int32_t) {
-  return z ? z->rows * LT_DISTILL_STATS * (int64_t)sizeof(float) : 0;
+  if (!z || z->rows < 1 || z->vocab < 1 || z->vocab > LT_MAX_VOCAB) return 0;
+  DistillParams p{};
+  p.z = rows_of(z);
+  p.rows = z->rows;
+  split_rows(p, z->dtype);
+  return p.splits == 1 ? 0 : p.rows * LT_DISTILL_STATS * (int64_t)sizeof(float) + parts_bytes(p);
 }
 
 lt_status lt_distill_forward(const lt_rows* z, const lt_teacher* t, double temperature, float* loss, float* stats,
-                             void*, int64_t, void* stream) {
+                             void* workspace, int64_t workspace_bytes, void* stream) {
   const lt_status st = distill_check(z, t, temperature);
   if (st != LT_OK || z->rows == 0) return st;
-  if (!loss || !stats) BAD("output: NULL");
-  ON_DEVICE(z->device);
+  if (!loss || !stats || (uintptr_t)stats % 16) BAD("output: NULL, or stats not 16 B aligned");
   DistillParams p = distill_params(z, t, temperature);
+  if (!workspace_ok(p, workspace, workspace_bytes)) BAD("workspace: %lld bytes, 16 B aligned, are needed", (long long)lt_distill_workspace(z, t->entries));
+  p.part = (float4*)workspace;
   p.loss = loss;
   p.stats = stats;
-  return launch(BY_TYPE(z->dtype, lt_distill_fwd), z->rows, NT, p, stream, "lt_distill_forward");
+  ON_DEVICE(z->device);
+  return launch_pass(p, z->dtype, SUMS, stream, "lt_distill_forward");
 }
 
 lt_status lt_distill_backward(const lt_rows* z, const lt_teacher* t, double temperature, const float* stats,
@@ -206,14 +445,14 @@ lt_status lt_distill_backward(const lt_rows* z, const lt_teacher* t, double temp
   lt_status st = distill_check(z, t, temperature);
   if (st == LT_OK) st = grad_check(z, grad, weight, weight_stride);
   if (st != LT_OK || z->rows == 0) return st;
-  if (!stats) BAD("stats: NULL");
-  ON_DEVICE(z->device);
+  if (!stats || (uintptr_t)stats % 16) BAD("stats: NULL or not 16 B aligned");
   DistillParams p = distill_params(z, t, temperature);
   p.stats = const_cast<float*>(stats);
   p.weight = weight;
   p.weight_stride = weight_stride;
   p.grad = rows_of(grad);
-  return launch(BY_TYPE(z->dtype, lt_distill_bwd), z->rows, NT, p, stream, "lt_distill_backward");
+  ON_DEVICE(z->device);
+  return launch_pass(p, z->dtype, GRAD, stream, "lt_distill_backward");
 }
 
 lt_status lt_distill_fused(const lt_rows* z, const lt_teacher* t, double temperature, const float* weight,
@@ -222,10 +461,19 @@ lt_status lt_distill_fused(const lt_rows* z, const lt_teacher* t, double tempera
   lt_status st = distill_check(z, t, temperature);
   if (st == LT_OK) st = grad_check(z, grad, weight, weight_stride);
   if (st != LT_OK || z->rows == 0) return st;
-  if (!workspace || workspace_bytes < lt_distill_workspace(z, t->entries)) BAD("workspace: %lld bytes", (long long)workspace_bytes);
-  st = lt_distill_forward(z, t, temperature, loss, (float*)workspace, nullptr, 0, stream);
-  if (st != LT_OK) return st;
-  return lt_distill_backward(z, t, temperature, (const float*)workspace, weight, weight_stride, grad, stream);
+  if (!loss) BAD("output: NULL");
+  DistillParams p = distill_params(z, t, temperature);
+  if (!workspace_ok(p, workspace, workspace_bytes)) BAD("workspace: %lld bytes, 16 B aligned, are needed", (long long)lt_distill_workspace(z, t->entries));
+  p.part = (float4*)workspace;
+  p.loss = loss;
+  p.stats = (float*)((char*)workspace + parts_bytes(p));
+  p.weight = weight;
+  p.weight_stride = weight_stride;
+  p.grad = rows_of(grad);
+  ON_DEVICE(z->device);
+  if (p.splits == 1) return launch_pass(p, z->dtype, BOTH, stream, "lt_distill_fused");
+  st = launch_pass(p, z->dtype, SUMS, stream, "lt_distill_fused");
+  return st != LT_OK ? st : launch_pass(p, z->dtype, GRAD, stream, "lt_distill_fused");
 }
 
 }  // extern "C"

@@ -36,12 +36,7 @@ struct F16 {
 struct BF16 {
   using raw = uint16_t;
   static __device__ __forceinline__ float get(raw v) { return __builtin_bit_cast(float, (uint32_t)v << 16); }
-  // to the nearest, ties to even; a NaN stays one
-  static __device__ __forceinline__ raw put(float v) {
-    const uint32_t b = __builtin_bit_cast(uint32_t, v);
-    if (v != v) return (raw)((b >> 16) | 0x40);
-    return (raw)((b + 0x7fff + ((b >> 16) & 1)) >> 16);
-  }
+  static __device__ __forceinline__ raw put(float v) { return __builtin_bit_cast(raw, (__bf16)v); }
 };
 
 // 16 bytes of a row, at any address its type allows (the loads and stores are
@@ -61,6 +56,23 @@ struct Vec {
   __device__ __forceinline__ void load(const typename T::raw* p) { b = *(const Bytes16*)p; }
   __device__ __forceinline__ void store(typename T::raw* p) const { *(Bytes16*)p = b; }
   __device__ __forceinline__ float get(int i) const;
+  // Rounded to the type, to the nearest.
+  __device__ __forceinline__ void put(const float* f) {
+    if constexpr (E == 4) {
+      for (int i = 0; i < 4; ++i) b.w[i] = __builtin_bit_cast(uint32_t, f[i]);
+    } else {
+      for (int i = 0; i < 4; ++i) b.w[i] = (uint32_t)T::put(f[2 * i]) | (uint32_t)T::put(f[2 * i + 1]) << 16;
+    }
+  }
+  // The first n < E of them.
+  __device__ __forceinline__ void store_part(typename T::raw* p, int n) const {
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (i < n) {
+        if constexpr (E == 4) p[i] = __builtin_bit_cast(float, b.w[i]);
+        else p[i] = (typename T::raw)(b.w[i >> 1] >> (i & 1) * 16);
+      }
+  }
   // What is computed from the logits ahead of this is not kept for later.
   __device__ __forceinline__ void keep() { asm volatile("" : "+v"(b.w[0]), "+v"(b.w[1]), "+v"(b.w[2]), "+v"(b.w[3])); }
   // The vector at `at` of a row's logits [.., end), `fill` behind them.

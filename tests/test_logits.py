@@ -114,8 +114,9 @@ def test_c_entries_refuse_rows(kw):
     lambda lib, x, t: lib.lt_distill_backward(C.byref(x), C.byref(t), 1.0, 4096, 4096, 1, None, None),
     lambda lib, x, t: lib.lt_distill_backward(C.byref(x), C.byref(t), 1.0, 4096, 4096, 1, C.byref(_desc(rows=3)), None),
     lambda lib, x, t: lib.lt_distill_backward(C.byref(x), C.byref(t), 1.0, 4096, 4096, 1, C.byref(_desc(dtype=2)), None),
-    lambda lib, x, t: lib.lt_distill_fused(C.byref(x), C.byref(t), 1.0, 4096, 1, 4096, C.byref(x), None, 1 << 20, None),
-    lambda lib, x, t: lib.lt_distill_fused(C.byref(x), C.byref(t), 1.0, 4096, 1, 4096, C.byref(x), 4096, 0, None),
+    lambda lib, x, t: lib.lt_distill_fused(C.byref(x), C.byref(t), 1.0, 4096, 1, None, C.byref(x), None, 0, None),
+    lambda lib, x, t: lib.lt_distill_fused(C.byref(_desc(vocab=200000)), C.byref(t), 1.0, 4096, 1, 4096,
+                                           C.byref(_desc(vocab=200000)), 4096, 0, None),
     lambda lib, x, t: lib.lt_verify_draft(None, 1.0, 4096, 4096, None, 0, None),
 ])
 def test_c_entries_refuse(call):
