@@ -45,6 +45,8 @@ struct __attribute__((packed, aligned(2))) Bytes16 {
   uint32_t w[4];
 };
 
+typedef uint32_t Words16 __attribute__((ext_vector_type(4), aligned(2)));
+
 __device__ __forceinline__ uint32_t twice(float v) { return __builtin_bit_cast(uint32_t, v); }
 __device__ __forceinline__ uint32_t twice(uint16_t v) { return (uint32_t)v << 16 | v; }
 
@@ -55,6 +57,18 @@ struct Vec {
   Bytes16 b;
   __device__ __forceinline__ void load(const typename T::raw* p) { b = *(const Bytes16*)p; }
   __device__ __forceinline__ void store(typename T::raw* p) const { *(Bytes16*)p = b; }
+  // The same past the caches: what is read or written for the last time.
+  __device__ __forceinline__ void load_last(const typename T::raw* p) {
+    const Words16 w = __builtin_nontemporal_load((const Words16*)p);
+    for (int i = 0; i < 4; ++i) b.w[i] = w[i];
+  }
+  __device__ __forceinline__ void store_past(typename T::raw* p) const {
+    // (the fences of asm: of this store and a plain one in the branches of an
+    // if, the compiler makes one plain store)
+    asm volatile("" ::: "memory");
+    __builtin_nontemporal_store(Words16{b.w[0], b.w[1], b.w[2], b.w[3]}, (Words16*)p);
+    asm volatile("" ::: "memory");
+  }
   __device__ __forceinline__ float get(int i) const;
   // Rounded to the type, to the nearest.
   __device__ __forceinline__ void put(const float* f) {
