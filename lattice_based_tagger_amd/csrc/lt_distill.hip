@@ -19,7 +19,7 @@ struct DistillParams {
   double inv_t;           // 1 / temperature
   float c;                // log2(e) / temperature
   int32_t splits;         // blocks of a row
-  int32_t chunk;          // logits of a block (a multiple of 8), the last one's fewer
+  int32_t chunk;          // of a row's numbers, to a block (a multiple of its step)
   float* loss;
   float* stats;           // [rows][LT_DISTILL_STATS]: m, the gradient's factors of exp2((z - m) c)
   float4* part;           // splits > 1: [rows][splits] reference, sums within and outside the entries
@@ -96,35 +96,30 @@ struct Sums {
   float m = LOWEST, in = 0.f, out = 0.f;
 };
 
-// One pass over z[v0 .. v1).
+// One pass over a row's logits with numbers in [v0, v1), from c0 on.
 template <class T, int NT, int U, int WINDOW, bool TAIL>
-__device__ __forceinline__ Sums sum_row(const typename T::raw* z, int v0, int v1, float c, const Entries<NT>& t,
+__device__ __forceinline__ Sums sum_row(const typename T::raw* row, int lead, int c0, int v0, int v1, float c, const Entries<NT>& t,
                                         DistillShared<NT, WINDOW>& sh) {
   constexpr int E = Vec<T>::E, STEP = NT * U * E;
   static_assert(WINDOW % STEP == 0 || WINDOW >= STEP, "a step lies in a window");
   const int tid = thread_of<NT>();
+  const typename T::raw* const z = row - lead;
   Sums o;
-  for (int w0 = v0; w0 < v1; w0 += WINDOW) {
+  for (int w0 = c0; w0 < v1; w0 += WINDOW) {
     const int w1 = min(v1, w0 + WINDOW);
     if (TAIL) {
       for (int i = tid; i < (w1 - w0 + 31) / 32; i += NT) sh.bits[i] = 0;
       sync<NT>();
 #pragma unroll
       for (int i = 0; i < Entries<NT>::N; ++i) {
-        const int at = t.id[i] - w0;
-        if (t.id[i] >= w0 && t.id[i] < w1) atomicOr(&sh.bits[at >> 5], 1u << (at & 31));
+        const int at = t.id[i] + lead - w0;
+        if (t.id[i] >= 0 && at >= 0 && at < w1 - w0) atomicOr(&sh.bits[at >> 5], 1u << (at & 31));
       }
       sync<NT>();
     }
     for (int base = w0; base < w1; base += STEP) {
       Vec<T> v[U];
-      if (base + STEP <= w1) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) v[u].load(z + base + (u * NT + tid) * E);
-      } else {
-#pragma unroll
-        for (int u = 0; u < U; ++u) v[u].load(z, base + (u * NT + tid) * E, w1, T::put(-INFINITY));
-      }
+      load_step<T, NT, U>(v, z, base, tid, v0, w1);
       uint32_t in[U];
       float t = -INFINITY;
 #pragma unroll
@@ -197,27 +192,20 @@ __device__ __forceinline__ float3 finish_row(const Entries<NT>& t, const typenam
   return make_float3(o.m, (float)(whole * inv_t / s), (float)((whole - (rest > 0 ? rest / qrest : 0)) * inv_t / s));
 }
 
-// The gradient of z[v0 .. v1): st from finish_row, w the row's weight.  The
+// The gradient of the logits with numbers in [v0, v1), from c0 on: st from finish_row, w the row's weight.  The
 // entries' own are written behind a barrier over what the others were given.
 template <class T, int NT, int U, int WINDOW, bool AGAIN>
-__device__ __forceinline__ void grad_row(const typename T::raw* z, typename T::raw* g, int v0, int v1, float c,
+__device__ __forceinline__ void grad_row(const typename T::raw* row, typename T::raw* grad, int lead, int c0, int v0, int v1, float c,
                                          float3 st, float w, double inv_t, const Entries<NT>& t,
                                          DistillShared<NT, WINDOW>& sh, int entries, bool past) {
   constexpr int E = Vec<T>::E, STEP = NT * U * E;
   const int tid = thread_of<NT>();
   const float out = st.z * w;
-  for (int base = v0; base < v1; base += STEP) {
+  const typename T::raw* const z = row - lead;
+  typename T::raw* const g = grad - lead;
+  for (int base = c0; base < v1; base += STEP) {
     Vec<T> v[U];
-    if (base + STEP <= v1) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (AGAIN) v[u].load_last(z + base + (u * NT + tid) * E);
-        else v[u].load(z + base + (u * NT + tid) * E);
-      }
-    } else {
-#pragma unroll
-      for (int u = 0; u < U; ++u) v[u].load(z, base + (u * NT + tid) * E, v1, T::put(-INFINITY));
-    }
+    load_step<T, NT, U, AGAIN>(v, z, base, tid, v0, v1);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float f[E];
@@ -225,11 +213,11 @@ __device__ __forceinline__ void grad_row(const typename T::raw* z, typename T::r
       for (int e = 0; e < E; ++e) f[e] = exp2_((v[u].get(e) - st.x) * c) * out;
       v[u].put(f);
       const int at = base + (u * NT + tid) * E;
-      if (at + E <= v1) {
+      if (at >= v0 && at + E <= v1) {
         if (past) v[u].store_past(g + at);
         else v[u].store(g + at);
       } else if (at < v1) {
-        v[u].store_part(g + at, v1 - at);
+        v[u].store_part(g, at, v0, v1);
       }
     }
   }
@@ -246,7 +234,7 @@ __device__ __forceinline__ void grad_row(const typename T::raw* z, typename T::r
 #pragma unroll
   for (int i = 0; i < Entries<NT>::N; ++i) {
     const int id = t.id[i];
-    if (id < v0 || id >= v1) continue;
+    if (id < 0 || id + lead < v0 || id + lead >= v1) continue;
     int alike = 0;                         // entries with this id, itself among them
     for (int j = 0; j < entries; j += 4) {
       const int4 o = *(const int4*)&sh.id[j];
@@ -257,7 +245,7 @@ __device__ __forceinline__ void grad_row(const typename T::raw* z, typename T::r
       mass = 0;
       for (int j = 0; j < entries; ++j) mass += sh.id[j] == id ? sh.mass[j] : 0.f;
     }
-    g[id] = T::put((exp2_((T::get(z[id]) - st.x) * c) * st.y - mass) * w);
+    grad[id] = T::put((exp2_((T::get(row[id]) - st.x) * c) * st.y - mass) * w);
   }
 }
 
@@ -270,16 +258,16 @@ __device__ __forceinline__ void grad_row(const typename T::raw* z, typename T::r
   const int64_t blk = (p.block0 + blockIdx.x) * GROUPS + group_of<NT>();                                  \
   if (blk >= p.rows * p.splits) return; /* (a wave as a whole) */                                         \
   const int64_t r = p.splits == 1 ? blk : blk / p.splits;                                                 \
-  const int v0 = p.splits == 1 ? 0 : (int)(blk % p.splits) * p.chunk;                                     \
-  const int v1 = p.splits == 1 ? p.z.vocab : min(p.z.vocab, v0 + p.chunk);                                \
   const typename T::raw* z = (const typename T::raw*)p.z.data + p.z.at(r);                                \
+  const int lead = lead_of<T>(z), c0 = p.splits == 1 ? 0 : (int)(blk % p.splits) * p.chunk;               \
+  const int v0 = max(lead, c0), v1 = min(lead + p.z.vocab, c0 + p.chunk);                                 \
   Entries<NT> t;                                                                                          \
   load_entries<NT>(p.t, r, p.z.vocab, p.inv_t, t, sh.sh)
 
 template <class T, int NT, int U, int WINDOW, bool TAIL>
 __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_distill_sums(DistillParams p) {
   GROUP_HEAD;
-  const Sums o = join<NT>(sum_row<T, NT, U, WINDOW, TAIL>(z, v0, v1, p.c, t, sh), p.c, sh.shf);
+  const Sums o = join<NT>(sum_row<T, NT, U, WINDOW, TAIL>(z, lead, c0, v0, v1, p.c, t, sh), p.c, sh.shf);
   if (p.splits > 1) {
     if (thread_of<NT>() == 0) p.part[blk] = make_float4(o.m, o.in, o.out, 0.f);
     return;
@@ -320,7 +308,7 @@ template <class T, int NT, int U, int WINDOW>
 __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_distill_grad(DistillParams p) {
   GROUP_HEAD;
   const float4 st = *(const float4*)(p.stats + r * LT_DISTILL_STATS);
-  grad_row<T, NT, U, WINDOW, false>(z, (typename T::raw*)p.grad.data + p.grad.at(r), v0, v1, p.c,
+  grad_row<T, NT, U, WINDOW, false>(z, (typename T::raw*)p.grad.data + p.grad.at(r), lead, c0, v0, v1, p.c,
                                     make_float3(st.x, st.y, st.z), p.weight[r * p.weight_stride], p.inv_t, t, sh,
                                     p.t.entries, p.past);
 }
@@ -330,14 +318,98 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_distill_grad(DistillPa
 // blocks are about to read again (4096 x 131072 bf16: 0.62 ms; with the stores
 // past the caches 0.50, with the loads too 0.47, 4.6 TB/s).
 template <class T, int NT, int U, int WINDOW, bool TAIL>
-__global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_distill_both(DistillParams p) {
+__global__ __launch_bounds__(NT == 64 ? 256 : NT, NT == 64 ? 1 : 8) void lt_distill_both(DistillParams p) {
   GROUP_HEAD;
-  const Sums o = join<NT>(sum_row<T, NT, U, WINDOW, TAIL>(z, v0, v1, p.c, t, sh), p.c, sh.shf);
+  const Sums o = join<NT>(sum_row<T, NT, U, WINDOW, TAIL>(z, lead, c0, v0, v1, p.c, t, sh), p.c, sh.shf);
   float loss;
   const float3 st = finish_row<T, NT>(t, z, o, p.inv_t, sh.sh, loss);
   if (thread_of<NT>() == 0) p.loss[r] = loss;
-  grad_row<T, NT, U, WINDOW, true>(z, (typename T::raw*)p.grad.data + p.grad.at(r), v0, v1, p.c, st,
+  grad_row<T, NT, U, WINDOW, true>(z, (typename T::raw*)p.grad.data + p.grad.at(r), lead, c0, v0, v1, p.c, st,
                                    p.weight[r * p.weight_stride], p.inv_t, t, sh, p.t.entries, p.past);
+}
+
+// Rows of at most FEW logits: a thread a row, the row in LDS, its entries a
+// mask of 64 bits.  The gradient is made of the logits alone (no stats).
+template <class T, bool LOSS, bool GRAD>
+__global__ __launch_bounds__(64) void lt_distill_few(DistillParams p) {
+  using raw = typename T::raw;
+  extern __shared__ float few[];           // [64][few_pitch(vocab)]
+  const int lane = threadIdx.x, vocab = p.z.vocab, pitch = few_pitch(vocab), n = p.t.entries;
+  const int64_t r0 = (p.block0 + blockIdx.x) * 64;
+  const int rows = (int)min((int64_t)64, p.rows - r0);
+  each_of_rows(rows, vocab, [&](int r, int v, int) {
+    few[r * pitch + v] = T::get(((const raw*)p.z.data + p.z.at(r0 + r))[v]);
+  });
+  __syncthreads();
+  const int64_t r = r0 + min(lane, rows - 1);
+  float* z = few + min(lane, rows - 1) * pitch;
+  const int64_t first = r * n;
+  // (the entries are read again where they are used: a cache line or two a row)
+  auto entry = [&](int j, int& id, double& v) {
+    const int64_t i = any_id(p.t.ids, first + j, p.t.ids_bytes);
+    if (i < 0 || i >= vocab) return false;
+    id = (int)i;
+    v = any_float(p.t.top, first + j, p.t.top_dtype) * p.inv_t;
+    return true;
+  };
+  int id = 0;
+  double v, ref = -INFINITY, sum = 0, rest = 0, norm = 0;
+  uint64_t mask = 0;
+  if (p.t.top_lse) ref = p.t.top_lse[r];
+  else
+    for (int j = 0; j < n; ++j)
+      if (entry(j, id, v)) ref = v > ref || v != v ? v : ref;
+  if (!p.t.top_lse && ref == -INFINITY) ref = 0;
+  for (int j = 0; j < n; ++j)
+    if (entry(j, id, v)) {
+      mask |= 1ull << id;
+      sum += exp(v - ref);
+    }
+  if (p.t.top_lse) {
+    if (sum < 1) rest = 1 - sum;
+  } else if (sum != 0) {
+    norm = log(sum);
+    sum = sum > 0 ? 1 : sum;               // (a NaN stays)
+  }
+  float m = LOWEST, in = 0.f, out = 0.f;
+  for (int i = 0; i < vocab; ++i) m = max2(m, z[i]);
+  for (int i = 0; i < vocab; ++i) {
+    const float e = exp2_((z[i] - m) * p.c);
+    const bool entry = mask >> i & 1;
+    in += entry ? e : 0.f;
+    out += entry ? 0.f : e;
+  }
+  const double s = (double)in + out, logs = log(s), qrest = out / s;
+  if (!(rest > 0 && qrest > 0)) rest = 0;
+  const double whole = sum + rest;
+  const float fin = s > 0 ? (float)(whole * p.inv_t / s) : 0.f;
+  const float fout = s > 0 ? (float)((whole - (rest > 0 ? rest / qrest : 0)) * p.inv_t / s) : 0.f;
+  if (LOSS) {
+    double loss = 0;
+    for (int j = 0; j < n; ++j)
+      if (entry(j, id, v)) {
+        const double logp = v - ref - norm, pj = exp(logp);
+        if (pj != 0) loss += pj * (logp - ((double)z[id] - m) * p.inv_t + logs);
+      }
+    if (rest > 0) loss += rest * (log(rest) - log(qrest));
+    if (lane < rows) {
+      p.loss[r] = (float)loss;
+      if (p.stats) *(float4*)(p.stats + r * LT_DISTILL_STATS) = make_float4(m, fin, fout, 0.f);
+    }
+  }
+  if (GRAD) {
+    const float w = p.weight[r * p.weight_stride];
+    if (lane < rows) {
+      for (int i = 0; i < vocab; ++i) z[i] = exp2_((z[i] - m) * p.c) * (mask >> i & 1 ? fin : fout);
+      for (int j = 0; j < n; ++j)
+        if (entry(j, id, v)) z[id] -= (float)(exp(v - ref - norm) * p.inv_t);
+      for (int i = 0; i < vocab; ++i) z[i] *= w;
+    }
+    __syncthreads();
+    each_of_rows(rows, vocab, [&](int r, int v, int) {
+      ((raw*)p.grad.data + p.grad.at(r0 + r))[v] = T::put(few[r * pitch + v]);
+    });
+  }
 }
 
 // ---- host ------------------------------------------------------------------
@@ -354,8 +426,8 @@ void split_rows(DistillParams& p, int dtype) {
     n = n < 256 ? n : 256;
   }
   const int64_t steps = (p.z.vocab + n * step - 1) / (n * step);
-  p.chunk = (int32_t)(n == 1 ? (int64_t)1 << 30 : steps * step);
-  p.splits = (int32_t)(((int64_t)p.z.vocab + p.chunk - 1) / p.chunk);
+  p.chunk = (int32_t)(n == 1 ? 0x7fffff80 : steps * step);
+  p.splits = (int32_t)(((int64_t)p.z.vocab + LEAD + p.chunk - 1) / p.chunk);
 }
 
 int64_t parts_bytes(const DistillParams& p) { return p.splits == 1 ? 0 : p.rows * p.splits * (int64_t)sizeof(float4); }
@@ -374,6 +446,14 @@ lt_status launch_group(const DistillParams& p, Pass pass, void* stream, const ch
 
 template <class T>
 lt_status launch_pass(const DistillParams& p, Pass pass, void* stream, const char* what) {
+  // (a wave a row takes 160 us for 131072 x 41 float32, a thread a row XX)
+  if (p.z.vocab <= FEW && p.rows >= 4096 && p.t.entries <= 64) {
+    const int64_t blocks = (p.rows + 63) / 64;
+    const int lds = 64 * few_pitch(p.z.vocab) * 4;
+    return pass == SUMS   ? launch(lt_distill_few<T, true, false>, blocks, 64, p, stream, what, lds)
+           : pass == GRAD ? launch(lt_distill_few<T, false, true>, blocks, 64, p, stream, what, lds)
+                          : launch(lt_distill_few<T, true, true>, blocks, 64, p, stream, what, lds);
+  }
   if (p.z.vocab <= 2048) return launch_group<T, 64, 16 / Vec<T>::E, 2048>(p, pass, stream, what);
   if (p.z.vocab <= 16384) return launch_group<T, 256, 4, 16384>(p, pass, stream, what);
   const lt_status st = launch_group<T, 512, 4, 1 << 18>(p, pass, stream, what);
@@ -482,7 +562,7 @@ lt_status lt_distill_fused(const lt_rows* z, const lt_teacher* t, double tempera
   if (!workspace_ok(p, workspace, workspace_bytes)) BAD("workspace: %lld bytes, 16 B aligned, are needed", (long long)lt_distill_workspace(z, t->entries));
   p.part = (float4*)workspace;
   p.loss = loss;
-  p.stats = (float*)((char*)workspace + parts_bytes(p));
+  p.stats = workspace ? (float*)((char*)workspace + parts_bytes(p)) : nullptr;
   p.weight = weight;
   p.weight_stride = weight_stride;
   p.grad = rows_of(grad);

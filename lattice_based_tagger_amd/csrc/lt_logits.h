@@ -48,6 +48,8 @@ struct __attribute__((packed, aligned(2))) Bytes16 {
 typedef uint32_t Words16 __attribute__((ext_vector_type(4), aligned(2)));
 
 __device__ __forceinline__ uint32_t twice(float v) { return __builtin_bit_cast(uint32_t, v); }
+__device__ __forceinline__ uint32_t bits_of(float v) { return __builtin_bit_cast(uint32_t, v); }
+__device__ __forceinline__ uint32_t bits_of(uint16_t v) { return v; }
 __device__ __forceinline__ uint32_t twice(uint16_t v) { return (uint32_t)v << 16 | v; }
 
 // The E = 16 / sizeof(raw) logits of a vector.
@@ -78,41 +80,67 @@ struct Vec {
       for (int i = 0; i < 4; ++i) b.w[i] = (uint32_t)T::put(f[2 * i]) | (uint32_t)T::put(f[2 * i + 1]) << 16;
     }
   }
-  // The first n < E of them.
-  __device__ __forceinline__ void store_part(typename T::raw* p, int n) const {
+  // What lies in [begin, end) of the vector that belongs at `at`.
+  __device__ __forceinline__ void store_part(typename T::raw* x, int at, int begin, int end) const {
 #pragma unroll
     for (int i = 0; i < E; ++i)
-      if (i < n) {
-        if constexpr (E == 4) p[i] = __builtin_bit_cast(float, b.w[i]);
-        else p[i] = (typename T::raw)(b.w[i >> 1] >> (i & 1) * 16);
+      if (at + i >= begin && at + i < end) {
+        if constexpr (E == 4) x[at + i] = __builtin_bit_cast(float, b.w[i]);
+        else x[at + i] = (typename T::raw)(b.w[i >> 1] >> (i & 1) * 16);
       }
   }
   // What is computed from the logits ahead of this is not kept for later.
   __device__ __forceinline__ void keep() { asm volatile("" : "+v"(b.w[0]), "+v"(b.w[1]), "+v"(b.w[2]), "+v"(b.w[3])); }
-  // The vector at `at` of a row's logits [.., end), `fill` behind them.
-  __device__ __forceinline__ void load(const typename T::raw* x, int at, int end, typename T::raw fill) {
-    if (at + E <= end) load(x + at);
-    else if (at < end) load_part(x + at, end - at, fill);
-    else b.w[0] = b.w[1] = b.w[2] = b.w[3] = twice(fill);
+  // The vector at `at` of logits that lie in [begin, end), `fill` around them.
+  // One that holds one of their ends is the whole vector beside it, shifted.
+  __device__ __forceinline__ void load(const typename T::raw* x, int at, int begin, int end, typename T::raw fill) {
+    if (!load_inner(x, at, begin, end, fill)) load_edge(x, at, begin, end, fill);
   }
-  // n < E logits, `fill` behind them (a rolled loop: few registers, taken once a row)
-  __device__ __forceinline__ void load_part(const typename T::raw* p, int n, typename T::raw fill) {
-    b.w[0] = b.w[1] = b.w[2] = b.w[3] = 0;
+  // The same; false where the vector holds an end (it is `fill` then).
+  __device__ __forceinline__ bool load_inner(const typename T::raw* x, int at, int begin, int end, typename T::raw fill) {
+    b.w[0] = b.w[1] = b.w[2] = b.w[3] = twice(fill);
+    if (at >= begin && at + E <= end) load(x + at);
+    else if (at < end && at + E > begin) return false;
+    return true;
+  }
+  __device__ __forceinline__ void load_edge(const typename T::raw* x, int at, int begin, int end, typename T::raw fill) {
+    constexpr int BITS = 8 * sizeof(typename T::raw);
+    const uint64_t f = (uint64_t)twice(fill) << 32 | twice(fill);
+    uint64_t lo, hi;
+    if (end - begin < E) {                 // a row of less than a vector
+      lo = hi = f;
 #pragma nounroll
-    for (int i = E - 1; i >= 0; --i) {
-      const typename T::raw v = i < n ? p[i] : fill;
-      if constexpr (E == 4) {
-        b.w[3] = b.w[2];
-        b.w[2] = b.w[1];
-        b.w[1] = b.w[0];
-        b.w[0] = __builtin_bit_cast(uint32_t, v);
-      } else {
-        b.w[3] = b.w[3] << 16 | b.w[2] >> 16;
-        b.w[2] = b.w[2] << 16 | b.w[1] >> 16;
-        b.w[1] = b.w[1] << 16 | b.w[0] >> 16;
-        b.w[0] = b.w[0] << 16 | v;
+      for (int i = max(at, begin); i < min(at + E, end); ++i) {
+        const int by = (i - at) * BITS;
+        const uint64_t field = (~0ull >> (64 - BITS)) << (by & 63), v = (uint64_t)bits_of(x[i]) << (by & 63);
+        if (by < 64) lo = (lo & ~field) | v;
+        else hi = (hi & ~field) | v;
+      }
+    } else {
+      const bool head = at < begin;
+      load(x + (head ? begin : end - E));
+      lo = (uint64_t)b.w[1] << 32 | b.w[0];
+      hi = (uint64_t)b.w[3] << 32 | b.w[2];
+      int by = (head ? begin - at : at + E - end) * BITS;      // 0 < by < 128
+      if (by >= 64) {
+        by -= 64;
+        if (head) hi = lo, lo = f;
+        else lo = hi, hi = f;
+      }
+      if (by) {
+        if (head) {
+          hi = hi << by | lo >> (64 - by);
+          lo = lo << by | f >> (64 - by);
+        } else {
+          lo = lo >> by | hi << (64 - by);
+          hi = hi >> by | f << (64 - by);
+        }
       }
     }
+    b.w[0] = (uint32_t)lo;
+    b.w[1] = (uint32_t)(lo >> 32);
+    b.w[2] = (uint32_t)hi;
+    b.w[3] = (uint32_t)(hi >> 32);
   }
 };
 template <>
@@ -126,6 +154,38 @@ __device__ __forceinline__ float Vec<F16>::get(int i) const {
 template <>
 __device__ __forceinline__ float Vec<BF16>::get(int i) const {
   return __builtin_bit_cast(float, i & 1 ? b.w[i >> 1] & 0xffff0000u : b.w[i >> 1] << 16);
+}
+
+// A step's vectors of a thread: U of them, NT vectors apart from `base` on, of
+// logits in [begin, end); LAST: past the caches.
+template <class T, int NT, int U, bool LAST = false>
+__device__ __forceinline__ void load_step(Vec<T> (&v)[U], const typename T::raw* x, int base, int tid, int begin, int end) {
+  constexpr int E = Vec<T>::E;
+  if (base >= begin && base + NT * U * E <= end) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (LAST) v[u].load_last(x + base + (u * NT + tid) * E);
+      else v[u].load(x + base + (u * NT + tid) * E);
+    }
+    return;
+  }
+  const typename T::raw fill = T::put(-INFINITY);
+  uint32_t edges = 0;
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (!v[u].load_inner(x, base + (u * NT + tid) * E, begin, end, fill)) edges |= 1u << u;
+  // (one copy of this for all u, and that once: else it takes 40 registers)
+#pragma nounroll
+  while (edges) {
+    const int at = __builtin_ctz(edges);
+    edges &= edges - 1;
+    Vec<T> e;
+    e.load_edge(x, base + (at * NT + tid) * E, begin, end, fill);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[u].b.w[i] = u == at ? e.b.w[i] : v[u].b.w[i];
+  }
 }
 
 // The larger of two, of three; a NaN gives way to a number.
@@ -271,6 +331,14 @@ __device__ __forceinline__ float of_order(uint32_t o) {
 // The order above the complement of the index: no two keys of a row are alike,
 // and of equal logits the first has the larger.
 __device__ __forceinline__ uint64_t order_key(float x, uint32_t id) { return ((uint64_t)order_of(x) << 32) | (uint32_t)~id; }
+
+// Rows lie at any address; their vectors lie on the memory's grid of 128 bytes.
+// A row's logits are numbered from the grid's last point before it: `lead` of
+// the numbers are no logits.  (Vectors from the row's own start took 18 to 20 %
+// longer where that is off the grid, as in rows of an odd vocabulary.)
+template <class T>
+__device__ __forceinline__ int lead_of(const typename T::raw* x) { return (int)((uintptr_t)x & 127) / (int)sizeof(typename T::raw); }
+constexpr int LEAD = 64;                   // more than any lead
 
 // ---- rows of a few logits ----------------------------------------------------
 // A wave takes 64 rows, a thread one of them, from LDS: the logits come in

@@ -14,7 +14,7 @@ struct TopParams {
   int64_t block0;         // of this launch
   int32_t k;
   int32_t splits;         // blocks of a row
-  int32_t chunk;          // logits of a block (a multiple of 8), the last one's fewer
+  int32_t chunk;          // of a row's numbers, to a block (a multiple of its step)
   float c;                // log2(e) / temperature
   void* values;
   int64_t* ids;
@@ -209,9 +209,12 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
   if (blk >= p.rows * p.splits) return;  // (a wave as a whole)
   const int64_t r = p.splits == 1 ? blk : blk / p.splits;
   const int split = p.splits == 1 ? 0 : (int)(blk % p.splits);
-  const raw* x = (const raw*)p.x.data + p.x.at(r);
-  const int v0 = split * p.chunk, v1 = min(p.x.vocab, v0 + p.chunk);
-  const int k = min(p.k, v1 - v0);
+  const raw* const row = (const raw*)p.x.data + p.x.at(r);
+  const int lead = lead_of<T>(row);
+  const raw* const x = row - lead;
+  const int c0 = split * p.chunk;        // the block's: [v0, v1) from c0 on
+  const int v0 = max(lead, c0), v1 = min(lead + p.x.vocab, c0 + p.chunk);
+  const int k = max(0, min(p.k, v1 - v0));
   const int per_wave = W == 1 ? min(63, k + 2 + k / 16) : (k + W - 1) / W + 1;
   float m = LOWEST, s = 0.f, tau = -INFINITY;
   int n = 0;                             // keys
@@ -221,7 +224,9 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
   // Above tau; or equal to it, and ahead of the last that a cut kept (in a
   // list, whose vectors lie in any order: of later steps none is ahead).
   uint32_t tie = 0xffffffffu;
-  auto counts = [&](float f, int id) { return f > tau || (f == tau && ~(uint32_t)id > tie); };
+  auto counts = [&](float f, int at) {
+    return at >= v0 && at < v1 && (f > tau || (f == tau && ~(uint32_t)(at - lead) > tie));
+  };
   auto cut = [&]() {
     const uint64_t least = cut_keys<NT, C>(buf, n, k, sh.hist, &sh.cnt2, sh.sh64);
     tau = of_order((uint32_t)(least >> 32));
@@ -234,12 +239,12 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
 #pragma nounroll
     for (int i0 = 0; i0 < nv; i0 += NT) {
       const int i = i0 + tid;
-      const int at = i < nv ? v0 + (of ? (int)of[i] : first + i) * E : v1;
+      const int at = i < nv ? c0 + (of ? (int)of[i] : first + i) * E : v1;
       Vec<T> v;
-      v.load(x, at, v1, T::put(-INFINITY));
+      v.load(x, at, v0, v1, T::put(-INFINITY));
       int mine = 0;
 #pragma unroll
-      for (int e = 0; e < E; ++e) mine += at + e < v1 && counts(v.get(e), at + e);
+      for (int e = 0; e < E; ++e) mine += counts(v.get(e), at + e);
       if (__any(mine)) {
         const int upto = wave_scan<Sum>(mine, 0);
         int pos = 0;
@@ -249,8 +254,8 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           const float f = v.get(e);
-          if (at + e < v1 && counts(f, at + e)) {
-            if (pos < C) buf[pos] = order_key(f, (uint32_t)(at + e));
+          if (counts(f, at + e)) {
+            if (pos < C) buf[pos] = order_key(f, (uint32_t)(at + e - lead));
             ++pos;
           }
         }
@@ -266,8 +271,8 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
           if (n > C - NT) cut();           // (room for a logit of every thread)
           if (tid == 0) sh.cnt = n;
           sync<NT>();
-          const float f = at + e < v1 ? T::get(x[at + e]) : -INFINITY;
-          if (at + e < v1 && counts(f, at + e)) buf[atomicAdd(&sh.cnt, 1)] = order_key(f, (uint32_t)(at + e));
+          const float f = at + e >= v0 && at + e < v1 ? T::get(x[at + e]) : -INFINITY;
+          if (counts(f, at + e)) buf[atomicAdd(&sh.cnt, 1)] = order_key(f, (uint32_t)(at + e - lead));
           sync<NT>();
           n = sh.cnt;
           sync<NT>();
@@ -277,16 +282,10 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
   };
 
   int have = 0;                          // vectors on the list
-  for (int base = v0; base < v1; base += STEP) {
+  for (int base = c0; base < v1; base += STEP) {
     Vec<T> v[U];
     float vm[U];
-    if (base + STEP <= v1) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) v[u].load(x + base + (u * NT + tid) * E);
-    } else {
-#pragma unroll
-      for (int u = 0; u < U; ++u) v[u].load(x, base + (u * NT + tid) * E, v1, T::put(-INFINITY));
-    }
+    load_step<T, NT, U>(v, x, base, tid, v0, v1);
     float t = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -307,7 +306,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
         s1 += exp2_((v[u].get(e + 1) - m) * p.c);
       }
     s += s0 + s1;
-    if (base == v0) {
+    if (base == c0) {
       // the per_wave-th largest of a wave's threads (from its leading 18 bits
       // down), and of the waves' the largest that k threads of the block are
       // above (the least where ties leave none: k threads reach that)
@@ -350,7 +349,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int at = pos + __builtin_amdgcn_mbcnt_hi((uint32_t)(b[u] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b[u], 0));
-        if (vm[u] > tau && at < CL) sh.list[at] = (uint32_t)((base - v0) / E + u * NT + tid);
+        if (vm[u] > tau && at < CL) sh.list[at] = (uint32_t)((base - c0) / E + u * NT + tid);
         pos += __popcll(b[u]);
       }
     }
@@ -362,7 +361,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
     if (last || over || n + have > k + k / 2 + 192) {
 #pragma nounroll
       for (int pass = 0; pass <= (int)over; ++pass)
-        expand(pass ? nullptr : sh.list, (base - v0) / E, pass ? min(NT * U, (v1 - base + E - 1) / E) : over ? was : have);
+        expand(pass ? nullptr : sh.list, (base - c0) / E, pass ? min(NT * U, (v1 - base + E - 1) / E) : over ? was : have);
       // the best k so far: fewer of the logits to come lie above the last of them
       if (n > k && (!last || n > 512)) cut();
       tie = 0xffffffffu;
@@ -377,17 +376,17 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
   const float top = block_reduce<NT, Max>(m, sh.shf);
   const float sum = block_reduce<NT, Sum>(s * exp2_((m - top) * p.c), sh.shf);
   if (sum != sum) {
-    best_by_passes<T, NT>(x, v0, v1, k, buf, sh.sh64);
+    best_by_passes<T, NT>(row, v0 - lead, v1 - lead, k, buf, sh.sh64);
   } else {
-    for (int base = v0; n < k && base < v1; base += NT * E) {
+    for (int base = c0; n < k && base < v1; base += NT * E) {
       // the first logits that equal tau: in order, a vector a thread (never
       // short of k: at least k logits reach tau)
       const int at = base + tid * E;
       Vec<T> v;
-      v.load(x, at, v1, T::put(-INFINITY));
+      v.load(x, at, v0, v1, T::put(-INFINITY));
       int mine = 0;
 #pragma unroll
-      for (int e = 0; e < E; ++e) mine += at + e < v1 && v.get(e) == tau;
+      for (int e = 0; e < E; ++e) mine += at + e >= v0 && at + e < v1 && v.get(e) == tau;
       const int upto = wave_scan<Sum>(mine, 0);
       if (lane == 63) sh.reach[wave] = upto;
       sync<NT>();
@@ -400,8 +399,8 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
       }
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if (at + e < v1 && v.get(e) == tau) {
-          if (pos < k) buf[pos] = order_key(tau, (uint32_t)(at + e));
+        if (at + e >= v0 && at + e < v1 && v.get(e) == tau) {
+          if (pos < k) buf[pos] = order_key(tau, (uint32_t)(at + e - lead));
           ++pos;
         }
       n = min(k, n + all);
@@ -415,7 +414,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
       const uint32_t id = ~(uint32_t)buf[j];
       p.ids[r * k + j] = id;
       // (the key holds a NaN as -inf)
-      ((raw*)p.values)[r * k + j] = sum != sum ? x[id] : T::put(of_order((uint32_t)(buf[j] >> 32)));
+      ((raw*)p.values)[r * k + j] = sum != sum ? row[id] : T::put(of_order((uint32_t)(buf[j] >> 32)));
     }
   } else {
     if (tid == 0) p.part_sums[blk] = make_float2(top, sum);
@@ -555,8 +554,8 @@ void split_rows(TopParams& p, int dtype) {
     n = n < JOIN / p.k ? n : JOIN / p.k;
   }
   const int64_t steps = (p.x.vocab + n * step - 1) / (n * step);
-  p.chunk = (int32_t)(n == 1 ? (int64_t)1 << 30 : steps * step);
-  p.splits = (int32_t)(((int64_t)p.x.vocab + p.chunk - 1) / p.chunk);
+  p.chunk = (int32_t)(n == 1 ? 0x7fffff80 : steps * step);
+  p.splits = (int32_t)(((int64_t)p.x.vocab + LEAD + p.chunk - 1) / p.chunk);
 }
 
 int64_t top_workspace(const TopParams& p) {

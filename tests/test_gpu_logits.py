@@ -190,6 +190,26 @@ def test_distill(dtype, tail, rows, vocab, k, pad, temperature):
     check_distill(z, ids, top, lse, temperature)
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('tail', [False, True])
+@pytest.mark.parametrize('vocab, k, pad', [(1, 1, 0), (2, 2, 0), (41, 5, 0), (64, 64, 0), (63, 7, 2), (65, 5, 0)])
+def test_distill_few_logits(dtype, tail, vocab, k, pad):
+    """Many rows of a few logits; masks, padding and repeated ids among them."""
+    z = rand((4121, vocab), dtype, vocab, pad=pad)
+    ids, top, lse = teacher(z, k, dtype, vocab + 1, tail, 0.8, empty=0.1)
+    ids[3::11, k // 2:] = -1
+    ids[5::13, 0] = vocab
+    if k > 4:
+        ids[7::17, 1] = ids[7::17, 2]
+        top[7::17] -= 2
+        top[8::19, 3] = -INF
+    if vocab > 2:
+        keep = z[9::23].gather(1, ids[9::23].clamp(0, vocab - 1))
+        z[9::23] = -INF
+        z[9::23] = z[9::23].scatter(1, ids[9::23].clamp(0, vocab - 1), keep)
+    check_distill(z, ids, top, lse, 0.8)
+
+
 @pytest.mark.parametrize('tail', [False, True])
 def test_distill_beyond_a_window_of_bits(tail):
     z = rand((2, 600007), torch.bfloat16, 4)
