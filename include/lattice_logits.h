@@ -119,7 +119,8 @@ lt_status lt_distill_fused(const lt_rows* z, const lt_teacher* t, double tempera
  *   token = the lowest v with w_v > 0 and w_0 + ... + w_v > sample_u[b] * sum w,
  *           else the last with w_v > 0; -1 if p_a is empty (a row of -inf)
  *   tokens[b] = x_0 .. x_{a-1}, token, -1 ...  [drafts + 1];  accepted[b] = a
- * Rows past lengths[b] are not read; lengths are taken as within [0, drafts].
+ * Logits are finite or -inf (a NaN counts as -inf).  Rows past lengths[b] are
+ * not read; lengths are taken as within [0, drafts].
  * Sums that decide the token are held in 64 bits. */
 typedef struct {
   const lt_rows* target;

@@ -350,7 +350,7 @@ def check_verify(**a):
 @pytest.mark.parametrize('batch, drafts, vocab, pad, temperature', [
     (1, 0, 5, 0, 1.0), (1, 1, 1, 0, 1.0), (5, 3, 2, 0, 1.0), (40, 4, 41, 0, 1.0), (7, 2, 64, 1, 0.8),
     (9, 5, 1000, 0, 1.0), (3, 8, 4097, 3, 1.5), (1, 4, 32000, 0, 1.0), (4, 3, 50261, 0, 0.6), (2, 2, 131072, 0, 1.0),
-    (300, 3, 700, 0, 1.0), (2, 20, 300, 0, 1.0)])
+    (300, 3, 700, 0, 1.0), (2, 20, 300, 0, 1.0), (260, 2, 9001, 1, 1.2), (257, 0, 40, 0, 1.0), (3, 1, 300007, 0, 1.0)])
 def test_verify(dtype, certain, batch, drafts, vocab, pad, temperature):
     a = drafted(batch, drafts, vocab, dtype, batch * 13 + vocab, certain, pad=pad)
     check_verify(temperature=temperature, **a)
