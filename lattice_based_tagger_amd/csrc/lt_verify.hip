@@ -5,32 +5,73 @@
 // relative error e of the sums moves it with a probability of about e times the
 // number of tokens that the line may fall beside: 131072 e.  A float32
 // exponential (1e-7) would move one in a hundred; all sums are held in 64 bits
-// and the exponential is good to 3e-13.
+// and the exponential is good to 1.1e-12.  It is what bounds these kernels: 18
+// instructions a logit, where memory would allow 14.
 #include "lt_logits.h"
 
 namespace {
 
-// 2^t for t <= 0 (0 below -1100; -inf is fine): 2^n 2^f, n the whole number
-// next to t, 2^f by its series, whose first term left out is below
-// (ln 2 / 2)^11 / 11! = 2.2e-13.
+// 2^t for -1020 < t < 1020: 2^n 2^f, n the whole number next to t, 2^f by the
+// polynomial of degree 8 through its values at the Chebyshev points of
+// [-1/2, 1/2] (relative error at most 1.1e-12; the series needs degree 10 for
+// that).  n is added to the exponent's bits.
 __device__ __forceinline__ double exp2_64(double t) {
   constexpr double BIG = 6755399441055744.0;       // 1.5 * 2^52: its last bits are whole numbers
-  t = fmax(t, -1100.0);
   const double b = t + BIG;
   const double f = t - (b - BIG);
-  double r = 7.0549116208011e-9;                   // (ln 2)^k / k!, k = 10 .. 0
-  r = fma(r, f, 1.0178086009239699e-7);
-  r = fma(r, f, 1.3215486790144307e-6);
-  r = fma(r, f, 1.5252733804059840e-5);
-  r = fma(r, f, 1.5403530393381610e-4);
-  r = fma(r, f, 1.3333558146428443e-3);
-  r = fma(r, f, 9.6181291076284772e-3);
-  r = fma(r, f, 5.5504108664821580e-2);
-  r = fma(r, f, 2.4022650695910071e-1);
-  r = fma(r, f, 6.9314718055994531e-1);
-  r = fma(r, f, 1.0);
-  return ldexp(r, (int)(uint32_t)__builtin_bit_cast(uint64_t, b));
+  double r = 1.325497460306718e-06;
+  r = fma(r, f, 1.531007807039615e-05);
+  r = fma(r, f, 0.00015403457039410448);
+  r = fma(r, f, 0.0013333450573018062);
+  r = fma(r, f, 0.009618129157656703);
+  r = fma(r, f, 0.055504109412010456);
+  r = fma(r, f, 0.24022650695821055);
+  r = fma(r, f, 0.6931471805459343);
+  r = fma(r, f, 0.9999999999999997);
+  const uint64_t bits = __builtin_bit_cast(uint64_t, r);
+  const uint32_t hi = (uint32_t)(bits >> 32) + ((uint32_t)__builtin_bit_cast(uint64_t, b) << 20);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)bits);
 }
+
+// Four at a time: a step of one takes 8 cycles or more until the next may use
+// it, and few waves are there to fill them.
+__device__ __forceinline__ void exp2_64(double (&t)[4]) {
+  constexpr double BIG = 6755399441055744.0;
+  constexpr double C[9] = {0.9999999999999997, 0.6931471805459343, 0.24022650695821055, 0.055504109412010456, 0.009618129157656703,
+                           0.0013333450573018062, 0.00015403457039410448, 1.531007807039615e-05, 1.325497460306718e-06};
+  double b[4], r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) b[i] = t[i] + BIG;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) t[i] -= b[i] - BIG;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = fma(C[8], t[i], C[7]);
+#pragma unroll
+  for (int k = 6; k >= 0; --k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = fma(r[i], t[i], C[k]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, r[i]);
+    const uint32_t hi = (uint32_t)(bits >> 32) + ((uint32_t)__builtin_bit_cast(uint64_t, b[i]) << 20);
+    t[i] = __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)bits);
+  }
+}
+
+// exp2((x - m) c) of logits no further than 1000 (in the exponent) below m;
+// lower ones are taken as that: 1e-301.
+constexpr double DEPTH = 1000;
+__device__ __forceinline__ float floor_of(float m, double c) { return (float)fmax((double)m - DEPTH / c, (double)LOWEST); }
+__device__ __forceinline__ double soft_exp(float x, float floor, double m, double c) {
+  return exp2_64(((double)max2(x, floor) - m) * c);
+}
+
+// Where a sequence stops, for the kernels that follow.
+struct StopNote {
+  double ps, qs;          // sums of the target's row, of the drafter's
+  float pm, qm;
+  int32_t a, pad;
+};
 
 struct VerifyParams {
   int64_t block0;         // of this launch
@@ -46,21 +87,29 @@ struct VerifyParams {
   int64_t* accepted;
   int32_t splits, chunk;  // blocks of a row, a block's numbers of it
   int32_t segments;       // of a row: 64 vectors each
+  int32_t weigh_splits, weigh_chunk;       // of the row that the token is drawn from
   double* weight;         // [batch][segments]: the weights' sums
+  struct StopNote* stop;  // [batch]
   double2* part;          // [batch * (2 drafts + 1)][splits]: reference and sum, targets first
 };
 
-// A row's softmax: exp2((x - m) c) * inv, inv 0 for a row of -inf.
+// A row's softmax: exp2((x - m) c) * inv, inv 0 for a row of -inf; 0 below the
+// floor.
 struct Soft {
-  float m = LOWEST;
+  float m = LOWEST, floor = LOWEST;
   double s = 0, inv = 0;
-  __device__ __forceinline__ double of(float x, double c) const { return exp2_64(((double)x - m) * c) * inv; }
+  __device__ __forceinline__ double of(float x, double c) const { return x >= floor ? soft_exp(x, floor, m, c) * inv : 0; }
+  __device__ __forceinline__ void finish(double c) {
+    floor = floor_of(m, c);
+    inv = s > 0 ? 1 / s : 0;
+  }
 };
 
 // The sum of exp2((x - m) c) over a row's numbers [v0, v1), from c0 on; a
 // thread's m is any logit not far below its largest.
 template <class T, int NT, int U>
-__device__ __forceinline__ Soft soft_part(const typename T::raw* row, int lead, int c0, int v0, int v1, double c) {
+__device__ __forceinline__ Soft soft_part(const typename T::raw* row, int lead, int c0, int v0, int v1, double c,
+                                          float* shf, double* shd) {
   constexpr int E = Vec<T>::E, STEP = NT * U * E;
   Soft o;
   for (int base = c0; base < v1; base += STEP) {
@@ -73,23 +122,35 @@ __device__ __forceinline__ Soft soft_part(const typename T::raw* row, int lead, 
       v[u].keep();
     }
     if (((double)t - o.m) * c > 300) {
-      o.s *= exp2_64(((double)o.m - t) * c);
+      o.s *= exp2_64(fmax(((double)o.m - t) * c, -DEPTH));
       o.m = t;
+      o.floor = floor_of(t, c);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int e = 0; e < E; ++e) o.s += exp2_64(((double)v[u].get(e) - o.m) * c);
+      for (int e = 0; e < E; e += 4) {
+        double t[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[i] = ((double)max2(v[u].get(e + i), o.floor) - o.m) * c;
+        exp2_64(t);
+        o.s += (t[0] + t[1]) + (t[2] + t[3]);
+      }
   }
-  return o;
-}
-
-template <int NT>
-__device__ __forceinline__ Soft join(Soft o, double c, float* shf, double* shd) {
   const float m = block_reduce<NT, Max>(o.m, shf);
-  o.s = block_reduce<NT, Sum>(o.s * exp2_64(((double)o.m - m) * c), shd);
+  o.s = block_reduce<NT, Sum>(o.m > -1e38f ? o.s * exp2_64(fmax(((double)o.m - m) * c, -DEPTH)) : 0, shd);
   o.m = m;
-  o.inv = o.s > 0 ? 1 / o.s : 0;
+  if (m <= -1e38f) {
+    // nothing but -inf and the type's lowest value: of these the sum above
+    // made one
+    double s = 0;
+    for (int at = v0 + threadIdx.x; at < v1; at += NT) {
+      const float x = T::get(row[at - lead]);
+      if (x >= LOWEST) s += exp2_64(fmax(((double)x - m) * c, -DEPTH));
+    }
+    o.s = block_reduce<NT, Sum>(s, shd);
+  }
+  o.finish(c);
   return o;
 }
 
@@ -122,7 +183,25 @@ __device__ __forceinline__ void weigh(const Stop<T>& st, int vocab, int c0, int 
     else vy = vx;
     double s = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) s += st.weight(vx.get(e), vy.get(e), at + e - lead, c);
+    for (int e = 0; e < E; e += 4) {
+      double t[4], q[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[i] = ((double)max2(vx.get(e + i), st.p.floor) - st.p.m) * c;
+      exp2_64(t);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[i] = vx.get(e + i) >= st.p.floor ? t[i] * st.p.inv : 0;
+      if (st.minus && y) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[i] = ((double)max2(vy.get(e + i), st.q.floor) - st.q.m) * c;
+        exp2_64(q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[i] = fmax(t[i] - (vy.get(e + i) >= st.q.floor ? q[i] * st.q.inv : 0), 0.0);
+      } else if (st.minus) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[i] = at + e + i - lead == st.id ? fmax(t[i] - 1.0, 0.0) : t[i];
+      }
+      s += (t[0] + t[1]) + (t[2] + t[3]);
+    }
     s = wave_reduce<Sum>(s, 0.0);
     if ((threadIdx.x & 63) == 0 && at < v1) weight[at / (64 * E)] = s;
   }
@@ -232,7 +311,7 @@ __device__ __forceinline__ void write_tokens(const VerifyParams& p, int64_t b, i
 // Batches that fill the card: a block takes a sequence, row by row up to where
 // it stops; what lies behind is not read.
 template <class T, int NT, int U>
-__global__ __launch_bounds__(NT, 8) void lt_verify_walk(VerifyParams p) {
+__global__ __launch_bounds__(NT, 4) void lt_verify_walk(VerifyParams p) {
   __shared__ float shf[NT / 64];
   __shared__ double shd[NT / 64];
   __shared__ int shi[2];
@@ -244,7 +323,7 @@ __global__ __launch_bounds__(NT, 8) void lt_verify_walk(VerifyParams p) {
   for (;; ++a) {
     st.x = target_row<T>(p, b, a);
     int lead = lead_of<T>(st.x);
-    st.p = join<NT>(soft_part<T, NT, U>(st.x, lead, 0, lead, lead + V, p.c), p.c, shf, shd);
+    st.p = soft_part<T, NT, U>(st.x, lead, 0, lead, lead + V, p.c, shf, shd);
     st.y = nullptr;
     if (a == n) break;
     st.id = any_id(p.ids, b * p.drafts + a, p.ids_bytes);
@@ -253,7 +332,7 @@ __global__ __launch_bounds__(NT, 8) void lt_verify_walk(VerifyParams p) {
     if (p.draft.data) {
       st.y = draft_row<T>(p, b, a);
       lead = lead_of<T>(st.y);
-      st.q = join<NT>(soft_part<T, NT, U>(st.y, lead, 0, lead, lead + V, p.c), p.c, shf, shd);
+      st.q = soft_part<T, NT, U>(st.y, lead, 0, lead, lead + V, p.c, shf, shd);
       q = there ? st.q.of(T::get(st.y[st.id]), p.c) : 0.0;
     }
     st.minus = true;
@@ -285,32 +364,25 @@ __global__ __launch_bounds__(SMALL_NT) void lt_verify_sums(VerifyParams p) {
   const typename T::raw* x = target ? target_row<T>(p, b, i) : draft_row<T>(p, b, i);
   const int lead = lead_of<T>(x), c0 = (int)(blk - row * p.splits) * p.chunk;
   const int v1 = min(lead + p.target.vocab, c0 + p.chunk);
-  const Soft o = join<NT>(soft_part<T, NT, U>(x, lead, c0, max(lead, c0), v1, p.c), p.c, shf, shd);
+  const Soft o = soft_part<T, NT, U>(x, lead, c0, max(lead, c0), v1, p.c, shf, shd);
   if (threadIdx.x == 0) p.part[blk] = make_double2(o.m, o.s);
 }
-
-struct WalkShared {
-  int a;
-  float shf[SMALL_NT / 64];
-  double shd[SMALL_NT / 64];
-  int shi[2];
-};
 
 // A row's chunks, one after another.
 __device__ __forceinline__ Soft join_parts(const double2* part, int splits, double c) {
   Soft o;
   for (int i = 0; i < splits; ++i) o.m = fmaxf(o.m, (float)part[i].x);
-  for (int i = 0; i < splits; ++i) o.s += part[i].y * exp2_64((part[i].x - o.m) * c);
-  o.inv = o.s > 0 ? 1 / o.s : 0;
+  for (int i = 0; i < splits; ++i) o.s += part[i].y * exp2_64(fmax((part[i].x - o.m) * c, -DEPTH));
+  o.finish(c);
   return o;
 }
 
 // Where sequence b stops, from the chunks' sums (every block that needs it does
 // the same): a thread a place.
 template <class T>
-__device__ __forceinline__ Stop<T> find_stop(const VerifyParams& p, int64_t b, WalkShared& sh, int& a) {
+__device__ __forceinline__ Stop<T> find_stop(const VerifyParams& p, int64_t b, int* sh_a, int& a) {
   const int n = length_of(p, b), V = p.target.vocab;
-  if (threadIdx.x == 0) sh.a = n;
+  if (threadIdx.x == 0) *sh_a = n;
   __syncthreads();
   const int64_t targets = p.batch * (p.drafts + 1);
   for (int i0 = 0; i0 < n; i0 += SMALL_NT) {
@@ -324,11 +396,11 @@ __device__ __forceinline__ Stop<T> find_stop(const VerifyParams& p, int64_t b, W
         if (p.draft.data)
           qx = join_parts(p.part + (targets + b * p.drafts + i) * p.splits, p.splits, p.c).of(T::get(draft_row<T>(p, b, i)[id]), p.c);
       }
-      if (!(there && p.accept_u[b * p.drafts + i] * qx < px)) atomicMin(&sh.a, i);
+      if (!(there && p.accept_u[b * p.drafts + i] * qx < px)) atomicMin(sh_a, i);
     }
   }
   __syncthreads();
-  a = sh.a;
+  a = *sh_a;
   Stop<T> st;
   st.x = target_row<T>(p, b, a);
   st.p = join_parts(p.part + (b * (p.drafts + 1) + a) * p.splits, p.splits, p.c);
@@ -345,23 +417,39 @@ __device__ __forceinline__ Stop<T> find_stop(const VerifyParams& p, int64_t b, W
 
 template <class T>
 __global__ __launch_bounds__(SMALL_NT) void lt_verify_weigh(VerifyParams p) {
-  __shared__ WalkShared sh;
-  const int64_t blk = p.block0 + blockIdx.x, b = blk / p.splits;
+  __shared__ int sh_a;
+  const int64_t blk = p.block0 + blockIdx.x, b = blk / p.weigh_splits;
   int a;
-  const Stop<T> st = find_stop<T>(p, b, sh, a);
-  const int c0 = (int)(blk - b * p.splits) * p.chunk;
-  weigh<T, SMALL_NT>(st, p.target.vocab, c0, c0 + p.chunk, p.c, p.weight + b * p.segments);
+  const Stop<T> st = find_stop<T>(p, b, &sh_a, a);
+  const int split = (int)(blk - b * p.weigh_splits), c0 = split * p.weigh_chunk;
+  if (split == 0 && threadIdx.x == 0) p.stop[b] = StopNote{st.p.s, st.q.s, st.p.m, st.q.m, a, 0};
+  weigh<T, SMALL_NT>(st, p.target.vocab, c0, c0 + p.weigh_chunk, p.c, p.weight + b * p.segments);
 }
 
 template <class T>
 __global__ __launch_bounds__(SMALL_NT) void lt_verify_draw(VerifyParams p) {
-  __shared__ WalkShared sh;
+  __shared__ double shd[SMALL_NT / 64];
+  __shared__ int shi[2];
   const int64_t b = p.block0 + blockIdx.x;
-  int a;
-  Stop<T> st = find_stop<T>(p, b, sh, a);
+  const StopNote note = p.stop[b];
+  Stop<T> st;
+  st.x = target_row<T>(p, b, note.a);
+  st.p.m = note.pm;
+  st.p.s = note.ps;
+  st.p.finish(p.c);
+  if (note.a < length_of(p, b)) {
+    st.minus = true;
+    st.id = any_id(p.ids, b * p.drafts + note.a, p.ids_bytes);
+    if (p.draft.data) {
+      st.y = draft_row<T>(p, b, note.a);
+      st.q.m = note.qm;
+      st.q.s = note.qs;
+      st.q.finish(p.c);
+    }
+  }
   const int segments = (lead_of<T>(st.x) + p.target.vocab + 64 * Vec<T>::E - 1) / (64 * Vec<T>::E);
-  const int token = draw<T, SMALL_NT>(st, p.target.vocab, p.sample_u[b], p.c, p.weight + b * p.segments, segments, sh.shd, sh.shi);
-  write_tokens<SMALL_NT>(p, b, a, token);
+  const int token = draw<T, SMALL_NT>(st, p.target.vocab, p.sample_u[b], p.c, p.weight + b * p.segments, segments, shd, shi);
+  write_tokens<SMALL_NT>(p, b, note.a, token);
 }
 
 // ---- host ------------------------------------------------------------------
@@ -372,28 +460,39 @@ void plan(VerifyParams& p, int dtype) {
   const int64_t numbers = (int64_t)p.target.vocab + LEAD, rows = p.batch * (p.drafts + 1 + (p.draft.data ? p.drafts : 0));
   p.segments = (int32_t)((numbers + 64 * e - 1) / (64 * e));
   int64_t n = (numbers + step - 1) / step;
-  n = n < 2048 / rows ? n : 2048 / rows;
+#ifndef XB
+#define XB 8192
+#endif
+  n = n < XB / rows ? n : XB / rows;
   n = n > 1 ? n : 1;
   const int64_t steps = (numbers + n * step - 1) / (n * step);
   p.chunk = (int32_t)(steps * step);
   p.splits = (int32_t)((numbers + p.chunk - 1) / p.chunk);
+  const int vectors = SMALL_NT * e;
+  n = (numbers + vectors - 1) / vectors;
+  n = n < 2048 / p.batch ? n : 2048 / p.batch;
+  n = n > 1 ? n : 1;
+  p.weigh_chunk = (int32_t)((numbers + n * vectors - 1) / (n * vectors) * vectors);
+  p.weigh_splits = (int32_t)((numbers + p.weigh_chunk - 1) / p.weigh_chunk);
 }
 
 int64_t weights_bytes(const VerifyParams& p) { return (p.batch * p.segments * (int64_t)sizeof(double) + 15) / 16 * 16; }
 
+int64_t parts_bytes(const VerifyParams& p) { return p.batch * (2 * p.drafts + 1) * p.splits * (int64_t)sizeof(double2); }
+
 int64_t need_bytes(const VerifyParams& p) {
-  return weights_bytes(p) + (p.batch >= MANY ? 0 : p.batch * (2 * p.drafts + 1) * p.splits * (int64_t)sizeof(double2));
+  return weights_bytes(p) + (p.batch >= MANY ? 0 : parts_bytes(p) + p.batch * (int64_t)sizeof(StopNote));
 }
 
 template <class T>
 lt_status launch_verify(const VerifyParams& p, void* stream) {
   const char* what = "lt_verify_draft";
   if (p.batch >= MANY)
-    return p.target.vocab > 8192 ? launch(lt_verify_walk<T, 1024, 2>, p.batch, 1024, p, stream, what)
+    return p.target.vocab > 8192 ? launch(lt_verify_walk<T, 512, 2>, p.batch, 512, p, stream, what)
                                  : launch(lt_verify_walk<T, 256, 2>, p.batch, 256, p, stream, what);
   const int64_t rows = p.batch * (p.drafts + 1 + (p.draft.data ? p.drafts : 0));
   lt_status st = launch(lt_verify_sums<T, 4>, rows * p.splits, SMALL_NT, p, stream, what);
-  if (st == LT_OK) st = launch(lt_verify_weigh<T>, p.batch * p.splits, SMALL_NT, p, stream, what);
+  if (st == LT_OK) st = launch(lt_verify_weigh<T>, p.batch * p.weigh_splits, SMALL_NT, p, stream, what);
   return st != LT_OK ? st : launch(lt_verify_draw<T>, p.batch, SMALL_NT, p, stream, what);
 }
 
@@ -449,6 +548,7 @@ lt_status lt_verify_draft(const lt_draft* d, double temperature, int64_t* tokens
     BAD("workspace: %lld bytes, 16 B aligned, are needed", (long long)need_bytes(p));
   p.weight = (double*)workspace;
   p.part = (double2*)((char*)workspace + weights_bytes(p));
+  p.stop = (StopNote*)((char*)p.part + parts_bytes(p));
   p.c = LOG2E / temperature;
   p.tokens = tokens;
   p.accepted = accepted;
