@@ -98,14 +98,16 @@ typedef struct {
 int64_t lt_distill_workspace(const lt_rows* z, int32_t entries);
 lt_status lt_distill_forward(const lt_rows* z, const lt_teacher* t, double temperature, float* loss, float* stats,
                              void* workspace, int64_t workspace_bytes, void* stream);
-/* grad: rows as z (its data, strides; same dtype and vocab) = weight[r * weight_stride] * d loss_r / d z.
+/* grad: rows as z (its data, strides; same dtype and vocab) =
+ * scale * weight[r * weight_stride] * d loss_r / d z; weight NULL: 1.
  * stats as the forward of the same arguments left them.  weight_stride 0 or 1. */
 lt_status lt_distill_backward(const lt_rows* z, const lt_teacher* t, double temperature, const float* stats,
-                              const float* weight, int64_t weight_stride, const lt_rows* grad, void* stream);
-/* Both at once, the logits read once where a row fits a block's registers. */
-lt_status lt_distill_fused(const lt_rows* z, const lt_teacher* t, double temperature, const float* weight,
-                           int64_t weight_stride, float* loss, const lt_rows* grad, void* workspace,
-                           int64_t workspace_bytes, void* stream);
+                              double scale, const float* weight, int64_t weight_stride, const lt_rows* grad,
+                              void* stream);
+/* Both at once. */
+lt_status lt_distill_fused(const lt_rows* z, const lt_teacher* t, double temperature, double scale,
+                           const float* weight, int64_t weight_stride, float* loss, const lt_rows* grad,
+                           void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---- verification of drafted tokens ----------------------------------------
  * target: rows = batch * (drafts + 1), row b * (drafts + 1) + i the target's

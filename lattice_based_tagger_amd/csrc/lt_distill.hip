@@ -23,11 +23,16 @@ struct DistillParams {
   float* loss;
   float* stats;           // [rows][LT_DISTILL_STATS]: m, the gradient's factors of exp2((z - m) c)
   float4* part;           // splits > 1: [rows][splits] reference, sums within and outside the entries
-  const float* weight;
+  float scale;
+  const float* weight;    // NULL: 1
   int64_t weight_stride;
   Rows grad;
   bool past;              // the gradient is written past the caches
 };
+
+__device__ __forceinline__ float weight_of(const DistillParams& p, int64_t r) {
+  return p.weight ? p.scale * p.weight[r * p.weight_stride] : p.scale;
+}
 
 // What a block (or a wave with a row of its own) keeps in LDS: the entries, and
 // a bit for each logit of a window that says whether it is one.
@@ -309,7 +314,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_distill_grad(DistillPa
   GROUP_HEAD;
   const float4 st = *(const float4*)(p.stats + r * LT_DISTILL_STATS);
   grad_row<T, NT, U, WINDOW, false>(z, (typename T::raw*)p.grad.data + p.grad.at(r), lead, c0, v0, v1, p.c,
-                                    make_float3(st.x, st.y, st.z), p.weight[r * p.weight_stride], p.inv_t, t, sh,
+                                    make_float3(st.x, st.y, st.z), weight_of(p, r), p.inv_t, t, sh,
                                     p.t.entries, p.past);
 }
 
@@ -325,7 +330,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, NT == 64 ? 1 : 8) void lt_dist
   const float3 st = finish_row<T, NT>(t, z, o, p.inv_t, sh.sh, loss);
   if (thread_of<NT>() == 0) p.loss[r] = loss;
   grad_row<T, NT, U, WINDOW, true>(z, (typename T::raw*)p.grad.data + p.grad.at(r), lead, c0, v0, v1, p.c, st,
-                                   p.weight[r * p.weight_stride], p.inv_t, t, sh, p.t.entries, p.past);
+                                   weight_of(p, r), p.inv_t, t, sh, p.t.entries, p.past);
 }
 
 // Rows of at most FEW logits: a thread a row, the row in LDS, its entries a
@@ -398,7 +403,7 @@ __global__ __launch_bounds__(64) void lt_distill_few(DistillParams p) {
     }
   }
   if (GRAD) {
-    const float w = p.weight[r * p.weight_stride];
+    const float w = weight_of(p, r);
     if (lane < rows) {
       for (int i = 0; i < vocab; ++i) z[i] = exp2_((z[i] - m) * p.c) * (mask >> i & 1 ? fin : fout);
       for (int j = 0; j < n; ++j)
@@ -479,12 +484,13 @@ lt_status distill_check(const lt_rows* z, const lt_teacher* t, double temperatur
   return LT_OK;
 }
 
-lt_status grad_check(const lt_rows* z, const lt_rows* g, const float* weight, int64_t weight_stride) {
+lt_status grad_check(const lt_rows* z, const lt_rows* g, double scale, int64_t weight_stride) {
   lt_status st;
   if (!rows_ok(g, "grad", &st)) return st;
   if (g->rows != z->rows || g->vocab != z->vocab || g->dtype != z->dtype || g->device != z->device)
     BAD("grad: not the logits' rows, vocab, dtype and device");
-  if (z->rows > 0 && !weight) BAD("weight: NULL");
+  if (z->rows > 0 && !g->data) BAD("grad: NULL");
+  if (!isfinite(scale)) BAD("scale %g", scale);
   if (weight_stride != 0 && weight_stride != 1) BAD("weight_stride %lld", (long long)weight_stride);
   return LT_OK;
 }
@@ -537,13 +543,15 @@ lt_status lt_distill_forward(const lt_rows* z, const lt_teacher* t, double tempe
 }
 
 lt_status lt_distill_backward(const lt_rows* z, const lt_teacher* t, double temperature, const float* stats,
-                              const float* weight, int64_t weight_stride, const lt_rows* grad, void* stream) {
+                              double scale, const float* weight, int64_t weight_stride, const lt_rows* grad,
+                              void* stream) {
   lt_status st = distill_check(z, t, temperature);
-  if (st == LT_OK) st = grad_check(z, grad, weight, weight_stride);
+  if (st == LT_OK) st = grad_check(z, grad, scale, weight_stride);
   if (st != LT_OK || z->rows == 0) return st;
   if (!stats || (uintptr_t)stats % 16) BAD("stats: NULL or not 16 B aligned");
   DistillParams p = distill_params(z, t, temperature);
   p.stats = const_cast<float*>(stats);
+  p.scale = (float)scale;
   p.weight = weight;
   p.weight_stride = weight_stride;
   p.grad = rows_of(grad);
@@ -551,11 +559,11 @@ lt_status lt_distill_backward(const lt_rows* z, const lt_teacher* t, double temp
   return launch_pass(p, z->dtype, GRAD, stream, "lt_distill_backward");
 }
 
-lt_status lt_distill_fused(const lt_rows* z, const lt_teacher* t, double temperature, const float* weight,
-                           int64_t weight_stride, float* loss, const lt_rows* grad, void* workspace,
-                           int64_t workspace_bytes, void* stream) {
+lt_status lt_distill_fused(const lt_rows* z, const lt_teacher* t, double temperature, double scale,
+                           const float* weight, int64_t weight_stride, float* loss, const lt_rows* grad,
+                           void* workspace, int64_t workspace_bytes, void* stream) {
   lt_status st = distill_check(z, t, temperature);
-  if (st == LT_OK) st = grad_check(z, grad, weight, weight_stride);
+  if (st == LT_OK) st = grad_check(z, grad, scale, weight_stride);
   if (st != LT_OK || z->rows == 0) return st;
   if (!loss) BAD("output: NULL");
   DistillParams p = distill_params(z, t, temperature);
@@ -563,6 +571,7 @@ lt_status lt_distill_fused(const lt_rows* z, const lt_teacher* t, double tempera
   p.part = (float4*)workspace;
   p.loss = loss;
   p.stats = workspace ? (float*)((char*)workspace + parts_bytes(p)) : nullptr;
+  p.scale = (float)scale;
   p.weight = weight;
   p.weight_stride = weight_stride;
   p.grad = rows_of(grad);

@@ -1,12 +1,15 @@
 // lt_verify.hip -- the verification of drafted tokens
 // (include/lattice_logits.h lt_verify_draft).
 //
-// A token is drawn where a running sum over the vocabulary crosses a line, so a
-// relative error e of the sums moves it with a probability of about e times the
-// number of tokens that the line may fall beside: 131072 e.  A float32
-// exponential (1e-7) would move one in a hundred; all sums are held in 64 bits
-// and the exponential is good to 1.1e-12.  It is what bounds these kernels: 18
-// instructions a logit, where memory would allow 14.
+// A drafted token is accepted by comparing two probabilities with a random
+// number: from sums in 32 bits, unless the two are within these sums' error
+// (some 2e-5) of each other; then the rows are summed again in 64 bits.  A token
+// is drawn where a running sum over the vocabulary crosses a
+// line, so a relative error e of the sums moves it with a probability of about
+// e times the number of tokens that the line may fall beside, 131072 e: the
+// one or two rows that it is drawn from are summed in 64 bits with an
+// exponential good to 1.1e-12.  That costs 35 issue slots a logit (a 64-bit
+// operation takes two), where memory allows 14; the sums in 32 bits take 9.
 #include "lt_logits.h"
 
 namespace {
@@ -66,10 +69,9 @@ __device__ __forceinline__ double soft_exp(float x, float floor, double m, doubl
   return exp2_64(((double)max2(x, floor) - m) * c);
 }
 
-// Where a sequence stops, for the kernels that follow.
+// Where a sequence stops and what its next token is drawn by, for the last kernel.
 struct StopNote {
-  double ps, qs;          // sums of the target's row, of the drafter's
-  float pm, qm;
+  float pm, qm;           // references of the target's row, of the drafter's
   int32_t a, pad;
 };
 
@@ -83,138 +85,348 @@ struct VerifyParams {
   int64_t batch;
   int32_t drafts, ids_bytes;
   double c;               // log2(e) / temperature
+  double margin;          // relative error of two probabilities by the sums in 32 bits
   int64_t* tokens;
   int64_t* accepted;
+  int32_t rounds;         // a launch for every place of the drafts; else one for all
+  int32_t place;          // of this launch
   int32_t splits, chunk;  // blocks of a row, a block's numbers of it
   int32_t segments;       // of a row: 64 vectors each
   int32_t weigh_splits, weigh_chunk;       // of the row that the token is drawn from
-  double* weight;         // [batch][segments]: the weights' sums
-  struct StopNote* stop;  // [batch]
-  double2* part;          // [batch * (2 drafts + 1)][splits]: reference and sum, targets first
+  float2* part;           // [batch * (2 drafts + 1)][splits]: reference and sum, targets first
+  double2* weight;        // [batch][segments]: sums of e_p and e_q where p > q
+  double2* sums;          // [batch][weigh_splits]: sums of e_p and e_q
+  int32_t* stopped;       // [batch], rounds: the place of the first token not accepted, or -1
+  StopNote* stop;         // [batch]
 };
 
-// A row's softmax: exp2((x - m) c) * inv, inv 0 for a row of -inf; 0 below the
-// floor.
-struct Soft {
-  float m = LOWEST, floor = LOWEST;
-  double s = 0, inv = 0;
-  __device__ __forceinline__ double of(float x, double c) const { return x >= floor ? soft_exp(x, floor, m, c) * inv : 0; }
-  __device__ __forceinline__ void finish(double c) {
-    floor = floor_of(m, c);
-    inv = s > 0 ? 1 / s : 0;
-  }
-};
+constexpr int NT = 256;
 
-// The sum of exp2((x - m) c) over a row's numbers [v0, v1), from c0 on; a
-// thread's m is any logit not far below its largest.
-template <class T, int NT, int U>
-__device__ __forceinline__ Soft soft_part(const typename T::raw* row, int lead, int c0, int v0, int v1, double c,
-                                          float* shf, double* shd) {
+// The sum of exp2((x - m) c) over a row's numbers [v0, v1), from c0 on, in 32
+// bits; a thread's m is any logit not far below its largest.
+template <class T, int U>
+__device__ __forceinline__ float2 sum_part(const typename T::raw* row, int lead, int c0, int v0, int v1, float c, float* shf) {
   constexpr int E = Vec<T>::E, STEP = NT * U * E;
-  Soft o;
+  float m = LOWEST, s = 0.f;
   for (int base = c0; base < v1; base += STEP) {
     Vec<T> v[U];
     load_step<T, NT, U>(v, row - lead, base, threadIdx.x, v0, v1);
-    float t = LOWEST;
+    float t = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       t = max2(t, max_of(v[u]));
       v[u].keep();
     }
-    if (((double)t - o.m) * c > 300) {
-      o.s *= exp2_64(fmax(((double)o.m - t) * c, -DEPTH));
-      o.m = t;
-      o.floor = floor_of(t, c);
+    if ((t - m) * c > 32.f) {
+      s *= exp2_((m - t) * c);
+      m = t;
     }
+    float s0 = 0.f, s1 = 0.f;
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int e = 0; e < E; e += 4) {
-        double t[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) t[i] = ((double)max2(v[u].get(e + i), o.floor) - o.m) * c;
-        exp2_64(t);
-        o.s += (t[0] + t[1]) + (t[2] + t[3]);
+      for (int e = 0; e < E; e += 2) {
+        const float f0 = exp2_((v[u].get(e) - m) * c), f1 = exp2_((v[u].get(e + 1) - m) * c);
+        s0 += f0;
+        s1 += f1;
       }
+    s += s0 + s1;
   }
-  const float m = block_reduce<NT, Max>(o.m, shf);
-  o.s = block_reduce<NT, Sum>(o.m > -1e38f ? o.s * exp2_64(fmax(((double)o.m - m) * c, -DEPTH)) : 0, shd);
-  o.m = m;
-  if (m <= -1e38f) {
-    // nothing but -inf and the type's lowest value: of these the sum above
-    // made one
-    double s = 0;
-    for (int at = v0 + threadIdx.x; at < v1; at += NT) {
-      const float x = T::get(row[at - lead]);
-      if (x >= LOWEST) s += exp2_64(fmax(((double)x - m) * c, -DEPTH));
-    }
-    o.s = block_reduce<NT, Sum>(s, shd);
-  }
-  o.finish(c);
-  return o;
+  const float top = block_reduce<NT, Max>(m, shf);
+  return make_float2(top, block_reduce<NT, Sum>(s * exp2_((m - top) * c), shf));
 }
 
-// Where a sequence stops: its rows there, and what the next token is drawn by.
-template <class T>
-struct Stop {
-  const typename T::raw *x = nullptr, *y = nullptr;        // the target's row; the drafter's
-  Soft p, q;
-  int64_t id = -1;        // the token that was not accepted
-  bool minus = false;     // weight max(p - q, 0); else p
-  __device__ __forceinline__ double weight(float fx, float fy, int v, double c) const {
-    const double w = p.of(fx, c);
-    if (!minus) return w;
-    return fmax(w - (y ? q.of(fy, c) : v == id ? 1.0 : 0.0), 0.0);
+// A row's softmax in 32 bits: exp2((x - m) c) / s.
+struct Soft {
+  float m = LOWEST;
+  double s = 0;
+  __device__ __forceinline__ double of(float x, double c) const {
+    const double t = ((double)x - m) * c;
+    return s > 0 && t > -DEPTH ? exp2_64(t) / s : 0;
   }
 };
 
-// The weights' sums of 64 vectors each, of the numbers [v0, v1) from c0 on.
-template <class T, int NT>
-__device__ __forceinline__ void weigh(const Stop<T>& st, int vocab, int c0, int c1, double c, double* weight) {
+// A row's chunks, one after another.
+__device__ __forceinline__ Soft join_parts(const float2* part, int splits, double c) {
+  Soft o;
+  for (int i = 0; i < splits; ++i) o.m = fmaxf(o.m, part[i].x);
+  for (int i = 0; i < splits; ++i) o.s += part[i].y * exp2_64(fmax(((double)part[i].x - o.m) * c, -DEPTH));
+  return o;
+}
+
+template <class T>
+__device__ __forceinline__ const typename T::raw* target_row(const VerifyParams& p, int64_t b, int i) {
+  return (const typename T::raw*)p.target.data + p.target.at(b * (p.drafts + 1) + i);
+}
+template <class T>
+__device__ __forceinline__ const typename T::raw* draft_row(const VerifyParams& p, int64_t b, int i) {
+  return (const typename T::raw*)p.draft.data + p.draft.at(b * p.drafts + i);
+}
+__device__ __forceinline__ int length_of(const VerifyParams& p, int64_t b) {
+  return p.lengths ? max(0, min(p.lengths[b], p.drafts)) : p.drafts;
+}
+__device__ __forceinline__ Soft target_soft(const VerifyParams& p, int64_t b, int i) {
+  return join_parts(p.part + (b * (p.drafts + 1) + i) * p.splits, p.splits, p.c);
+}
+__device__ __forceinline__ Soft draft_soft(const VerifyParams& p, int64_t b, int i) {
+  return join_parts(p.part + (p.batch * (p.drafts + 1) + b * p.drafts + i) * p.splits, p.splits, p.c);
+}
+
+// Whether token i of sequence b is accepted: by its rows' sums in 32 bits; CLOSE
+// where these leave it open.
+enum Verdict { REFUSED, ACCEPTED, CLOSE };
+template <class T>
+__device__ __forceinline__ Verdict accepts(const VerifyParams& p, int64_t b, int i) {
+  const int64_t id = any_id(p.ids, b * p.drafts + i, p.ids_bytes);
+  if (id < 0 || id >= p.target.vocab) return REFUSED;
+  const double px = target_soft(p, b, i).of(T::get(target_row<T>(p, b, i)[id]), p.c);
+  const double qx = p.draft.data ? draft_soft(p, b, i).of(T::get(draft_row<T>(p, b, i)[id]), p.c) : 1.0;
+  const double line = p.accept_u[b * p.drafts + i] * qx;
+  if (fabs(px - line) <= p.margin * px && px > 0) return CLOSE;
+  return line < px ? ACCEPTED : REFUSED;
+}
+
+// The sum of exp2((x - m) c) of a row in 64 bits, by the block.
+template <class T>
+__device__ __forceinline__ double sum_row(const typename T::raw* row, int vocab, float m, double c, double* shd) {
   constexpr int E = Vec<T>::E;
-  const int lead = lead_of<T>(st.x), v1 = min(c1, lead + vocab);
-  const typename T::raw* const x = st.x - lead;
-  const typename T::raw* const y = st.y ? st.y - lead : nullptr;       // (at any address)
-  for (int base = c0; base < v1; base += NT * E) {
-    const int at = base + threadIdx.x * E;
-    Vec<T> vx, vy;
-    vx.load(x, at, lead, lead + vocab, T::put(-INFINITY));
-    if (st.minus && y) vy.load(y, at, lead, lead + vocab, T::put(-INFINITY));
-    else vy = vx;
-    double s = 0;
-#pragma unroll
+  const int lead = lead_of<T>(row);
+  const float floor = floor_of(m, c);
+  double s = 0;
+  for (int at = threadIdx.x * E; at < lead + vocab; at += NT * E) {
+    Vec<T> v;
+    v.load(row - lead, at, lead, lead + vocab, T::put(-INFINITY));
+#pragma nounroll
     for (int e = 0; e < E; e += 4) {
-      double t[4], q[4];
+      double t[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) t[i] = ((double)max2(vx.get(e + i), st.p.floor) - st.p.m) * c;
-      exp2_64(t);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) t[i] = vx.get(e + i) >= st.p.floor ? t[i] * st.p.inv : 0;
-      if (st.minus && y) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) q[i] = ((double)max2(vy.get(e + i), st.q.floor) - st.q.m) * c;
-        exp2_64(q);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) t[i] = fmax(t[i] - (vy.get(e + i) >= st.q.floor ? q[i] * st.q.inv : 0), 0.0);
-      } else if (st.minus) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) t[i] = at + e + i - lead == st.id ? fmax(t[i] - 1.0, 0.0) : t[i];
+      for (int i = 0; i < 4; ++i) {
+        const float x = E == 4 || e == 0 ? v.get(i) : v.get(E == 4 ? i : i + 4);
+        t[i] = x >= floor ? ((double)x - m) * c : -DEPTH;
       }
+      exp2_64(t);
       s += (t[0] + t[1]) + (t[2] + t[3]);
     }
-    s = wave_reduce<Sum>(s, 0.0);
-    if ((threadIdx.x & 63) == 0 && at < v1) weight[at / (64 * E)] = s;
+  }
+  return block_reduce<NT, Sum>(s, shd);
+}
+
+// The same by sums in 64 bits, by the block.
+template <class T>
+__device__ __forceinline__ bool accepts_exactly(const VerifyParams& p, int64_t b, int i, double* shd) {
+  const int id = (int)any_id(p.ids, b * p.drafts + i, p.ids_bytes);
+  double ratio = p.accept_u[b * p.drafts + i];             // u q / p
+#pragma nounroll
+  for (int side = 0; side < (p.draft.data ? 2 : 1); ++side) {
+    const typename T::raw* x = side ? draft_row<T>(p, b, i) : target_row<T>(p, b, i);
+    const float m = (side ? draft_soft(p, b, i) : target_soft(p, b, i)).m;
+    const double e = exp2_64(fmax(((double)T::get(x[id]) - m) * p.c, -DEPTH)), s = sum_row<T>(x, p.target.vocab, m, p.c, shd);
+    ratio = side ? ratio * (e / s) : ratio / (e / s);
+  }
+  return ratio < 1;
+}
+
+// Chunks' sums: of every row that counts, or in rounds of those of one place,
+// where every block first sees whether the token ahead of it was accepted.
+template <class T, int U, bool ROUNDS>
+__global__ __launch_bounds__(NT) void lt_verify_sums(VerifyParams p) {
+  __shared__ float shf[NT / 64];
+  const int64_t blk = p.block0 + blockIdx.x, row = blk / p.splits;
+  const int split = (int)(blk - row * p.splits);
+  const int64_t targets = ROUNDS ? p.batch : p.batch * (p.drafts + 1);
+  const bool target = row < targets;
+  const int64_t of = target ? row : row - targets, places = ROUNDS ? 1 : target ? p.drafts + 1 : p.drafts;
+  const int64_t b = of / places;
+  const int i = ROUNDS ? p.place : (int)(of - b * places), n = length_of(p, b);
+  if (target ? i > n : i >= n) return;
+  if constexpr (ROUNDS) {
+    const bool writes = target && split == 0 && threadIdx.x == 0;
+    __shared__ double shd[NT / 64];
+    if (i == 0) {
+      if (writes) p.stopped[b] = -1;
+    } else {
+      // (a block of this launch may write it, but only what this one finds too)
+      const int at = p.stopped[b];
+      if (at >= 0 && at < i - 1) return;
+      const Verdict v = accepts<T>(p, b, i - 1);
+      if (v == REFUSED || (v == CLOSE && !accepts_exactly<T>(p, b, i - 1, shd))) {
+        if (writes) p.stopped[b] = i - 1;
+        return;
+      }
+    }
+  }
+  const typename T::raw* x = target ? target_row<T>(p, b, i) : draft_row<T>(p, b, i);
+  const int lead = lead_of<T>(x), c0 = split * p.chunk, v1 = min(lead + p.target.vocab, c0 + p.chunk);
+  const float2 o = sum_part<T, U>(x, lead, c0, max(lead, c0), v1, (float)p.c, shf);
+  if (threadIdx.x == 0) p.part[((target ? b * (p.drafts + 1) : p.batch * (p.drafts + 1) + b * p.drafts) + i) * p.splits + split] = o;
+}
+
+// The place where sequence b stops.  (One launch for all: from the sums, a
+// thread a place.)
+template <class T>
+__device__ __forceinline__ int find_stop(const VerifyParams& p, int64_t b, int* sh_a, int* sh_close, double* shd) {
+  const int n = length_of(p, b);
+  if (p.rounds) {
+    const int at = p.stopped[b];
+    return at < 0 ? n : at;
+  }
+  for (int from = 0;;) {
+    if (threadIdx.x == 0) *sh_a = *sh_close = n;
+    __syncthreads();
+    for (int i = from + threadIdx.x; i < n; i += NT) {
+      const Verdict v = accepts<T>(p, b, i);
+      if (v == REFUSED) atomicMin(sh_a, i);
+      if (v == CLOSE) atomicMin(sh_close, i);
+    }
+    __syncthreads();
+    const int a = *sh_a, close = *sh_close;
+    __syncthreads();
+    if (close >= a) return a;              // (both n: none)
+    if (!accepts_exactly<T>(p, b, close, shd)) return close;
+    from = close + 1;
   }
 }
 
-// The token: the first whose running sum of weights passes u of the whole,
-// else the last with a weight.  All of a block gets it.
-template <class T, int NT>
-__device__ __forceinline__ int draw(Stop<T>& st, int vocab, float u, double c, const double* weight, int segments,
-                                    double* shd, int* shi) {
+// What the next token is drawn by: e_p, or max(e_p - ratio e_q, 0), e_p and e_q
+// the exponentials of the target's and the drafter's logits and ratio the
+// quotient of their sums -- a multiple of max(p - q, 0); without a drafter's
+// row, e_p of all but the token that was not accepted.
+template <class T>
+struct Stop {
+  const typename T::raw *x = nullptr, *y = nullptr;
+  float pm = LOWEST, qm = LOWEST, pfloor = LOWEST, qfloor = LOWEST;
+  int id = -1;
+  double ratio = 0;
+  __device__ __forceinline__ void floors(double c) {
+    pfloor = floor_of(pm, c);
+    qfloor = floor_of(qm, c);
+  }
+  __device__ __forceinline__ double ep(float f, double c) const { return f >= pfloor ? soft_exp(f, pfloor, pm, c) : 0; }
+  __device__ __forceinline__ double eq(float f, double c) const { return f >= qfloor ? soft_exp(f, qfloor, qm, c) : 0; }
+  __device__ __forceinline__ double weight(int v, double c) const {
+    if (v == id) return 0;
+    const double w = ep(T::get(x[v]), c);
+    return y ? fmax(w - ratio * eq(T::get(y[v]), c), 0.0) : w;
+  }
+};
+
+template <class T>
+__device__ __forceinline__ Stop<T> stop_at(const VerifyParams& p, int64_t b, int a) {
+  Stop<T> st;
+  st.x = target_row<T>(p, b, a);
+  if (a < length_of(p, b)) {
+    if (p.draft.data) {
+      st.y = draft_row<T>(p, b, a);
+    } else {
+      const int64_t id = any_id(p.ids, b * p.drafts + a, p.ids_bytes);
+      st.id = id >= 0 && id < p.target.vocab ? (int)id : -1;
+    }
+  }
+  return st;
+}
+
+// One pass in 64 bits over the rows that the token is drawn from: the sums of
+// e_p and e_q of all, and of 64 vectors each where e_p > ratio e_q, ratio as the
+// sums in 32 bits give it.  (With the exact ratio, known when all is summed, a
+// segment's weight is then e_p - ratio e_q of its two sums: a token that the
+// ratio's last bits would put on the other side has no weight to speak of.)
+template <class T>
+__global__ __launch_bounds__(NT) void lt_verify_weigh(VerifyParams p) {
+  constexpr int E = Vec<T>::E;
+  __shared__ int sh_a, sh_close;
+  __shared__ double shd[NT / 64];
+  const int64_t blk = p.block0 + blockIdx.x, b = blk / p.weigh_splits;
+  const int split = (int)(blk - b * p.weigh_splits), c0 = split * p.weigh_chunk;
+  const int a = find_stop<T>(p, b, &sh_a, &sh_close, shd);
+  Stop<T> st = stop_at<T>(p, b, a);
+  const Soft ps = target_soft(p, b, a);
+  st.pm = ps.m;
+  if (st.y) {
+    const Soft qs = draft_soft(p, b, a);
+    st.qm = qs.m;
+    st.ratio = qs.s > 0 ? ps.s / qs.s : 0;
+  }
+  st.floors(p.c);
+  if (split == 0 && threadIdx.x == 0) p.stop[b] = StopNote{st.pm, st.qm, a, 0};
+  const int lead = lead_of<T>(st.x), end = lead + p.target.vocab, v1 = min(c0 + p.weigh_chunk, end);
+  const typename T::raw* const x = st.x - lead;
+  const typename T::raw* const y = st.y ? st.y - lead : nullptr;       // (at any address)
+  double sp = 0, sq = 0;
+  for (int base = c0; base < v1; base += NT * E) {
+    const int at = base + threadIdx.x * E;
+    Vec<T> vx, vy;
+    vx.load(x, at, lead, end, T::put(-INFINITY));
+    if (y) vy.load(y, at, lead, end, T::put(-INFINITY));
+    double wp = 0, wq = 0;
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+      double t[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[i] = ((double)max2(vx.get(e + i), st.pfloor) - st.pm) * p.c;
+      exp2_64(t);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[i] = vx.get(e + i) >= st.pfloor ? t[i] : 0;
+      sp += (t[0] + t[1]) + (t[2] + t[3]);
+      if (y) {
+        double q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[i] = ((double)max2(vy.get(e + i), st.qfloor) - st.qm) * p.c;
+        exp2_64(q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          q[i] = vy.get(e + i) >= st.qfloor ? q[i] : 0;
+          sq += q[i];
+          const bool more = t[i] > st.ratio * q[i];
+          wp += more ? t[i] : 0;
+          wq += more ? q[i] : 0;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) wp += at + e + i - lead == st.id ? 0 : t[i];
+      }
+    }
+    wp = wave_reduce<Sum>(wp, 0.0);
+    if (y) wq = wave_reduce<Sum>(wq, 0.0);
+    if ((threadIdx.x & 63) == 0 && at < v1) p.weight[b * p.segments + at / (64 * E)] = make_double2(wp, wq);
+  }
+  sp = block_reduce<NT, Sum>(sp, shd);
+  if (y) sq = block_reduce<NT, Sum>(sq, shd);
+  if (threadIdx.x == 0) p.sums[blk] = make_double2(sp, sq);
+}
+
+// The token: the first whose running sum of weights passes u of the whole, else
+// the last with a weight; where all weights are 0 (p and q alike), drawn by p.
+template <class T>
+__global__ __launch_bounds__(NT) void lt_verify_draw(VerifyParams p) {
   constexpr int SEG = 64 * Vec<T>::E;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lead = lead_of<T>(st.x);
-  // sums of the segments, `before` each NT of them, in their order
+  __shared__ double shd[NT / 64];
+  __shared__ int first, last;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t b = p.block0 + blockIdx.x;
+  const StopNote note = p.stop[b];
+  Stop<T> st = stop_at<T>(p, b, note.a);
+  st.pm = note.pm;
+  st.qm = note.qm;
+  st.floors(p.c);
+  const int lead = lead_of<T>(st.x), end = lead + p.target.vocab, segments = (end + SEG - 1) / SEG;
+  double sp = 0, sq = 0;
+  for (int i = tid; i < p.weigh_splits; i += NT) {
+    const double2 s = p.sums[b * p.weigh_splits + i];
+    sp += s.x;
+    sq += s.y;
+  }
+  sp = block_reduce<NT, Sum>(sp, shd);
+  if (st.y) {
+    sq = block_reduce<NT, Sum>(sq, shd);
+    st.ratio = sq > 0 ? sp / sq : 0;
+  }
+  const double2* weights = p.weight + b * p.segments;
+  auto segment = [&](int s) {
+    if (s >= segments) return 0.0;
+    const double2 w = weights[s];
+    return st.y ? fmax(w.x - st.ratio * w.y, 0.0) : w.x;
+  };
+  // running sums over a block's threads, `before` ahead of them; all: the last's
   auto scan = [&](double w, double before, double& all) {
     double cum = wave_scan<Sum>(w, 0.0);
     if (lane == 63) shd[wave] = cum;
@@ -229,271 +441,121 @@ __device__ __forceinline__ int draw(Stop<T>& st, int vocab, float u, double c, c
     __syncthreads();
     return cum;
   };
-  double total = 0;
-  for (int s0 = 0; s0 < segments; s0 += NT) total += s0 + tid < segments ? weight[s0 + tid] : 0.0;
-  total = block_reduce<NT, Sum>(total, shd);
-  int begin = lead, end = lead + vocab;
-  double before = 0;
-  const bool whole = !(total > 0);         // p and q alike: then it is drawn by p
-  if (whole) {
-    st.minus = false;
-    total = st.p.inv > 0 ? 1 : 0;
-  }
-  const double line = u * total;
-  if (!whole) {
-    if (tid == 0) shi[0] = 0x7fffffff, shi[1] = -1;
+  // The first of [from, to) whose sum passes the line, else the last with a
+  // weight, else -1; and the sum ahead of it.
+  auto cross = [&](int from, int to, double line, double& before, auto weight) {
+    if (tid == 0) first = 0x7fffffff, last = -1;
     __syncthreads();
-    double ahead = 0;
-    for (int s0 = 0; s0 < segments; s0 += NT) {
-      const int s = s0 + tid;
-      const double w = s < segments ? weight[s] : 0.0;
+    for (int i0 = from; i0 < to; i0 += NT) {
+      const double w = i0 + tid < to ? weight(i0 + tid) : 0.0;
       double all;
-      const double cum = scan(w, ahead, all);
+      const double cum = scan(w, before, all);
       if (w > 0) {
-        if (cum > line) atomicMin(&shi[0], s);
-        atomicMax(&shi[1], s);
+        if (cum > line) atomicMin(&first, i0 + tid);
+        atomicMax(&last, i0 + tid);
       }
+      __syncthreads();
+      if (first != 0x7fffffff) break;
+      before = all;
+    }
+    __syncthreads();
+    const int at = first != 0x7fffffff ? first : last;
+    __syncthreads();
+    return at;
+  };
+  double total = 0;
+  for (int s = tid; s < segments; s += NT) total += segment(s);
+  total = block_reduce<NT, Sum>(total, shd);
+  auto of_token = [&](int v) { return st.weight(v, p.c); };
+  int token = -1;
+  if (total > 0) {
+    const double line = p.sample_u[b] * total;
+    double before = 0;
+    const int s = cross(0, segments, line, before, segment);
+    // (ahead of segment s: what lies in the steps before its own, and in its own)
+    double ahead = 0, all;
+    for (int s0 = 0; s0 < s; s0 += NT) {
+      (void)scan(s0 + tid < s ? segment(s0 + tid) : 0.0, ahead, all);
       ahead = all;
     }
-    __syncthreads();
-    const int s = shi[0] != 0x7fffffff ? shi[0] : shi[1];
-    __syncthreads();
-    // what lies before it, summed as above
-    double part = 0;
-    for (int s0 = 0; s0 < s; s0 += NT) {
-      double all;
-      (void)scan(s0 + tid < s ? weight[s0 + tid] : 0.0, part, all);
-      part = all;
+    token = cross(max(0, s * SEG - lead), min(p.target.vocab, (s + 1) * SEG - lead), line, ahead, of_token);
+    if (token < 0) {
+      before = 0;                          // (a segment of rounding errors)
+      token = cross(0, p.target.vocab, line, before, of_token);
     }
-    before = part;
-    begin = max(begin, s * SEG);
-    end = min(end, (s + 1) * SEG);
   }
-  if (tid == 0) shi[0] = 0x7fffffff, shi[1] = -1;
-  __syncthreads();
-  for (int base = begin; base < end; base += NT) {
-    const int at = base + tid, v = at - lead;
-    double w = 0;
-    if (at < end) w = st.weight(T::get(st.x[v]), st.y ? T::get(st.y[v]) : 0.f, v, c);
-    double all;
-    const double cum = scan(w, before, all);
-    if (w > 0) {
-      if (cum > line) atomicMin(&shi[0], v);
-      atomicMax(&shi[1], v);
-    }
-    before = all;
-    __syncthreads();
-    if (shi[0] != 0x7fffffff) break;
-  }
-  __syncthreads();
-  return shi[0] != 0x7fffffff ? shi[0] : shi[1];
-}
-
-template <class T>
-__device__ __forceinline__ const typename T::raw* target_row(const VerifyParams& p, int64_t b, int i) {
-  return (const typename T::raw*)p.target.data + p.target.at(b * (p.drafts + 1) + i);
-}
-template <class T>
-__device__ __forceinline__ const typename T::raw* draft_row(const VerifyParams& p, int64_t b, int i) {
-  return (const typename T::raw*)p.draft.data + p.draft.at(b * p.drafts + i);
-}
-__device__ __forceinline__ int length_of(const VerifyParams& p, int64_t b) {
-  return p.lengths ? max(0, min(p.lengths[b], p.drafts)) : p.drafts;
-}
-
-template <int NT>
-__device__ __forceinline__ void write_tokens(const VerifyParams& p, int64_t b, int a, int token) {
-  if (threadIdx.x == 0) p.accepted[b] = a;
-  for (int i = threadIdx.x; i <= p.drafts; i += NT)
-    p.tokens[b * (p.drafts + 1) + i] = i < a ? any_id(p.ids, b * p.drafts + i, p.ids_bytes) : i == a ? token : -1;
-}
-
-// Batches that fill the card: a block takes a sequence, row by row up to where
-// it stops; what lies behind is not read.
-template <class T, int NT, int U>
-__global__ __launch_bounds__(NT, 4) void lt_verify_walk(VerifyParams p) {
-  __shared__ float shf[NT / 64];
-  __shared__ double shd[NT / 64];
-  __shared__ int shi[2];
-  const int V = p.target.vocab;
-  const int64_t b = p.block0 + blockIdx.x;
-  const int n = length_of(p, b);
-  Stop<T> st;
-  int a = 0;
-  for (;; ++a) {
-    st.x = target_row<T>(p, b, a);
-    int lead = lead_of<T>(st.x);
-    st.p = soft_part<T, NT, U>(st.x, lead, 0, lead, lead + V, p.c, shf, shd);
+  if (token < 0 && sp > 0) {
     st.y = nullptr;
-    if (a == n) break;
-    st.id = any_id(p.ids, b * p.drafts + a, p.ids_bytes);
-    const bool there = st.id >= 0 && st.id < V;
-    double q = 1;
-    if (p.draft.data) {
-      st.y = draft_row<T>(p, b, a);
-      lead = lead_of<T>(st.y);
-      st.q = soft_part<T, NT, U>(st.y, lead, 0, lead, lead + V, p.c, shf, shd);
-      q = there ? st.q.of(T::get(st.y[st.id]), p.c) : 0.0;
-    }
-    st.minus = true;
-    if (!(there && p.accept_u[b * p.drafts + a] * q < st.p.of(T::get(st.x[st.id]), p.c))) break;
-    st.minus = false;
+    st.id = -1;
+    double before = 0;
+    token = cross(0, p.target.vocab, p.sample_u[b] * sp, before, of_token);
   }
-  double* const weight = p.weight + b * p.segments;
-  const int lead = lead_of<T>(st.x), segments = (lead + V + 64 * Vec<T>::E - 1) / (64 * Vec<T>::E);
-  weigh<T, NT>(st, V, 0, lead + V, p.c, weight);
-  __syncthreads();
-  const int token = draw<T, NT>(st, V, p.sample_u[b], p.c, weight, segments, shd, shi);
-  write_tokens<NT>(p, b, a, token);
-}
-
-// ---- smaller batches: all rows at once, in chunks --------------------------------
-constexpr int SMALL_NT = 256;
-
-// Chunks' sums of every row that counts.
-template <class T, int U>
-__global__ __launch_bounds__(SMALL_NT) void lt_verify_sums(VerifyParams p) {
-  constexpr int NT = SMALL_NT;
-  __shared__ float shf[NT / 64];
-  __shared__ double shd[NT / 64];
-  const int64_t blk = p.block0 + blockIdx.x, row = blk / p.splits, targets = p.batch * (p.drafts + 1);
-  const bool target = row < targets;
-  const int64_t b = target ? row / (p.drafts + 1) : (row - targets) / p.drafts;
-  const int i = (int)(target ? row - b * (p.drafts + 1) : row - targets - b * p.drafts), n = length_of(p, b);
-  if (target ? i > n : i >= n) return;
-  const typename T::raw* x = target ? target_row<T>(p, b, i) : draft_row<T>(p, b, i);
-  const int lead = lead_of<T>(x), c0 = (int)(blk - row * p.splits) * p.chunk;
-  const int v1 = min(lead + p.target.vocab, c0 + p.chunk);
-  const Soft o = soft_part<T, NT, U>(x, lead, c0, max(lead, c0), v1, p.c, shf, shd);
-  if (threadIdx.x == 0) p.part[blk] = make_double2(o.m, o.s);
-}
-
-// A row's chunks, one after another.
-__device__ __forceinline__ Soft join_parts(const double2* part, int splits, double c) {
-  Soft o;
-  for (int i = 0; i < splits; ++i) o.m = fmaxf(o.m, (float)part[i].x);
-  for (int i = 0; i < splits; ++i) o.s += part[i].y * exp2_64(fmax((part[i].x - o.m) * c, -DEPTH));
-  o.finish(c);
-  return o;
-}
-
-// Where sequence b stops, from the chunks' sums (every block that needs it does
-// the same): a thread a place.
-template <class T>
-__device__ __forceinline__ Stop<T> find_stop(const VerifyParams& p, int64_t b, int* sh_a, int& a) {
-  const int n = length_of(p, b), V = p.target.vocab;
-  if (threadIdx.x == 0) *sh_a = n;
-  __syncthreads();
-  const int64_t targets = p.batch * (p.drafts + 1);
-  for (int i0 = 0; i0 < n; i0 += SMALL_NT) {
-    const int i = i0 + threadIdx.x;
-    if (i < n) {
-      const int64_t id = any_id(p.ids, b * p.drafts + i, p.ids_bytes);
-      const bool there = id >= 0 && id < V;
-      double px = 0, qx = there ? 1 : 0;
-      if (there) {
-        px = join_parts(p.part + (b * (p.drafts + 1) + i) * p.splits, p.splits, p.c).of(T::get(target_row<T>(p, b, i)[id]), p.c);
-        if (p.draft.data)
-          qx = join_parts(p.part + (targets + b * p.drafts + i) * p.splits, p.splits, p.c).of(T::get(draft_row<T>(p, b, i)[id]), p.c);
-      }
-      if (!(there && p.accept_u[b * p.drafts + i] * qx < px)) atomicMin(sh_a, i);
-    }
-  }
-  __syncthreads();
-  a = *sh_a;
-  Stop<T> st;
-  st.x = target_row<T>(p, b, a);
-  st.p = join_parts(p.part + (b * (p.drafts + 1) + a) * p.splits, p.splits, p.c);
-  if (a < n) {
-    st.minus = true;
-    st.id = any_id(p.ids, b * p.drafts + a, p.ids_bytes);
-    if (p.draft.data) {
-      st.y = draft_row<T>(p, b, a);
-      st.q = join_parts(p.part + (targets + b * p.drafts + a) * p.splits, p.splits, p.c);
-    }
-  }
-  return st;
-}
-
-template <class T>
-__global__ __launch_bounds__(SMALL_NT) void lt_verify_weigh(VerifyParams p) {
-  __shared__ int sh_a;
-  const int64_t blk = p.block0 + blockIdx.x, b = blk / p.weigh_splits;
-  int a;
-  const Stop<T> st = find_stop<T>(p, b, &sh_a, a);
-  const int split = (int)(blk - b * p.weigh_splits), c0 = split * p.weigh_chunk;
-  if (split == 0 && threadIdx.x == 0) p.stop[b] = StopNote{st.p.s, st.q.s, st.p.m, st.q.m, a, 0};
-  weigh<T, SMALL_NT>(st, p.target.vocab, c0, c0 + p.weigh_chunk, p.c, p.weight + b * p.segments);
-}
-
-template <class T>
-__global__ __launch_bounds__(SMALL_NT) void lt_verify_draw(VerifyParams p) {
-  __shared__ double shd[SMALL_NT / 64];
-  __shared__ int shi[2];
-  const int64_t b = p.block0 + blockIdx.x;
-  const StopNote note = p.stop[b];
-  Stop<T> st;
-  st.x = target_row<T>(p, b, note.a);
-  st.p.m = note.pm;
-  st.p.s = note.ps;
-  st.p.finish(p.c);
-  if (note.a < length_of(p, b)) {
-    st.minus = true;
-    st.id = any_id(p.ids, b * p.drafts + note.a, p.ids_bytes);
-    if (p.draft.data) {
-      st.y = draft_row<T>(p, b, note.a);
-      st.q.m = note.qm;
-      st.q.s = note.qs;
-      st.q.finish(p.c);
-    }
-  }
-  const int segments = (lead_of<T>(st.x) + p.target.vocab + 64 * Vec<T>::E - 1) / (64 * Vec<T>::E);
-  const int token = draw<T, SMALL_NT>(st, p.target.vocab, p.sample_u[b], p.c, p.weight + b * p.segments, segments, shd, shi);
-  write_tokens<SMALL_NT>(p, b, note.a, token);
+  if (tid == 0) p.accepted[b] = note.a;
+  for (int i = tid; i <= p.drafts; i += NT)
+    p.tokens[b * (p.drafts + 1) + i] = i < note.a ? any_id(p.ids, b * p.drafts + i, p.ids_bytes) : i == note.a ? token : -1;
 }
 
 // ---- host ------------------------------------------------------------------
-constexpr int64_t MANY = 256;              // sequences that fill the card's CUs
+// Rounds read no row behind the one where a sequence stops; each costs a
+// launch's time and waits for its slowest block.  (512 x 7 drafts of 131072
+// bf16, 268 MB a place: 0.45 ms, all at once 0.51; 64 x 5, 34 MB: 0.15 and 0.08.)
+constexpr int64_t ROUND_BYTES = (int64_t)128 << 20;
+
+int64_t chunks(int64_t numbers, int64_t step, int64_t rows, int64_t blocks) {
+  int64_t n = (numbers + step - 1) / step;
+  n = n < blocks / rows ? n : blocks / rows;
+  return n > 1 ? n : 1;
+}
 
 void plan(VerifyParams& p, int dtype) {
-  const int e = dtype == LT_F32 ? 4 : 8, step = SMALL_NT * 4 * e;
-  const int64_t numbers = (int64_t)p.target.vocab + LEAD, rows = p.batch * (p.drafts + 1 + (p.draft.data ? p.drafts : 0));
+  const int e = dtype == LT_F32 ? 4 : 8, step = NT * 4 * e, vectors = NT * e;
+  const int64_t numbers = (int64_t)p.target.vocab + LEAD, kinds = p.draft.data ? 2 : 1;
+  p.rounds = p.batch * kinds * p.target.vocab * dtype_bytes(dtype) >= ROUND_BYTES && p.drafts > 0;
   p.segments = (int32_t)((numbers + 64 * e - 1) / (64 * e));
-  int64_t n = (numbers + step - 1) / step;
-#ifndef XB
-#define XB 8192
-#endif
-  n = n < XB / rows ? n : XB / rows;
-  n = n > 1 ? n : 1;
-  const int64_t steps = (numbers + n * step - 1) / (n * step);
-  p.chunk = (int32_t)(steps * step);
+  // blocks enough that those of rows that do not count leave the card full
+  int64_t n = chunks(numbers, step, p.batch * kinds * (p.rounds ? 1 : p.drafts + 1), 8192);
+  p.chunk = (int32_t)((numbers + n * step - 1) / (n * step) * step);
   p.splits = (int32_t)((numbers + p.chunk - 1) / p.chunk);
-  const int vectors = SMALL_NT * e;
-  n = (numbers + vectors - 1) / vectors;
-  n = n < 2048 / p.batch ? n : 2048 / p.batch;
-  n = n > 1 ? n : 1;
+  // of each sum: a thread's additions one after another (16 of a step, the
+  // steps), 30 to join them, 3 roundings of an exponent of 12 and one of its
+  // power of 2; twice that for two
+  p.margin = 2 * (16 + p.chunk / step + 30 + p.splits + 3 * 12 + 2) * 0x1p-24;
+  n = chunks(numbers, vectors, p.batch, 4096);
   p.weigh_chunk = (int32_t)((numbers + n * vectors - 1) / (n * vectors) * vectors);
   p.weigh_splits = (int32_t)((numbers + p.weigh_chunk - 1) / p.weigh_chunk);
 }
 
-int64_t weights_bytes(const VerifyParams& p) { return (p.batch * p.segments * (int64_t)sizeof(double) + 15) / 16 * 16; }
-
-int64_t parts_bytes(const VerifyParams& p) { return p.batch * (2 * p.drafts + 1) * p.splits * (int64_t)sizeof(double2); }
-
-int64_t need_bytes(const VerifyParams& p) {
-  return weights_bytes(p) + (p.batch >= MANY ? 0 : parts_bytes(p) + p.batch * (int64_t)sizeof(StopNote));
+// The workspace's arrays, from `at` on; its bytes.
+int64_t lay_out(VerifyParams& p, char* at) {
+  int64_t n = 0;
+  auto take = [&](int64_t bytes) {
+    char* const q = at + n;
+    n += (bytes + 15) / 16 * 16;
+    return q;
+  };
+  p.weight = (double2*)take(p.batch * p.segments * (int64_t)sizeof(double2));
+  p.sums = (double2*)take(p.batch * p.weigh_splits * (int64_t)sizeof(double2));
+  p.part = (float2*)take(p.batch * (2 * p.drafts + 1) * p.splits * (int64_t)sizeof(float2));
+  p.stop = (StopNote*)take(p.batch * (int64_t)sizeof(StopNote));
+  p.stopped = (int32_t*)take(p.batch * (int64_t)sizeof(int32_t));
+  return n;
 }
 
 template <class T>
-lt_status launch_verify(const VerifyParams& p, void* stream) {
+lt_status launch_verify(VerifyParams& p, void* stream) {
   const char* what = "lt_verify_draft";
-  if (p.batch >= MANY)
-    return p.target.vocab > 8192 ? launch(lt_verify_walk<T, 512, 2>, p.batch, 512, p, stream, what)
-                                 : launch(lt_verify_walk<T, 256, 2>, p.batch, 256, p, stream, what);
-  const int64_t rows = p.batch * (p.drafts + 1 + (p.draft.data ? p.drafts : 0));
-  lt_status st = launch(lt_verify_sums<T, 4>, rows * p.splits, SMALL_NT, p, stream, what);
-  if (st == LT_OK) st = launch(lt_verify_weigh<T>, p.batch * p.weigh_splits, SMALL_NT, p, stream, what);
-  return st != LT_OK ? st : launch(lt_verify_draw<T>, p.batch, SMALL_NT, p, stream, what);
+  lt_status st = LT_OK;
+  if (p.rounds) {
+    for (p.place = 0; p.place <= p.drafts && st == LT_OK; ++p.place) {
+      const int64_t rows = p.batch * (p.draft.data && p.place < p.drafts ? 2 : 1);
+      st = launch(lt_verify_sums<T, 4, true>, rows * p.splits, NT, p, stream, what);
+    }
+  } else {
+    const int64_t rows = p.batch * (p.drafts + 1 + (p.draft.data ? p.drafts : 0));
+    st = launch(lt_verify_sums<T, 4, false>, rows * p.splits, NT, p, stream, what);
+  }
+  if (st == LT_OK) st = launch(lt_verify_weigh<T>, p.batch * p.weigh_splits, NT, p, stream, what);
+  return st != LT_OK ? st : launch(lt_verify_draw<T>, p.batch, NT, p, stream, what);
 }
 
 lt_status check(const lt_draft* d) {
@@ -533,7 +595,8 @@ extern "C" {
 
 int64_t lt_verify_workspace(const lt_draft* d) {
   if (check(d) != LT_OK || d->batch == 0) return 0;
-  return need_bytes(verify_params(d));
+  VerifyParams p = verify_params(d);
+  return lay_out(p, nullptr);
 }
 
 lt_status lt_verify_draft(const lt_draft* d, double temperature, int64_t* tokens, int64_t* accepted, void* workspace,
@@ -544,11 +607,9 @@ lt_status lt_verify_draft(const lt_draft* d, double temperature, int64_t* tokens
   if (d->batch == 0) return LT_OK;
   if (!tokens || !accepted || !d->sample_u || (d->drafts > 0 && (!d->ids || !d->accept_u))) BAD("NULL argument");
   VerifyParams p = verify_params(d);
-  if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need_bytes(p))
-    BAD("workspace: %lld bytes, 16 B aligned, are needed", (long long)need_bytes(p));
-  p.weight = (double*)workspace;
-  p.part = (double2*)((char*)workspace + weights_bytes(p));
-  p.stop = (StopNote*)((char*)p.part + parts_bytes(p));
+  const int64_t need = lay_out(p, (char*)workspace);
+  if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need)
+    BAD("workspace: %lld bytes, 16 B aligned, are needed", (long long)need);
   p.c = LOG2E / temperature;
   p.tokens = tokens;
   p.accepted = accepted;

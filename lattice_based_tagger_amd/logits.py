@@ -29,7 +29,6 @@ float32 at least.
 """
 
 import ctypes as C
-import math
 import threading
 from collections import namedtuple
 
@@ -81,8 +80,8 @@ def bind(lib):
         'lt_top_logits': (i32, [vp, i32, f64, vp, vp, vp, vp, i64, vp]),
         'lt_distill_workspace': (i64, [vp, i32]),
         'lt_distill_forward': (i32, [vp, vp, f64, vp, vp, vp, i64, vp]),
-        'lt_distill_backward': (i32, [vp, vp, f64, vp, vp, i64, vp, vp]),
-        'lt_distill_fused': (i32, [vp, vp, f64, vp, i64, vp, vp, vp, i64, vp]),
+        'lt_distill_backward': (i32, [vp, vp, f64, vp, f64, vp, i64, vp, vp]),
+        'lt_distill_fused': (i32, [vp, vp, f64, f64, vp, i64, vp, vp, vp, i64, vp]),
         'lt_verify_workspace': (i64, [vp]),
         'lt_verify_draft': (i32, [vp, f64, vp, vp, vp, i64, vp]),
     }
@@ -129,25 +128,29 @@ def _logits(x, what):
 
 def _rows(x, what):
     """lt_rows of ``x``: its leading dimensions as rows of at most two strides."""
-    dims = [(n, s) for n, s in zip(x.shape[:-1], x.stride()[:-1]) if n != 1]
-    runs = []                        # from the innermost out, dimensions that one stride spans joined
-    for n, s in reversed(dims):
-        if runs and s == runs[-1][0] * runs[-1][1]:
-            runs[-1][0] *= n
-        else:
-            runs.append([n, s])
-    if len(runs) > 2 and x.numel():
-        raise ValueError('%s: the leading dimensions %s need more than two strides %s; pass a contiguous tensor'
-                         % (what, tuple(x.shape[:-1]), x.stride()[:-1]))
-    rows = math.prod(x.shape[:-1])
-    if rows == 0 or not runs:
-        inner, outer_s, inner_s = 1, 0, 0
-    elif len(runs) == 1:
-        inner, outer_s, inner_s = 1, runs[0][1], 0
+    vocab = x.shape[-1]
+    if x.is_contiguous():
+        rows, inner, outer_s, inner_s = x.numel() // vocab, 1, vocab, 0
     else:
-        inner, outer_s, inner_s = runs[0][0], runs[1][1], runs[0][1]
-    return _Rows(x.data_ptr(), _DTYPES[x.dtype], x.device.index if x.device.index is not None else -1, rows, inner,
-                 outer_s, inner_s, x.shape[-1])
+        runs = []                    # from the innermost out, dimensions that one stride spans joined
+        for n, s in zip(reversed(x.shape[:-1]), reversed(x.stride()[:-1])):
+            if n == 1:
+                continue
+            if runs and s == runs[-1][0] * runs[-1][1]:
+                runs[-1][0] *= n
+            else:
+                runs.append([n, s])
+        if len(runs) > 2 and x.numel():
+            raise ValueError('%s: the leading dimensions %s need more than two strides %s; pass a contiguous tensor'
+                             % (what, tuple(x.shape[:-1]), x.stride()[:-1]))
+        rows = x.numel() // vocab
+        if rows == 0 or not runs:
+            inner, outer_s, inner_s = 1, 0, 0
+        elif len(runs) == 1:
+            inner, outer_s, inner_s = 1, runs[0][1], 0
+        else:
+            inner, outer_s, inner_s = runs[0][0], runs[1][1], runs[0][1]
+    return _Rows(x.data_ptr(), _DTYPES[x.dtype], x.device.index or 0, rows, inner, outer_s, inner_s, vocab)
 
 
 def _temperature(t):
@@ -158,17 +161,23 @@ def _temperature(t):
 
 
 def _beside(t, shape, dtypes, what, like):
-    """A further argument: its type, shape and device."""
+    """A further argument: its type, shape and device; contiguous."""
     if not isinstance(t, torch.Tensor):
         raise TypeError('%s must be a torch.Tensor, not %s' % (what, type(t).__name__))
     if t.dtype not in dtypes:
         raise TypeError('%s must be %s, not %s' % (what, ' or '.join(str(d).replace('torch.', '') for d in dtypes),
                                                    t.dtype))
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError('%s must be %s, not %s' % (what, tuple(shape), tuple(t.shape)))
     if t.device != like.device:
         raise ValueError('%s is on %s, the logits are on %s' % (what, t.device, like.device))
-    return t.detach().contiguous()
+    if t.requires_grad:
+        t = t.detach()
+    return t if t.is_contiguous() else t.contiguous()
+
+
+_IDS = (torch.int64, torch.int32)
+_F32 = (torch.float32,)
 
 
 def _on_gpu(x):
@@ -176,12 +185,18 @@ def _on_gpu(x):
         raise ValueError('the logits are on %s: these operators run on a GPU (there is no CPU path)' % x.device)
 
 
+# (the handle alone: torch.cuda.current_stream makes an object around it, 2 us)
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
+
+
 def _stream(x):
+    if _raw_stream is not None:
+        return _raw_stream(x.device.index)
     return torch.cuda.current_stream(x.device).cuda_stream
 
 
 def _scratch(n, x):
-    return torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+    return x.new_empty((n,), dtype=torch.uint8) if n else None
 
 
 def _ptr(t):
@@ -203,18 +218,19 @@ def top_logits(logits, k, temperature=1.0):
     if not 1 <= k <= min(MAX_TOP, logits.shape[-1]):
         raise ValueError('k must be within 1 .. min(vocab, %d), not %d' % (MAX_TOP, k))
     temperature = _temperature(temperature)
-    x = logits.detach()
-    rows = _rows(x, 'logits')
-    _on_gpu(x)
+    rows = _rows(logits, 'logits')
+    _on_gpu(logits)
     lib = _load()
-    lead = x.shape[:-1]
-    out = TopLogits(torch.empty(lead + (k,), dtype=x.dtype, device=x.device),
-                    torch.empty(lead + (k,), dtype=torch.int64, device=x.device),
-                    torch.empty(lead, dtype=torch.float32, device=x.device))
-    work = _scratch(lib.lt_top_logits_workspace(C.byref(rows), k), x)
-    _capi.check(lib.lt_top_logits(C.byref(rows), k, temperature, out.values.data_ptr(), out.ids.data_ptr(),
-                                  out.lse.data_ptr(), _ptr(work), work.numel() if work is not None else 0,
-                                  _stream(x)))
+    lead = logits.shape[:-1]
+    many = lead + (k,)
+    out = TopLogits(logits.new_empty(many), logits.new_empty(many, dtype=torch.int64),
+                    logits.new_empty(lead, dtype=torch.float32))
+    size = lib.lt_top_logits_workspace(C.byref(rows), k)
+    work = _scratch(size, logits)
+    status = lib.lt_top_logits(C.byref(rows), k, temperature, out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(),
+                               _ptr(work), size, _stream(logits))
+    if status:
+        _capi.check(status)
     return out
 
 
@@ -227,11 +243,11 @@ def _teacher(x, ids, top, lse):
     n = ids.shape[-1]
     if not 1 <= n <= MAX_TOP:
         raise ValueError('a teacher row has 1 .. %d entries, not %d' % (MAX_TOP, n))
-    lead = tuple(x.shape[:-1])
-    ids = _beside(ids, lead + (n,), (torch.int64, torch.int32), 'top_ids', x)
-    top = _beside(top, lead + (n,), tuple(_DTYPES), 'top_values', x)
+    lead = x.shape[:-1]
+    ids = _beside(ids, lead + (n,), _IDS, 'top_ids', x)
+    top = _beside(top, lead + (n,), _DTYPES, 'top_values', x)
     if lse is not None:
-        lse = _beside(lse, lead, (torch.float32,), 'top_lse', x)
+        lse = _beside(lse, lead, _F32, 'top_lse', x)
     return ids, top, lse
 
 
@@ -242,23 +258,23 @@ def _teacher_desc(ids, top, lse):
 def _grad_like(x):
     """Memory for a gradient whose rows lie as ``x``'s do, where those do not
     overlap: rows of one alignment load and store alike."""
+    if x.is_contiguous():
+        return x.new_empty(x.shape)
     v = x.shape[-1]
     pitch = x.stride(-2) if x.dim() > 1 else v
-    if x.dim() < 2 or pitch < v or pitch > v + 1024 or pitch == v:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    return torch.empty(x.shape[:-1] + (pitch,), dtype=x.dtype, device=x.device)[..., :v]
+    if pitch <= v or pitch > v + 1024:
+        return x.new_empty(x.shape)
+    return x.new_empty(x.shape[:-1] + (pitch,))[..., :v]
 
 
 def _weight(w, x):
-    """(tensor, stride) of the rows' weights: a number or a tensor [...]."""
-    if isinstance(w, torch.Tensor) and w.dim() == 0:
+    """(tensor, stride) of the rows' weights, a tensor [...] or of no dimension."""
+    if w.dim() == 0:
         w = w.expand(x.shape[:-1])
-    elif not isinstance(w, torch.Tensor):
-        return torch.full((1,), float(w), dtype=torch.float32, device=x.device), 0
-    if w.dtype == torch.float32 and w.device == x.device and tuple(w.shape) == tuple(x.shape[:-1]) and w.numel() and \
+    if w.dtype == torch.float32 and w.device == x.device and w.shape == x.shape[:-1] and w.numel() and \
             all(s == 0 or n == 1 for n, s in zip(w.shape, w.stride())):
         return w.detach(), 0             # one weight for every row (a sum's or a mean's gradient)
-    return _beside(w, x.shape[:-1], (torch.float32,), 'weight', x), 1
+    return _beside(w, x.shape[:-1], _F32, 'weight', x), 1
 
 
 class _Distill(torch.autograd.Function):
@@ -266,11 +282,14 @@ class _Distill(torch.autograd.Function):
     def forward(ctx, x, ids, top, lse, temperature):
         lib = _load()
         rows, t = _rows(x, 'logits'), _teacher_desc(ids, top, lse)
-        loss = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-        stats = torch.empty(rows.rows * _STATS, dtype=torch.float32, device=x.device)
-        work = _scratch(lib.lt_distill_workspace(C.byref(rows), t.entries), x)
-        _capi.check(lib.lt_distill_forward(C.byref(rows), C.byref(t), temperature, loss.data_ptr(), stats.data_ptr(),
-                                           _ptr(work), work.numel() if work is not None else 0, _stream(x)))
+        loss = x.new_empty(x.shape[:-1], dtype=torch.float32)
+        stats = x.new_empty((rows.rows * _STATS,), dtype=torch.float32)
+        size = lib.lt_distill_workspace(C.byref(rows), t.entries)
+        work = _scratch(size, x)
+        status = lib.lt_distill_forward(C.byref(rows), C.byref(t), temperature, loss.data_ptr(), stats.data_ptr(),
+                                        _ptr(work), size, _stream(x))
+        if status:
+            _capi.check(status)
         ctx.save_for_backward(x, ids, top, lse, stats)
         ctx.temperature = temperature
         return loss
@@ -284,8 +303,10 @@ class _Distill(torch.autograd.Function):
         w, stride = _weight(g, x)
         grad = _grad_like(x)
         out = _rows(grad, 'grad')
-        _capi.check(lib.lt_distill_backward(C.byref(rows), C.byref(t), ctx.temperature, stats.data_ptr(),
-                                            w.data_ptr(), stride, C.byref(out), _stream(x)))
+        status = lib.lt_distill_backward(C.byref(rows), C.byref(t), ctx.temperature, stats.data_ptr(), 1.0,
+                                         w.data_ptr(), stride, C.byref(out), _stream(x))
+        if status:
+            _capi.check(status)
         return grad, None, None, None, None
 
 
@@ -311,7 +332,8 @@ def distill_loss(logits, top_ids, top_values, top_lse=None, temperature=1.0):
     _logits(logits, 'logits')
     ids, top, lse = _teacher(logits, top_ids, top_values, top_lse)
     temperature = _temperature(temperature)
-    _rows(logits, 'logits')
+    if not logits.is_contiguous():
+        _rows(logits, 'logits')
     _on_gpu(logits)
     return _Distill.apply(logits, ids, top, lse, temperature)
 
@@ -325,21 +347,24 @@ def distill_loss_grad(logits, top_ids, top_values, weight, top_lse=None, tempera
     _logits(logits, 'logits')
     ids, top, lse = _teacher(logits, top_ids, top_values, top_lse)
     temperature = _temperature(temperature)
-    x = logits.detach()
-    rows = _rows(x, 'logits')
+    rows = _rows(logits, 'logits')
+    w, stride, scale = None, 0, 1.0
     if isinstance(weight, torch.Tensor):
-        w, stride = _weight(weight, x)
-    _on_gpu(x)
+        w, stride = _weight(weight, logits)
+    else:
+        scale = float(weight)
+    _on_gpu(logits)
     lib = _load()
-    if not isinstance(weight, torch.Tensor):
-        w, stride = _weight(weight, x)
     t = _teacher_desc(ids, top, lse)
-    loss = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    grad = _grad_like(x)
+    loss = logits.new_empty(logits.shape[:-1], dtype=torch.float32)
+    grad = _grad_like(logits)
     out = _rows(grad, 'grad')
-    work = _scratch(lib.lt_distill_workspace(C.byref(rows), t.entries), x)
-    _capi.check(lib.lt_distill_fused(C.byref(rows), C.byref(t), temperature, w.data_ptr(), stride, loss.data_ptr(),
-                                     C.byref(out), _ptr(work), work.numel() if work is not None else 0, _stream(x)))
+    size = lib.lt_distill_workspace(C.byref(rows), t.entries)
+    work = _scratch(size, logits)
+    status = lib.lt_distill_fused(C.byref(rows), C.byref(t), temperature, scale, _ptr(w), stride, loss.data_ptr(),
+                                  C.byref(out), _ptr(work), size, _stream(logits))
+    if status:
+        _capi.check(status)
     return loss, grad
 
 
@@ -373,26 +398,28 @@ def verify_draft(target, draft_ids, accept_u, sample_u, draft=None, lengths=None
     drafts = places - 1
     if drafts > MAX_DRAFTS:
         raise ValueError('at most %d drafted tokens, not %d' % (MAX_DRAFTS, drafts))
-    ids = _beside(draft_ids, (batch, drafts), (torch.int64, torch.int32), 'draft_ids', target)
-    au = _beside(accept_u, (batch, drafts), (torch.float32,), 'accept_u', target)
-    su = _beside(sample_u, (batch,), (torch.float32,), 'sample_u', target)
+    ids = _beside(draft_ids, (batch, drafts), _IDS, 'draft_ids', target)
+    au = _beside(accept_u, (batch, drafts), _F32, 'accept_u', target)
+    su = _beside(sample_u, (batch,), _F32, 'sample_u', target)
     if lengths is not None:
         lengths = _beside(lengths, (batch,), (torch.int32,), 'lengths', target)
-    x, y = target.detach(), None
+    y = None
     if draft is not None:
         _logits(draft, 'draft')
-        if tuple(draft.shape) != (batch, drafts, vocab) or draft.dtype != target.dtype or draft.device != target.device:
+        if draft.shape != (batch, drafts, vocab) or draft.dtype != target.dtype or draft.device != target.device:
             raise ValueError('draft must be %s of %s on %s' % ((batch, drafts, vocab), target.dtype, target.device))
-        y = _rows(draft.detach(), 'draft')
+        y = _rows(draft, 'draft')
     temperature = _temperature(temperature)
-    rows = _rows(x, 'target')
-    _on_gpu(x)
+    rows = _rows(target, 'target')
+    _on_gpu(target)
     lib = _load()
     d = _Draft(C.addressof(rows), None if y is None else C.addressof(y), ids.data_ptr(), au.data_ptr(), su.data_ptr(),
                _ptr(lengths), batch, drafts, ids.element_size())
-    out = Verified(torch.empty((batch, places), dtype=torch.int64, device=x.device),
-                   torch.empty((batch,), dtype=torch.int64, device=x.device))
-    work = _scratch(lib.lt_verify_workspace(C.byref(d)), x)
-    _capi.check(lib.lt_verify_draft(C.byref(d), temperature, out.tokens.data_ptr(), out.accepted.data_ptr(),
-                                    _ptr(work), work.numel() if work is not None else 0, _stream(x)))
+    out = Verified(ids.new_empty((batch, places), dtype=torch.int64), ids.new_empty((batch,), dtype=torch.int64))
+    size = lib.lt_verify_workspace(C.byref(d))
+    work = _scratch(size, target)
+    status = lib.lt_verify_draft(C.byref(d), temperature, out[0].data_ptr(), out[1].data_ptr(), _ptr(work), size,
+                                 _stream(target))
+    if status:
+        _capi.check(status)
     return out

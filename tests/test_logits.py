@@ -97,8 +97,13 @@ def test_c_entries_refuse_rows(kw):
     t = logits._Teacher(4096, 4096, None, 1, 8, 0)
     assert lib.lt_top_logits(C.byref(x), 1, 1.0, 4096, 4096, 4096, None, 0, None) == -1
     assert lib.lt_distill_forward(C.byref(x), C.byref(t), 1.0, 4096, 4096, None, 0, None) == -1
-    assert lib.lt_distill_fused(C.byref(x), C.byref(t), 1.0, 4096, 1, 4096, C.byref(x), 4096, 1 << 20, None) == -1
+    assert lib.lt_distill_fused(C.byref(x), C.byref(t), 1.0, 1.0, 4096, 1, 4096, C.byref(x), 4096, 1 << 20, None) == -1
     assert _capi.load().lt_last_error()
+
+
+def _backward(lib, x, t, grad, stats=4096, scale=1.0, stride=1):
+    return lib.lt_distill_backward(C.byref(x), C.byref(t), 1.0, stats, scale, 4096, stride,
+                                   None if grad is None else C.byref(grad), None)
 
 
 @pytest.mark.parametrize('call', [
@@ -109,13 +114,16 @@ def test_c_entries_refuse_rows(kw):
     lambda lib, x, t: lib.lt_top_logits(C.byref(x), 1, 1.0, None, 4096, 4096, None, 0, None),
     lambda lib, x, t: lib.lt_distill_forward(C.byref(x), None, 1.0, 4096, 4096, None, 0, None),
     lambda lib, x, t: lib.lt_distill_forward(C.byref(x), C.byref(t), 1.0, None, 4096, None, 0, None),
-    lambda lib, x, t: lib.lt_distill_backward(C.byref(x), C.byref(t), 1.0, 4096, None, 1, C.byref(x), None),
-    lambda lib, x, t: lib.lt_distill_backward(C.byref(x), C.byref(t), 1.0, 4096, 4096, 2, C.byref(x), None),
-    lambda lib, x, t: lib.lt_distill_backward(C.byref(x), C.byref(t), 1.0, 4096, 4096, 1, None, None),
-    lambda lib, x, t: lib.lt_distill_backward(C.byref(x), C.byref(t), 1.0, 4096, 4096, 1, C.byref(_desc(rows=3)), None),
-    lambda lib, x, t: lib.lt_distill_backward(C.byref(x), C.byref(t), 1.0, 4096, 4096, 1, C.byref(_desc(dtype=2)), None),
-    lambda lib, x, t: lib.lt_distill_fused(C.byref(x), C.byref(t), 1.0, 4096, 1, None, C.byref(x), None, 0, None),
-    lambda lib, x, t: lib.lt_distill_fused(C.byref(_desc(vocab=200000)), C.byref(t), 1.0, 4096, 1, 4096,
+    lambda lib, x, t: _backward(lib, x, t, x, stats=None),
+    lambda lib, x, t: _backward(lib, x, t, x, stats=4100),
+    lambda lib, x, t: _backward(lib, x, t, x, scale=float('nan')),
+    lambda lib, x, t: _backward(lib, x, t, x, stride=2),
+    lambda lib, x, t: _backward(lib, x, t, None),
+    lambda lib, x, t: _backward(lib, x, t, _desc(rows=3)),
+    lambda lib, x, t: _backward(lib, x, t, _desc(dtype=2)),
+    lambda lib, x, t: _backward(lib, x, t, _desc(device=1)),
+    lambda lib, x, t: lib.lt_distill_fused(C.byref(x), C.byref(t), 1.0, 1.0, 4096, 1, None, C.byref(x), None, 0, None),
+    lambda lib, x, t: lib.lt_distill_fused(C.byref(_desc(vocab=200000)), C.byref(t), 1.0, 1.0, 4096, 1, 4096,
                                            C.byref(_desc(vocab=200000)), 4096, 0, None),
     lambda lib, x, t: lib.lt_verify_draft(None, 1.0, 4096, 4096, None, 0, None),
 ])
@@ -158,13 +166,14 @@ def test_rows_of_views():
         return r.rows, r.inner, r.stride_outer, r.stride_inner
     x = torch.zeros(4, 6, 10)
     assert lay(x) == (24, 1, 10, 0)
+    assert lay(x.transpose(0, 1).contiguous()) == (24, 1, 10, 0)
     assert lay(x[:, :-1]) == (20, 5, 60, 10)
     assert lay(x[..., :7]) == (24, 1, 10, 0)
-    assert lay(x[0, 0]) == (1, 1, 0, 0)
+    assert lay(x[0, 0]) == (1, 1, 10, 0)
     assert lay(x[:1]) == (6, 1, 10, 0)
     assert lay(x[0, :1].expand(5, 10)) == (5, 1, 0, 0)
     assert lay(x.transpose(0, 1)) == (24, 4, 10, 60)
-    assert lay(x[:0]) == (0, 1, 0, 0)
+    assert lay(x[:0]) == (0, 1, 10, 0)
 
 
 def test_plain_distillation_is_the_divergence():
