@@ -342,9 +342,7 @@ __global__ __launch_bounds__(64) void lt_distill_few(DistillParams p) {
   const int lane = threadIdx.x, vocab = p.z.vocab, pitch = few_pitch(vocab), n = p.t.entries;
   const int64_t r0 = (p.block0 + blockIdx.x) * 64;
   const int rows = (int)min((int64_t)64, p.rows - r0);
-  each_of_rows(rows, vocab, [&](int r, int v, int) {
-    few[r * pitch + v] = T::get(((const raw*)p.z.data + p.z.at(r0 + r))[v]);
-  });
+  load_few<T>(p.z, r0, rows, few, pitch);
   __syncthreads();
   const int64_t r = r0 + min(lane, rows - 1);
   float* z = few + min(lane, rows - 1) * pitch;
@@ -411,28 +409,48 @@ __global__ __launch_bounds__(64) void lt_distill_few(DistillParams p) {
       for (int i = 0; i < vocab; ++i) z[i] *= w;
     }
     __syncthreads();
-    each_of_rows(rows, vocab, [&](int r, int v, int) {
-      ((raw*)p.grad.data + p.grad.at(r0 + r))[v] = T::put(few[r * pitch + v]);
-    });
+    raw* const g = (raw*)p.grad.data;
+    if (p.grad.inner == 1 && p.grad.stride_outer == vocab)
+      each_of_rows(rows, vocab, [&](int r, int v, int i) { g[r0 * vocab + i] = T::put(few[r * pitch + v]); });
+    else
+      each_of_rows(rows, vocab, [&](int r, int v, int) { g[p.grad.at(r0 + r) + v] = T::put(few[r * pitch + v]); });
   }
 }
 
 // ---- host ------------------------------------------------------------------
 enum Pass { SUMS, GRAD, BOTH };
 
-// Chunks of a row: one where the rows fill the card or a row is a few steps of
-// a block.
-void split_rows(DistillParams& p, int dtype) {
+// Chunks of a row, of a whole number of steps of a block.
+void split_rows(DistillParams& p, int step, int64_t n) {
+  const int64_t steps = (p.z.vocab + LEAD + n * step - 1) / (n * step);
+  p.chunk = (int32_t)(n <= 1 ? 0x7fffff80 : steps * step);
+  p.splits = (int32_t)(((int64_t)p.z.vocab + LEAD + p.chunk - 1) / p.chunk);
+}
+
+// For the sums: one where the rows fill the card or a row is a few steps --
+// chunks have to be joined, in a launch of its own.  (Loss and gradient of 8 x
+// 32000 bf16 in one launch 11 us, in three 16 and the gaps between them; of 64 x
+// 131072 in three 24 us.)
+void split_sums(DistillParams& p, int dtype) {
   const int step = 512 * 4 * (dtype == LT_F32 ? 4 : 8);
   int64_t n = 1;
-  if (p.z.vocab > 16384 && p.rows < 256) {
+  if (p.z.vocab > 6 * step && p.rows < 256) {
     n = (p.z.vocab + step - 1) / step;
     n = n < 512 / p.rows ? n : 512 / p.rows;
     n = n < 256 ? n : 256;
   }
-  const int64_t steps = (p.z.vocab + n * step - 1) / (n * step);
-  p.chunk = (int32_t)(n == 1 ? 0x7fffff80 : steps * step);
-  p.splits = (int32_t)(((int64_t)p.z.vocab + LEAD + p.chunk - 1) / p.chunk);
+  split_rows(p, step, n);
+}
+
+// For the gradient, which needs no joining: blocks enough for the card.
+void split_grad(DistillParams& p, int dtype) {
+  const int step = 512 * 4 * (dtype == LT_F32 ? 4 : 8);
+  int64_t n = 1;
+  if (p.z.vocab > 16384 && p.rows < 512) {
+    n = (p.z.vocab + step - 1) / step;
+    n = n < 1024 / p.rows ? n : 1024 / p.rows;
+  }
+  split_rows(p, step, n);
 }
 
 int64_t parts_bytes(const DistillParams& p) { return p.splits == 1 ? 0 : p.rows * p.splits * (int64_t)sizeof(float4); }
@@ -502,7 +520,7 @@ DistillParams distill_params(const lt_rows* z, const lt_teacher* t, double tempe
   p.rows = z->rows;
   p.inv_t = 1 / temperature;
   p.c = (float)(LOG2E / temperature);
-  split_rows(p, z->dtype);
+  split_sums(p, z->dtype);
   // Logits and gradient of more than the last cache's 256 MB: by the time that
   // the gradient is read, it would be gone.  A smaller one is left there, and so
   // are rows short enough to be found again in the L2 (131072 x 2000: 0.37 ms
@@ -524,7 +542,7 @@ int64_t lt_distill_workspace(const lt_rows* z, int32_t) {
   DistillParams p{};
   p.z = rows_of(z);
   p.rows = z->rows;
-  split_rows(p, z->dtype);
+  split_sums(p, z->dtype);
   return p.splits == 1 ? 0 : p.rows * LT_DISTILL_STATS * (int64_t)sizeof(float) + parts_bytes(p);
 }
 
@@ -555,6 +573,7 @@ lt_status lt_distill_backward(const lt_rows* z, const lt_teacher* t, double temp
   p.weight = weight;
   p.weight_stride = weight_stride;
   p.grad = rows_of(grad);
+  split_grad(p, z->dtype);
   ON_DEVICE(z->device);
   return launch_pass(p, z->dtype, GRAD, stream, "lt_distill_backward");
 }
@@ -578,6 +597,7 @@ lt_status lt_distill_fused(const lt_rows* z, const lt_teacher* t, double tempera
   ON_DEVICE(z->device);
   if (p.splits == 1) return launch_pass(p, z->dtype, BOTH, stream, "lt_distill_fused");
   st = launch_pass(p, z->dtype, SUMS, stream, "lt_distill_fused");
+  split_grad(p, z->dtype);
   return st != LT_OK ? st : launch_pass(p, z->dtype, GRAD, stream, "lt_distill_fused");
 }
 

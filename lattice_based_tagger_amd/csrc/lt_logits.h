@@ -362,6 +362,34 @@ __device__ __forceinline__ void each_of_rows(int rows, int vocab, F f) {
   }
 }
 
+// Rows r0 .. r0 + rows (at most 64) to LDS.
+template <class T>
+__device__ __forceinline__ void load_few(const Rows& x, int64_t r0, int rows, float* few, int pitch) {
+  using raw = typename T::raw;
+  const raw* const data = (const raw*)x.data;
+  const int vocab = x.vocab, lane = threadIdx.x & 63, n = rows * vocab;
+  if (x.inner != 1 || x.stride_outer != vocab) {
+    each_of_rows(rows, vocab, [&](int r, int v, int) { few[r * pitch + v] = T::get(data[x.at(r0 + r) + v]); });
+    return;
+  }
+  // contiguous: eight loads under way at a time
+  const raw* const from = data + r0 * vocab;
+  const int dr = 64 / vocab, dv = 64 - dr * vocab;
+  int r = lane / vocab, v = lane - r * vocab;
+  for (int i0 = lane; i0 < n; i0 += 64 * 8) {
+    raw f[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = from[min(i0 + 64 * j, n - 1)];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (i0 + 64 * j < n) few[r * pitch + v] = T::get(f[j]);
+      r += dr;
+      v += dv;
+      if (v >= vocab) v -= vocab, ++r;
+    }
+  }
+}
+
 // ---- host ------------------------------------------------------------------
 #define BAD(...) return lt::set_error(LT_EINVAL, __VA_ARGS__)
 

@@ -463,9 +463,7 @@ __global__ __launch_bounds__(64) void lt_top_few(TopParams p) {
   const int lane = threadIdx.x, vocab = p.x.vocab, pitch = few_pitch(vocab);
   const int64_t r0 = (p.block0 + blockIdx.x) * 64;
   const int rows = (int)min((int64_t)64, p.rows - r0);
-  each_of_rows(rows, vocab, [&](int r, int v, int) {
-    few[r * pitch + v] = T::get(((const raw*)p.x.data + p.x.at(r0 + r))[v]);
-  });
+  load_few<T>(p.x, r0, rows, few, pitch);
   __syncthreads();
   const float* x = few + min(lane, rows - 1) * pitch;
   uint32_t best[K];
@@ -543,12 +541,12 @@ __global__ __launch_bounds__(256) void lt_top_small(TopParams p) {
 }
 
 // Chunks of a row: one where the rows fill the card or a row is a few steps of
-// a block; else a step or more each.  (131072 bf16, k 20, one row: 22 us whole,
-// 17 us in 8 chunks and joined; 64 rows: 27 and 18 us.)
+// a block; else a step or more each.  (64 x 131072 bf16, k 20: 27 us whole; in
+// 8 chunks 10 us, and 4 us to join them in a launch of its own.)
 void split_rows(TopParams& p, int dtype) {
   const int step = 512 * 4 * (dtype == LT_F32 ? 4 : 8);
   int64_t n = 1;
-  if (p.x.vocab > 2 * step && p.rows < 256) {
+  if (p.x.vocab > 6 * step && p.rows < 256) {
     n = (p.x.vocab + step - 1) / step;
     n = n < 512 / p.rows ? n : 512 / p.rows;
     n = n < JOIN / p.k ? n : JOIN / p.k;
