@@ -375,12 +375,17 @@ __global__ __launch_bounds__(64) void lt_distill_few(DistillParams p) {
     sum = sum > 0 ? 1 : sum;               // (a NaN stays)
   }
   float m = LOWEST, in = 0.f, out = 0.f;
-  for (int i = 0; i < vocab; ++i) m = max2(m, z[i]);
-  for (int i = 0; i < vocab; ++i) {
-    const float e = exp2_((z[i] - m) * p.c);
-    const bool entry = mask >> i & 1;
-    in += entry ? e : 0.f;
-    out += entry ? 0.f : e;
+  for (int i = 0; i < vocab; i += 4) m = max2(max3(m, z[i], z[i + 1]), max2(z[i + 2], z[i + 3]));
+  for (int i = 0; i < vocab; i += 4) {
+    float e[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) e[j] = exp2_((z[i + j] - m) * p.c);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool entry = mask >> (i + j) & 1;
+      in += entry ? e[j] : 0.f;
+      out += entry ? 0.f : e[j];
+    }
   }
   const double s = (double)in + out, logs = log(s), qrest = out / s;
   if (!(rest > 0 && qrest > 0)) rest = 0;
@@ -403,10 +408,15 @@ __global__ __launch_bounds__(64) void lt_distill_few(DistillParams p) {
   if (GRAD) {
     const float w = weight_of(p, r);
     if (lane < rows) {
-      for (int i = 0; i < vocab; ++i) z[i] = exp2_((z[i] - m) * p.c) * (mask >> i & 1 ? fin : fout);
+      for (int i = 0; i < vocab; i += 4) {
+        float e[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) e[j] = exp2_((z[i + j] - m) * p.c) * (mask >> (i + j) & 1 ? fin : fout) * w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) z[i + j] = e[j];
+      }
       for (int j = 0; j < n; ++j)
-        if (entry(j, id, v)) z[id] -= (float)(exp(v - ref - norm) * p.inv_t);
-      for (int i = 0; i < vocab; ++i) z[i] *= w;
+        if (entry(j, id, v)) z[id] -= (float)(exp(v - ref - norm) * p.inv_t) * w;
     }
     __syncthreads();
     raw* const g = (raw*)p.grad.data;

@@ -347,7 +347,9 @@ constexpr int LEAD = 64;                   // more than any lead
 // fall on different banks.
 constexpr int FEW = 64;                    // logits of such a row, at most
 
-__host__ __device__ inline int few_pitch(int vocab) { return vocab | 1; }
+// Behind a row's logits, up to a multiple of 4, lie -inf: what goes over a row
+// takes 4 at a time (a read of LDS that is waited for costs 100 cycles).
+__host__ __device__ inline int few_pitch(int vocab) { return ((vocab + 3) & ~3) | 1; }
 
 // f(row of the 64, v, its place among all) for every logit, 64 at a time
 template <class F>
@@ -368,6 +370,7 @@ __device__ __forceinline__ void load_few(const Rows& x, int64_t r0, int rows, fl
   using raw = typename T::raw;
   const raw* const data = (const raw*)x.data;
   const int vocab = x.vocab, lane = threadIdx.x & 63, n = rows * vocab;
+  for (int v = vocab; v & 3; ++v) few[lane * pitch + v] = -INFINITY;
   if (x.inner != 1 || x.stride_outer != vocab) {
     each_of_rows(rows, vocab, [&](int r, int v, int) { few[r * pitch + v] = T::get(data[x.at(r0 + r) + v]); });
     return;

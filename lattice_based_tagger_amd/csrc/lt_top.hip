@@ -471,20 +471,30 @@ __global__ __launch_bounds__(64) void lt_top_few(TopParams p) {
 #pragma unroll
   for (int j = 0; j < K; ++j) best[j] = 0, id[j] = 0;
   float m = LOWEST;
-  for (int v = 0; v < vocab; ++v) {
-    const float f = x[v];
-    m = max2(m, f);
-    const uint32_t o = order_of(f);
-    // (behind an equal one, which came earlier)
+  for (int v0 = 0; v0 < vocab; v0 += 4) {
+    float f[4];
 #pragma unroll
-    for (int j = K - 1; j >= 0; --j) {
-      const bool here = o > best[j], ahead = j > 0 && o > best[j > 0 ? j - 1 : 0];
-      best[j] = ahead ? best[j > 0 ? j - 1 : 0] : here ? o : best[j];
-      id[j] = ahead ? id[j > 0 ? j - 1 : 0] : here ? v : id[j];
+    for (int i = 0; i < 4; ++i) f[i] = x[v0 + i];
+    m = max2(max3(m, f[0], f[1]), max2(f[2], f[3]));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t o = v0 + i < vocab ? order_of(f[i]) : 0;
+      // (behind an equal one, which came earlier)
+#pragma unroll
+      for (int j = K - 1; j >= 0; --j) {
+        const bool here = o > best[j], ahead = j > 0 && o > best[j > 0 ? j - 1 : 0];
+        best[j] = ahead ? best[j > 0 ? j - 1 : 0] : here ? o : best[j];
+        id[j] = ahead ? id[j > 0 ? j - 1 : 0] : here ? v0 + i : id[j];
+      }
     }
   }
   float s = 0.f;
-  for (int v = 0; v < vocab; ++v) s += exp2_((x[v] - m) * p.c);
+  for (int v0 = 0; v0 < vocab; v0 += 4) {
+    float e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = exp2_((x[v0 + i] - m) * p.c);
+    s += (e[0] + e[1]) + (e[2] + e[3]);
+  }
   if (lane < rows) p.lse[r0 + lane] = log_sum(m, s, p.c);
   // results by way of LDS, so that the rows' are written together
   raw* val = (raw*)(few + 64 * pitch);
