@@ -46,7 +46,10 @@ struct DistillShared {
 };
 
 // A thread's entries of the teacher's row, j = i * NT + thread: logits that are
-// no entry have id -1 and p 0.  All in 64 bits: what is left of 1 is used.
+// no entry have id -1 and p 0.  p in 64 bits: what is left of 1 is used.
+// Logarithms are to the base 2.  (A library's logarithm or exponential of 64
+// bits takes 60 operations or more of two slots each: for every row of 2000
+// logits they took longer than the logits.)
 template <int NT>
 struct Entries {
   static constexpr int N = MAXK / NT > 1 ? MAXK / NT : 1;
@@ -55,9 +58,13 @@ struct Entries {
   double sum, rest;       // of the row
 };
 
+// 2^t for t <= 0 or little more, 0 far below.
+__device__ __forceinline__ double exp2_or_0(double t) { return t < -1000 ? 0.0 : exp2_64(t); }
+
 template <int NT>
 __device__ __forceinline__ void load_entries(const Teacher& t, int64_t r, int vocab, double inv_t, Entries<NT>& o,
                                              double* sh) {
+  const double c = inv_t * LOG2E;
   double m = -INFINITY, s = 0;
 #pragma unroll
   for (int i = 0; i < Entries<NT>::N; ++i) {
@@ -68,25 +75,28 @@ __device__ __forceinline__ void load_entries(const Teacher& t, int64_t r, int vo
       const int64_t id = any_id(t.ids, r * t.entries + j, t.ids_bytes);
       if (id >= 0 && id < vocab) {
         o.id[i] = (int)id;
-        o.logp[i] = any_float(t.top, r * t.entries + j, t.top_dtype) * inv_t;
+        o.logp[i] = any_float(t.top, r * t.entries + j, t.top_dtype) * c;
       }
     }
     m = o.logp[i] > m || o.logp[i] != o.logp[i] ? o.logp[i] : m;
   }
-  double ref = t.top_lse ? (double)t.top_lse[r] : block_reduce<NT, Max>(m, sh);
+  double ref = t.top_lse ? (double)t.top_lse[r] * LOG2E : block_reduce<NT, Max>(m, sh);
   if (!t.top_lse && ref == -INFINITY) ref = 0;
 #pragma unroll
   for (int i = 0; i < Entries<NT>::N; ++i) {
     o.logp[i] -= ref;
-    o.p[i] = o.id[i] < 0 ? 0.0 : exp(o.logp[i]);
-    s += o.p[i];
+    o.p[i] = 0;
+    if (i * NT < t.entries) {              // (for all threads)
+      o.p[i] = o.id[i] < 0 ? 0.0 : exp2_or_0(o.logp[i]);
+      s += o.p[i];
+    }
   }
   o.sum = block_reduce<NT, Sum>(s, sh);
   o.rest = 0;
   if (t.top_lse) {
     if (o.sum < 1) o.rest = 1 - o.sum;
   } else if (o.sum != 0) {
-    const double logs = log(o.sum), inv = 1 / o.sum;
+    const double logs = log2_((float)o.sum), inv = 1 / o.sum;
 #pragma unroll
     for (int i = 0; i < Entries<NT>::N; ++i) {
       o.logp[i] -= logs;
@@ -178,23 +188,32 @@ __device__ __forceinline__ Sums join(Sums o, float c, float* shf) {
   return o;
 }
 
-// Loss and the gradient's factors of a row from its sums.  (z: the row.)
+// Loss and the gradient's factors of a row from its sums.
+__device__ __forceinline__ float3 factors(Sums o, double sum, double& rest, double inv_t, float& qrest) {
+  const float s = o.in + o.out;
+  qrest = o.out / s;
+  if (!(rest > 0 && qrest > 0)) rest = 0;
+  const double whole = sum + rest;
+  if (!(s > 0)) return make_float3(o.m, 0.f, 0.f);
+  const float other = rest > 0 ? (float)rest / qrest : 0.f;
+  return make_float3(o.m, (float)(whole * inv_t) / s, (float)((whole - other) * inv_t) / s);
+}
+
+// (z: the row.)
 template <class T, int NT>
 __device__ __forceinline__ float3 finish_row(const Entries<NT>& t, const typename T::raw* z, Sums o, double inv_t,
                                              double* sh, float& loss) {
-  const double s = (double)o.in + o.out, logs = log(s);
-  double l = 0;
+  const double logs = log2_(o.in + o.out), c = inv_t * LOG2E;
+  double l = 0, rest = t.rest;
 #pragma unroll
   for (int i = 0; i < Entries<NT>::N; ++i)
-    if (t.id[i] >= 0 && t.p[i] != 0) l += t.p[i] * (t.logp[i] - ((double)T::get(z[t.id[i]]) - o.m) * inv_t + logs);
+    if (t.id[i] >= 0 && t.p[i] != 0) l += t.p[i] * (t.logp[i] - ((double)T::get(z[t.id[i]]) - o.m) * c + logs);
   l = block_reduce<NT, Sum>(l, sh);
-  const double qrest = o.out / s;
-  const double rest = t.rest > 0 && qrest > 0 ? t.rest : 0;
-  if (rest > 0) l += rest * (log(rest) - log(qrest));
-  loss = (float)l;
-  const double whole = t.sum + rest;
-  if (!(s > 0)) return make_float3(o.m, 0.f, 0.f);
-  return make_float3(o.m, (float)(whole * inv_t / s), (float)((whole - (rest > 0 ? rest / qrest : 0)) * inv_t / s));
+  float qrest;
+  const float3 st = factors(o, t.sum, rest, inv_t, qrest);
+  if (rest > 0) l += rest * (log2_((float)rest) - log2_(qrest));
+  loss = (float)(l * LN2);
+  return st;
 }
 
 // The gradient of the logits with numbers in [v0, v1), from c0 on: st from finish_row, w the row's weight.  The
@@ -347,18 +366,19 @@ __global__ __launch_bounds__(64) void lt_distill_few(DistillParams p) {
   const int64_t r = r0 + min(lane, rows - 1);
   float* z = few + min(lane, rows - 1) * pitch;
   const int64_t first = r * n;
+  const double c = p.inv_t * LOG2E;
   // (the entries are read again where they are used: a cache line or two a row)
   auto entry = [&](int j, int& id, double& v) {
     const int64_t i = any_id(p.t.ids, first + j, p.t.ids_bytes);
     if (i < 0 || i >= vocab) return false;
     id = (int)i;
-    v = any_float(p.t.top, first + j, p.t.top_dtype) * p.inv_t;
+    v = any_float(p.t.top, first + j, p.t.top_dtype) * c;
     return true;
   };
   int id = 0;
   double v, ref = -INFINITY, sum = 0, rest = 0, norm = 0;
   uint64_t mask = 0;
-  if (p.t.top_lse) ref = p.t.top_lse[r];
+  if (p.t.top_lse) ref = p.t.top_lse[r] * LOG2E;
   else
     for (int j = 0; j < n; ++j)
       if (entry(j, id, v)) ref = v > ref || v != v ? v : ref;
@@ -366,43 +386,41 @@ __global__ __launch_bounds__(64) void lt_distill_few(DistillParams p) {
   for (int j = 0; j < n; ++j)
     if (entry(j, id, v)) {
       mask |= 1ull << id;
-      sum += exp(v - ref);
+      sum += exp2_or_0(v - ref);
     }
   if (p.t.top_lse) {
     if (sum < 1) rest = 1 - sum;
   } else if (sum != 0) {
-    norm = log(sum);
+    norm = log2_((float)sum);
     sum = sum > 0 ? 1 : sum;               // (a NaN stays)
   }
-  float m = LOWEST, in = 0.f, out = 0.f;
-  for (int i = 0; i < vocab; i += 4) m = max2(max3(m, z[i], z[i + 1]), max2(z[i + 2], z[i + 3]));
+  Sums o;
+  for (int i = 0; i < vocab; i += 4) o.m = max2(max3(o.m, z[i], z[i + 1]), max2(z[i + 2], z[i + 3]));
   for (int i = 0; i < vocab; i += 4) {
     float e[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) e[j] = exp2_((z[i + j] - m) * p.c);
+    for (int j = 0; j < 4; ++j) e[j] = exp2_((z[i + j] - o.m) * p.c);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const bool entry = mask >> (i + j) & 1;
-      in += entry ? e[j] : 0.f;
-      out += entry ? 0.f : e[j];
+      o.in += entry ? e[j] : 0.f;
+      o.out += entry ? 0.f : e[j];
     }
   }
-  const double s = (double)in + out, logs = log(s), qrest = out / s;
-  if (!(rest > 0 && qrest > 0)) rest = 0;
-  const double whole = sum + rest;
-  const float fin = s > 0 ? (float)(whole * p.inv_t / s) : 0.f;
-  const float fout = s > 0 ? (float)((whole - (rest > 0 ? rest / qrest : 0)) * p.inv_t / s) : 0.f;
+  float qrest;
+  const float3 st = factors(o, sum, rest, p.inv_t, qrest);
   if (LOSS) {
     double loss = 0;
+    const double logs = log2_(o.in + o.out);
     for (int j = 0; j < n; ++j)
       if (entry(j, id, v)) {
-        const double logp = v - ref - norm, pj = exp(logp);
-        if (pj != 0) loss += pj * (logp - ((double)z[id] - m) * p.inv_t + logs);
+        const double logp = v - ref - norm, pj = exp2_or_0(logp);
+        if (pj != 0) loss += pj * (logp - ((double)z[id] - o.m) * c + logs);
       }
-    if (rest > 0) loss += rest * (log(rest) - log(qrest));
+    if (rest > 0) loss += rest * (log2_((float)rest) - log2_(qrest));
     if (lane < rows) {
-      p.loss[r] = (float)loss;
-      if (p.stats) *(float4*)(p.stats + r * LT_DISTILL_STATS) = make_float4(m, fin, fout, 0.f);
+      p.loss[r] = (float)(loss * LN2);
+      if (p.stats) *(float4*)(p.stats + r * LT_DISTILL_STATS) = make_float4(st.x, st.y, st.z, 0.f);
     }
   }
   if (GRAD) {
@@ -411,12 +429,12 @@ __global__ __launch_bounds__(64) void lt_distill_few(DistillParams p) {
       for (int i = 0; i < vocab; i += 4) {
         float e[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) e[j] = exp2_((z[i + j] - m) * p.c) * (mask >> (i + j) & 1 ? fin : fout) * w;
+        for (int j = 0; j < 4; ++j) e[j] = exp2_((z[i + j] - o.m) * p.c) * (mask >> (i + j) & 1 ? st.y : st.z) * w;
 #pragma unroll
         for (int j = 0; j < 4; ++j) z[i + j] = e[j];
       }
       for (int j = 0; j < n; ++j)
-        if (entry(j, id, v)) z[id] -= (float)(exp(v - ref - norm) * p.inv_t) * w;
+        if (entry(j, id, v)) z[id] -= (float)(exp2_or_0(v - ref - norm) * p.inv_t) * w;
     }
     __syncthreads();
     raw* const g = (raw*)p.grad.data;

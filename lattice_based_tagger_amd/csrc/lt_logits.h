@@ -13,6 +13,7 @@ namespace {
 
 constexpr int MAXK = LT_MAX_TOP;
 constexpr float LOWEST = -3.4028234663852886e38f;
+constexpr double LOG2E = 1.4426950408889634, LN2 = 0.6931471805599453;
 
 struct Rows {
   const void* data;
@@ -207,6 +208,34 @@ __device__ __forceinline__ float max_of(const Vec<T>& v) {
 
 // 2^x of the hardware: within an ulp, 0 below the normal numbers.
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// 2^t for -1020 < t < 1020: 2^n 2^f, n the whole number next to t, 2^f by the
+// polynomial of degree 8 through its values at the Chebyshev points of
+// [-1/2, 1/2] (relative error at most 1.1e-12; the series needs degree 10 for
+// that).  n is added to the exponent's bits.
+__device__ __forceinline__ double exp2_64(double t) {
+  constexpr double BIG = 6755399441055744.0;       // 1.5 * 2^52: its last bits are whole numbers
+  const double b = t + BIG;
+  const double f = t - (b - BIG);
+  double r = 1.325497460306718e-06;
+  r = fma(r, f, 1.531007807039615e-05);
+  r = fma(r, f, 0.00015403457039410448);
+  r = fma(r, f, 0.0013333450573018062);
+  r = fma(r, f, 0.009618129157656703);
+  r = fma(r, f, 0.055504109412010456);
+  r = fma(r, f, 0.24022650695821055);
+  r = fma(r, f, 0.6931471805459343);
+  r = fma(r, f, 0.9999999999999997);
+  const uint64_t bits = __builtin_bit_cast(uint64_t, r);
+  const uint32_t hi = (uint32_t)(bits >> 32) + ((uint32_t)__builtin_bit_cast(uint64_t, b) << 20);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)bits);
+}
+
+// log2 of a sum in 32 bits, good to 2^-23 absolutely (the hardware's logarithm
+// of the whole would be good to 2^-23 of its value, up to 30 here).
+__device__ __forceinline__ double log2_(float s) {
+  return (double)__builtin_amdgcn_frexp_expf(s) + (double)__builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(s));
+}
 
 __device__ __forceinline__ float any_float(const void* p, int64_t i, int dtype) {
   if (dtype == LT_F32) return ((const float*)p)[i];
@@ -453,7 +482,5 @@ lt_status launch(void (*kernel)(P), int64_t blocks, int threads, P p, void* stre
 #define ON_DEVICE(d)                                                                                   \
   OnDevice on(d);                                                                                      \
   if (on.err != hipSuccess) return lt::set_error(LT_EHIP, "device %d: %s", (int)(d), hipGetErrorString(on.err))
-
-constexpr double LOG2E = 1.4426950408889634;
 
 }  // namespace

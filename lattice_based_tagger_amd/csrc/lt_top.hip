@@ -16,6 +16,7 @@ struct TopParams {
   int32_t splits;         // blocks of a row
   int32_t chunk;          // of a row's numbers, to a block (a multiple of its step)
   float c;                // log2(e) / temperature
+  double inv_t;           // 1 / temperature
   void* values;
   int64_t* ids;
   float* lse;
@@ -23,10 +24,9 @@ struct TopParams {
   float2* part_sums;      // [rows][splits]: reference and sum
 };
 
-// The sum behind a log-sum-exp: that of exp2((x - m) c), m any logit at most 32
-// (in the exponent) below the largest seen.
-__device__ __forceinline__ float log_sum(float m, float s, float c) {
-  return m == INFINITY ? m : (float)((double)m * (c * 0.6931471805599453) + (double)__builtin_amdgcn_logf(s) * 0.6931471805599453);
+// The log-sum-exp of a row whose exp2((x - m) c) sum up to s.
+__device__ __forceinline__ float log_sum(float m, float s, double inv_t) {
+  return m == INFINITY ? m : (float)(m * inv_t + log2_(s) * LN2);
 }
 
 // The key of lane ^ X: by the data-parallel primitives where they can, else by
@@ -409,7 +409,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
     sort_keys<NT, C>(buf, n, k);
   }
   if (p.splits == 1) {
-    if (tid == 0) p.lse[r] = log_sum(top, sum, p.c);
+    if (tid == 0) p.lse[r] = log_sum(top, sum, p.inv_t);
     for (int j = tid; j < k; j += NT) {
       const uint32_t id = ~(uint32_t)buf[j];
       p.ids[r * k + j] = id;
@@ -444,7 +444,7 @@ __global__ __launch_bounds__(256) void lt_top_join(TopParams p) {
     left = p.k;
   }
   sort_keys<NT, C>(sh.buf, left, p.k);
-  if (tid == 0) p.lse[r] = log_sum(m, s, p.c);
+  if (tid == 0) p.lse[r] = log_sum(m, s, p.inv_t);
   const typename T::raw* x = (const typename T::raw*)p.x.data + p.x.at(r);
   for (int j = tid; j < p.k; j += NT) {
     const uint32_t id = ~(uint32_t)sh.buf[j];
@@ -495,7 +495,7 @@ __global__ __launch_bounds__(64) void lt_top_few(TopParams p) {
     for (int i = 0; i < 4; ++i) e[i] = exp2_((x[v0 + i] - m) * p.c);
     s += (e[0] + e[1]) + (e[2] + e[3]);
   }
-  if (lane < rows) p.lse[r0 + lane] = log_sum(m, s, p.c);
+  if (lane < rows) p.lse[r0 + lane] = log_sum(m, s, p.inv_t);
   // results by way of LDS, so that the rows' are written together
   raw* val = (raw*)(few + 64 * pitch);
   uint8_t* at = (uint8_t*)(val + 64 * p.k);
@@ -538,7 +538,7 @@ __global__ __launch_bounds__(256) void lt_top_small(TopParams p) {
   s = wave_reduce<Sum>(s, 0.f);
   sync<64>();
   sort_keys<64, SMALL>(buf, vocab, p.k);
-  if (lane == 0) p.lse[r] = log_sum(m, s, p.c);
+  if (lane == 0) p.lse[r] = log_sum(m, s, p.inv_t);
 #pragma unroll
   for (int i = 0; i < SMALL / 64; ++i) {
     const int j = i * 64 + lane;
@@ -630,6 +630,7 @@ lt_status lt_top_logits(const lt_rows* x, int32_t k, double temperature, void* v
   p.rows = x->rows;
   p.k = k;
   p.c = (float)(LOG2E / temperature);
+  p.inv_t = 1 / temperature;
   p.values = values;
   p.ids = ids;
   p.lse = lse;

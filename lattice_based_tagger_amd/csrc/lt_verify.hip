@@ -14,28 +14,6 @@
 
 namespace {
 
-// 2^t for -1020 < t < 1020: 2^n 2^f, n the whole number next to t, 2^f by the
-// polynomial of degree 8 through its values at the Chebyshev points of
-// [-1/2, 1/2] (relative error at most 1.1e-12; the series needs degree 10 for
-// that).  n is added to the exponent's bits.
-__device__ __forceinline__ double exp2_64(double t) {
-  constexpr double BIG = 6755399441055744.0;       // 1.5 * 2^52: its last bits are whole numbers
-  const double b = t + BIG;
-  const double f = t - (b - BIG);
-  double r = 1.325497460306718e-06;
-  r = fma(r, f, 1.531007807039615e-05);
-  r = fma(r, f, 0.00015403457039410448);
-  r = fma(r, f, 0.0013333450573018062);
-  r = fma(r, f, 0.009618129157656703);
-  r = fma(r, f, 0.055504109412010456);
-  r = fma(r, f, 0.24022650695821055);
-  r = fma(r, f, 0.6931471805459343);
-  r = fma(r, f, 0.9999999999999997);
-  const uint64_t bits = __builtin_bit_cast(uint64_t, r);
-  const uint32_t hi = (uint32_t)(bits >> 32) + ((uint32_t)__builtin_bit_cast(uint64_t, b) << 20);
-  return __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)bits);
-}
-
 // Four at a time: a step of one takes 8 cycles or more until the next may use
 // it, and few waves are there to fill them.
 __device__ __forceinline__ void exp2_64(double (&t)[4]) {
