@@ -10,6 +10,8 @@
 // one or two rows that it is drawn from are summed in 64 bits with an
 // exponential good to 1.1e-12.  That costs 35 issue slots a logit (a 64-bit
 // operation takes two), where memory allows 14; the sums in 32 bits take 9.
+#include <type_traits>
+
 #include "lt_logits.h"
 
 namespace {
@@ -127,7 +129,9 @@ struct Soft {
 // A row's chunks, one after another.
 __device__ __forceinline__ Soft join_parts(const float2* part, int splits, double c) {
   Soft o;
+#pragma unroll 8
   for (int i = 0; i < splits; ++i) o.m = fmaxf(o.m, part[i].x);
+#pragma unroll 4
   for (int i = 0; i < splits; ++i) o.s += part[i].y * exp2_64(fmax(((double)part[i].x - o.m) * c, -DEPTH));
   return o;
 }
@@ -404,43 +408,62 @@ __global__ __launch_bounds__(NT) void lt_verify_draw(VerifyParams p) {
     const double2 w = weights[s];
     return st.y ? fmax(w.x - st.ratio * w.y, 0.0) : w.x;
   };
-  // running sums over a block's threads, `before` ahead of them; all: the last's
-  auto scan = [&](double w, double before, double& all) {
-    double cum = wave_scan<Sum>(w, 0.0);
-    if (lane == 63) shd[wave] = cum;
-    __syncthreads();
-    cum += before;
-    all = before;
-#pragma unroll
-    for (int i = 0; i < NT / 64; ++i) {
-      if (i < wave) cum += shd[i];
-      all += shd[i];
-    }
-    __syncthreads();
-    return cum;
-  };
-  // The first of [from, to) whose sum passes the line, else the last with a
-  // weight, else -1; and the sum ahead of it.
-  auto cross = [&](int from, int to, double line, double& before, auto weight) {
+  // The first of [from, to) whose running sum (from `before` on) passes the
+  // line, else the last with a weight, else -1; before: the sum ahead of it.
+  // A thread takes Q neighbours at a time.
+  auto cross = [&](auto q, int from, int to, double line, double& before, auto weight) {
+    constexpr int Q = decltype(q)::value;
     if (tid == 0) first = 0x7fffffff, last = -1;
-    __syncthreads();
-    for (int i0 = from; i0 < to; i0 += NT) {
-      const double w = i0 + tid < to ? weight(i0 + tid) : 0.0;
-      double all;
-      const double cum = scan(w, before, all);
-      if (w > 0) {
-        if (cum > line) atomicMin(&first, i0 + tid);
-        atomicMax(&last, i0 + tid);
+    double ahead = 0, last_ahead = 0;      // of this thread's first past the line, of its last with a weight
+    int mine = -1, my_last = -1;
+    for (int i0 = from; i0 < to; i0 += NT * Q) {
+      const int i = i0 + tid * Q;
+      double w[Q], sum = 0;
+#pragma unroll
+      for (int j = 0; j < Q; ++j) w[j] = i + j < to ? weight(i + j) : 0.0;
+#pragma unroll
+      for (int j = 0; j < Q; ++j) sum += w[j];
+      double cum = wave_scan<Sum>(sum, 0.0);
+      if (lane == 63) shd[wave] = cum;
+      __syncthreads();
+      double all = before;
+      cum += before - sum;
+#pragma unroll
+      for (int k = 0; k < NT / 64; ++k) {
+        if (k < wave) cum += shd[k];
+        all += shd[k];
       }
+#pragma unroll
+      for (int j = 0; j < Q; ++j) {
+        if (w[j] > 0) {
+          if (mine < 0 && cum + w[j] > line) mine = i + j, ahead = cum;
+          my_last = i + j, last_ahead = cum;
+        }
+        cum += w[j];
+      }
+      if (mine >= 0) atomicMin(&first, mine);
       __syncthreads();
       if (first != 0x7fffffff) break;
       before = all;
     }
     __syncthreads();
-    const int at = first != 0x7fffffff ? first : last;
+    int at = first;
+    if (at == 0x7fffffff) {
+      atomicMax(&last, my_last);
+      __syncthreads();
+      at = last;
+      mine = my_last;
+      ahead = last_ahead;
+    }
+    if (at >= 0 && mine == at) shd[0] = ahead;
+    __syncthreads();
+    before = shd[0];
     __syncthreads();
     return at;
   };
+  using std::integral_constant;
+  constexpr integral_constant<int, 4> FOUR;
+  constexpr integral_constant<int, SEG / NT> STEP;
   double total = 0;
   for (int s = tid; s < segments; s += NT) total += segment(s);
   total = block_reduce<NT, Sum>(total, shd);
@@ -449,24 +472,18 @@ __global__ __launch_bounds__(NT) void lt_verify_draw(VerifyParams p) {
   if (total > 0) {
     const double line = p.sample_u[b] * total;
     double before = 0;
-    const int s = cross(0, segments, line, before, segment);
-    // (ahead of segment s: what lies in the steps before its own, and in its own)
-    double ahead = 0, all;
-    for (int s0 = 0; s0 < s; s0 += NT) {
-      (void)scan(s0 + tid < s ? segment(s0 + tid) : 0.0, ahead, all);
-      ahead = all;
-    }
-    token = cross(max(0, s * SEG - lead), min(p.target.vocab, (s + 1) * SEG - lead), line, ahead, of_token);
+    const int s = cross(FOUR, 0, segments, line, before, segment);
+    token = cross(STEP, max(0, s * SEG - lead), min(p.target.vocab, (s + 1) * SEG - lead), line, before, of_token);
     if (token < 0) {
       before = 0;                          // (a segment of rounding errors)
-      token = cross(0, p.target.vocab, line, before, of_token);
+      token = cross(STEP, 0, p.target.vocab, line, before, of_token);
     }
   }
   if (token < 0 && sp > 0) {
     st.y = nullptr;
     st.id = -1;
     double before = 0;
-    token = cross(0, p.target.vocab, p.sample_u[b] * sp, before, of_token);
+    token = cross(STEP, 0, p.target.vocab, p.sample_u[b] * sp, before, of_token);
   }
   if (tid == 0) p.accepted[b] = note.a;
   for (int i = tid; i <= p.drafts; i += NT)
@@ -498,7 +515,7 @@ void plan(VerifyParams& p, int dtype) {
   // steps), 30 to join them, 3 roundings of an exponent of 12 and one of its
   // power of 2; twice that for two
   p.margin = 2 * (16 + p.chunk / step + 30 + p.splits + 3 * 12 + 2) * 0x1p-24;
-  n = chunks(numbers, vectors, p.batch, 4096);
+  n = chunks(numbers, vectors, p.batch, 1024);
   p.weigh_chunk = (int32_t)((numbers + n * vectors - 1) / (n * vectors) * vectors);
   p.weigh_splits = (int32_t)((numbers + p.weigh_chunk - 1) / p.weigh_chunk);
 }
