@@ -555,15 +555,16 @@ __global__ __launch_bounds__(256) void lt_top_small(TopParams p) {
 // 8 chunks 10 us, and 4 us to join them in a launch of its own.)
 void split_rows(TopParams& p, int dtype) {
   const int step = 512 * 4 * (dtype == LT_F32 ? 4 : 8);
+  const int64_t numbers = (int64_t)p.x.vocab + LEAD;
   int64_t n = 1;
   if (p.x.vocab > 6 * step && p.rows < 256) {
-    n = (p.x.vocab + step - 1) / step;
+    n = (numbers + step - 1) / step;
     n = n < 512 / p.rows ? n : 512 / p.rows;
     n = n < JOIN / p.k ? n : JOIN / p.k;
   }
-  const int64_t steps = (p.x.vocab + n * step - 1) / (n * step);
+  const int64_t steps = (numbers + n * step - 1) / (n * step);
   p.chunk = (int32_t)(n == 1 ? 0x7fffff80 : steps * step);
-  p.splits = (int32_t)(((int64_t)p.x.vocab + LEAD + p.chunk - 1) / p.chunk);
+  p.splits = (int32_t)((numbers + p.chunk - 1) / p.chunk);     // at most n: JOIN keys hold
 }
 
 int64_t top_workspace(const TopParams& p) {

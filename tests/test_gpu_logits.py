@@ -119,6 +119,16 @@ def test_top_views():
     assert got.values.shape == (4, 0, 9) and got.lse.shape == (4, 0)
 
 
+@pytest.mark.parametrize('vocab, k', [(131072, 256), (131072, 16), (262144, 255), (114688, 128)])
+def test_top_chunks_off_the_grid(vocab, k):
+    """Chunks that a row starting off the grid of its vectors overruns by a few logits."""
+    for dtype in (torch.bfloat16, torch.float32):
+        x = rand((2, vocab + 5), dtype, 90)
+        x[:, -30:] += 20                                # the best behind the last whole chunk
+        check_top(x[:1, 5:], k)
+        check_top(x[:, 3:3 + vocab], k)
+
+
 def test_top_many_rows():
     """More rows than blocks are ever resident, of a tag set and of a small vocabulary."""
     check_top(rand((20011, 13), torch.float32, 1), 13)

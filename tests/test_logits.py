@@ -44,6 +44,7 @@ TOP = torch.zeros(2, 3, 4)
     (ValueError, 'adjacent', lambda: logits.top_logits(X.transpose(1, 2), 1)),
     (ValueError, 'two strides', lambda: logits.top_logits(torch.zeros(4, 4, 4, 9)[::2, ::2, ::2], 1)),
     (ValueError, 'k must be', lambda: logits.top_logits(X, 0)),
+    (TypeError, 'integer', lambda: logits.top_logits(X, 2.5)),
     (ValueError, 'k must be', lambda: logits.top_logits(X, 11)),
     (ValueError, 'k must be', lambda: logits.top_logits(torch.zeros(1, 1000), 257)),
     (ValueError, 'temperature', lambda: logits.top_logits(X, 1, temperature=0)),
@@ -141,6 +142,20 @@ def test_c_entry_refuses_a_short_workspace():
         assert b'workspace' in _capi.load().lt_last_error()
     assert lib.lt_top_logits_workspace(C.byref(_desc(rows=1000, vocab=200000)), 20) == 0
     assert lib.lt_top_logits_workspace(None, 20) == 0
+
+
+@pytest.mark.parametrize('dtype', [0, 1, 2])
+def test_chunks_of_a_row_fit_their_join(dtype):
+    """What is joined of a row's chunks -- the workspace is rows * chunks * (8 k + 8)
+    bytes -- is at most 1024 keys, however the row divides."""
+    lib = logits._load()
+    for rows in (1, 2, 3, 7, 60, 255):
+        for vocab in [16384 * n + d for n in (4, 6, 7, 8, 13, 64, 1000) for d in (-65, -1, 0, 1, 63)]:
+            for k in (1, 5, 16, 127, 128, 129, 255, 256):
+                x = _desc(rows=rows, vocab=vocab, stride_outer=vocab, dtype=dtype)
+                need = lib.lt_top_logits_workspace(C.byref(x), k)
+                assert need % (rows * (8 * k + 8)) == 0
+                assert need // (rows * (8 * k + 8)) * k <= 1024
 
 
 @pytest.mark.parametrize('entries, ids_bytes, dtype', [(0, 8, 0), (257, 8, 0), (1, 2, 0), (1, 8, 3)])
