@@ -29,6 +29,7 @@ float32 at least.
 """
 
 import ctypes as C
+import operator
 import threading
 from collections import namedtuple
 
@@ -214,7 +215,7 @@ def top_logits(logits, k, temperature=1.0):
     (-inf for a row of -inf, NaN where the row holds a NaN).
     ``1 <= k <= min(vocab, 256)``.  Not differentiable."""
     _logits(logits, 'logits')
-    k = int(k)
+    k = operator.index(k)
     if not 1 <= k <= min(MAX_TOP, logits.shape[-1]):
         raise ValueError('k must be within 1 .. min(vocab, %d), not %d' % (MAX_TOP, k))
     temperature = _temperature(temperature)
