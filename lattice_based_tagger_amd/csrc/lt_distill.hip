@@ -617,7 +617,7 @@ lt_status lt_distill_fused(const lt_rows* z, const lt_teacher* t, double tempera
   if (!workspace_ok(p, workspace, workspace_bytes)) BAD("workspace: %lld bytes, 16 B aligned, are needed", (long long)lt_distill_workspace(z, t->entries));
   p.part = (float4*)workspace;
   p.loss = loss;
-  p.stats = workspace ? (float*)((char*)workspace + parts_bytes(p)) : nullptr;
+  p.stats = p.splits > 1 ? (float*)((char*)workspace + parts_bytes(p)) : nullptr;
   p.scale = (float)scale;
   p.weight = weight;
   p.weight_stride = weight_stride;

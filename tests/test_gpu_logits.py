@@ -2,6 +2,7 @@
 CPU), with its bounds: the k best and whole numbers exactly, the rest within
 the rounding of float32 sums and of the output's type."""
 
+import ctypes as C
 import math
 
 import pytest
@@ -291,6 +292,24 @@ def test_distill_types_and_views():
     check_distill(one.expand(3, 1001), *teacher(one.expand(3, 1001), 6, torch.float32, 16, True, 1.0))
     ids, top, lse = teacher(one[None], 6, torch.float32, 16, True, 1.0)
     check_distill(one, ids[0], top[0], lse[0], weight=torch.tensor(0.5).cuda())
+
+
+@pytest.mark.parametrize('rows, vocab', [(5000, 41), (300, 41), (70, 1200), (300, 20000)])
+def test_distill_leaves_a_workspace_it_needs_not(rows, vocab):
+    """A caller's scratch memory that a call has no use for stays as it is."""
+    z = rand((rows, vocab), torch.float32, 21)
+    ids, top, lse = teacher(z, 5, torch.float32, 22, True, 1.0)
+    lib = logits._load()
+    x, t = logits._rows(z, 'logits'), logits._teacher_desc(ids, top, lse)
+    assert lib.lt_distill_workspace(C.byref(x), 5) == 0
+    work = torch.full((rows * 16,), 77, dtype=torch.uint8, device='cuda')
+    loss, grad = torch.empty(rows, device='cuda'), torch.empty_like(z)
+    out = logits._rows(grad, 'grad')
+    assert lib.lt_distill_fused(C.byref(x), C.byref(t), 1.0, 1.0, None, 0, loss.data_ptr(), C.byref(out),
+                                work.data_ptr(), 0, logits._stream(z)) == 0
+    want = logits.distill_loss_grad(z, ids, top, 1.0, top_lse=lse)
+    assert torch.equal(loss, want[0]) and torch.equal(grad, want[1])
+    assert (work == 77).all()
 
 
 def test_distill_weights():
