@@ -16,7 +16,7 @@
  * synchronise, and may be captured into a graph.  Scratch memory is the
  * caller's: a buffer of at least lt_*_workspace bytes, 16 B aligned, that no
  * other call uses until this one's kernels are complete (its contents need
- * not be kept nor cleared).  The stream must be of the same device and of the
+ * not be kept nor cleared; NULL where 0 bytes are needed).  The stream must be of the same device and of the
  * HIP runtime this library is bound to (lt_hip_library).  Calls may be made
  * from several threads at once.  Errors as in lattice_decode.h (lt_status,
  * lt_last_error).
@@ -80,8 +80,8 @@ lt_status lt_top_logits(const lt_rows* x, int32_t k, double temperature, void* v
  *   d loss / d z_v = 1/temperature * (P q_v - sum_{id_j = v} p_j)       v an entry
  *                    1/temperature * (P - p_rest / q_rest) q_v         else
  *     with P = sum p_j + p_rest
- * A row without entries has loss 0 and gradient 0.  An id that a row repeats
- * counts once for each time.  The teacher is a constant.
+ * A row without entries has loss 0 and gradient 0, whatever its logits, top and
+ * top_lse hold.  An id that a row repeats counts once for each time.  The teacher is a constant.
  * 1 <= K <= LT_MAX_TOP. */
 typedef struct {
   const void* ids;        /* [rows][entries] int32 or int64 */
@@ -94,13 +94,14 @@ typedef struct {
 
 #define LT_DISTILL_STATS 4   /* floats a row that the forward leaves for the backward */
 
-/* loss[rows]; stats[rows * LT_DISTILL_STATS]. */
+/* loss[rows]; stats[rows * LT_DISTILL_STATS], 16 B aligned. */
 int64_t lt_distill_workspace(const lt_rows* z, int32_t entries);
 lt_status lt_distill_forward(const lt_rows* z, const lt_teacher* t, double temperature, float* loss, float* stats,
                              void* workspace, int64_t workspace_bytes, void* stream);
 /* grad: rows as z (its data, strides; same dtype and vocab) =
  * scale * weight[r * weight_stride] * d loss_r / d z; weight NULL: 1.
- * stats as the forward of the same arguments left them.  weight_stride 0 or 1. */
+ * stats as the forward of the same arguments left them.  weight_stride 0 or 1.
+ * No row of grad overlaps a row of z or another of its own. */
 lt_status lt_distill_backward(const lt_rows* z, const lt_teacher* t, double temperature, const float* stats,
                               double scale, const float* weight, int64_t weight_stride, const lt_rows* grad,
                               void* stream);

@@ -56,7 +56,14 @@ struct Entries {
   int id[N];
   double p[N], logp[N];
   double sum, rest;       // of the row
+  // Nothing to learn: no entry, or none with a weight.  Loss and gradient are 0
+  // whatever the logits are (a padded position's are often NaN); they are not read.
+  __device__ __forceinline__ bool blank() const { return sum == 0 && rest == 0; }
 };
+
+// With top_lse, an entry too unlikely for its p to be more than 0 still tells its
+// row from one without entries.
+constexpr double TRACE = 1e-300;
 
 // 2^t for t <= 0 or little more, 0 far below.
 __device__ __forceinline__ double exp2_or_0(double t) { return t < -1000 ? 0.0 : exp2_64(t); }
@@ -88,13 +95,13 @@ __device__ __forceinline__ void load_entries(const Teacher& t, int64_t r, int vo
     o.p[i] = 0;
     if (i * NT < t.entries) {              // (for all threads)
       o.p[i] = o.id[i] < 0 ? 0.0 : exp2_or_0(o.logp[i]);
-      s += o.p[i];
+      s += t.top_lse && o.id[i] >= 0 && o.p[i] == 0 ? TRACE : o.p[i];
     }
   }
   o.sum = block_reduce<NT, Sum>(s, sh);
   o.rest = 0;
   if (t.top_lse) {
-    if (o.sum < 1) o.rest = 1 - o.sum;
+    if (o.sum > 0 && o.sum < 1) o.rest = 1 - o.sum;
   } else if (o.sum != 0) {
     const double logs = log2_((float)o.sum), inv = 1 / o.sum;
 #pragma unroll
@@ -227,6 +234,15 @@ __device__ __forceinline__ void grad_row(const typename T::raw* row, typename T:
   const float out = st.z * w;
   const typename T::raw* const z = row - lead;
   typename T::raw* const g = grad - lead;
+  if (t.blank()) {
+    Vec<T> none;
+    none.b = {};
+    for (int at = c0 + tid * E; at < v1; at += NT * E) {
+      if (at >= v0 && at + E <= v1) none.store(g + at);
+      else none.store_part(g, at, v0, v1);
+    }
+    return;
+  }
   for (int base = c0; base < v1; base += STEP) {
     Vec<T> v[U];
     load_step<T, NT, U, AGAIN>(v, z, base, tid, v0, v1);
@@ -291,7 +307,8 @@ __device__ __forceinline__ void grad_row(const typename T::raw* row, typename T:
 template <class T, int NT, int U, int WINDOW, bool TAIL>
 __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_distill_sums(DistillParams p) {
   GROUP_HEAD;
-  const Sums o = join<NT>(sum_row<T, NT, U, WINDOW, TAIL>(z, lead, c0, v0, v1, p.c, t, sh), p.c, sh.shf);
+  Sums o;
+  if (!t.blank()) o = join<NT>(sum_row<T, NT, U, WINDOW, TAIL>(z, lead, c0, v0, v1, p.c, t, sh), p.c, sh.shf);
   if (p.splits > 1) {
     if (thread_of<NT>() == 0) p.part[blk] = make_float4(o.m, o.in, o.out, 0.f);
     return;
@@ -344,7 +361,8 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_distill_grad(DistillPa
 template <class T, int NT, int U, int WINDOW, bool TAIL>
 __global__ __launch_bounds__(NT == 64 ? 256 : NT, NT == 64 ? 1 : 8) void lt_distill_both(DistillParams p) {
   GROUP_HEAD;
-  const Sums o = join<NT>(sum_row<T, NT, U, WINDOW, TAIL>(z, lead, c0, v0, v1, p.c, t, sh), p.c, sh.shf);
+  Sums o;
+  if (!t.blank()) o = join<NT>(sum_row<T, NT, U, WINDOW, TAIL>(z, lead, c0, v0, v1, p.c, t, sh), p.c, sh.shf);
   float loss;
   const float3 st = finish_row<T, NT>(t, z, o, p.inv_t, sh.sh, loss);
   if (thread_of<NT>() == 0) p.loss[r] = loss;
@@ -386,14 +404,16 @@ __global__ __launch_bounds__(64) void lt_distill_few(DistillParams p) {
   for (int j = 0; j < n; ++j)
     if (entry(j, id, v)) {
       mask |= 1ull << id;
-      sum += exp2_or_0(v - ref);
+      const double pj = exp2_or_0(v - ref);
+      sum += p.t.top_lse && pj == 0 ? TRACE : pj;
     }
   if (p.t.top_lse) {
-    if (sum < 1) rest = 1 - sum;
+    if (sum > 0 && sum < 1) rest = 1 - sum;
   } else if (sum != 0) {
     norm = log2_((float)sum);
     sum = sum > 0 ? 1 : sum;               // (a NaN stays)
   }
+  const bool blank = sum == 0 && rest == 0;
   Sums o;
   for (int i = 0; i < vocab; i += 4) o.m = max2(max3(o.m, z[i], z[i + 1]), max2(z[i + 2], z[i + 3]));
   for (int i = 0; i < vocab; i += 4) {
@@ -431,9 +451,9 @@ __global__ __launch_bounds__(64) void lt_distill_few(DistillParams p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) e[j] = exp2_((z[i + j] - o.m) * p.c) * (mask >> (i + j) & 1 ? st.y : st.z) * w;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) z[i + j] = e[j];
+        for (int j = 0; j < 4; ++j) z[i + j] = blank ? 0.f : e[j];
       }
-      for (int j = 0; j < n; ++j)
+      for (int j = 0; j < n && !blank; ++j)
         if (entry(j, id, v)) z[id] -= (float)(exp2_or_0(v - ref - norm) * p.inv_t) * w;
     }
     __syncthreads();

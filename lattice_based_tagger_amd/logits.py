@@ -327,7 +327,8 @@ def distill_loss(logits, top_ids, top_values, top_lse=None, temperature=1.0):
       of the vocabulary as one more place with what is left of 1 (left out
       where the student's logits leave it nothing).
 
-    A row without entries -- padding: every id -1 -- has loss 0 and gradient 0.
+    A row without entries -- padding: every id -1 -- has loss 0 and gradient 0,
+    whatever its logits are.
     No factor temperature^2 is applied, and no reduction.  The teacher is a
     constant: no gradient flows to it, and there is no second derivative."""
     _logits(logits, 'logits')

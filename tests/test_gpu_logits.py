@@ -254,6 +254,50 @@ def test_distill_masks(vocab):
     assert torch.isfinite(loss).all() and torch.isfinite(grad).all()
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('rows, vocab, pad', [(4200, 41, 0), (40, 41, 0), (40, 1999, 1), (40, 16383, 0), (40, 70001, 0),
+                                              (600, 20000, 3)])
+def test_distill_blank_rows(dtype, rows, vocab, pad):
+    """Padded positions hold anything: logits of NaN, infinities or -inf throughout,
+    entries of NaN, a log-sum-exp of NaN.  Their loss and gradient are 0, the
+    others' what they are without them."""
+    z = rand((rows, vocab), dtype, 23, pad=pad)
+    ids, top, lse = teacher(z, 4, dtype, 24, True, 1.0)
+    weight = torch.rand(rows, generator=torch.Generator().manual_seed(3)).cuda()
+    blank = torch.arange(rows, device='cuda') % 5 > 2
+    for use in (None, lse):
+        want = logits.distill_loss_grad(z, ids, top, weight, top_lse=use)
+        i, t, l = ids.clone(), top.clone(), None if use is None else use.clone()
+        x = torch.empty(rows, vocab + pad, dtype=dtype, device='cuda')[:, :vocab].copy_(z)
+        i[blank] = -1
+        i[blank, 1:] = vocab
+        for n, v in enumerate((math.nan, INF, -INF)):
+            x[3 + 5 * n::15] = v
+            x[4 + 5 * n::15, ::3] = v
+            t[3 + 5 * n::15] = v
+            if l is not None:
+                l[3 + 5 * n::15] = v
+        x.requires_grad_()
+        loss = logits.distill_loss(x, i, t, top_lse=l)
+        grad, = torch.autograd.grad(loss, x, weight)
+        for got in ((loss.detach(), grad), logits.distill_loss_grad(x.detach(), i, t, weight, top_lse=l)):
+            assert not got[0][blank].any() and not got[1][blank].any()
+            assert torch.equal(got[0][~blank], want[0][~blank])
+            assert (got[1][~blank].float() - want[1][~blank].float()).abs().max() <= \
+                4 * plain.HALF_STEP[dtype] * want[1][~blank].float().abs().max()
+
+
+def test_distill_unlikely_entries():
+    """With the teacher's log-sum-exp, entries whose p is 0 in 64 bits too: all of
+    the mass is the rest's, and the loss -log q_rest."""
+    for vocab in (30, 41, 1200, 70000):
+        rows = 4200 if vocab == 41 else 3
+        z = rand((rows, vocab), torch.float32, 25)
+        ids, top, _ = teacher(z, 4, torch.float32, 26, False, 1.0)
+        check_distill(z, ids, torch.full_like(top, -900.0), torch.zeros(rows, device='cuda'))
+        check_distill(z, ids, torch.full_like(top, -INF), torch.zeros(rows, device='cuda'))
+
+
 def test_distill_repeated_ids():
     z = rand((5, 500), torch.float32, 8)
     ids, top, lse = teacher(z, 12, torch.float32, 9, True, 1.0)
