@@ -257,13 +257,14 @@ def _teacher_desc(ids, top, lse):
 
 
 def _grad_like(x):
-    """Memory for a gradient whose rows lie as ``x``'s do, where those do not
-    overlap: rows of one alignment load and store alike."""
+    """Memory for a gradient.  Rows with a little between them, as a projection
+    padded for its alignment leaves, get the same: rows of one alignment load and
+    store alike."""
     if x.is_contiguous():
         return x.new_empty(x.shape)
     v = x.shape[-1]
     pitch = x.stride(-2) if x.dim() > 1 else v
-    if pitch <= v or pitch > v + 1024:
+    if pitch <= v or pitch > v + v // 8:
         return x.new_empty(x.shape)
     return x.new_empty(x.shape[:-1] + (pitch,))[..., :v]
 

@@ -356,6 +356,17 @@ def test_distill_leaves_a_workspace_it_needs_not(rows, vocab):
     assert (work == 77).all()
 
 
+def test_distill_gradients_memory():
+    """A gradient lies as its logits do where these have a few elements between
+    their rows; else it is contiguous."""
+    for shape, pad, pitch in (((5, 1000), 24, 1024), ((5, 1000), 1048, 1000), ((5, 41), 471, 41), ((2, 3, 800), 8, 808)):
+        z = rand(shape, torch.bfloat16, 27, pad=pad)
+        ids, top, _ = teacher(z, 3, torch.bfloat16, 28, False, 1.0)
+        _, grad = logits.distill_loss_grad(z, ids, top, 1.0)
+        assert grad.stride(-2) == pitch and grad.untyped_storage().nbytes() <= 2 * pitch * z[..., 0].numel()
+        check_distill(z, ids, top)
+
+
 def test_distill_weights():
     """Gradients of sums, means and numbers; of a broadcast input."""
     z = rand((6, 400), torch.float32, 17)
@@ -473,6 +484,90 @@ def test_verify_edges():
     a['accept_u'][2] = 1 - 2.0 ** -24
     a['target'][3, 0, a['draft_ids'][3, 0]] = -INF
     check_verify(**a)
+
+
+@pytest.mark.parametrize('certain, batch, drafts, vocab', [(False, 120, 3, 300007), (True, 290, 2, 262144)])
+def test_verify_large_batches(certain, batch, drafts, vocab):
+    """More than 128 MB of logits at a place, which are taken place by place: drafts
+    of every length, refused and accepted ones, and ones that sums in 32 bits leave
+    open; what lies behind a draft's end is not read."""
+    a = drafted(batch, drafts, vocab, torch.bfloat16, 41, certain, noise=0.1)
+    n = torch.arange(batch, dtype=torch.int32) % (drafts + 1)
+    n[:40] = drafts
+    if not certain:
+        for b in range(4, 24, 4):                      # alike: accepted, exactly
+            a['draft'][b] = a['target'][b, :drafts]
+            a['accept_u'][b] = 1 - 2.0 ** -24
+    a['draft_ids'][5, 0] = -1
+    a['draft_ids'][6, drafts - 1] = vocab
+    a['target'][7, 0, :-9] = -INF
+    for b in range(40, batch):
+        a['target'][b, n[b] + 1:] = math.nan
+        a['draft_ids'][b, n[b]:] = 2 ** 50
+        a['accept_u'][b, n[b]:] = math.nan
+        if not certain:
+            a['draft'][b, n[b]:] = math.nan
+    got = check_verify(lengths=n.cuda(), **a)
+    # (of 262144 words the likeliest has a probability of some 0.05: few are accepted)
+    assert set(got.accepted.tolist()) >= ({0, 1} if certain else set(range(drafts + 1)))
+
+
+# ---- many logits ------------------------------------------------------------
+
+def check_last(x, got, n, exact):
+    """Loss and gradient of all rows at once, of the last n as a copy of them alone
+    gives: exactly, or, where the copy's rows lie otherwise on the vectors' grid or
+    are divided among blocks, within what sums of another order may differ by --
+    6 delta of the loss (three logarithms of sums), 4 delta of q <= 1 in each
+    gradient, and its rounding."""
+    top, lse = got.values.roll(1, 0), got.lse.roll(1, 0)
+    for tail in (None, lse):
+        cut = lambda t: None if t is None else t[-n:].clone()
+        loss, grad = logits.distill_loss_grad(x, got.ids, top, 0.5, top_lse=tail)
+        want = logits.distill_loss_grad(cut(x), cut(got.ids), cut(top), 0.5, top_lse=cut(tail))
+        assert want[1].any()
+        if exact:
+            assert torch.equal(loss[-n:], want[0]) and torch.equal(grad[-n:], want[1])
+        else:
+            d = plain.delta(x.shape[-1])
+            assert (loss[-n:] - want[0]).abs().max() <= 6 * d + 2.0 ** -23 * want[0].abs().max()
+            off = (grad[-n:].float() - want[1].float()).abs()
+            assert (off <= 8 * d * 0.5 + 2 * plain.HALF_STEP[x.dtype] * want[1].float().abs()).all()
+        del grad
+
+
+def test_offsets_beyond_32_bits():
+    """Rows that begin behind 2^31 logits: as a copy of them alone gives."""
+    x = torch.empty(66000, 32769, dtype=torch.bfloat16, device='cuda').normal_(0, 3)
+    assert x.numel() > 2 ** 31
+    got = logits.top_logits(x, 20)
+    want = check_top(x[-3:].clone(), 20)
+    assert same(got.values[-3:], want.values) and torch.equal(got.ids[-3:], want.ids)
+    check_last(x, got, 3, False)
+    y = x.view(-1)[:66000 * 32768].view(33000, 2, 32768)
+    ids = y[:, :1].argmax(-1)
+    u = torch.rand(33000, device='cuda')
+    got = logits.verify_draft(y, ids, u[:, None], u)
+    want = check_verify(target=y[-3:].clone(), draft_ids=ids[-3:], accept_u=u[-3:, None], sample_u=u[-3:])
+    assert torch.equal(got.tokens[-3:], want.tokens) and torch.equal(got.accepted[-3:], want.accepted)
+
+
+def test_more_blocks_than_a_launch_takes():
+    """2^21 blocks of four rows, and some more."""
+    x = torch.empty(9000001, 65, dtype=torch.bfloat16, device='cuda').normal_(0, 3)
+    got = logits.top_logits(x, 2)
+    want = check_top(x[-70:].clone(), 2)
+    assert same(got.values[-70:], want.values) and torch.equal(got.ids[-70:], want.ids)
+    check_last(x, got, 70, False)
+
+
+def test_few_logits_beyond_32_bits():
+    x = torch.empty(53000001, 41, dtype=torch.bfloat16, device='cuda').normal_(0, 3)
+    assert x.numel() > 2 ** 31
+    got = logits.top_logits(x, 2)
+    want = check_top(x[-5000:].clone(), 2)
+    assert same(got.values[-5000:], want.values) and torch.equal(got.ids[-5000:], want.ids)
+    check_last(x, got, 5000, True)
 
 
 def test_verify_views_and_ids():

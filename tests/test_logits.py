@@ -144,6 +144,27 @@ def test_c_entry_refuses_a_short_workspace():
     assert lib.lt_top_logits_workspace(None, 20) == 0
 
 
+def test_c_entry_refuses_a_short_workspace_of_a_draft():
+    lib = logits._load()
+    for batch, drafts, vocab in ((1, 0, 5), (3, 4, 50000), (300, 2, 131072)):
+        x = _desc(rows=batch * (drafts + 1), vocab=vocab, stride_outer=vocab, dtype=2)
+        y = _desc(rows=batch * drafts, vocab=vocab, stride_outer=vocab, dtype=2)
+        d = logits._Draft(C.addressof(x), C.addressof(y), 4096, 4096, 4096, None, batch, drafts, 8)
+        need = lib.lt_verify_workspace(C.byref(d))
+        assert need > 0
+        for at, size in ((None, need), (4096, need - 1), (4104, need)):
+            assert lib.lt_verify_draft(C.byref(d), 1.0, 4096, 4096, at, size, None) == -1
+            assert b'workspace' in _capi.load().lt_last_error()
+    z = _desc(rows=3, vocab=200000, stride_outer=200000)
+    t = logits._Teacher(4096, 4096, None, 5, 8, 0)
+    need = lib.lt_distill_workspace(C.byref(z), 5)
+    assert need > 0
+    for at, size in ((None, need), (4096, need - 1), (4104, need)):
+        assert lib.lt_distill_forward(C.byref(z), C.byref(t), 1.0, 4096, 4096, at, size, None) == -1
+        assert lib.lt_distill_fused(C.byref(z), C.byref(t), 1.0, 1.0, None, 0, 4096, C.byref(z), at, size, None) == -1
+        assert b'workspace' in _capi.load().lt_last_error()
+
+
 @pytest.mark.parametrize('dtype', [0, 1, 2])
 def test_chunks_of_a_row_fit_their_join(dtype):
     """What is joined of a row's chunks -- the workspace is rows * chunks * (8 k + 8)
