@@ -51,14 +51,19 @@ __device__ __forceinline__ void exchange(uint64_t& key) {
   key = (key > other) == ((threadIdx.x & BIT) == 0) ? key : other;
 }
 
-// A wave's 64 keys, largest in lane 0: a bitonic sort, every merge's first
-// exchange with the mirrored lane, so that all go the same way.
-__device__ __forceinline__ uint64_t sort_wave(uint64_t key) {
+// A wave's keys, n of them (else 0), largest in lane 0: a bitonic sort, every
+// merge's first exchange with the mirrored lane, so that all go the same way.
+// (n is the same for all; lanes behind the power of two that holds it are not
+// sorted.)
+__device__ __forceinline__ uint64_t sort_wave(uint64_t key, int n) {
   exchange<1, 1>(key);
   exchange<3, 2>(key), exchange<1, 1>(key);
   exchange<7, 4>(key), exchange<2, 2>(key), exchange<1, 1>(key);
+  if (n <= 8) return key;
   exchange<15, 8>(key), exchange<4, 4>(key), exchange<2, 2>(key), exchange<1, 1>(key);
+  if (n <= 16) return key;
   exchange<31, 16>(key), exchange<8, 8>(key), exchange<4, 4>(key), exchange<2, 2>(key), exchange<1, 1>(key);
+  if (n <= 32) return key;
   exchange<63, 32>(key), exchange<16, 16>(key), exchange<8, 8>(key), exchange<4, 4>(key), exchange<2, 2>(key), exchange<1, 1>(key);
   return key;
 }
@@ -74,7 +79,7 @@ __device__ __forceinline__ void sort_keys(uint64_t* buf, int n, int k) {
   for (int i = 0; i < C / NT; ++i) {
     key[i] = 0;
     if (i * NT + (tid & ~63) < n) {
-      key[i] = sort_wave(i * NT + tid < n ? buf[i * NT + tid] : 0);
+      key[i] = sort_wave(i * NT + tid < n ? buf[i * NT + tid] : 0, n);
       if (n > 64 || NT == 64) buf[i * NT + tid] = key[i];
     }
   }
@@ -102,8 +107,9 @@ __device__ __forceinline__ void sort_keys(uint64_t* buf, int n, int k) {
 }
 
 // Keeps the k largest of the keys buf[0 .. n), k < n <= C, in any order, and
-// returns a key that they reach and the others do not: the k-th is found eight bits at a time, from the leading bit in which the keys
-// differ, by counting the keys of every value of the eight.  hist: 256 counts,
+// returns a key that they reach and the others do not: the k-th is found eight
+// bits at a time, from the leading bit in which the keys differ, by counting the
+// keys of every value of the eight.  hist: 256 counts,
 // cnt: one more, sh: NT / 64 keys.
 template <int NT, int C>
 __device__ __forceinline__ uint64_t cut_keys(uint64_t* buf, int n, int k, int* hist, int* cnt, uint64_t* sh) {
@@ -215,7 +221,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
   const int c0 = split * p.chunk;        // the block's: [v0, v1) from c0 on
   const int v0 = max(lead, c0), v1 = min(lead + p.x.vocab, c0 + p.chunk);
   const int k = max(0, min(p.k, v1 - v0));
-  const int per_wave = W == 1 ? min(63, k + 2 + k / 16) : (k + W - 1) / W + 1;
+  const int per_wave = W == 1 ? k + 2 + k / 16 : (k + W - 1) / W + 1;
   float m = LOWEST, s = 0.f, tau = -INFINITY;
   int n = 0;                             // keys
   if (tid == 0) sh.cnt = sh.listed = 0;
@@ -512,41 +518,157 @@ __global__ __launch_bounds__(64) void lt_top_few(TopParams p) {
   }
 }
 
-// Rows of at most SMALL logits: a wave takes one and sorts all of it.
-constexpr int SMALL = 256;
-
+// A single logit in a vector's place.
 template <class T>
-__global__ __launch_bounds__(256) void lt_top_small(TopParams p) {
+struct One {
+  static constexpr int E = 1;
+  float f;
+  __device__ __forceinline__ void load(const typename T::raw* p) { f = T::get(*p); }
+  __device__ __forceinline__ void load(const typename T::raw* x, int at, int, int end, typename T::raw) {
+    f = at < end ? T::get(x[at]) : -INFINITY;
+  }
+  __device__ __forceinline__ float get(int) const { return f; }
+  __device__ __forceinline__ void keep() {}
+};
+template <class T>
+__device__ __forceinline__ float max_of(const One<T>& v) {
+  return v.f;
+}
+
+// Rows that a wave holds in its registers, U vectors a lane.  The k-th largest
+// is found from below by its bits, from the leading one down: of the lanes'
+// largest logits, of the vectors' or of all logits, the fewest that are at least
+// twice as many as k -- k logits reach what is found, and not many more.  Those
+// become keys in LDS, which are sorted.  Its instructions bound it, but for long
+// rows and a small k: 65536 x 2000 bf16, k 5: 54 us (4.9 TB/s), k 100: 131;
+// 65536 x 200, k 5: 33 (a wave that sorts all of the row 108).
+// Rows where more than C logits reach it (equal ones, mostly) or where it is
+// -inf: the k-th is found among all logits in all its bits, and of those that
+// equal it the first are taken.
+template <class T, class V, int U, int C>
+__global__ __launch_bounds__(256) void lt_top_wave(TopParams p) {
   using raw = typename T::raw;
-  __shared__ uint64_t keys[4][SMALL];
-  const int lane = threadIdx.x & 63, vocab = p.x.vocab;
+  constexpr int E = V::E;
+  __shared__ __attribute__((aligned(16))) uint64_t keys[4][C];
   uint64_t* const buf = keys[group_of<64>()];
+  const int lane = threadIdx.x & 63, vocab = p.x.vocab, k = p.k;
   const int64_t r = (p.block0 + blockIdx.x) * 4 + group_of<64>();
   if (r >= p.rows) return;                 // (a wave as a whole)
-  const raw* x = (const raw*)p.x.data + p.x.at(r);
-  float f[SMALL / 64], m = LOWEST, s = 0.f;
+  const raw* const x = (const raw*)p.x.data + p.x.at(r);
+  V v[U];
 #pragma unroll
-  for (int i = 0; i < SMALL / 64; ++i) f[i] = i * 64 + lane < vocab ? T::get(x[i * 64 + lane]) : -INFINITY;
-#pragma unroll
-  for (int i = 0; i < SMALL / 64; ++i) m = max2(m, f[i]);
-  m = wave_reduce<Max>(m, LOWEST);
-#pragma unroll
-  for (int i = 0; i < SMALL / 64; ++i) {
-    s += exp2_((f[i] - m) * p.c);
-    if (i * 64 + lane < vocab) buf[i * 64 + lane] = order_key(f[i], (uint32_t)(i * 64 + lane));
+  for (int u = 0; u < U; ++u) {
+    const int at = (u * 64 + lane) * E;
+    if ((u + 1) * 64 * E <= vocab) v[u].load(x + at);
+    else v[u].load(x, at, 0, vocab, T::put(-INFINITY));
   }
-  s = wave_reduce<Sum>(s, 0.f);
-  sync<64>();
-  sort_keys<64, SMALL>(buf, vocab, p.k);
-  if (lane == 0) p.lse[r] = log_sum(m, s, p.inv_t);
+  float vm[U], m = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < SMALL / 64; ++i) {
-    const int j = i * 64 + lane;
-    if (j < p.k) {
-      const uint32_t id = ~(uint32_t)buf[j];
-      p.ids[r * p.k + j] = id;
-      ((raw*)p.values)[r * p.k + j] = s != s ? x[id] : T::put(of_order((uint32_t)(buf[j] >> 32)));
+  for (int u = 0; u < U; ++u) {
+    vm[u] = max_of(v[u]);
+    m = max2(m, vm[u]);
+    v[u].keep();
+  }
+  const float top = max2(wave_reduce<Max>(m, -INFINITY), LOWEST);
+  float s[2] = {0.f, 0.f};
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) s[(u * E + e) & 1] += exp2_((v[u].get(e) - top) * p.c);
+    v[u].keep();
+  }
+  const float sum = wave_reduce<Sum>(s[0] + s[1], 0.f);
+  if (lane == 0) p.lse[r] = log_sum(top, sum, p.inv_t);
+  int n = 0;
+  uint64_t key = 0;
+  if (sum != sum) {
+    best_by_passes<T, 64>(x, 0, vocab, k, buf, nullptr);
+    n = k;
+  } else {
+    uint32_t th = 0;
+    // (18 bits: all of a 16-bit logit's)
+    if (k * 2 <= min(64, (vocab + E - 1) / E)) {
+      const uint32_t o = order_of(m);
+#pragma unroll 2
+      for (int bit = 31; bit >= 14; --bit) {
+        const uint32_t cand = th | 1u << bit;
+        if (__popcll(__ballot(o >= cand)) >= k) th = cand;
+      }
+    } else if (U > 1 && E > 1 && k * (2 * E) <= vocab) {
+      uint32_t o[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) o[u] = order_of(vm[u]);
+#pragma nounroll
+      for (int bit = 31; bit >= 14; --bit) {
+        const uint32_t cand = th | 1u << bit;
+        int c = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) c += __popcll(__ballot(o[u] >= cand));
+        if (c >= k) th = cand;
+      }
+    } else {
+#pragma nounroll
+      for (int bit = 31; bit >= 14; --bit) {
+        const float f = of_order(th | 1u << bit);
+        int c = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int e = 0; e < E; ++e) c += __popcll(__ballot(v[u].get(e) >= f));
+        if (c < k) continue;
+        th |= 1u << bit;
+        if (c <= ((k + 63) & ~63)) break;
+      }
     }
+    float tau = of_order(th);
+    if (th > order_of(-INFINITY)) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float f = v[u].get(e);
+          const uint64_t b = __ballot(f >= tau);
+          if (b) {
+            const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
+            if (f >= tau && at < C) buf[at] = order_key(f, (uint32_t)((u * 64 + lane) * E + e));
+            n += __popcll(b);
+          }
+        }
+    } else {
+      n = C + 1;
+    }
+    if (n > C) {
+      th = 0;
+#pragma nounroll
+      for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t cand = th | 1u << bit;
+        int c = 0;
+#pragma nounroll
+        for (int i = lane; i < vocab; i += 64) c += order_of(T::get(x[i])) >= cand;
+        if (wave_reduce<Sum>(c, 0) >= k) th = cand;
+      }
+      n = 0;
+      // (first those above it, then those that equal it, in order)
+      for (int pass = 0; pass < 2; ++pass)
+        for (int i0 = 0; i0 < vocab && n < k; i0 += 64) {
+          const uint32_t o = i0 + lane < vocab ? order_of(T::get(x[i0 + lane])) : 0;
+          const bool mine = pass ? o == th : o > th;
+          const uint64_t b = __ballot(mine);
+          const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
+          if (mine && at < k) buf[at] = (uint64_t)o << 32 | (uint32_t)~(i0 + lane);
+          n = min(k, n + __popcll(b));
+        }
+    }
+    sync<64>();
+    if (n > 64) sort_keys<64, C>(buf, n, k);
+    else key = sort_wave(lane < n ? buf[lane] : 0, n);
+  }
+  for (int j = lane; j < k; j += 64) {
+    if (n > 64 || sum != sum) key = buf[j];
+    const uint32_t id = ~(uint32_t)key;
+    p.ids[r * k + j] = id;
+    // (the key holds a NaN as -inf)
+    ((raw*)p.values)[r * k + j] = sum != sum ? x[id] : T::put(of_order((uint32_t)(key >> 32)));
   }
 }
 
@@ -571,29 +693,47 @@ int64_t top_workspace(const TopParams& p) {
   return p.splits == 1 ? 0 : p.rows * p.splits * (int64_t)(p.k * sizeof(uint64_t) + sizeof(float2));
 }
 
+// (65536 rows of 100 logits, k 5: 28 us by single logits, 68 by vectors; of 300:
+// 35 by a vector a lane, 39 by two.)
+template <class T, int C>
+auto wave_kernel(int vocab) -> void (*)(TopParams) {
+  using V = Vec<T>;
+  if (vocab <= 128) return lt_top_wave<T, One<T>, 2, C>;
+  if (vocab <= 256) return lt_top_wave<T, One<T>, 4, C>;
+  if (vocab <= 64 * V::E) return lt_top_wave<T, V, 1, C>;
+  if (vocab <= 128 * V::E) return lt_top_wave<T, V, 2, C>;
+  return vocab <= 256 * V::E ? lt_top_wave<T, V, 4, C> : lt_top_wave<T, V, 32 / V::E, C>;
+}
+
 template <class T>
 lt_status launch_top(TopParams& p, void* stream) {
-    // Few logits a row, few of them wanted, and rows enough: a thread a row.
-  // (131072 x 41 float32, k 5: 23 us, a wave a row 158 us; 4096 x 128, k 16 the
-  // other way round: 65 and 19.)
-  if (p.x.vocab <= FEW && p.k <= 8 && p.rows >= 4096) {
+  // Few logits a row, few of them wanted, and rows enough: a thread a row.
+  // (131072 x 41 float32, k 5: 15 us, a wave a row 49; 16384 x 64, k 8: 16 and 12.)
+  if (p.x.vocab <= FEW && p.k <= 8 && p.rows >= 16384) {
     const int64_t blocks = (p.rows + 63) / 64;
     const int lds = 64 * (few_pitch(p.x.vocab) * 4 + p.k * (int)(sizeof(typename T::raw) + 1));
     if (p.k == 1) return launch(lt_top_few<T, 1>, blocks, 64, p, stream, "lt_top_logits", lds);
     if (p.k <= 5) return launch(lt_top_few<T, 5>, blocks, 64, p, stream, "lt_top_logits", lds);
     return launch(lt_top_few<T, 8>, blocks, 64, p, stream, "lt_top_logits", lds);
   }
-  if (p.x.vocab <= SMALL) return launch(lt_top_small<T>, (p.rows + 3) / 4, 256, p, stream, "lt_top_logits");
+  const int64_t fours = (p.rows + 3) / 4;
+  if (p.x.vocab <= 2048)
+    return launch(p.k <= 128 ? wave_kernel<T, 256>(p.x.vocab) : wave_kernel<T, 512>(p.x.vocab), fours, 256, p, stream, "lt_top_logits");
   if (p.splits > 1) {
     const lt_status st = launch(lt_top_k<T, 512, 4, 1024, 1024>, p.rows * p.splits, 512, p, stream, "lt_top_logits");
     return st != LT_OK ? st : launch(lt_top_join<T>, p.rows, 256, p, stream, "lt_top_logits");
   }
-  if (p.k > 62 && p.x.vocab <= 2048)
-    return launch(lt_top_k<T, 256, 8 / Vec<T>::E, 2048, 256 * 8 / Vec<T>::E>, p.rows * p.splits, 256, p, stream, "lt_top_logits");
-  if (p.k > 192 || p.x.vocab > 8192) return launch(lt_top_k<T, 512, 4, 1024, 1024>, p.rows * p.splits, 512, p, stream, "lt_top_logits");
-  if (p.k > 62 || p.x.vocab > 2048) return launch(lt_top_k<T, 256, 4, 1024, 512>, p.rows * p.splits, 256, p, stream, "lt_top_logits");
-  if (p.x.vocab > 1024) return launch(lt_top_k<T, 64, 4, 256, 128>, (p.rows + 3) / 4, 256, p, stream, "lt_top_logits");
-  return launch(lt_top_k<T, 64, 2, 256, 128>, (p.rows + 3) / 4, 256, p, stream, "lt_top_logits");
+  // Longer rows: a wave a row, 256 threads or 512.  Fewer threads wait for each
+  // other less, more find enough to do in few rows and hold a k of their size.
+  // (bf16, us: 16384 x 6000, k 5: 48, 96, -; k 32: 96, 97, -; 2048 x 6000, k 32:
+  // 27, 18, -; 4096 x 16000, k 60: 76, 42, 61; k 200: -, 97, 68; 16384 x 8000, k
+  // 200: -, 187, 241; 256 x 50000, k 60: 83, 24, 17.)  Of 256 threads at most 252
+  // take part in finding the first bound.
+  if (p.k <= 32 && p.x.vocab <= 8192 && p.rows >= 2048)
+    return launch(lt_top_k<T, 64, 4, 256, 128>, fours, 256, p, stream, "lt_top_logits");
+  if (p.k > 252 || (p.k > 192 && p.x.vocab > 8192) || (p.rows < 512 && p.x.vocab > 32768))
+    return launch(lt_top_k<T, 512, 4, 1024, 1024>, p.rows, 512, p, stream, "lt_top_logits");
+  return launch(lt_top_k<T, 256, 4, 1024, 512>, p.rows, 256, p, stream, "lt_top_logits");
 }
 
 }  // namespace

@@ -130,6 +130,31 @@ def test_top_chunks_off_the_grid(vocab, k):
         check_top(x[:, 3:3 + vocab], k)
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('vocab', [65, 127, 128, 129, 255, 256, 257, 511, 512, 513, 1023, 1024, 1025, 2047, 2048, 2049])
+def test_top_of_a_wave(dtype, vocab):
+    """Every k's way through rows about the sizes of a wave's registers: distinct
+    logits, many equal ones, and masks that leave fewer than k."""
+    for k in (1, 16, 32, 33, 50, 64, 65, 128, 129, 200, 256):
+        if k > vocab:
+            continue
+        x = rand((24, vocab), dtype, vocab + k, pad=k % 3)
+        x[4:8] = x[4:8].round()
+        x[8:12] = (x[8:12] / 4).round()
+        x[12:14, k // 2:] = -INF
+        x[14:16, :vocab - k] = -INF
+        x[16] = 1.0
+        x[17, ::2] = -0.0
+        x[17, 1::2] = 0.0
+        x[18] = LOWEST[dtype]
+        x[19] = -INF
+        x[20, -1] = math.nan
+        x[21, 0] = INF
+        x[22] = torch.sort(x[22].float()).values.to(dtype)
+        x[23] = -x[22]
+        check_top(x, k)
+
+
 def test_top_many_rows():
     """More rows than blocks are ever resident, of a tag set and of a small vocabulary."""
     check_top(rand((20011, 13), torch.float32, 1), 13)
