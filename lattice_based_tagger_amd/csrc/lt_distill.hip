@@ -34,7 +34,7 @@ __device__ __forceinline__ float weight_of(const DistillParams& p, int64_t r) {
   return p.weight ? p.scale * p.weight[r * p.weight_stride] : p.scale;
 }
 
-// What a block (or a wave with a row of its own) keeps in LDS: the entries, and
+// What a block keeps in LDS: the entries, and
 // a bit for each logit of a window that says whether it is one.
 template <int NT, int WINDOW>
 struct DistillShared {
@@ -50,9 +50,9 @@ struct DistillShared {
 // Logarithms are to the base 2.  (A library's logarithm or exponential of 64
 // bits takes 60 operations or more of two slots each: for every row of 2000
 // logits they took longer than the logits.)
-template <int NT>
+template <int NT, int N_ = (MAXK / NT > 1 ? MAXK / NT : 1)>
 struct Entries {
-  static constexpr int N = MAXK / NT > 1 ? MAXK / NT : 1;
+  static constexpr int N = N_;
   int id[N];
   double p[N], logp[N];
   double sum, rest;       // of the row
@@ -68,30 +68,36 @@ constexpr double TRACE = 1e-300;
 // 2^t for t <= 0 or little more, 0 far below.
 __device__ __forceinline__ double exp2_or_0(double t) { return t < -1000 ? 0.0 : exp2_64(t); }
 
-template <int NT>
-__device__ __forceinline__ void load_entries(const Teacher& t, int64_t r, int vocab, double inv_t, Entries<NT>& o,
+template <int NT, int N>
+__device__ __forceinline__ void load_entries(const Teacher& t, int64_t r, int vocab, double inv_t, Entries<NT, N>& o,
                                              double* sh) {
   const double c = inv_t * LOG2E;
-  double m = -INFINITY, s = 0;
+  float m = -INFINITY, top[N];
+  double s = 0;
 #pragma unroll
-  for (int i = 0; i < Entries<NT>::N; ++i) {
+  for (int i = 0; i < N; ++i) {
     const int j = i * NT + thread_of<NT>();
     o.id[i] = -1;
-    o.logp[i] = -INFINITY;
+    top[i] = -INFINITY;
     if (j < t.entries) {
       const int64_t id = any_id(t.ids, r * t.entries + j, t.ids_bytes);
       if (id >= 0 && id < vocab) {
         o.id[i] = (int)id;
-        o.logp[i] = any_float(t.top, r * t.entries + j, t.top_dtype) * c;
+        top[i] = any_float(t.top, r * t.entries + j, t.top_dtype);
       }
     }
-    m = o.logp[i] > m || o.logp[i] != o.logp[i] ? o.logp[i] : m;
+    m = max2(m, top[i]);
   }
-  double ref = t.top_lse ? (double)t.top_lse[r] * LOG2E : block_reduce<NT, Max>(m, sh);
-  if (!t.top_lse && ref == -INFINITY) ref = 0;
+  double ref;
+  if (t.top_lse) {
+    ref = (double)t.top_lse[r] * LOG2E;
+  } else {
+    m = block_reduce<NT, Max>(m, (float*)sh);
+    ref = m == -INFINITY ? 0 : m * c;
+  }
 #pragma unroll
-  for (int i = 0; i < Entries<NT>::N; ++i) {
-    o.logp[i] -= ref;
+  for (int i = 0; i < N; ++i) {
+    o.logp[i] = top[i] * c - ref;
     o.p[i] = 0;
     if (i * NT < t.entries) {              // (for all threads)
       o.p[i] = o.id[i] < 0 ? 0.0 : exp2_or_0(o.logp[i]);
@@ -103,9 +109,14 @@ __device__ __forceinline__ void load_entries(const Teacher& t, int64_t r, int vo
   if (t.top_lse) {
     if (o.sum > 0 && o.sum < 1) o.rest = 1 - o.sum;
   } else if (o.sum != 0) {
-    const double logs = log2_((float)o.sum), inv = 1 / o.sum;
+    // (a reciprocal good to 2^-20 or so, and two steps of Newton's: a division
+    // takes three times as long)
+    double inv = __builtin_amdgcn_rcp(o.sum);
+    inv = fma(fma(-o.sum, inv, 1.0), inv, inv);
+    inv = fma(fma(-o.sum, inv, 1.0), inv, inv);
+    const double logs = log2_((float)o.sum);
 #pragma unroll
-    for (int i = 0; i < Entries<NT>::N; ++i) {
+    for (int i = 0; i < N; ++i) {
       o.logp[i] -= logs;
       o.p[i] *= inv;
     }
@@ -197,30 +208,37 @@ __device__ __forceinline__ Sums join(Sums o, float c, float* shf) {
 
 // Loss and the gradient's factors of a row from its sums.
 __device__ __forceinline__ float3 factors(Sums o, double sum, double& rest, double inv_t, float& qrest) {
-  const float s = o.in + o.out;
-  qrest = o.out / s;
+  const float s = o.in + o.out, inv = 1 / s;
+  qrest = o.out * inv;
   if (!(rest > 0 && qrest > 0)) rest = 0;
   const double whole = sum + rest;
   if (!(s > 0)) return make_float3(o.m, 0.f, 0.f);
   const float other = rest > 0 ? (float)rest / qrest : 0.f;
-  return make_float3(o.m, (float)(whole * inv_t) / s, (float)((whole - other) * inv_t) / s);
+  return make_float3(o.m, (float)(whole * inv_t) * inv, (float)((whole - other) * inv_t) * inv);
 }
 
-// (z: the row.)
-template <class T, int NT>
-__device__ __forceinline__ float3 finish_row(const Entries<NT>& t, const typename T::raw* z, Sums o, double inv_t,
+// (zi: the logits of the entries.)
+template <int NT, int N>
+__device__ __forceinline__ float3 finish_row(const Entries<NT, N>& t, const float (&zi)[N], Sums o, double inv_t,
                                              double* sh, float& loss) {
   const double logs = log2_(o.in + o.out), c = inv_t * LOG2E;
   double l = 0, rest = t.rest;
 #pragma unroll
-  for (int i = 0; i < Entries<NT>::N; ++i)
-    if (t.id[i] >= 0 && t.p[i] != 0) l += t.p[i] * (t.logp[i] - ((double)T::get(z[t.id[i]]) - o.m) * c + logs);
+  for (int i = 0; i < N; ++i)
+    if (t.id[i] >= 0 && t.p[i] != 0) l += t.p[i] * (t.logp[i] - ((double)zi[i] - o.m) * c + logs);
   l = block_reduce<NT, Sum>(l, sh);
   float qrest;
   const float3 st = factors(o, t.sum, rest, inv_t, qrest);
   if (rest > 0) l += rest * (log2_((float)rest) - log2_(qrest));
   loss = (float)(l * LN2);
   return st;
+}
+
+// (z: the row.)
+template <class T, int NT, int N>
+__device__ __forceinline__ void load_zi(const Entries<NT, N>& t, const typename T::raw* z, float (&zi)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) zi[i] = t.id[i] >= 0 ? T::get(z[t.id[i]]) : 0.f;
 }
 
 // The gradient of the logits with numbers in [v0, v1), from c0 on: st from finish_row, w the row's weight.  The
@@ -270,7 +288,6 @@ __device__ __forceinline__ void grad_row(const typename T::raw* row, typename T:
     }
   }
   sync<NT>();
-  if (NT == 64) __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
 #pragma unroll
   for (int i = 0; i < Entries<NT>::N; ++i) {
     const int id = t.id[i];
@@ -289,33 +306,30 @@ __device__ __forceinline__ void grad_row(const typename T::raw* row, typename T:
   }
 }
 
-// Logits of a row and threads that take it: a wave, four of them a block, up to
-// 2048; else a block.
-#define GROUP_HEAD                                                                                        \
-  constexpr int GROUPS = NT == 64 ? 4 : 1;                                                                \
-  __shared__ __attribute__((aligned(16))) DistillShared<NT, WINDOW> shared[GROUPS];                       \
-  DistillShared<NT, WINDOW>& sh = shared[group_of<NT>()];                                                 \
-  const int64_t blk = (p.block0 + blockIdx.x) * GROUPS + group_of<NT>();                                  \
-  if (blk >= p.rows * p.splits) return; /* (a wave as a whole) */                                         \
-  const int64_t r = p.splits == 1 ? blk : blk / p.splits;                                                 \
+// A block's row, and the part of it that is the block's.
+#define BLOCK_HEAD                                                                                        \
+  __shared__ __attribute__((aligned(16))) DistillShared<NT, WINDOW> sh;                                   \
+  const int64_t blk = p.block0 + blockIdx.x, r = p.splits == 1 ? blk : blk / p.splits;                    \
   const typename T::raw* z = (const typename T::raw*)p.z.data + p.z.at(r);                                \
   const int lead = lead_of<T>(z), c0 = p.splits == 1 ? 0 : (int)(blk % p.splits) * p.chunk;               \
   const int v0 = max(lead, c0), v1 = min(lead + p.z.vocab, c0 + p.chunk);                                 \
   Entries<NT> t;                                                                                          \
-  load_entries<NT>(p.t, r, p.z.vocab, p.inv_t, t, sh.sh)
+  load_entries(p.t, r, p.z.vocab, p.inv_t, t, sh.sh)
 
 template <class T, int NT, int U, int WINDOW, bool TAIL>
-__global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_distill_sums(DistillParams p) {
-  GROUP_HEAD;
+__global__ __launch_bounds__(NT) void lt_distill_sums(DistillParams p) {
+  BLOCK_HEAD;
   Sums o;
   if (!t.blank()) o = join<NT>(sum_row<T, NT, U, WINDOW, TAIL>(z, lead, c0, v0, v1, p.c, t, sh), p.c, sh.shf);
   if (p.splits > 1) {
-    if (thread_of<NT>() == 0) p.part[blk] = make_float4(o.m, o.in, o.out, 0.f);
+    if (threadIdx.x == 0) p.part[blk] = make_float4(o.m, o.in, o.out, 0.f);
     return;
   }
   float loss;
-  const float3 st = finish_row<T, NT>(t, z, o, p.inv_t, sh.sh, loss);
-  if (thread_of<NT>() == 0) {
+  float zi[Entries<NT>::N];
+  load_zi<T>(t, z, zi);
+  const float3 st = finish_row(t, zi, o, p.inv_t, sh.sh, loss);
+  if (threadIdx.x == 0) {
     p.loss[r] = loss;
     *(float4*)(p.stats + r * LT_DISTILL_STATS) = make_float4(st.x, st.y, st.z, 0.f);
   }
@@ -328,7 +342,7 @@ __global__ __launch_bounds__(256) void lt_distill_join(DistillParams p) {
   __shared__ DistillShared<NT, 32> sh;
   const int64_t r = p.block0 + blockIdx.x;
   Entries<NT> t;
-  load_entries<NT>(p.t, r, p.z.vocab, p.inv_t, t, sh.sh);
+  load_entries(p.t, r, p.z.vocab, p.inv_t, t, sh.sh);
   Sums o;
   if ((int)threadIdx.x < p.splits) {       // (at most NT chunks)
     const float4 part = p.part[r * p.splits + threadIdx.x];
@@ -338,7 +352,9 @@ __global__ __launch_bounds__(256) void lt_distill_join(DistillParams p) {
   }
   o = join<NT>(o, p.c, sh.shf);
   float loss;
-  const float3 st = finish_row<T, NT>(t, (const typename T::raw*)p.z.data + p.z.at(r), o, p.inv_t, sh.sh, loss);
+  float zi[Entries<NT>::N];
+  load_zi<T>(t, (const typename T::raw*)p.z.data + p.z.at(r), zi);
+  const float3 st = finish_row(t, zi, o, p.inv_t, sh.sh, loss);
   if (threadIdx.x == 0) {
     p.loss[r] = loss;
     *(float4*)(p.stats + r * LT_DISTILL_STATS) = make_float4(st.x, st.y, st.z, 0.f);
@@ -346,8 +362,8 @@ __global__ __launch_bounds__(256) void lt_distill_join(DistillParams p) {
 }
 
 template <class T, int NT, int U, int WINDOW>
-__global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_distill_grad(DistillParams p) {
-  GROUP_HEAD;
+__global__ __launch_bounds__(NT) void lt_distill_grad(DistillParams p) {
+  BLOCK_HEAD;
   const float4 st = *(const float4*)(p.stats + r * LT_DISTILL_STATS);
   grad_row<T, NT, U, WINDOW, false>(z, (typename T::raw*)p.grad.data + p.grad.at(r), lead, c0, v0, v1, p.c,
                                     make_float3(st.x, st.y, st.z), weight_of(p, r), p.inv_t, t, sh,
@@ -359,15 +375,147 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_distill_grad(DistillPa
 // blocks are about to read again (4096 x 131072 bf16: 0.62 ms; with the stores
 // past the caches 0.50, with the loads too 0.47, 4.6 TB/s).
 template <class T, int NT, int U, int WINDOW, bool TAIL>
-__global__ __launch_bounds__(NT == 64 ? 256 : NT, NT == 64 ? 1 : 8) void lt_distill_both(DistillParams p) {
-  GROUP_HEAD;
+__global__ __launch_bounds__(NT, 8) void lt_distill_both(DistillParams p) {
+  BLOCK_HEAD;
   Sums o;
   if (!t.blank()) o = join<NT>(sum_row<T, NT, U, WINDOW, TAIL>(z, lead, c0, v0, v1, p.c, t, sh), p.c, sh.shf);
   float loss;
-  const float3 st = finish_row<T, NT>(t, z, o, p.inv_t, sh.sh, loss);
-  if (thread_of<NT>() == 0) p.loss[r] = loss;
+  float zi[Entries<NT>::N];
+  load_zi<T>(t, z, zi);
+  const float3 st = finish_row(t, zi, o, p.inv_t, sh.sh, loss);
+  if (threadIdx.x == 0) p.loss[r] = loss;
   grad_row<T, NT, U, WINDOW, true>(z, (typename T::raw*)p.grad.data + p.grad.at(r), lead, c0, v0, v1, p.c, st,
                                    weight_of(p, r), p.inv_t, t, sh, p.t.entries, p.past);
+}
+
+// Rows that a wave holds in its registers, U vectors a lane: read once, their
+// exponentials too taken once for the loss and the gradient.  N * 64 entries at
+// most.  The sum within the entries is that of the entries' own logits, each
+// once; the sum of all else leaves them out by a mask of bits in LDS (all less
+// the entries' would lose what is left where that is little).
+template <int N>
+struct WaveShared {
+  uint32_t bits[64];
+  int id[N * 64];
+  float mass[N * 64];
+};
+
+template <class T, class V, int U, int N, bool TAIL, bool LOSS, bool GRAD>
+__global__ __launch_bounds__(256) void lt_distill_wave(DistillParams p) {
+  using raw = typename T::raw;
+  constexpr int E = V::E;
+  __shared__ WaveShared<N> shared[4];
+  WaveShared<N>& sh = shared[group_of<64>()];
+  const int lane = threadIdx.x & 63, vocab = p.z.vocab;
+  const int64_t r = (p.block0 + blockIdx.x) * 4 + group_of<64>();
+  if (r >= p.rows) return;                 // (a wave as a whole)
+  const raw* const x = (const raw*)p.z.data + p.z.at(r);
+  V v[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int at = (u * 64 + lane) * E;
+    if ((u + 1) * 64 * E <= vocab) v[u].load(x + at);
+    else v[u].load(x, at, 0, vocab, T::put(-INFINITY));
+  }
+  Entries<64, N> t;
+  load_entries(p.t, r, vocab, p.inv_t, t, nullptr);
+  const bool blank = t.blank();
+  float zi[N];
+  load_zi<T>(t, x, zi);
+  // a bit for each logit that is an entry; `first`: of those with this id
+  bool first[N];
+  sh.bits[lane] = 0;
+  sync<64>();
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    first[i] = t.id[i] >= 0 && !(atomicOr(&sh.bits[t.id[i] >> 5], 1u << (t.id[i] & 31)) >> (t.id[i] & 31) & 1);
+  sync<64>();
+  float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (LOSS) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      m = max2(m, max_of(v[u]));
+      v[u].keep();
+    }
+    st.x = max2(wave_reduce<Max>(m, -INFINITY), LOWEST);
+  } else {
+    st = *(const float4*)(p.stats + r * LT_DISTILL_STATS);
+  }
+  float f[U][E], out[2] = {0.f, 0.f};
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    int others = -1;
+    if (LOSS && TAIL) {
+      const int at = min((u * 64 + lane) * E, vocab - 1);
+      others = ~(sh.bits[at >> 5] >> (at & 31 & ~(E - 1)));
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      f[u][e] = exp2_((v[u].get(e) - st.x) * p.c);
+      if (LOSS && TAIL) out[e & 1] += __builtin_bit_cast(float, __builtin_bit_cast(int, f[u][e]) & (others << (31 - e) >> 31));
+      else if (LOSS) out[e & 1] += f[u][e];
+    }
+  }
+  if (LOSS) {
+    Sums o;
+    o.m = st.x;
+    o.out = wave_reduce<Sum>(out[0] + out[1], 0.f);
+    if (TAIL) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) o.in += first[i] ? exp2_((zi[i] - st.x) * p.c) : 0.f;
+      o.in = wave_reduce<Sum>(o.in, 0.f);
+    }
+    float loss;
+    const float3 q = finish_row(t, zi, o, p.inv_t, nullptr, loss);
+    st = make_float4(q.x, q.y, q.z, 0.f);
+    if (lane == 0) {
+      p.loss[r] = blank ? 0.f : loss;
+      if (!GRAD) *(float4*)(p.stats + r * LT_DISTILL_STATS) = st;
+    }
+  }
+  if (!GRAD) return;
+  const float w = weight_of(p, r), all = st.z * w;
+  raw* const g = (raw*)p.grad.data + p.grad.at(r);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int at = (u * 64 + lane) * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[u][e] = blank ? 0.f : f[u][e] * all;
+    if constexpr (E == 1) {
+      if (at < vocab) g[at] = T::put(f[u][0]);
+    } else {
+      v[u].put(f[u]);
+      if (at + E <= vocab) v[u].store(g + at);
+      else if (at < vocab) v[u].store_part(g, at, 0, vocab);
+    }
+  }
+  if (blank) return;
+  // the entries' own, over that
+  float mass[N];
+  bool again = false;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    mass[i] = (float)(t.p[i] * p.inv_t);
+    again |= t.id[i] >= 0 && !first[i];
+  }
+  if (__any(again)) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      sh.id[i * 64 + lane] = t.id[i];
+      sh.mass[i * 64 + lane] = mass[i];
+      mass[i] = 0;
+    }
+    sync<64>();
+#pragma nounroll
+    for (int j = 0; j < p.t.entries; ++j)
+#pragma unroll
+      for (int i = 0; i < N; ++i) mass[i] += sh.id[j] == t.id[i] ? sh.mass[j] : 0.f;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (t.id[i] >= 0) g[t.id[i]] = T::put((exp2_((zi[i] - st.x) * p.c) * st.y - mass[i]) * w);
 }
 
 // Rows of at most FEW logits: a thread a row, the row in LDS, its entries a
@@ -504,9 +652,9 @@ void split_grad(DistillParams& p, int dtype) {
 int64_t parts_bytes(const DistillParams& p) { return p.splits == 1 ? 0 : p.rows * p.splits * (int64_t)sizeof(float4); }
 
 template <class T, int NT, int U, int WINDOW>
-lt_status launch_group(const DistillParams& p, Pass pass, void* stream, const char* what) {
-  const int64_t blocks = NT == 64 ? (p.rows + 3) / 4 : p.rows * p.splits;
-  const int threads = NT == 64 ? 256 : NT;
+lt_status launch_block(const DistillParams& p, Pass pass, void* stream, const char* what) {
+  const int64_t blocks = p.rows * p.splits;
+  constexpr int threads = NT;
   if (pass == GRAD) return launch(lt_distill_grad<T, NT, U, WINDOW>, blocks, threads, p, stream, what);
   if (pass == SUMS)
     return p.t.top_lse ? launch(lt_distill_sums<T, NT, U, WINDOW, true>, blocks, threads, p, stream, what)
@@ -515,19 +663,47 @@ lt_status launch_group(const DistillParams& p, Pass pass, void* stream, const ch
                      : launch(lt_distill_both<T, NT, U, WINDOW, false>, blocks, threads, p, stream, what);
 }
 
+template <class T, class V, int U, int N, bool TAIL>
+lt_status launch_wave(const DistillParams& p, Pass pass, void* stream, const char* what) {
+  const int64_t blocks = (p.rows + 3) / 4;
+  return pass == SUMS   ? launch(lt_distill_wave<T, V, U, N, TAIL, true, false>, blocks, 256, p, stream, what)
+         : pass == GRAD ? launch(lt_distill_wave<T, V, U, N, false, false, true>, blocks, 256, p, stream, what)
+                        : launch(lt_distill_wave<T, V, U, N, TAIL, true, true>, blocks, 256, p, stream, what);
+}
+
+template <class T, class V, int U>
+lt_status launch_wave(const DistillParams& p, Pass pass, void* stream, const char* what) {
+  if (p.t.entries <= 64)
+    return p.t.top_lse ? launch_wave<T, V, U, 1, true>(p, pass, stream, what) : launch_wave<T, V, U, 1, false>(p, pass, stream, what);
+  return p.t.top_lse ? launch_wave<T, V, U, 4, true>(p, pass, stream, what) : launch_wave<T, V, U, 4, false>(p, pass, stream, what);
+}
+
 template <class T>
 lt_status launch_pass(const DistillParams& p, Pass pass, void* stream, const char* what) {
-  // (a wave a row takes 160 us for 131072 x 41 float32, a thread a row XX)
-  if (p.z.vocab <= FEW && p.rows >= 4096 && p.t.entries <= 64) {
+  // Rows of few logits, and enough of them: a thread a row, which goes through
+  // its entries one after another.  (Loss and gradient of float32, us, a wave a
+  // row the second: 131072 x 41, 3 entries 23, 60; 12 entries 41, 60; 16384 x 41,
+  // 12 entries 25, 17.)
+  if (p.z.vocab <= FEW && p.rows >= 65536 && p.t.entries <= 16) {
     const int64_t blocks = (p.rows + 63) / 64;
     const int lds = 64 * few_pitch(p.z.vocab) * 4;
     return pass == SUMS   ? launch(lt_distill_few<T, true, false>, blocks, 64, p, stream, what, lds)
            : pass == GRAD ? launch(lt_distill_few<T, false, true>, blocks, 64, p, stream, what, lds)
                           : launch(lt_distill_few<T, true, true>, blocks, 64, p, stream, what, lds);
   }
-  if (p.z.vocab <= 2048) return launch_group<T, 64, 16 / Vec<T>::E, 2048>(p, pass, stream, what);
-  if (p.z.vocab <= 16384) return launch_group<T, 256, 4, 16384>(p, pass, stream, what);
-  const lt_status st = launch_group<T, 512, 4, 1 << 18>(p, pass, stream, what);
+  // (65536 x 2000 bf16, 32 entries: 123 us, 4.3 TB/s; 65536 x 200, 8 entries: 47, by
+  // its instructions; a wave that reads the row twice 190 and 82.)
+  if (p.z.vocab <= 2048) {
+    using W = Vec<T>;
+    if (p.z.vocab <= 128) return launch_wave<T, One<T>, 2>(p, pass, stream, what);
+    if (p.z.vocab <= 256) return launch_wave<T, One<T>, 4>(p, pass, stream, what);
+    if (p.z.vocab <= 64 * W::E) return launch_wave<T, W, 1>(p, pass, stream, what);
+    if (p.z.vocab <= 128 * W::E) return launch_wave<T, W, 2>(p, pass, stream, what);
+    if (p.z.vocab <= 256 * W::E) return launch_wave<T, W, 4>(p, pass, stream, what);
+    return launch_wave<T, W, 32 / W::E>(p, pass, stream, what);
+  }
+  if (p.z.vocab <= 16384) return launch_block<T, 256, 4, 16384>(p, pass, stream, what);
+  const lt_status st = launch_block<T, 512, 4, 1 << 18>(p, pass, stream, what);
   if (st != LT_OK || pass != SUMS || p.splits == 1) return st;
   return launch(lt_distill_join<T>, p.rows, 256, p, stream, what);
 }

@@ -206,6 +206,23 @@ __device__ __forceinline__ float max_of(const Vec<T>& v) {
   else return max3(max3(max3(v.get(0), v.get(1), v.get(2)), v.get(3), v.get(4)), max2(v.get(5), v.get(6)), v.get(7));
 }
 
+// A single logit in a vector's place.
+template <class T>
+struct One {
+  static constexpr int E = 1;
+  float f;
+  __device__ __forceinline__ void load(const typename T::raw* p) { f = T::get(*p); }
+  __device__ __forceinline__ void load(const typename T::raw* x, int at, int, int end, typename T::raw) {
+    f = at < end ? T::get(x[at]) : -INFINITY;
+  }
+  __device__ __forceinline__ float get(int) const { return f; }
+  __device__ __forceinline__ void keep() {}
+};
+template <class T>
+__device__ __forceinline__ float max_of(const One<T>& v) {
+  return v.f;
+}
+
 // 2^x of the hardware: within an ulp, 0 below the normal numbers.
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 

@@ -518,23 +518,6 @@ __global__ __launch_bounds__(64) void lt_top_few(TopParams p) {
   }
 }
 
-// A single logit in a vector's place.
-template <class T>
-struct One {
-  static constexpr int E = 1;
-  float f;
-  __device__ __forceinline__ void load(const typename T::raw* p) { f = T::get(*p); }
-  __device__ __forceinline__ void load(const typename T::raw* x, int at, int, int end, typename T::raw) {
-    f = at < end ? T::get(x[at]) : -INFINITY;
-  }
-  __device__ __forceinline__ float get(int) const { return f; }
-  __device__ __forceinline__ void keep() {}
-};
-template <class T>
-__device__ __forceinline__ float max_of(const One<T>& v) {
-  return v.f;
-}
-
 // Rows that a wave holds in its registers, U vectors a lane.  The k-th largest
 // is found from below by its bits, from the leading one down: of the lanes'
 // largest logits, of the vectors' or of all logits, the fewest that are at least

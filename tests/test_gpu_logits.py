@@ -246,6 +246,71 @@ def test_distill_few_logits(dtype, tail, vocab, k, pad):
     check_distill(z, ids, top, lse, 0.8)
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('tail', [False, True])
+@pytest.mark.parametrize('vocab, k, pad', [(1, 1, 0), (2, 2, 0), (41, 5, 0), (64, 16, 0), (63, 7, 2), (64, 17, 0)])
+def test_distill_many_rows_of_few_logits(dtype, tail, vocab, k, pad):
+    """811 rows, masks, padding and repeated ids among them, over and over: all as
+    the first time."""
+    n, times = 811, 82
+    z = rand((n, vocab), dtype, vocab)
+    ids, top, lse = teacher(z, k, dtype, vocab + 1, tail, 0.8, empty=0.1)
+    ids[3::11, k // 2:] = -1
+    ids[5::13, 0] = vocab
+    if k > 4:
+        ids[7::17, 1] = ids[7::17, 2]
+        top[7::17] -= 2
+        top[8::19, 3] = -INF
+    if vocab > 2:
+        keep = z[9::23].gather(1, ids[9::23].clamp(0, vocab - 1))
+        z[9::23] = -INF
+        z[9::23] = z[9::23].scatter(1, ids[9::23].clamp(0, vocab - 1), keep)
+    weight = torch.rand(n, generator=torch.Generator().manual_seed(4)).cuda()
+    many = lambda t: None if t is None else t.repeat(times, *[1] * (t.dim() - 1))
+    x = torch.zeros(n * times, vocab + pad, dtype=dtype, device='cuda')[:, :vocab]
+    x[:] = many(z)
+    blank = ((ids < 0) | (ids >= vocab)).all(-1)
+    x[many(blank)] = math.nan
+    loss, grad, loss_tol, grad_tol = plain.distill(z, ids, top, lse, 0.8, weight)
+    grad_tol = grad_tol + plain.type_tolerance(grad, dtype)
+    leaf = x.detach().requires_grad_()
+    got = logits.distill_loss(leaf, many(ids), many(top), top_lse=many(lse), temperature=0.8)
+    g, = torch.autograd.grad(got, leaf, many(weight))
+    for got, g in ((got.detach(), g), logits.distill_loss_grad(x, many(ids), many(top), many(weight), top_lse=many(lse),
+                                                               temperature=0.8)):
+        near(got[:n], loss, loss_tol)
+        near(g[:n], grad, grad_tol)
+        assert torch.equal(got.view(times, n), got[:n].expand(times, n))
+        assert torch.equal(g.reshape(times, n, vocab), g[:n].expand(times, n, vocab))
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('tail', [False, True])
+@pytest.mark.parametrize('vocab', [65, 127, 128, 129, 256, 257, 512, 513, 1023, 1024, 1025, 2047, 2048, 2049])
+def test_distill_of_a_wave(dtype, tail, vocab):
+    """Rows about the sizes of a wave's registers, with few entries and with many;
+    masks, repeated ids and an empty row among them."""
+    for k in (1, 60, 64, 65, 256):
+        if k > vocab:
+            continue
+        z = rand((12, vocab), dtype, vocab + k, pad=k % 5)
+        ids, top, lse = teacher(z, k, dtype, vocab + 1, tail, 1.0)
+        ids[1] = -1
+        ids[2, k // 2:] = vocab
+        z[3, ::2] = -INF
+        z[3].scatter_(0, ids[3], 0.0)
+        if k > 1:
+            ids[4, k // 2:] = ids[4, :k - k // 2].clone()
+            ids[5] = ids[5, 0]
+            top[4:6] -= 4
+        keep = z[6].gather(0, ids[6])                  # nothing but the entries is left
+        z[6] = -INF
+        z[6].scatter_(0, ids[6], keep)
+        z[7] = LOWEST[dtype]
+        z[7].scatter_(0, ids[7], 0.5)
+        check_distill(z, ids, top, lse)
+
+
 @pytest.mark.parametrize('tail', [False, True])
 def test_distill_beyond_a_window_of_bits(tail):
     z = rand((2, 600007), torch.bfloat16, 4)
