@@ -395,7 +395,7 @@ __global__ __launch_bounds__(NT, 8) void lt_distill_both(DistillParams p) {
 // the entries' would lose what is left where that is little).
 template <int N>
 struct WaveShared {
-  uint32_t bits[64];
+  uint32_t bits[128];
   int id[N * 64];
   float mass[N * 64];
 };
@@ -424,7 +424,7 @@ __global__ __launch_bounds__(256) void lt_distill_wave(DistillParams p) {
   load_zi<T>(t, x, zi);
   // a bit for each logit that is an entry; `first`: of those with this id
   bool first[N];
-  sh.bits[lane] = 0;
+  for (int i = lane; i < U * 2 * E; i += 64) sh.bits[i] = 0;
   sync<64>();
 #pragma unroll
   for (int i = 0; i < N; ++i)
@@ -691,17 +691,17 @@ lt_status launch_pass(const DistillParams& p, Pass pass, void* stream, const cha
            : pass == GRAD ? launch(lt_distill_few<T, false, true>, blocks, 64, p, stream, what, lds)
                           : launch(lt_distill_few<T, true, true>, blocks, 64, p, stream, what, lds);
   }
-  // (65536 x 2000 bf16, 32 entries: 123 us, 4.3 TB/s; 65536 x 200, 8 entries: 47, by
-  // its instructions; a wave that reads the row twice 190 and 82.)
-  if (p.z.vocab <= 2048) {
-    using W = Vec<T>;
-    if (p.z.vocab <= 128) return launch_wave<T, One<T>, 2>(p, pass, stream, what);
-    if (p.z.vocab <= 256) return launch_wave<T, One<T>, 4>(p, pass, stream, what);
-    if (p.z.vocab <= 64 * W::E) return launch_wave<T, W, 1>(p, pass, stream, what);
-    if (p.z.vocab <= 128 * W::E) return launch_wave<T, W, 2>(p, pass, stream, what);
-    if (p.z.vocab <= 256 * W::E) return launch_wave<T, W, 4>(p, pass, stream, what);
-    return launch_wave<T, W, 32 / W::E>(p, pass, stream, what);
-  }
+  // Rows that fit a wave's registers.  (65536 x 2000 bf16, 32 entries: 123 us, 4.3
+  // TB/s; 65536 x 200, 8 entries: 47, by its instructions; a wave that reads the
+  // row twice 190 and 82.  16384 x 4000: 68 us, a block of 256 threads 100.)
+  using W = Vec<T>;
+  if (p.z.vocab <= 128) return launch_wave<T, One<T>, 2>(p, pass, stream, what);
+  if (p.z.vocab <= 256) return launch_wave<T, One<T>, 4>(p, pass, stream, what);
+  if (p.z.vocab <= 64 * W::E) return launch_wave<T, W, 1>(p, pass, stream, what);
+  if (p.z.vocab <= 128 * W::E) return launch_wave<T, W, 2>(p, pass, stream, what);
+  if (p.z.vocab <= 256 * W::E) return launch_wave<T, W, 4>(p, pass, stream, what);
+  if (p.z.vocab <= 512 * W::E) return launch_wave<T, W, 8>(p, pass, stream, what);
+  // (4096 x 8000 bf16: 40 us by 256 threads, 57 by 512; 4096 x 131072: 508 and 468.)
   if (p.z.vocab <= 16384) return launch_block<T, 256, 4, 16384>(p, pass, stream, what);
   const lt_status st = launch_block<T, 512, 4, 1 << 18>(p, pass, stream, what);
   if (st != LT_OK || pass != SUMS || p.splits == 1) return st;

@@ -677,7 +677,8 @@ int64_t top_workspace(const TopParams& p) {
 }
 
 // (65536 rows of 100 logits, k 5: 28 us by single logits, 68 by vectors; of 300:
-// 35 by a vector a lane, 39 by two.)
+// 35 by a vector a lane, 39 by two.  16384 rows of 4000, k 100: 66 us, lt_top_k
+// of 256 threads 105.)
 template <class T, int C>
 auto wave_kernel(int vocab) -> void (*)(TopParams) {
   using V = Vec<T>;
@@ -685,7 +686,7 @@ auto wave_kernel(int vocab) -> void (*)(TopParams) {
   if (vocab <= 256) return lt_top_wave<T, One<T>, 4, C>;
   if (vocab <= 64 * V::E) return lt_top_wave<T, V, 1, C>;
   if (vocab <= 128 * V::E) return lt_top_wave<T, V, 2, C>;
-  return vocab <= 256 * V::E ? lt_top_wave<T, V, 4, C> : lt_top_wave<T, V, 32 / V::E, C>;
+  return vocab <= 256 * V::E ? lt_top_wave<T, V, 4, C> : lt_top_wave<T, V, 8, C>;
 }
 
 template <class T>
@@ -700,7 +701,7 @@ lt_status launch_top(TopParams& p, void* stream) {
     return launch(lt_top_few<T, 8>, blocks, 64, p, stream, "lt_top_logits", lds);
   }
   const int64_t fours = (p.rows + 3) / 4;
-  if (p.x.vocab <= 2048)
+  if (p.x.vocab <= 512 * Vec<T>::E)
     return launch(p.k <= 128 ? wave_kernel<T, 256>(p.x.vocab) : wave_kernel<T, 512>(p.x.vocab), fours, 256, p, stream, "lt_top_logits");
   if (p.splits > 1) {
     const lt_status st = launch(lt_top_k<T, 512, 4, 1024, 1024>, p.rows * p.splits, 512, p, stream, "lt_top_logits");

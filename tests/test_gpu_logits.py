@@ -131,7 +131,8 @@ def test_top_chunks_off_the_grid(vocab, k):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
-@pytest.mark.parametrize('vocab', [65, 127, 128, 129, 255, 256, 257, 511, 512, 513, 1023, 1024, 1025, 2047, 2048, 2049])
+@pytest.mark.parametrize('vocab', [65, 127, 128, 129, 255, 256, 257, 511, 512, 513, 1023, 1024, 1025, 2047, 2048, 2049,
+                                   4095, 4096, 4097])
 def test_top_of_a_wave(dtype, vocab):
     """Every k's way through rows about the sizes of a wave's registers: distinct
     logits, many equal ones, and masks that leave fewer than k."""
@@ -286,7 +287,7 @@ def test_distill_many_rows_of_few_logits(dtype, tail, vocab, k, pad):
 
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('tail', [False, True])
-@pytest.mark.parametrize('vocab', [65, 127, 128, 129, 256, 257, 512, 513, 1023, 1024, 1025, 2047, 2048, 2049])
+@pytest.mark.parametrize('vocab', [65, 127, 128, 129, 256, 257, 512, 513, 1023, 1024, 1025, 2047, 2048, 2049, 4095, 4096, 4097])
 def test_distill_of_a_wave(dtype, tail, vocab):
     """Rows about the sizes of a wave's registers, with few entries and with many;
     masks, repeated ids and an empty row among them."""
