@@ -372,8 +372,9 @@ __global__ __launch_bounds__(NT) void lt_distill_grad(DistillParams p) {
 
 // Both: the second pass finds the row in the caches.  It reads past them, and
 // the gradient is written past them: kept, they push out the rows that other
-// blocks are about to read again (4096 x 131072 bf16: 0.62 ms; with the stores
-// past the caches 0.50, with the loads too 0.47, 4.6 TB/s).
+// blocks are about to read again (4096 x 131072 bf16: 570 us; with the stores
+// past the caches 500, with the loads too 467, 4.6 TB/s; 32768 x 16000: 518 and
+// 461).
 template <class T, int NT, int U, int WINDOW, bool TAIL>
 __global__ __launch_bounds__(NT, 8) void lt_distill_both(DistillParams p) {
   BLOCK_HEAD;
@@ -746,10 +747,8 @@ DistillParams distill_params(const lt_rows* z, const lt_teacher* t, double tempe
   p.c = (float)(LOG2E / temperature);
   split_sums(p, z->dtype);
   // Logits and gradient of more than the last cache's 256 MB: by the time that
-  // the gradient is read, it would be gone.  A smaller one is left there, and so
-  // are rows short enough to be found again in the L2 (131072 x 2000: 0.37 ms
-  // plain, 0.40 past the caches).
-  p.past = p.z.vocab > 16384 && 2 * p.rows * p.z.vocab * dtype_bytes(z->dtype) > (int64_t)256 << 20;
+  // the gradient is read, it would be gone; a smaller one is left there.
+  p.past = 2 * p.rows * p.z.vocab * dtype_bytes(z->dtype) > (int64_t)256 << 20;
   return p;
 }
 

@@ -351,19 +351,6 @@ __device__ __forceinline__ T block_reduce(T v, T* sh) {
   return v;
 }
 
-// sum of exp2((x - m) c) over what a thread has seen; m is LOWEST at first, so
-// that a -inf logit adds 0 and a row of the type's lowest value adds 1 each.
-struct Running {
-  float m = LOWEST, s = 0.f;
-  __device__ __forceinline__ void add(float x, float c) {
-    if (x > m) {
-      s *= exp2f((m - x) * c);
-      m = x;
-    }
-    s += exp2f((x - m) * c);
-  }
-};
-
 // A logit as a whole number in the order of the values (NaN as -inf, -0 as 0).
 __device__ __forceinline__ uint32_t order_of(float x) {
   x = x != x ? -INFINITY : x + 0.f;
@@ -495,7 +482,6 @@ lt_status launch(void (*kernel)(P), int64_t blocks, int threads, P p, void* stre
   return LT_OK;
 }
 
-#define BY_TYPE(dtype, kernel) ((dtype) == LT_F32 ? kernel<F32> : (dtype) == LT_F16 ? kernel<F16> : kernel<BF16>)
 #define ON_DEVICE(d)                                                                                   \
   OnDevice on(d);                                                                                      \
   if (on.err != hipSuccess) return lt::set_error(LT_EHIP, "device %d: %s", (int)(d), hipGetErrorString(on.err))
