@@ -10,6 +10,8 @@ Public surface (mirrors the reference's ``lattice_tagger.beam``,
     Tagger, Word, tag constants
     evaluate_batch (BeamScoreFunctions.evaluate for many paths on the GPU)
     modelpack (trained-model files: save / load)
+    logits (imported by itself, with torch: top logits, distillation,
+    verification of drafts, for models that give logits)
 
 Decoding runs in hand-written HIP kernels for gfx950 (``csrc/``) behind the
 C-ABI ``include/lattice_decode.h``; see DESIGN.md.

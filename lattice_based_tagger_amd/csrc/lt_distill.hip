@@ -316,6 +316,9 @@ __device__ __forceinline__ void grad_row(const typename T::raw* row, typename T:
   Entries<NT> t;                                                                                          \
   load_entries(p.t, r, p.z.vocab, p.inv_t, t, sh.sh)
 
+// Loss and statistics, or the gradient from them: one pass each, bound by memory
+// (2039 x 50261 bf16, 32 entries with the tail: 49 us, 4.2 TB/s, and 65 us, 6.3
+// TB/s with what of the logits is still in the last cache).
 template <class T, int NT, int U, int WINDOW, bool TAIL>
 __global__ __launch_bounds__(NT) void lt_distill_sums(DistillParams p) {
   BLOCK_HEAD;
@@ -520,7 +523,10 @@ __global__ __launch_bounds__(256) void lt_distill_wave(DistillParams p) {
 }
 
 // Rows of at most FEW logits: a thread a row, the row in LDS, its entries a
-// mask of 64 bits.  The gradient is made of the logits alone (no stats).
+// mask of 64 bits.  The gradient is made of the logits alone (no stats).  131072 x
+// 41 float32, 5 entries: loss 17 us, gradient 24, where reading the logits and
+// writing the gradient take 4 each: its instructions bound it, those in 64 bits
+// for every entry foremost.
 template <class T, bool LOSS, bool GRAD>
 __global__ __launch_bounds__(64) void lt_distill_few(DistillParams p) {
   using raw = typename T::raw;
