@@ -49,7 +49,12 @@ __device__ __forceinline__ void exp2_64(double (&t)[4]) {
 // exp2((x - m) c) of logits no further than 1000 (in the exponent) below m;
 // lower ones are taken as that: 1e-301.
 constexpr double DEPTH = 1000;
-__device__ __forceinline__ float floor_of(float m, double c) { return (float)fmax((double)m - DEPTH / c, (double)LOWEST); }
+// (The float next above it where the nearest one lies below: at the lowest
+// temperatures floats are hundreds of exponents apart.)
+__device__ __forceinline__ float floor_of(float m, double c) {
+  const float f = (float)fmax((double)m - DEPTH / c, (double)LOWEST);
+  return ((double)f - m) * c >= -DEPTH ? f : nextafterf(f, INFINITY);
+}
 __device__ __forceinline__ double soft_exp(float x, float floor, double m, double c) {
   return exp2_64(((double)max2(x, floor) - m) * c);
 }

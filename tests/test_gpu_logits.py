@@ -577,6 +577,24 @@ def test_verify_edges():
     check_verify(**a)
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('certain', [False, True])
+def test_verify_lowest_temperature(dtype, certain):
+    """Logits a step of their type apart, which at 1e-6 are hundreds of powers of 2:
+    the best ones share all the mass."""
+    g = torch.Generator().manual_seed(50)
+    for top in (2000.0, -2000.0, 28672.0):
+        step = 2.0 ** (math.floor(math.log2(abs(top))) + 1) * plain.HALF_STEP[dtype]
+        below = torch.randint(0, 12, (6, 4, 700), generator=g).double()
+        below[:, :, 100:103] = 0
+        x = (top - below * step).to(dtype).cuda()
+        assert (x[:, :, 100:103] == top).all() and (x <= top).all()
+        ids = torch.randint(100, 104, (6, 3), generator=g).cuda()
+        a = dict(target=x, draft_ids=ids, accept_u=0.05 + 0.9 * torch.rand(6, 3, generator=g).cuda(),
+                 sample_u=0.05 + 0.9 * torch.rand(6, generator=g).cuda(), draft=None if certain else x.roll(1, -1)[:, :3])
+        check_verify(temperature=1e-6, **a)
+
+
 @pytest.mark.parametrize('certain, batch, drafts, vocab', [(False, 120, 3, 300007), (True, 290, 2, 262144)])
 def test_verify_large_batches(certain, batch, drafts, vocab):
     """More than 128 MB of logits at a place, which are taken place by place: drafts
