@@ -65,8 +65,8 @@ struct Entries {
 // row from one without entries.
 constexpr double TRACE = 1e-300;
 
-// 2^t for t <= 0 or little more, 0 far below.
-__device__ __forceinline__ double exp2_or_0(double t) { return t < -1000 ? 0.0 : exp2_64(t); }
+// 2^t; 0 far below, infinite far above (a log-sum-exp that is not the entries').
+__device__ __forceinline__ double exp2_or_0(double t) { return t < -1000 ? 0.0 : t > 1000 ? INFINITY : exp2_64(t); }
 
 template <int NT, int N>
 __device__ __forceinline__ void load_entries(const Teacher& t, int64_t r, int vocab, double inv_t, Entries<NT, N>& o,

@@ -411,6 +411,21 @@ def test_distill_impossible_entry():
     assert torch.isfinite(grad).all() and grad[0, ids[0, 1]] < 0
 
 
+@pytest.mark.parametrize('rows, vocab', [(3, 41), (65600, 41), (3, 1200), (3, 20000), (3, 200000)])
+def test_distill_wrong_log_sum_exp(rows, vocab):
+    """Entries that the given log-sum-exp makes likelier than a double holds: not
+    finite, in their row alone."""
+    z = rand((rows, vocab), torch.float32, 29)
+    ids, top, lse = teacher(z, 4, torch.float32, 30, True, 1.0)
+    want = logits.distill_loss_grad(z, ids, top, 1.0, top_lse=lse)
+    bad = lse.clone()
+    bad[1] = top[1, 0] - 1500.0
+    loss, grad = logits.distill_loss_grad(z, ids, top, 1.0, top_lse=bad)
+    assert not loss[1].isfinite() and not grad[1].isfinite().all()
+    assert torch.equal(loss[2:], want[0][2:]) and torch.equal(grad[2:], want[1][2:])
+    assert torch.equal(loss[0], want[0][0]) and torch.equal(grad[0], want[1][0])
+
+
 def test_distill_types_and_views():
     z = rand((3, 5, 1001), torch.bfloat16, 12)
     view = z[:, :-1]
