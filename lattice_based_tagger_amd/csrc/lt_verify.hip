@@ -386,76 +386,86 @@ __global__ __launch_bounds__(NT) void lt_verify_weigh(VerifyParams p) {
   if (threadIdx.x == 0) p.sums[blk] = make_double2(sp, sq);
 }
 
+struct Two {
+  double x, y;
+  __device__ __forceinline__ Two operator+(Two o) const { return {x + o.x, y + o.y}; }
+};
+template <> __device__ __forceinline__ Two neutral<Sum, Two>() { return {0, 0}; }
+
 // The token: the first whose running sum of weights passes u of the whole, else
 // the last with a weight; where all weights are 0 (p and q alike), drawn by p.
 template <class T>
 __global__ __launch_bounds__(NT) void lt_verify_draw(VerifyParams p) {
   constexpr int SEG = 64 * Vec<T>::E;
   __shared__ double shd[NT / 64];
+  __shared__ Two sh2[NT / 64];
   __shared__ int first, last;
+  constexpr int Q = 4;                     // segments of a thread
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t b = p.block0 + blockIdx.x;
+  // what can be read at once: a load that waits for another takes a microsecond
+  const double2* const weights = p.weight + b * p.segments;
   const StopNote note = p.stop[b];
+  const double u = p.sample_u[b];
+  const int64_t drafted = tid < p.drafts ? any_id(p.ids, b * p.drafts + tid, p.ids_bytes) : -1;
+  double2 own[Q];
+#pragma unroll
+  for (int j = 0; j < Q; ++j) own[j] = tid * Q + j < p.segments ? weights[tid * Q + j] : make_double2(0, 0);
+  Two sums{0, 0};
+  for (int i = tid; i < p.weigh_splits; i += NT) {
+    const double2 s = p.sums[b * p.weigh_splits + i];
+    sums = sums + Two{s.x, s.y};
+  }
   Stop<T> st = stop_at<T>(p, b, note.a);
   st.pm = note.pm;
   st.qm = note.qm;
   st.floors(p.c);
   const int lead = lead_of<T>(st.x), end = lead + p.target.vocab, segments = (end + SEG - 1) / SEG;
-  double sp = 0, sq = 0;
-  for (int i = tid; i < p.weigh_splits; i += NT) {
-    const double2 s = p.sums[b * p.weigh_splits + i];
-    sp += s.x;
-    sq += s.y;
-  }
-  sp = block_reduce<NT, Sum>(sp, shd);
-  if (st.y) {
-    sq = block_reduce<NT, Sum>(sq, shd);
-    st.ratio = sq > 0 ? sp / sq : 0;
-  }
-  const double2* weights = p.weight + b * p.segments;
-  auto segment = [&](int s) {
-    if (s >= segments) return 0.0;
-    const double2 w = weights[s];
-    return st.y ? fmax(w.x - st.ratio * w.y, 0.0) : w.x;
-  };
-  // The first of [from, to) whose running sum (from `before` on) passes the
-  // line, else the last with a weight, else -1; before: the sum ahead of it.
-  // A thread takes Q neighbours at a time.
-  auto cross = [&](auto q, int from, int to, double line, double& before, auto weight) {
-    constexpr int Q = decltype(q)::value;
+  sums = block_reduce<NT, Sum>(sums, sh2);
+  const double sp = sums.x;
+  if (st.y) st.ratio = sums.y > 0 ? sp / sums.y : 0;
+  auto segment_of = [&](double2 w) { return st.y ? fmax(w.x - st.ratio * w.y, 0.0) : w.x; };
+  // Of Q neighbours' weights of a thread, the first of which is number i: the first
+  // whose running sum (from `before` on) passes the line.  -- found: 0x7fffffff or
+  // that; before: the sum of all.  A thread's own in `mine`, its last with a weight
+  // in `my_last`, with the sum ahead of each.
+  int mine = -1, my_last = -1;
+  double ahead = 0, last_ahead = 0;
+  auto begin = [&]() {
     if (tid == 0) first = 0x7fffffff, last = -1;
-    double ahead = 0, last_ahead = 0;      // of this thread's first past the line, of its last with a weight
-    int mine = -1, my_last = -1;
-    for (int i0 = from; i0 < to; i0 += NT * Q) {
-      const int i = i0 + tid * Q;
-      double w[Q], sum = 0;
+    mine = my_last = -1;
+  };
+  auto pass = [&](auto& w, int i, auto line_of, double& before) {
+    constexpr int N = sizeof(w) / sizeof(double);
+    double sum = 0;
 #pragma unroll
-      for (int j = 0; j < Q; ++j) w[j] = i + j < to ? weight(i + j) : 0.0;
+    for (int j = 0; j < N; ++j) sum += w[j];
+    double cum = wave_scan<Sum>(sum, 0.0);
+    if (lane == 63) shd[wave] = cum;
+    __syncthreads();
+    double all = before;
+    cum += before - sum;
 #pragma unroll
-      for (int j = 0; j < Q; ++j) sum += w[j];
-      double cum = wave_scan<Sum>(sum, 0.0);
-      if (lane == 63) shd[wave] = cum;
-      __syncthreads();
-      double all = before;
-      cum += before - sum;
-#pragma unroll
-      for (int k = 0; k < NT / 64; ++k) {
-        if (k < wave) cum += shd[k];
-        all += shd[k];
-      }
-#pragma unroll
-      for (int j = 0; j < Q; ++j) {
-        if (w[j] > 0) {
-          if (mine < 0 && cum + w[j] > line) mine = i + j, ahead = cum;
-          my_last = i + j, last_ahead = cum;
-        }
-        cum += w[j];
-      }
-      if (mine >= 0) atomicMin(&first, mine);
-      __syncthreads();
-      if (first != 0x7fffffff) break;
-      before = all;
+    for (int k = 0; k < NT / 64; ++k) {
+      if (k < wave) cum += shd[k];
+      all += shd[k];
     }
+    const double line = line_of(all);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (w[j] > 0) {
+        if (mine < 0 && cum + w[j] > line) mine = i + j, ahead = cum;
+        my_last = i + j, last_ahead = cum;
+      }
+      cum += w[j];
+    }
+    if (mine >= 0) atomicMin(&first, mine);
+    __syncthreads();
+    before = all;
+    return first;
+  };
+  // That one, else the last with a weight, else -1; before: the sum ahead of it.
+  auto settle = [&](double& before) {
     __syncthreads();
     int at = first;
     if (at == 0x7fffffff) {
@@ -471,19 +481,40 @@ __global__ __launch_bounds__(NT) void lt_verify_draw(VerifyParams p) {
     __syncthreads();
     return at;
   };
+  // The same over [from, to), N neighbours of a thread at a time.
+  auto cross = [&](auto n, int from, int to, double line, double& before, auto weight) {
+    constexpr int N = decltype(n)::value;
+    begin();
+    for (int i0 = from; i0 < to; i0 += NT * N) {
+      double w[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) w[j] = i0 + tid * N + j < to ? weight(i0 + tid * N + j) : 0.0;
+      if (pass(w, i0 + tid * N, [&](double) { return line; }, before) != 0x7fffffff) break;
+    }
+    return settle(before);
+  };
   using std::integral_constant;
-  constexpr integral_constant<int, 4> FOUR;
+  constexpr integral_constant<int, Q> MANY;
   constexpr integral_constant<int, SEG / NT> STEP;
-  double total = 0;
-  for (int s = tid; s < segments; s += NT) total += segment(s);
-  total = block_reduce<NT, Sum>(total, shd);
   auto of_token = [&](int v) { return st.weight(v, p.c); };
-  int token = -1;
-  if (total > 0) {
-    const double line = p.sample_u[b] * total;
-    double before = 0;
-    const int s = cross(FOUR, 0, segments, line, before, segment);
-    token = cross(STEP, max(0, s * SEG - lead), min(p.target.vocab, (s + 1) * SEG - lead), line, before, of_token);
+  double line = 0, before = 0;
+  int at, token = -1;
+  if (segments <= NT * Q) {
+    double w[Q];
+#pragma unroll
+    for (int j = 0; j < Q; ++j) w[j] = tid * Q + j < segments ? segment_of(own[j]) : 0;
+    begin();
+    pass(w, tid * Q, [&](double all) { return line = u * all; }, before);
+    at = settle(before);
+  } else {
+    double total = 0;
+    auto segment = [&](int s) { return segment_of(weights[s]); };
+    for (int s = tid; s < segments; s += NT) total += segment(s);
+    line = u * block_reduce<NT, Sum>(total, shd);
+    at = cross(MANY, 0, segments, line, before, segment);
+  }
+  if (at >= 0) {
+    token = cross(STEP, max(0, at * SEG - lead), min(p.target.vocab, (at + 1) * SEG - lead), line, before, of_token);
     if (token < 0) {
       before = 0;                          // (a segment of rounding errors)
       token = cross(STEP, 0, p.target.vocab, line, before, of_token);
@@ -492,12 +523,12 @@ __global__ __launch_bounds__(NT) void lt_verify_draw(VerifyParams p) {
   if (token < 0 && sp > 0) {
     st.y = nullptr;
     st.id = -1;
-    double before = 0;
-    token = cross(STEP, 0, p.target.vocab, p.sample_u[b] * sp, before, of_token);
+    before = 0;
+    token = cross(STEP, 0, p.target.vocab, u * sp, before, of_token);
   }
   if (tid == 0) p.accepted[b] = note.a;
   for (int i = tid; i <= p.drafts; i += NT)
-    p.tokens[b * (p.drafts + 1) + i] = i < note.a ? any_id(p.ids, b * p.drafts + i, p.ids_bytes) : i == note.a ? token : -1;
+    p.tokens[b * (p.drafts + 1) + i] = i < note.a ? drafted : i == note.a ? token : -1;
 }
 
 // ---- host ------------------------------------------------------------------
