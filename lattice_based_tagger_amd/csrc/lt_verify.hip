@@ -128,8 +128,8 @@ __device__ __forceinline__ float2 sum_part(const typename T::raw* row, int lead,
 
 // A row's softmax in 32 bits: exp2((x - m) c) / s.
 struct Soft {
-  float m = LOWEST;
-  double s = 0;
+  float m;
+  double s;
   __device__ __forceinline__ double of(float x, double c) const {
     const double t = ((double)x - m) * c;
     return s > 0 && t > -DEPTH ? exp2_64(t) / s : 0;
@@ -138,7 +138,7 @@ struct Soft {
 
 // A row's chunks, one after another.
 __device__ __forceinline__ Soft join_parts(const float2* part, int splits, double c) {
-  Soft o;
+  Soft o{LOWEST, 0};
 #pragma unroll 8
   for (int i = 0; i < splits; ++i) o.m = fmaxf(o.m, part[i].x);
 #pragma unroll 4
@@ -164,16 +164,15 @@ __device__ __forceinline__ Soft draft_soft(const VerifyParams& p, int64_t b, int
   return join_parts(p.part + (p.batch * (p.drafts + 1) + b * p.drafts + i) * p.splits, p.splits, p.c);
 }
 
-// Whether token i of sequence b is accepted: by its rows' sums in 32 bits; CLOSE
-// where these leave it open.
+// Whether token i of sequence b is accepted: by its rows' sums in 32 bits (ps, qs
+// give them); CLOSE where these leave it open.
 enum Verdict { REFUSED, ACCEPTED, CLOSE };
-template <class T>
-__device__ __forceinline__ Verdict accepts(const VerifyParams& p, int64_t b, int i) {
-  const int64_t id = any_id(p.ids, b * p.drafts + i, p.ids_bytes);
+template <class T, class P, class Q>
+__device__ __forceinline__ Verdict accepts(const VerifyParams& p, int64_t b, int i, int64_t id, float u, P ps, Q qs) {
   if (id < 0 || id >= p.target.vocab) return REFUSED;
-  const double px = target_soft(p, b, i).of(T::get(target_row<T>(p, b, i)[id]), p.c);
-  const double qx = p.draft.data ? draft_soft(p, b, i).of(T::get(draft_row<T>(p, b, i)[id]), p.c) : 1.0;
-  const double line = p.accept_u[b * p.drafts + i] * qx;
+  const double px = ps().of(T::get(target_row<T>(p, b, i)[id]), p.c);
+  const double qx = p.draft.data ? qs().of(T::get(draft_row<T>(p, b, i)[id]), p.c) : 1.0;
+  const double line = u * qx;
   if (fabs(px - line) <= p.margin * px && px > 0) return CLOSE;
   return line < px ? ACCEPTED : REFUSED;
 }
@@ -240,7 +239,8 @@ __global__ __launch_bounds__(NT) void lt_verify_sums(VerifyParams p) {
       // (a block of this launch may write it, but only what this one finds too)
       const int at = p.stopped[b];
       if (at >= 0 && at < i - 1) return;
-      const Verdict v = accepts<T>(p, b, i - 1);
+      const Verdict v = accepts<T>(p, b, i - 1, any_id(p.ids, b * p.drafts + i - 1, p.ids_bytes), p.accept_u[b * p.drafts + i - 1],
+                                   [&] { return target_soft(p, b, i - 1); }, [&] { return draft_soft(p, b, i - 1); });
       if (v == REFUSED || (v == CLOSE && !accepts_exactly<T>(p, b, i - 1, shd))) {
         if (writes) p.stopped[b] = i - 1;
         return;
@@ -253,30 +253,59 @@ __global__ __launch_bounds__(NT) void lt_verify_sums(VerifyParams p) {
   if (threadIdx.x == 0) p.part[((target ? b * (p.drafts + 1) : p.batch * (p.drafts + 1) + b * p.drafts) + i) * p.splits + split] = o;
 }
 
-// The place where sequence b stops.  (One launch for all: from the sums, a
-// thread a place.)
+// The place where sequence b stops, and the sums of its rows there.  (One launch
+// for all: a thread a place, which reads ahead of the sequence's length what may
+// be behind it.)
+struct StopShared {
+  int a, close;
+  Soft p, q;
+};
 template <class T>
-__device__ __forceinline__ int find_stop(const VerifyParams& p, int64_t b, int* sh_a, int* sh_close, double* shd) {
-  const int n = length_of(p, b);
+__device__ __forceinline__ int find_stop(const VerifyParams& p, int64_t b, StopShared& sh, double* shd, Soft& ps, Soft& qs) {
+  const int tid = threadIdx.x;
+  int a;
   if (p.rounds) {
-    const int at = p.stopped[b];
-    return at < 0 ? n : at;
-  }
-  for (int from = 0;;) {
-    if (threadIdx.x == 0) *sh_a = *sh_close = n;
-    __syncthreads();
-    for (int i = from + threadIdx.x; i < n; i += NT) {
-      const Verdict v = accepts<T>(p, b, i);
-      if (v == REFUSED) atomicMin(sh_a, i);
-      if (v == CLOSE) atomicMin(sh_close, i);
+    a = p.stopped[b];
+    if (a < 0) a = length_of(p, b);
+  } else {
+    Soft tp, tq;
+    int64_t id = -1;
+    float u = 0;
+    if (tid <= p.drafts) tp = target_soft(p, b, tid);
+    if (tid < p.drafts) {
+      id = any_id(p.ids, b * p.drafts + tid, p.ids_bytes);
+      u = p.accept_u[b * p.drafts + tid];
+      if (p.draft.data) tq = draft_soft(p, b, tid);
     }
-    __syncthreads();
-    const int a = *sh_a, close = *sh_close;
-    __syncthreads();
-    if (close >= a) return a;              // (both n: none)
-    if (!accepts_exactly<T>(p, b, close, shd)) return close;
-    from = close + 1;
+    const int n = length_of(p, b);
+    const Verdict v = tid < n ? accepts<T>(p, b, tid, id, u, [&] { return tp; }, [&] { return tq; }) : ACCEPTED;
+    for (int from = 0;;) {
+      if (tid == 0) sh.a = sh.close = n;
+      __syncthreads();
+      if (v == REFUSED && tid >= from) atomicMin(&sh.a, tid);
+      if (v == CLOSE && tid >= from) atomicMin(&sh.close, tid);
+      __syncthreads();
+      a = sh.a;
+      const int close = sh.close;
+      __syncthreads();
+      if (close >= a) break;               // (both n: none)
+      if (!accepts_exactly<T>(p, b, close, shd)) {
+        a = close;
+        break;
+      }
+      from = close + 1;
+    }
+    if (a < NT) {
+      if (tid == a) sh.p = tp, sh.q = tq;
+      __syncthreads();
+      ps = sh.p;
+      qs = sh.q;
+      return a;
+    }
   }
+  ps = target_soft(p, b, a);
+  if (p.draft.data && a < p.drafts) qs = draft_soft(p, b, a);
+  return a;
 }
 
 // What the next token is drawn by: e_p, or max(e_p - ratio e_q, 0), e_p and e_q
@@ -325,16 +354,15 @@ __device__ __forceinline__ Stop<T> stop_at(const VerifyParams& p, int64_t b, int
 template <class T>
 __global__ __launch_bounds__(NT) void lt_verify_weigh(VerifyParams p) {
   constexpr int E = Vec<T>::E;
-  __shared__ int sh_a, sh_close;
+  __shared__ StopShared sh;
   __shared__ double shd[NT / 64];
   const int64_t blk = p.block0 + blockIdx.x, b = blk / p.weigh_splits;
   const int split = (int)(blk - b * p.weigh_splits), c0 = split * p.weigh_chunk;
-  const int a = find_stop<T>(p, b, &sh_a, &sh_close, shd);
+  Soft ps{LOWEST, 0}, qs{LOWEST, 0};
+  const int a = find_stop<T>(p, b, sh, shd, ps, qs);
   Stop<T> st = stop_at<T>(p, b, a);
-  const Soft ps = target_soft(p, b, a);
   st.pm = ps.m;
   if (st.y) {
-    const Soft qs = draft_soft(p, b, a);
     st.qm = qs.m;
     st.ratio = qs.s > 0 ? ps.s / qs.s : 0;
   }
