@@ -561,9 +561,12 @@ __global__ __launch_bounds__(NT) void lt_verify_draw(VerifyParams p) {
 
 // ---- host ------------------------------------------------------------------
 // Rounds read no row behind the one where a sequence stops; each costs a
-// launch's time and waits for its slowest block.  (512 x 7 drafts of 131072
-// bf16, 268 MB a place: 0.45 ms, all at once 0.51; 64 x 5, 34 MB: 0.15 and 0.08.)
-constexpr int64_t ROUND_BYTES = (int64_t)128 << 20;
+// launch's time and waits for its slowest block.  They pay where a place's rows
+// are large and the drafts are many; with lengths, of which about half counts,
+// twice as many.  (131072 bf16, us, all at once the second: 512 x 7 drafts 430,
+// 488; 350 x 7 336, 355; 512 x 4 350, 354; 260 x 7 284, 282; 512 x 2 274, 263;
+// 64 x 5 138, 69; up to 7 each 512 375, 364.)
+constexpr int64_t ROUND_BYTES = (int64_t)128 << 20, ROUNDS_BYTES = (int64_t)1 << 30;
 
 int64_t chunks(int64_t numbers, int64_t step, int64_t rows, int64_t blocks) {
   int64_t n = (numbers + step - 1) / step;
@@ -574,10 +577,13 @@ int64_t chunks(int64_t numbers, int64_t step, int64_t rows, int64_t blocks) {
 void plan(VerifyParams& p, int dtype) {
   const int e = dtype == LT_F32 ? 4 : 8, step = NT * 4 * e, vectors = NT * e;
   const int64_t numbers = (int64_t)p.target.vocab + LEAD, kinds = p.draft.data ? 2 : 1;
-  p.rounds = p.batch * kinds * p.target.vocab * dtype_bytes(dtype) >= ROUND_BYTES && p.drafts > 0;
+  const int64_t place = p.batch * kinds * p.target.vocab * dtype_bytes(dtype);
+  p.rounds = place >= ROUND_BYTES && place * p.drafts >= (p.lengths ? 2 : 1) * ROUNDS_BYTES;
   p.segments = (int32_t)((numbers + 64 * e - 1) / (64 * e));
-  // blocks enough that those of rows that do not count leave the card full
-  int64_t n = chunks(numbers, step, p.batch * kinds * (p.rounds ? 1 : p.drafts + 1), 8192);
+  // blocks enough that those of rows that do not count leave the card full; in
+  // rounds fewer, of which each first finds what was accepted (512 x 7 drafts: 429
+  // us of 4096 blocks, 445 of 8192; 400 x 3 of 50261 float32 179 and 195)
+  int64_t n = p.rounds ? chunks(numbers, step, p.batch * kinds, 4096) : chunks(numbers, step, p.batch * kinds * (p.drafts + 1), 8192);
   p.chunk = (int32_t)((numbers + n * step - 1) / (n * step) * step);
   p.splits = (int32_t)((numbers + p.chunk - 1) / p.chunk);
   // of each sum: a thread's additions one after another (16 of a step, the

@@ -610,6 +610,32 @@ def test_verify_lowest_temperature(dtype, certain):
         check_verify(temperature=1e-6, **a)
 
 
+@pytest.mark.parametrize('certain, batch, drafts, vocab, dtype, ragged', [
+    (False, 300, 7, 131072, torch.bfloat16, False), (True, 180, 8, 200003, torch.float32, False),
+    (False, 700, 4, 100003, torch.float16, True), (True, 500, 16, 150000, torch.bfloat16, True)])
+def test_verify_place_by_place(certain, batch, drafts, vocab, dtype, ragged):
+    """Gigabytes of logits, which are taken a place at a time: drafts refused at every
+    place, some that sums in 32 bits leave open, one without any token."""
+    g = torch.Generator('cuda').manual_seed(batch)
+    x = torch.empty(batch, drafts + 1, vocab, dtype=dtype, device='cuda').normal_(0, 2, generator=g)
+    best = x.argmax(-1, keepdim=True)
+    x.scatter_add_(2, best, torch.full_like(best, 8, dtype=dtype))
+    n = (torch.arange(batch) % (drafts + 1)).int().cuda() if ragged else None
+    ids, draft = best[:, :drafts, 0].clone(), None
+    ids[1::19, 1] = vocab
+    if not certain:
+        draft = x[:, :drafts].clone()
+        draft[3::4] += torch.empty_like(draft[3::4]).normal_(0, 0.3, generator=g)
+    u = torch.rand(batch, drafts, generator=g, device='cuda')
+    u[::4] = 1 - 2.0 ** -24                            # (p and q alike: accepted, by their sums in 64 bits)
+    x[2, 1] = -INF
+    a = dict(target=x, draft_ids=ids, sample_u=torch.rand(batch, generator=g, device='cuda'), draft=draft, lengths=n)
+    check_verify(accept_u=u, **a)
+    # the noise refuses some at every place (of the largest u the sum rounds to 1,
+    # which is none of [0, 1))
+    check_verify(accept_u=(0.9 + 0.1 * u).clamp(max=1 - 2.0 ** -24), **a)
+
+
 @pytest.mark.parametrize('certain, batch, drafts, vocab', [(False, 120, 3, 300007), (True, 290, 2, 262144)])
 def test_verify_large_batches(certain, batch, drafts, vocab):
     """More than 128 MB of logits at a place, which are taken place by place: drafts
