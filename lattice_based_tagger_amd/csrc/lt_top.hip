@@ -532,10 +532,10 @@ __global__ __launch_bounds__(64) void lt_top_few(TopParams p) {
 // Rows where more than C logits reach it (equal ones, mostly) or where it is
 // -inf: the k-th is found among all logits in all its bits, and of those that
 // equal it the first are taken.
-template <class T, class V, int U, int C>
+template <class T, class V, int U>
 __global__ __launch_bounds__(256) void lt_top_wave(TopParams p) {
   using raw = typename T::raw;
-  constexpr int E = V::E;
+  constexpr int E = V::E, C = 2 * MAXK;
   __shared__ __attribute__((aligned(16))) uint64_t keys[4][C];
   uint64_t* const buf = keys[group_of<64>()];
   const int lane = threadIdx.x & 63, vocab = p.x.vocab, k = p.k;
@@ -683,20 +683,21 @@ int64_t top_workspace(const TopParams& p) {
 // (65536 rows of 100 logits, k 5: 28 us by single logits, 68 by vectors; of 300:
 // 35 by a vector a lane, 39 by two.  16384 rows of 4000, k 100: 66 us, lt_top_k
 // of 256 threads 105.)
-template <class T, int C>
+template <class T>
 auto wave_kernel(int vocab) -> void (*)(TopParams) {
   using V = Vec<T>;
-  if (vocab <= 128) return lt_top_wave<T, One<T>, 2, C>;
-  if (vocab <= 256) return lt_top_wave<T, One<T>, 4, C>;
-  if (vocab <= 64 * V::E) return lt_top_wave<T, V, 1, C>;
-  if (vocab <= 128 * V::E) return lt_top_wave<T, V, 2, C>;
-  return vocab <= 256 * V::E ? lt_top_wave<T, V, 4, C> : lt_top_wave<T, V, 8, C>;
+  if (vocab <= 128) return lt_top_wave<T, One<T>, 2>;
+  if (vocab <= 256) return lt_top_wave<T, One<T>, 4>;
+  if (vocab <= 64 * V::E) return lt_top_wave<T, V, 1>;
+  if (vocab <= 128 * V::E) return lt_top_wave<T, V, 2>;
+  return vocab <= 256 * V::E ? lt_top_wave<T, V, 4> : lt_top_wave<T, V, 8>;
 }
 
 template <class T>
 lt_status launch_top(TopParams& p, void* stream) {
   // Few logits a row, few of them wanted, and rows enough: a thread a row.
-  // (131072 x 41 float32, k 5: 15 us, a wave a row 49; 16384 x 64, k 8: 16 and 12.)
+  // (131072 x 41 float32, k 5: 15 us, a wave a row 49; 16384 x 64, k 8: 16 and 12.
+  // Registers for 1 logit 13 us, for 5 15, for 8 19.)
   if (p.x.vocab <= FEW && p.k <= 8 && p.rows >= 16384) {
     const int64_t blocks = (p.rows + 63) / 64;
     const int lds = 64 * (few_pitch(p.x.vocab) * 4 + p.k * (int)(sizeof(typename T::raw) + 1));
@@ -706,7 +707,7 @@ lt_status launch_top(TopParams& p, void* stream) {
   }
   const int64_t fours = (p.rows + 3) / 4;
   if (p.x.vocab <= 512 * Vec<T>::E)
-    return launch(p.k <= 128 ? wave_kernel<T, 256>(p.x.vocab) : wave_kernel<T, 512>(p.x.vocab), fours, 256, p, stream, "lt_top_logits");
+    return launch(wave_kernel<T>(p.x.vocab), fours, 256, p, stream, "lt_top_logits");
   if (p.splits > 1) {
     const lt_status st = launch(lt_top_k<T, 512, 4, 1024, 1024>, p.rows * p.splits, 512, p, stream, "lt_top_logits");
     return st != LT_OK ? st : launch(lt_top_join<T>, p.rows, 256, p, stream, "lt_top_logits");
@@ -715,8 +716,8 @@ lt_status launch_top(TopParams& p, void* stream) {
   // other less, more find enough to do in few rows and hold a k of their size.
   // (bf16, us: 16384 x 6000, k 5: 48, 96, -; k 32: 96, 97, -; 2048 x 6000, k 32:
   // 27, 18, -; 4096 x 16000, k 60: 76, 42, 61; k 200: -, 97, 68; 16384 x 8000, k
-  // 200: -, 187, 241; 256 x 50000, k 60: 83, 24, 17.)  Of 256 threads at most 252
-  // take part in finding the first bound.
+  // 200: -, 187, 241; 256 x 50000, k 60: 83, 24, 17.)  Beyond k 252 the first
+  // bound of 256 threads would need more of a wave's threads than it has.
   if (p.k <= 32 && p.x.vocab <= 8192 && p.rows >= 2048)
     return launch(lt_top_k<T, 64, 4, 256, 128>, fours, 256, p, stream, "lt_top_logits");
   if (p.k > 252 || (p.k > 192 && p.x.vocab > 8192) || (p.rows < 512 && p.x.vocab > 8192))

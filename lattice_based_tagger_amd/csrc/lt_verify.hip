@@ -632,8 +632,10 @@ lt_status check(const lt_draft* d) {
   lt_status st;
   if (!d) BAD("draft: NULL");
   if (!rows_ok(d->target, "target", &st)) return st;
-  if (d->batch < 0 || d->drafts < 0 || d->drafts > LT_MAX_DRAFTS) BAD("batch %lld, drafts %d (0 .. %d)", (long long)d->batch, d->drafts, LT_MAX_DRAFTS);
-  if (d->target->rows != d->batch * (d->drafts + 1)) BAD("target: %lld rows, batch * (drafts + 1) = %lld", (long long)d->target->rows, (long long)(d->batch * (d->drafts + 1)));
+  if (d->batch < 0 || d->drafts < 0 || d->drafts > LT_MAX_DRAFTS)
+    BAD("batch %lld, drafts %d (0 .. %d)", (long long)d->batch, d->drafts, LT_MAX_DRAFTS);
+  if (d->target->rows != d->batch * (d->drafts + 1))
+    BAD("target: %lld rows, batch * (drafts + 1) = %lld", (long long)d->target->rows, (long long)(d->batch * (d->drafts + 1)));
   if (d->ids_bytes != 4 && d->ids_bytes != 8) BAD("ids of %d bytes", d->ids_bytes);
   if (d->draft) {
     if (!rows_ok(d->draft, "draft", &st)) return st;
