@@ -2,8 +2,8 @@
 # TSan over lt_lookup.cpp, lt_packer.cpp and the host half of lt_capi.cpp /
 # lt_comm.cpp).  The host sources are compiled by g++ with the sanitizer; the
 # device sources (lt_decode.hip, lt_results.hip, lt_top.hip, lt_distill.hip,
-# lt_verify.hip) by hipcc for gfx950 without one (GPU sanitizers are not
-# available on the pool).  The CPU test suite then runs against the instrumented library (LT_LIBRARY) with the sanitizer runtime
+# lt_verify.hip) by hipcc for gfx950 without one.  The CPU test suite then runs
+# against the instrumented library (LT_LIBRARY) with the sanitizer runtime
 # preloaded into the interpreter:
 #
 #   make check-asan     # AddressSanitizer + UndefinedBehaviorSanitizer
