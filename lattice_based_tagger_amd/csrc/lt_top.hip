@@ -160,22 +160,6 @@ __device__ __forceinline__ uint64_t cut_keys(uint64_t* buf, int n, int k, int* h
   return at_least;
 }
 
-// The k best of x[v0 .. v1) one after another, k passes: rows with a NaN.
-template <class T, int NT>
-__device__ void best_by_passes(const typename T::raw* x, int v0, int v1, int k, uint64_t* out, uint64_t* sh) {
-  uint64_t below = ~0ull;
-  for (int j = 0; j < k; ++j) {
-    uint64_t best = 0;
-    for (int v = v0 + thread_of<NT>(); v < v1; v += NT) {
-      const uint64_t key = order_key(T::get(x[v]), (uint32_t)v);
-      if (key < below && key > best) best = key;
-    }
-    below = block_reduce<NT, Max>(best, sh);
-    if (thread_of<NT>() == 0) out[j] = below;
-  }
-  sync<NT>();
-}
-
 // One pass over a row (or a chunk of it).  A step takes U vectors of 16 bytes
 // a thread.  From the first step's largest logit of every thread comes a
 // bound tau that at least k logits reach; a vector with a logit above it goes
@@ -384,39 +368,37 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
   }
   const float top = block_reduce<NT, Max>(m, sh.shf);
   const float sum = block_reduce<NT, Sum>(s * exp2_((m - top) * p.c), sh.shf);
-  if (sum != sum) {
-    best_by_passes<T, NT>(row, v0 - lead, v1 - lead, k, buf, sh.sh64);
-  } else {
-    for (int base = c0; n < k && base < v1; base += NT * E) {
-      // the first logits that equal tau: in order, a vector a thread (never
-      // short of k: at least k logits reach tau)
-      const int at = base + tid * E;
-      Vec<T> v;
-      v.load(x, at, v0, v1, T::put(-INFINITY));
-      int mine = 0;
+  // (a NaN as -inf, which nothing else is less than)
+  auto equals = [&](float f, int at) { return at >= v0 && at < v1 && (tau == -INFINITY ? !(f > tau) : f == tau); };
+  for (int base = c0; n < k && base < v1; base += NT * E) {
+    // the first logits that equal tau: in order, a vector a thread (never
+    // short of k: at least k logits reach tau)
+    const int at = base + tid * E;
+    Vec<T> v;
+    v.load(x, at, v0, v1, T::put(-INFINITY));
+    int mine = 0;
 #pragma unroll
-      for (int e = 0; e < E; ++e) mine += at + e >= v0 && at + e < v1 && v.get(e) == tau;
-      const int upto = wave_scan<Sum>(mine, 0);
-      if (lane == 63) sh.reach[wave] = upto;
-      sync<NT>();
-      int pos = n + upto - mine, all = 0;
+    for (int e = 0; e < E; ++e) mine += equals(v.get(e), at + e);
+    const int upto = wave_scan<Sum>(mine, 0);
+    if (lane == 63) sh.reach[wave] = upto;
+    sync<NT>();
+    int pos = n + upto - mine, all = 0;
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const int c = sh.reach[w];
-        if (w < wave) pos += c;
-        all += c;
-      }
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (at + e >= v0 && at + e < v1 && v.get(e) == tau) {
-          if (pos < k) buf[pos] = order_key(tau, (uint32_t)(at + e - lead));
-          ++pos;
-        }
-      n = min(k, n + all);
-      sync<NT>();
+    for (int w = 0; w < W; ++w) {
+      const int c = sh.reach[w];
+      if (w < wave) pos += c;
+      all += c;
     }
-    sort_keys<NT, C>(buf, n, k);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (equals(v.get(e), at + e)) {
+        if (pos < k) buf[pos] = order_key(tau, (uint32_t)(at + e - lead));
+        ++pos;
+      }
+    n = min(k, n + all);
+    sync<NT>();
   }
+  sort_keys<NT, C>(buf, n, k);
   if (p.splits == 1) {
     if (tid == 0) p.lse[r] = log_sum(top, sum, p.inv_t);
     for (int j = tid; j < k; j += NT) {
@@ -522,16 +504,25 @@ __global__ __launch_bounds__(64) void lt_top_few(TopParams p) {
   }
 }
 
+// What is made of this inside a loop is made there each time: the numbers of all
+// of a lane's logits, made ahead of the loop, took 40 registers.
+__device__ __forceinline__ int renewed(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
 // Rows that a wave holds in its registers, U vectors a lane.  The k-th largest
 // is found from below by its bits, from the leading one down: of the lanes'
 // largest logits, of the vectors' or of all logits, the fewest that are at least
 // twice as many as k -- k logits reach what is found, and not many more.  Those
 // become keys in LDS, which are sorted.  Its instructions bound it, but for long
-// rows and a small k: 65536 x 2000 bf16, k 5: 54 us (4.9 TB/s), k 100: 131;
-// 65536 x 200, k 5: 33 (a wave that sorts all of the row 108).
+// rows and a small k: 65536 x 2000 bf16, k 5: 61 us (4.4 TB/s), k 100: 138;
+// 65536 x 200, k 5: 32 (a wave that sorts all of the row 108).
 // Rows where more than C logits reach it (equal ones, mostly) or where it is
-// -inf: the k-th is found among all logits in all its bits, and of those that
-// equal it the first are taken.
+// -inf, and rows with a NaN: the bound is raised to the largest logit if k equal
+// it, else by a search among all logits, which ends when few enough reach it or at
+// the k-th itself; then only those above it become keys, and the first of those
+// that equal it (65536 x 2000 bf16, k 5: 61 us, constant rows 172).
 template <class T, class V, int U>
 __global__ __launch_bounds__(256) void lt_top_wave(TopParams p) {
   using raw = typename T::raw;
@@ -556,6 +547,7 @@ __global__ __launch_bounds__(256) void lt_top_wave(TopParams p) {
     m = max2(m, vm[u]);
     v[u].keep();
   }
+  m = max2(m, -INFINITY);                  // (of NaNs alone)
   const float top = max2(wave_reduce<Max>(m, -INFINITY), LOWEST);
   float s[2] = {0.f, 0.f};
 #pragma unroll
@@ -568,90 +560,131 @@ __global__ __launch_bounds__(256) void lt_top_wave(TopParams p) {
   if (lane == 0) p.lse[r] = log_sum(top, sum, p.inv_t);
   int n = 0;
   uint64_t key = 0;
-  if (sum != sum) {
-    best_by_passes<T, 64>(x, 0, vocab, k, buf, nullptr);
-    n = k;
-  } else {
-    uint32_t th = 0;
-    // (18 bits: all of a 16-bit logit's)
-    if (k * 2 <= min(64, (vocab + E - 1) / E)) {
-      const uint32_t o = order_of(m);
+  uint32_t th = 0;
+  // (18 bits: all of a 16-bit logit's)
+  if (k * 2 <= min(64, (vocab + E - 1) / E)) {
+    const uint32_t o = order_of(m);
 #pragma unroll 2
-      for (int bit = 31; bit >= 14; --bit) {
-        const uint32_t cand = th | 1u << bit;
-        if (__popcll(__ballot(o >= cand)) >= k) th = cand;
-      }
-    } else if (U > 1 && E > 1 && k * (2 * E) <= vocab) {
-      uint32_t o[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) o[u] = order_of(vm[u]);
-#pragma nounroll
-      for (int bit = 31; bit >= 14; --bit) {
-        const uint32_t cand = th | 1u << bit;
-        int c = 0;
-#pragma unroll
-        for (int u = 0; u < U; ++u) c += __popcll(__ballot(o[u] >= cand));
-        if (c >= k) th = cand;
-      }
-    } else {
-#pragma nounroll
-      for (int bit = 31; bit >= 14; --bit) {
-        const float f = of_order(th | 1u << bit);
-        int c = 0;
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int e = 0; e < E; ++e) c += __popcll(__ballot(v[u].get(e) >= f));
-        if (c < k) continue;
-        th |= 1u << bit;
-        if (c <= ((k + 63) & ~63)) break;
-      }
+    for (int bit = 31; bit >= 14; --bit) {
+      const uint32_t cand = th | 1u << bit;
+      if (__popcll(__ballot(o >= cand)) >= k) th = cand;
     }
-    float tau = of_order(th);
-    if (th > order_of(-INFINITY)) {
+  } else if (U > 1 && E > 1 && k * (2 * E) <= vocab) {
+    uint32_t o[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) o[u] = order_of(vm[u]);
+#pragma nounroll
+    for (int bit = 31; bit >= 14; --bit) {
+      const uint32_t cand = th | 1u << bit;
+      int c = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) c += __popcll(__ballot(o[u] >= cand));
+      if (c >= k) th = cand;
+    }
+  } else {
+#pragma nounroll
+    for (int bit = 31; bit >= 14; --bit) {
+      const float f = of_order(th | 1u << bit);
+      int c = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        V w = v[u];
+        // (64 logits of a lane take too many registers as floats: 16384 x 4000, k
+        // 200 99 us, unpacked each time 86; 32 do not: 65536 x 2000, k 256 304, 331)
+        if (U * E > 32) w.keep();
+#pragma unroll
+        for (int e = 0; e < E; ++e) c += __popcll(__ballot(w.get(e) >= f));
+      }
+      if (c < k) continue;
+      th |= 1u << bit;
+      if (c <= ((k + 63) & ~63)) break;
+    }
+  }
+  float tau = of_order(th);
+  if (th > order_of(-INFINITY)) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float f = v[u].get(e);
+        const uint64_t b = __ballot(f >= tau);
+        if (b) {
+          const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
+          if (f >= tau && at < C) buf[at] = order_key(f, (uint32_t)((u * 64 + lane) * E + e));
+          n += __popcll(b);
+        }
+      }
+  } else {
+    n = C + 1;
+  }
+  if (n > C) {
+    // Logits that reach f, which is above -inf (so does no NaN).
+    auto reach = [&](float f) {
+      int c = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        V w = v[u];
+        w.keep();
+#pragma unroll
+        for (int e = 0; e < E; ++e) c += __popcll(__ballot(w.get(e) >= f));
+      }
+      return c;
+    };
+    th = order_of(LOWEST);
+    int c = reach(LOWEST);
+    if (c > C) {
+      th = order_of(top);
+      c = reach(top);
+      if (c < k) {
+        th = 0;
+#pragma nounroll
+        for (int bit = 31; bit >= 0; --bit) {
+          const int d = reach(of_order(th | 1u << bit));
+          if (d < k) continue;
+          th |= 1u << bit;
+          c = d;
+          if (c <= C) break;
+        }
+      }
+      th += c > C;
+    }
+    tau = of_order(th);
+    // those that reach th, then, if these are less than k, the first of those next
+    // below it (-inf, or a NaN in its place, below the lowest)
+    const float next = of_order(th - 1);
+    n = 0;
+#pragma nounroll
+    for (int below = 0; below < 2; ++below)
 #pragma unroll
       for (int u = 0; u < U; ++u)
+        if (!below || n < k) {
+          V w = v[u];
+          w.keep();
+          const int first = renewed((u * 64 + lane) * E);
+          auto counts = [&](int e) {
+            const float f = w.get(e);
+            return below ? first + e < vocab && (next == -INFINITY ? !(f > next) : f == next) : f >= tau;
+          };
+          int mine = 0;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float f = v[u].get(e);
-          const uint64_t b = __ballot(f >= tau);
-          if (b) {
-            const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
-            if (f >= tau && at < C) buf[at] = order_key(f, (uint32_t)((u * 64 + lane) * E + e));
-            n += __popcll(b);
-          }
+          for (int e = 0; e < E; ++e) mine += counts(e);
+          const int upto = wave_scan<Sum>(mine, 0);
+          int at = n + upto - mine;
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (counts(e)) {
+              if (at < (below ? k : C)) buf[at] = order_key(below ? next : w.get(e), (uint32_t)(first + e));
+              ++at;
+            }
+          n += lane_value(upto, 63);
+          if (below) n = min(k, n);
         }
-    } else {
-      n = C + 1;
-    }
-    if (n > C) {
-      th = 0;
-#pragma nounroll
-      for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t cand = th | 1u << bit;
-        int c = 0;
-#pragma nounroll
-        for (int i = lane; i < vocab; i += 64) c += order_of(T::get(x[i])) >= cand;
-        if (wave_reduce<Sum>(c, 0) >= k) th = cand;
-      }
-      n = 0;
-      // (first those above it, then those that equal it, in order)
-      for (int pass = 0; pass < 2; ++pass)
-        for (int i0 = 0; i0 < vocab && n < k; i0 += 64) {
-          const uint32_t o = i0 + lane < vocab ? order_of(T::get(x[i0 + lane])) : 0;
-          const bool mine = pass ? o == th : o > th;
-          const uint64_t b = __ballot(mine);
-          const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
-          if (mine && at < k) buf[at] = (uint64_t)o << 32 | (uint32_t)~(i0 + lane);
-          n = min(k, n + __popcll(b));
-        }
-    }
-    sync<64>();
-    if (n > 64) sort_keys<64, C>(buf, n, k);
-    else key = sort_wave(lane < n ? buf[lane] : 0, n);
   }
+  sync<64>();
+  if (n > 64) sort_keys<64, C>(buf, n, k);
+  else key = sort_wave(lane < n ? buf[lane] : 0, n);
   for (int j = lane; j < k; j += 64) {
-    if (n > 64 || sum != sum) key = buf[j];
+    if (n > 64) key = buf[j];
     const uint32_t id = ~(uint32_t)key;
     p.ids[r * k + j] = id;
     // (the key holds a NaN as -inf)

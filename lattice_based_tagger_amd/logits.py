@@ -212,7 +212,7 @@ def top_logits(logits, k, temperature=1.0):
     ``values`` ``[..., k]`` in the logits' type, largest first, ties to the
     lowest index (a NaN counts as -inf); ``ids`` ``[..., k]`` int64; ``lse``
     ``[...]`` float32 = log sum exp(logits / temperature) over the whole row
-    (-inf for a row of -inf, NaN where the row holds a NaN).
+    (-inf for a row of -inf, NaN where the row holds a NaN and no +inf).
     ``1 <= k <= min(vocab, 256)``.  Not differentiable."""
     _logits(logits, 'logits')
     k = operator.index(k)

@@ -31,6 +31,7 @@ def top_logits(x, k, temperature=1.0):
     order = torch.where(x.isnan(), torch.tensor(-INF, dtype=torch.float64), x)
     ids = torch.sort(order, dim=-1, descending=True, stable=True).indices[..., :k]
     lse = torch.logsumexp(x / temperature, -1)
+    lse = torch.where((x == INF).any(-1), torch.tensor(INF, dtype=torch.float64), lse)   # (beside a NaN too)
     return x.gather(-1, ids), ids, lse
 
 

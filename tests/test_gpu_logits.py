@@ -156,6 +156,39 @@ def test_top_of_a_wave(dtype, vocab):
         check_top(x, k)
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('vocab, k', [(100, 60), (700, 60), (2000, 200), (4000, 256), (9000, 100), (140000, 20)])
+def test_top_ties_and_nan(dtype, vocab, k):
+    """More equal logits than are kept beside the k best, and a NaN or -inf among the
+    k: by their indices."""
+    x = rand((14, vocab), dtype, vocab)
+    x[0] = 1.0
+    x[1, ::2] = 7.5                                    # half of the row the largest
+    x[2] = x[2].clamp(-9.0, -1.0)                      # many at the k-th
+    x[3] = -INF
+    x[4] = -INF
+    x[4, 5::vocab // 30] = 2.0                         # fewer than k are left
+    x[5] = math.nan
+    x[6, 1::3] = math.nan
+    x[7] = -INF
+    x[7, ::3] = math.nan                               # alike, by their indices
+    x[7, 7] = 0.5
+    x[8] = math.nan
+    x[8, ::2] = 3.0
+    x[9] = LOWEST[dtype]
+    x[9, ::3] = -INF
+    x[10] = INF
+    x[10, 3] = math.nan
+    x[11] = torch.where(x[11] > 0, 0.0, -0.0)
+    x[12] = torch.sort(x[12].float()).values.to(dtype)
+    x[13] = (x[13] * 0).add(torch.arange(vocab, device='cuda') % 7)
+    check_top(x, k)
+    many = x.repeat(200, 1)
+    got = logits.top_logits(many, k)
+    want = logits.top_logits(many[:14].clone(), k)
+    assert torch.equal(got.ids.view(200, 14, k), want.ids.expand(200, 14, k))
+
+
 def test_top_many_rows():
     """More rows than blocks are ever resident, of a tag set and of a small vocabulary."""
     check_top(rand((20011, 13), torch.float32, 1), 13)
