@@ -92,12 +92,15 @@ struct VerifyParams {
 
 constexpr int NT = 256;
 
-// The sum of exp2((x - m) c) over a row's numbers [v0, v1), from c0 on, in 32
-// bits; a thread's m is any logit not far below its largest.
-template <class T, int U>
-__device__ __forceinline__ float2 sum_part(const typename T::raw* row, int lead, int c0, int v0, int v1, float c, float* shf) {
+// A thread's part of the sum of exp2((x - m) c) over a row's numbers [v0, v1),
+// from c0 on, in 32 bits; m is any logit not far below its largest.  CLEAN: with
+// -inf for a NaN (a selection for every logit).
+template <class T, int U, bool CLEAN>
+__device__ __forceinline__ void sum_thread(const typename T::raw* row, int lead, int c0, int v0, int v1, float c, float& m, float& s) {
   constexpr int E = Vec<T>::E, STEP = NT * U * E;
-  float m = LOWEST, s = 0.f;
+  m = LOWEST;
+  s = 0.f;
+  auto of = [](float x) { return CLEAN && x != x ? -INFINITY : x; };
   for (int base = c0; base < v1; base += STEP) {
     Vec<T> v[U];
     load_step<T, NT, U>(v, row - lead, base, threadIdx.x, v0, v1);
@@ -116,14 +119,27 @@ __device__ __forceinline__ float2 sum_part(const typename T::raw* row, int lead,
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int e = 0; e < E; e += 2) {
-        const float f0 = exp2_((v[u].get(e) - m) * c), f1 = exp2_((v[u].get(e + 1) - m) * c);
+        const float f0 = exp2_((of(v[u].get(e)) - m) * c), f1 = exp2_((of(v[u].get(e + 1)) - m) * c);
         s0 += f0;
         s1 += f1;
       }
     s += s0 + s1;
   }
-  const float top = block_reduce<NT, Max>(m, shf);
-  return make_float2(top, block_reduce<NT, Sum>(s * exp2_((m - top) * c), shf));
+}
+
+// The block's.  A sum that is no number is taken again without the NaN (of an
+// infinite logit, which is none that the rows may hold, it stays one).
+template <class T, int U>
+__device__ __forceinline__ float2 sum_part(const typename T::raw* row, int lead, int c0, int v0, int v1, float c, float* shf) {
+  float m, s;
+  sum_thread<T, U, false>(row, lead, c0, v0, v1, c, m, s);
+  float top = block_reduce<NT, Max>(m, shf), sum = block_reduce<NT, Sum>(s * exp2_((m - top) * c), shf);
+  if (sum != sum) {                        // (for the block as a whole)
+    sum_thread<T, U, true>(row, lead, c0, v0, v1, c, m, s);
+    top = block_reduce<NT, Max>(m, shf);
+    sum = block_reduce<NT, Sum>(s * exp2_((m - top) * c), shf);
+  }
+  return make_float2(top, sum);
 }
 
 // A row's softmax in 32 bits: exp2((x - m) c) / s.

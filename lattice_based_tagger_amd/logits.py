@@ -393,7 +393,7 @@ def verify_draft(target, draft_ids, accept_u, sample_u, draft=None, lengths=None
     running sum exceeds ``sample_u`` of the whole.  Then the tokens are
     distributed as drawn from the target.  ``tokens`` holds the accepted ones,
     the next one, then -1 (the next one is -1 where the target's row is
-    -inf throughout)."""
+    -inf throughout).  Logits are finite or -inf; a NaN counts as -inf."""
     _logits(target, 'target')
     if target.dim() != 3 or target.shape[1] < 1:
         raise ValueError('target must be [batch, drafts + 1, vocab], not %s' % (tuple(target.shape),))
