@@ -222,8 +222,11 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
   };
   auto cut = [&]() {
     const uint64_t least = cut_keys<NT, C>(buf, n, k, sh.hist, &sh.cnt2, sh.sh64);
-    tau = of_order((uint32_t)(least >> 32));
-    tie = max((uint32_t)least, 1u) - 1;
+    // (The order next below that of 0 is no logit's: it reads as -0, which compares
+    // as 0.  A cut there keeps every 0 so far, and one of a lower index to come.)
+    const bool zero = (uint32_t)(least >> 32) == order_of(0.f) - 1;
+    tau = zero ? 0.f : of_order((uint32_t)(least >> 32));
+    tie = zero ? 0 : max((uint32_t)least, 1u) - 1;
     n = k;
   };
 
