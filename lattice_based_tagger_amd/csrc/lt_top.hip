@@ -29,6 +29,14 @@ __device__ __forceinline__ float log_sum(float m, float s, double inv_t) {
   return m == INFINITY ? m : (float)(m * inv_t + log2_(s) * LN2);
 }
 
+// The logit of a key, row[id]: read again where the key does not tell it, a NaN
+// (in a row whose sum is none: held as -inf) and a -0 (held as 0).
+template <class T>
+__device__ __forceinline__ typename T::raw logit_of(uint64_t key, float sum, const typename T::raw* row) {
+  const uint32_t order = (uint32_t)(key >> 32);
+  return sum != sum || order == order_of(0.f) ? row[~(uint32_t)key] : T::put(of_order(order));
+}
+
 // The key of lane ^ X: by the data-parallel primitives where they can, else by
 // the LDS crossbar.
 template <int X>
@@ -405,10 +413,8 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
   if (p.splits == 1) {
     if (tid == 0) p.lse[r] = log_sum(top, sum, p.inv_t);
     for (int j = tid; j < k; j += NT) {
-      const uint32_t id = ~(uint32_t)buf[j];
-      p.ids[r * k + j] = id;
-      // (the key holds a NaN as -inf)
-      ((raw*)p.values)[r * k + j] = sum != sum ? row[id] : T::put(of_order((uint32_t)(buf[j] >> 32)));
+      p.ids[r * k + j] = ~(uint32_t)buf[j];
+      ((raw*)p.values)[r * k + j] = logit_of<T>(buf[j], sum, row);
     }
   } else {
     if (tid == 0) p.part_sums[blk] = make_float2(top, sum);
@@ -441,9 +447,8 @@ __global__ __launch_bounds__(256) void lt_top_join(TopParams p) {
   if (tid == 0) p.lse[r] = log_sum(m, s, p.inv_t);
   const typename T::raw* x = (const typename T::raw*)p.x.data + p.x.at(r);
   for (int j = tid; j < p.k; j += NT) {
-    const uint32_t id = ~(uint32_t)sh.buf[j];
-    p.ids[r * p.k + j] = id;
-    ((typename T::raw*)p.values)[r * p.k + j] = s != s ? x[id] : T::put(of_order((uint32_t)(sh.buf[j] >> 32)));
+    p.ids[r * p.k + j] = ~(uint32_t)sh.buf[j];
+    ((typename T::raw*)p.values)[r * p.k + j] = logit_of<T>(sh.buf[j], s, x);
   }
 }
 
@@ -688,10 +693,8 @@ __global__ __launch_bounds__(256) void lt_top_wave(TopParams p) {
   else key = sort_wave(lane < n ? buf[lane] : 0, n);
   for (int j = lane; j < k; j += 64) {
     if (n > 64) key = buf[j];
-    const uint32_t id = ~(uint32_t)key;
-    p.ids[r * k + j] = id;
-    // (the key holds a NaN as -inf)
-    ((raw*)p.values)[r * k + j] = sum != sum ? x[id] : T::put(of_order((uint32_t)(key >> 32)));
+    p.ids[r * k + j] = ~(uint32_t)key;
+    ((raw*)p.values)[r * k + j] = logit_of<T>(key, sum, x);
   }
 }
 

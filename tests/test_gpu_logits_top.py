@@ -1,4 +1,5 @@
-"""``top_logits`` where a bound that a row's logits are cut at falls on zero."""
+"""``top_logits`` where a bound that a row's logits are cut at falls on zero, and
+the sign of zeros."""
 
 import pytest
 import torch
@@ -52,3 +53,23 @@ def test_rising_ties_about_zero(dtype, rows, vocab, k):
     x[torch.rand(rows, vocab, generator=g) < 2.0 * k / vocab] = 0.0
     x[::3] += 1
     check(x.to(dtype).cuda(), k)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('rows, vocab, k', [
+    (16500, 41, 1), (16500, 41, 5), (16500, 60, 8), (7, 41, 9), (7, 100, 3), (7, 200, 40), (7, 700, 100), (7, 2000, 64),
+    (2100, 7000, 20), (600, 9000, 100), (5, 9000, 256), (5, 40000, 256), (3, 140000, 20)])
+def test_the_sign_of_zeros(dtype, rows, vocab, k):
+    """-0 and 0 are equal, by their indices; each comes back as it is."""
+    g = torch.Generator().manual_seed(vocab)
+    x = torch.randint(-3, 1, (rows, vocab), generator=g).float()
+    x = torch.where(torch.rand(rows, vocab, generator=g) < 0.5, x.abs().neg(), x)
+    x[0] = -0.0
+    x[1, ::2] = -x[1, ::2].abs()
+    x[2, 3:] = -0.0
+    assert (x == 0).any() and x[0].signbit().all()
+    x = x.to(dtype).cuda()
+    check(x, k)
+    got = logits.top_logits(x, k)
+    assert torch.equal(got.values.float().signbit(), x.gather(1, got.ids).float().signbit())
+    assert got.values[0].float().signbit().all()
