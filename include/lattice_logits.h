@@ -76,7 +76,9 @@ lt_status lt_top_logits(const lt_rows* x, int32_t k, double temperature, void* v
  *     p_j = exp(top_j / temperature - top_lse),  p_rest = max(0, 1 - sum p_j),
  *     q_rest = the q_v of every v that is no entry, summed
  *   loss = sum_j p_j (log p_j - log q_{id_j}) + p_rest (log p_rest - log q_rest)
- *     (the last term is left out where q_rest = 0)
+ *     (the last term is left out, p_rest = 0, where the others are masked: each is
+ *     -inf, or each the type's lowest value and more than 745 temperatures below the
+ *     row's largest logit; else q_rest may be as small as logits can make it)
  *   d loss / d z_v = 1/temperature * (P q_v - sum_{id_j = v} p_j)       v an entry
  *                    1/temperature * (P - p_rest / q_rest) q_v         else
  *     with P = sum p_j + p_rest

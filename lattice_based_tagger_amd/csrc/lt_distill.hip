@@ -1,5 +1,7 @@
 // lt_distill.hip -- the distillation loss against a teacher's top logits and
 // its gradient (include/lattice_logits.h lt_distill_*).
+#include <type_traits>
+
 #include "lt_logits.h"
 
 namespace {
@@ -21,8 +23,8 @@ struct DistillParams {
   int32_t splits;         // blocks of a row
   int32_t chunk;          // of a row's numbers, to a block (a multiple of its step)
   float* loss;
-  float* stats;           // [rows][LT_DISTILL_STATS]: m, the gradient's factors of exp2((z - m) c)
-  float4* part;           // splits > 1: [rows][splits] reference, sums within and outside the entries
+  float* stats;           // [rows][LT_DISTILL_STATS]: Factors
+  float2* part;           // splits > 1: [rows][splits] reference and sum, its sign set where an id came again
   float scale;
   const float* weight;    // NULL: 1
   int64_t weight_stride;
@@ -42,7 +44,7 @@ struct DistillShared {
   float mass[MAXK];
   uint32_t bits[WINDOW / 32];
   double sh[NT / 64];
-  float shf[NT / 64];
+  int again;                               // an id came more than once
 };
 
 // A thread's entries of the teacher's row, j = i * NT + thread: logits that are
@@ -124,15 +126,41 @@ __device__ __forceinline__ void load_entries(const Teacher& t, int64_t r, int vo
   }
 }
 
-// sums of exp2((z - m) c) of a thread: within the entries (TAIL) and of all else
+// first: of a block's entries that are one logit the first alone (ids: MAXK in LDS,
+// -1 behind the row's).  Which of several waves' an atomic finds first varies from
+// call to call, and so would the order of a sum.
+template <int NT>
+__device__ __forceinline__ void only_first(const Entries<NT>& t, const int* ids, int entries, bool (&first)[1]) {
+  const int own = threadIdx.x, id = t.id[0];
+  bool before = false;
+  for (int j = 0; j < entries; j += 16) {
+    int4 o[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = ((const int4*)&ids[j])[k];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int left = own - (j + k * 4);
+      before |= (o[k].x == id && left > 0) | (o[k].y == id && left > 1) | (o[k].z == id && left > 2) | (o[k].w == id && left > 3);
+    }
+  }
+  first[0] = id >= 0 && !before;
+}
+
+// A sum of exp2((z - m) c), and its reference m.
 struct Sums {
-  float m = LOWEST, in = 0.f, out = 0.f;
+  float m = LOWEST, s = 0.f;
 };
 
-// One pass over a row's logits with numbers in [v0, v1), from c0 on.
+// One pass over a row's logits with numbers in [v0, v1), from c0 on: the sum of
+// all, or, with the tail (TAIL), of all that are no entries.  These have a
+// reference of their own: beside a larger entry's their sum would lose its bits,
+// or all of it -- 87 temperatures below it nothing is left of it in 32 bits, where
+// the loss is to be 87 and the gradient p_rest.  first: of the entries in these
+// windows that are one logit, whether it is the one that was seen first
+// (sh.again: some were seen again).
 template <class T, int NT, int U, int WINDOW, bool TAIL>
 __device__ __forceinline__ Sums sum_row(const typename T::raw* row, int lead, int c0, int v0, int v1, float c, const Entries<NT>& t,
-                                        DistillShared<NT, WINDOW>& sh) {
+                                        DistillShared<NT, WINDOW>& sh, bool (&first)[Entries<NT>::N]) {
   constexpr int E = Vec<T>::E, STEP = NT * U * E;
   static_assert(WINDOW % STEP == 0 || WINDOW >= STEP, "a step lies in a window");
   const int tid = thread_of<NT>();
@@ -146,92 +174,149 @@ __device__ __forceinline__ Sums sum_row(const typename T::raw* row, int lead, in
 #pragma unroll
       for (int i = 0; i < Entries<NT>::N; ++i) {
         const int at = t.id[i] + lead - w0;
-        if (t.id[i] >= 0 && at >= 0 && at < w1 - w0) atomicOr(&sh.bits[at >> 5], 1u << (at & 31));
+        if (t.id[i] >= 0 && at >= 0 && at < w1 - w0) {
+          first[i] = !(atomicOr(&sh.bits[at >> 5], 1u << (at & 31)) >> (at & 31) & 1);
+          if (!first[i]) sh.again = 1;
+        }
       }
       sync<NT>();
     }
     for (int base = w0; base < w1; base += STEP) {
       Vec<T> v[U];
       load_step<T, NT, U>(v, z, base, tid, v0, w1);
-      uint32_t in[U];
       float t = -INFINITY;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (TAIL) {
           const int at = min(base + (u * NT + tid) * E, w1 - 1) - w0;
-          in[u] = (sh.bits[at >> 5] >> (at & 31 & ~(E - 1))) & ((1u << E) - 1);
+          const uint32_t in = (sh.bits[at >> 5] >> (at & 31 & ~(E - 1))) & ((1u << E) - 1);
+          if (__any(in)) v[u].mask(in);
         }
         t = max2(t, max_of(v[u]));
         v[u].keep();
       }
       if ((t - o.m) * c > 32.f) {
-        const float f = exp2_((o.m - t) * c);
-        o.in *= f;
-        o.out *= f;
+        o.s *= exp2_((o.m - t) * c);
         o.m = t;
       }
       float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (TAIL && __any(in[u])) {
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int e = 0; e < E; ++e) {
-            const float f = exp2_((v[u].get(e) - o.m) * c);
-            const bool entry = in[u] >> e & 1;
-            o.in += entry ? f : 0.f;
-            s0 += entry ? 0.f : f;
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < E; e += 2) {
-            s0 += exp2_((v[u].get(e) - o.m) * c);
-            s1 += exp2_((v[u].get(e + 1) - o.m) * c);
-          }
+        for (int e = 0; e < E; e += 2) {
+          s0 += exp2_((v[u].get(e) - o.m) * c);
+          s1 += exp2_((v[u].get(e + 1) - o.m) * c);
         }
-      }
-      o.out += s0 + s1;
+      o.s += s0 + s1;
     }
     if (TAIL) sync<NT>();
   }
   return o;
 }
 
+// Two at once: a thread's sum and, of the entries beside it, the row's.
+struct Two {
+  float a, b;
+};
+struct Max2 {
+  static __device__ __forceinline__ Two of(Two x, Two y) { return {max2(x.a, y.a), max2(x.b, y.b)}; }
+};
+struct Sum2 {
+  static __device__ __forceinline__ Two of(Two x, Two y) { return {x.a + y.a, x.b + y.b}; }
+};
+template <> __device__ __forceinline__ Two neutral<Max2, Two>() { return {-INFINITY, -INFINITY}; }
+template <> __device__ __forceinline__ Two neutral<Sum2, Two>() { return {0.f, 0.f}; }
+
 // The sums of a group's threads, or of a row's chunks.
 template <int NT>
-__device__ __forceinline__ Sums join(Sums o, float c, float* shf) {
-  const float m = block_reduce<NT, Max>(o.m, shf), f = exp2_((o.m - m) * c);
-  o.in = block_reduce<NT, Sum>(o.in * f, shf);
-  o.out = block_reduce<NT, Sum>(o.out * f, shf);
-  o.m = m;
-  return o;
+__device__ __forceinline__ Sums join(Sums o, float c, double* sh) {
+  const float m = block_reduce<NT, Max>(o.m, (float*)sh);
+  return {m, block_reduce<NT, Sum>(o.s * exp2_((o.m - m) * c), (float*)sh)};
+}
+// The same of all but the entries, and, with the entries' logits zi, each once
+// (`first` tells) however often the row repeats it, of the row.
+template <int NT>
+__device__ __forceinline__ Sums join(Sums o, const float (&zi)[Entries<NT>::N], const bool (&first)[Entries<NT>::N], float c,
+                                     double* sh, Sums& all) {
+  float in = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < Entries<NT>::N; ++i) in = first[i] ? max2(in, zi[i]) : in;
+  const Two m = block_reduce<NT, Max2>(Two{o.m, max2(o.m, in)}, (Two*)sh);
+  in = 0.f;
+#pragma unroll
+  for (int i = 0; i < Entries<NT>::N; ++i) in += first[i] ? exp2_((zi[i] - m.b) * c) : 0.f;
+  const Two s = block_reduce<NT, Sum2>(Two{o.s * exp2_((o.m - m.a) * c), in}, (Two*)sh);
+  all = {m.b, s.b + s.a * exp2_((m.a - m.b) * c)};
+  return {m.a, s.a};
 }
 
-// Loss and the gradient's factors of a row from its sums.
-__device__ __forceinline__ float3 factors(Sums o, double sum, double& rest, double inv_t, float& qrest) {
-  const float s = o.in + o.out, inv = 1 / s;
-  qrest = o.out * inv;
-  if (!(rest > 0 && qrest > 0)) rest = 0;
+// 2^t, t <= 0.
+__device__ __forceinline__ float exp2_of(double t) {
+  if (t < -160) return 0.f;
+  const double n = rint(t);
+  return ldexpf(exp2_((float)(t - n)), (int)n);
+}
+
+// What the gradient of a row is made of: an entry's is exp2((z - m) entry) less
+// its mass, another's exp2((z - other_m) other).
+struct Factors {
+  float other_m, other, m, entry;
+};
+__device__ __forceinline__ Factors of_stats(const float* stats, int64_t r) {
+  const float4 v = *(const float4*)(stats + r * LT_DISTILL_STATS);
+  return {v.x, v.y, v.z, v.w};
+}
+__device__ __forceinline__ void put_stats(float* stats, int64_t r, Factors f) {
+  *(float4*)(stats + r * LT_DISTILL_STATS) = make_float4(f.other_m, f.other, f.m, f.entry);
+}
+
+// From the row's sum and that of all but its entries (where that is not known,
+// the row's).  p_rest becomes 0 where these have nothing: all of them are -inf, or
+// all the type's lowest value -- a mask -- and so far below the largest logit that
+// 64 bits hold nothing of them.  Else q_rest may lie as far below as logits can:
+// log_rest is its logarithm, and with
+//   q_v = q_rest r_v,  r_v = exp2((z - other_m) c) / others.s
+// the gradient (P - p_rest / q_rest) q_v is (P q_rest - p_rest) r_v, which neither
+// under- nor overflows.  log_s: the row's sum's, to the base 2 as all.
+constexpr double GONE = 745;               // exp(-745) is the least in 64 bits
+template <class T, bool TAIL>
+__device__ __forceinline__ Factors factors(Sums all, Sums others, double sum, double& rest, double inv_t, double log_s,
+                                           double& log_rest) {
+  if (!TAIL) {
+    const float entry = all.s > 0 ? (float)(sum * inv_t) * (1 / all.s) : 0.f;
+    return {all.m, entry, all.m, entry};
+  }
+  double t = 0;
+  float far = 1;
+  if (others.m != all.m) {
+    t = ((double)others.m - all.m) * (inv_t * LOG2E);
+    far = exp2_of(t);
+  }
+  if (!(others.s > 0) || (others.m <= T::lowest && -t > GONE * LOG2E)) rest = 0;
+  log_rest = t + log2_(others.s) - log_s;
   const double whole = sum + rest;
-  if (!(s > 0)) return make_float3(o.m, 0.f, 0.f);
-  const float other = rest > 0 ? (float)rest / qrest : 0.f;
-  return make_float3(o.m, (float)(whole * inv_t) * inv, (float)((whole - other) * inv_t) * inv);
+  if (!(all.s > 0)) return {others.m, 0.f, all.m, 0.f};
+  const float inv = 1 / all.s, entry = (float)(whole * inv_t) * inv;
+  if (!(rest > 0)) return {others.m, entry * far, all.m, entry};
+  const float qrest = others.s * inv * far;
+  return {others.m, (float)((whole * qrest - rest) * inv_t) / others.s, all.m, entry};
 }
 
-// (zi: the logits of the entries.)
-template <int NT, int N>
-__device__ __forceinline__ float3 finish_row(const Entries<NT, N>& t, const float (&zi)[N], Sums o, double inv_t,
-                                             double* sh, float& loss) {
-  const double logs = log2_(o.in + o.out), c = inv_t * LOG2E;
-  double l = 0, rest = t.rest;
+// Loss and the gradient's factors of a row from its sums (zi: the logits of the
+// entries).
+template <class T, bool TAIL, int NT, int N>
+__device__ __forceinline__ Factors finish_row(const Entries<NT, N>& t, const float (&zi)[N], Sums all, Sums others, double inv_t,
+                                              double* sh, float& loss) {
+  const double logs = log2_(all.s), c = inv_t * LOG2E;
+  double l = 0, rest = t.rest, log_rest;
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    if (t.id[i] >= 0 && t.p[i] != 0) l += t.p[i] * (t.logp[i] - ((double)zi[i] - o.m) * c + logs);
+    if (t.id[i] >= 0 && t.p[i] != 0) l += t.p[i] * (t.logp[i] - ((double)zi[i] - all.m) * c + logs);
   l = block_reduce<NT, Sum>(l, sh);
-  float qrest;
-  const float3 st = factors(o, t.sum, rest, inv_t, qrest);
-  if (rest > 0) l += rest * (log2_((float)rest) - log2_(qrest));
+  const Factors f = factors<T, TAIL>(all, others, t.sum, rest, inv_t, logs, log_rest);
+  if (TAIL && rest > 0) l += rest * (log2_((float)rest) - log_rest);
   loss = (float)(l * LN2);
-  return st;
+  return f;
 }
 
 // (z: the row.)
@@ -241,16 +326,16 @@ __device__ __forceinline__ void load_zi(const Entries<NT, N>& t, const typename 
   for (int i = 0; i < N; ++i) zi[i] = t.id[i] >= 0 ? T::get(z[t.id[i]]) : 0.f;
 }
 
-// The gradient of the logits with numbers in [v0, v1), from c0 on: st from
-// finish_row, w the row's weight.  The entries' own are written behind a barrier
-// over what the others were given.
+// The gradient of the logits with numbers in [v0, v1), from c0 on; w: the row's
+// weight.  The entries' own are written behind a barrier over what the others
+// were given.
 template <class T, int NT, int U, int WINDOW, bool AGAIN>
 __device__ __forceinline__ void grad_row(const typename T::raw* row, typename T::raw* grad, int lead, int c0, int v0,
-                                         int v1, float c, float3 st, float w, double inv_t, const Entries<NT>& t,
+                                         int v1, float c, Factors st, float w, double inv_t, const Entries<NT>& t,
                                          DistillShared<NT, WINDOW>& sh, int entries, bool past) {
   constexpr int E = Vec<T>::E, STEP = NT * U * E;
   const int tid = thread_of<NT>();
-  const float out = st.z * w;
+  const float out = st.other * w;
   const typename T::raw* const z = row - lead;
   typename T::raw* const g = grad - lead;
   if (t.blank()) {
@@ -269,7 +354,7 @@ __device__ __forceinline__ void grad_row(const typename T::raw* row, typename T:
     for (int u = 0; u < U; ++u) {
       float f[E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) f[e] = exp2_((v[u].get(e) - st.x) * c) * out;
+      for (int e = 0; e < E; ++e) f[e] = exp2_((v[u].get(e) - st.other_m) * c) * out;
       v[u].put(f);
       const int at = base + (u * NT + tid) * E;
       if (at >= v0 && at + E <= v1) {
@@ -303,7 +388,7 @@ __device__ __forceinline__ void grad_row(const typename T::raw* row, typename T:
       mass = 0;
       for (int j = 0; j < entries; ++j) mass += sh.id[j] == id ? sh.mass[j] : 0.f;
     }
-    grad[id] = T::put((exp2_((T::get(row[id]) - st.x) * c) * st.y - mass) * w);
+    grad[id] = T::put((exp2_((T::get(row[id]) - st.m) * c) * st.entry - mass) * w);
   }
 }
 
@@ -317,61 +402,87 @@ __device__ __forceinline__ void grad_row(const typename T::raw* row, typename T:
   Entries<NT> t;                                                                                          \
   load_entries(p.t, r, p.z.vocab, p.inv_t, t, sh.sh)
 
+// Its pass: o, the sum of all that are no entries (without the tail: of all), and
+// the row's.
+#define PASS                                                                                              \
+  float zi[Entries<NT>::N];                                                                               \
+  bool first[Entries<NT>::N] = {};                                                                        \
+  load_zi<T>(t, z, zi);                                                                                   \
+  Sums o, all;                                                                                            \
+  if (threadIdx.x == 0) sh.again = 0;                                                                     \
+  if (!t.blank()) {                                                                                       \
+    o = sum_row<T, NT, U, WINDOW, TAIL>(z, lead, c0, v0, v1, p.c, t, sh, first);                          \
+    if (TAIL && p.splits == 1) {                                                                          \
+      if (sh.again) {                                                                                     \
+        if ((int)threadIdx.x < MAXK) sh.id[threadIdx.x] = t.id[0];                                        \
+        __syncthreads();                                                                                  \
+        only_first<NT>(t, sh.id, p.t.entries, first);                                                     \
+      }                                                                                                   \
+      o = join<NT>(o, zi, first, p.c, sh.sh, all);                                                        \
+    } else {                                                                                              \
+      all = o = join<NT>(o, p.c, sh.sh);                                                                  \
+    }                                                                                                     \
+  }
+
 // Loss and statistics, or the gradient from them: one pass each, bound by memory
 // (2039 x 50261 bf16, 32 entries with the tail: 49 us, 4.2 TB/s, and 65 us, 6.3
 // TB/s with what of the logits is still in the last cache).
 template <class T, int NT, int U, int WINDOW, bool TAIL>
 __global__ __launch_bounds__(NT) void lt_distill_sums(DistillParams p) {
   BLOCK_HEAD;
-  Sums o;
-  if (!t.blank()) o = join<NT>(sum_row<T, NT, U, WINDOW, TAIL>(z, lead, c0, v0, v1, p.c, t, sh), p.c, sh.shf);
+  PASS;
   if (p.splits > 1) {
-    if (threadIdx.x == 0) p.part[blk] = make_float4(o.m, o.in, o.out, 0.f);
+    if (threadIdx.x == 0) p.part[blk] = make_float2(o.m, TAIL && !t.blank() && sh.again ? -o.s : o.s);
     return;
   }
   float loss;
-  float zi[Entries<NT>::N];
-  load_zi<T>(t, z, zi);
-  const float3 st = finish_row(t, zi, o, p.inv_t, sh.sh, loss);
+  const Factors st = finish_row<T, TAIL>(t, zi, all, o, p.inv_t, sh.sh, loss);
   if (threadIdx.x == 0) {
     p.loss[r] = loss;
-    *(float4*)(p.stats + r * LT_DISTILL_STATS) = make_float4(st.x, st.y, st.z, 0.f);
+    put_stats(p.stats, r, st);
   }
 }
 
 // A row's chunks joined.
-template <class T>
+template <class T, bool TAIL>
 __global__ __launch_bounds__(256) void lt_distill_join(DistillParams p) {
   constexpr int NT = 256;
-  __shared__ DistillShared<NT, 32> sh;
+  __shared__ __attribute__((aligned(16))) DistillShared<NT, 32> sh;
   const int64_t r = p.block0 + blockIdx.x;
   Entries<NT> t;
   load_entries(p.t, r, p.z.vocab, p.inv_t, t, sh.sh);
   Sums o;
+  bool again = false;
   if ((int)threadIdx.x < p.splits) {       // (at most NT chunks)
-    const float4 part = p.part[r * p.splits + threadIdx.x];
+    const float2 part = p.part[r * p.splits + threadIdx.x];
     o.m = part.x;
-    o.in = part.y;
-    o.out = part.z;
+    o.s = fabsf(part.y);
+    again = signbit(part.y);
   }
-  o = join<NT>(o, p.c, sh.shf);
-  float loss;
   float zi[Entries<NT>::N];
   load_zi<T>(t, (const typename T::raw*)p.z.data + p.z.at(r), zi);
-  const float3 st = finish_row(t, zi, o, p.inv_t, sh.sh, loss);
+  Sums all;
+  if (TAIL) {
+    bool first[1] = {t.id[0] >= 0};
+    sh.id[threadIdx.x] = t.id[0];
+    if (__syncthreads_or(again)) only_first<NT>(t, sh.id, p.t.entries, first);
+    o = join<NT>(o, zi, first, p.c, sh.sh, all);
+  } else {
+    all = o = join<NT>(o, p.c, sh.sh);
+  }
+  float loss;
+  const Factors st = finish_row<T, TAIL>(t, zi, all, o, p.inv_t, sh.sh, loss);
   if (threadIdx.x == 0) {
     p.loss[r] = loss;
-    *(float4*)(p.stats + r * LT_DISTILL_STATS) = make_float4(st.x, st.y, st.z, 0.f);
+    put_stats(p.stats, r, st);
   }
 }
 
 template <class T, int NT, int U, int WINDOW>
 __global__ __launch_bounds__(NT) void lt_distill_grad(DistillParams p) {
   BLOCK_HEAD;
-  const float4 st = *(const float4*)(p.stats + r * LT_DISTILL_STATS);
   grad_row<T, NT, U, WINDOW, false>(z, (typename T::raw*)p.grad.data + p.grad.at(r), lead, c0, v0, v1, p.c,
-                                    make_float3(st.x, st.y, st.z), weight_of(p, r), p.inv_t, t, sh,
-                                    p.t.entries, p.past);
+                                    of_stats(p.stats, r), weight_of(p, r), p.inv_t, t, sh, p.t.entries, p.past);
 }
 
 // Both: the second pass finds the row in the caches.  It reads past them, and
@@ -382,12 +493,9 @@ __global__ __launch_bounds__(NT) void lt_distill_grad(DistillParams p) {
 template <class T, int NT, int U, int WINDOW, bool TAIL>
 __global__ __launch_bounds__(NT, 8) void lt_distill_both(DistillParams p) {
   BLOCK_HEAD;
-  Sums o;
-  if (!t.blank()) o = join<NT>(sum_row<T, NT, U, WINDOW, TAIL>(z, lead, c0, v0, v1, p.c, t, sh), p.c, sh.shf);
+  PASS;
   float loss;
-  float zi[Entries<NT>::N];
-  load_zi<T>(t, z, zi);
-  const float3 st = finish_row(t, zi, o, p.inv_t, sh.sh, loss);
+  const Factors st = finish_row<T, TAIL>(t, zi, all, o, p.inv_t, sh.sh, loss);
   if (threadIdx.x == 0) p.loss[r] = loss;
   grad_row<T, NT, U, WINDOW, true>(z, (typename T::raw*)p.grad.data + p.grad.at(r), lead, c0, v0, v1, p.c, st,
                                    weight_of(p, r), p.inv_t, t, sh, p.t.entries, p.past);
@@ -396,8 +504,8 @@ __global__ __launch_bounds__(NT, 8) void lt_distill_both(DistillParams p) {
 // Rows that a wave holds in its registers, U vectors a lane: read once, their
 // exponentials too taken once for the loss and the gradient.  N * 64 entries at
 // most.  The sum within the entries is that of the entries' own logits, each
-// once; the sum of all else leaves them out by a mask of bits in LDS (all less
-// the entries' would lose what is left where that is little).
+// once; the row's others are summed beside the largest of their own, with -inf in
+// the entries' places (a mask of bits in LDS tells them).
 template <int N>
 struct WaveShared {
   uint32_t bits[128];
@@ -405,8 +513,11 @@ struct WaveShared {
   float mass[N * 64];
 };
 
+// (Of 16-bit rows up to 2048 with many entries and the tail the compiler takes one
+// register more than six waves a SIMD leave: 65536 x 2000 bf16, 100 entries 152 us
+// by six, 159 by five.)
 template <class T, class V, int U, int N, bool TAIL, bool LOSS, bool GRAD>
-__global__ __launch_bounds__(256) void lt_distill_wave(DistillParams p) {
+__global__ __launch_bounds__(256, (TAIL && N > 1 && U == 4 && V::E == 8 ? 6 : 1)) void lt_distill_wave(DistillParams p) {
   using raw = typename T::raw;
   constexpr int E = V::E;
   __shared__ WaveShared<N> shared[4];
@@ -435,52 +546,55 @@ __global__ __launch_bounds__(256) void lt_distill_wave(DistillParams p) {
   for (int i = 0; i < N; ++i)
     first[i] = t.id[i] >= 0 && !(atomicOr(&sh.bits[t.id[i] >> 5], 1u << (t.id[i] & 31)) >> (t.id[i] & 31) & 1);
   sync<64>();
-  float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
+  Factors st{0.f, 0.f, 0.f, 0.f};
   if (LOSS) {
     float m = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      if (TAIL) {
+        const int at = min((u * 64 + lane) * E, vocab - 1);
+        v[u].mask(sh.bits[at >> 5] >> (at & 31 & ~(E - 1)));
+      }
       m = max2(m, max_of(v[u]));
       v[u].keep();
     }
-    st.x = max2(wave_reduce<Max>(m, -INFINITY), LOWEST);
+    st.m = st.other_m = max2(wave_reduce<Max>(m, -INFINITY), LOWEST);
+    if (TAIL) {
+      // (the entries' sum too beside the others' largest, unless that lies so far
+      // below that the roundings of their exponents would count)
+      float in = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < N; ++i) in = first[i] ? max2(in, zi[i]) : in;
+      if (__any((in - st.m) * p.c > 16.f)) st.m = max2(st.m, wave_reduce<Max>(in, -INFINITY));
+    }
   } else {
-    st = *(const float4*)(p.stats + r * LT_DISTILL_STATS);
+    st = of_stats(p.stats, r);
   }
   float f[U][E], out[2] = {0.f, 0.f};
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    int others = -1;
-    if (LOSS && TAIL) {
-      const int at = min((u * 64 + lane) * E, vocab - 1);
-      others = ~(sh.bits[at >> 5] >> (at & 31 & ~(E - 1)));
-    }
+  for (int u = 0; u < U; ++u)
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      f[u][e] = exp2_((v[u].get(e) - st.x) * p.c);
-      if (LOSS && TAIL) out[e & 1] += __builtin_bit_cast(float, __builtin_bit_cast(int, f[u][e]) & (others << (31 - e) >> 31));
-      else if (LOSS) out[e & 1] += f[u][e];
+      f[u][e] = exp2_((v[u].get(e) - st.other_m) * p.c);
+      if (LOSS) out[e & 1] += f[u][e];
     }
-  }
   if (LOSS) {
-    Sums o;
-    o.m = st.x;
-    o.out = wave_reduce<Sum>(out[0] + out[1], 0.f);
+    Sums rest{st.other_m, wave_reduce<Sum>(out[0] + out[1], 0.f)}, all = rest;
     if (TAIL) {
+      float in = 0.f;
 #pragma unroll
-      for (int i = 0; i < N; ++i) o.in += first[i] ? exp2_((zi[i] - st.x) * p.c) : 0.f;
-      o.in = wave_reduce<Sum>(o.in, 0.f);
+      for (int i = 0; i < N; ++i) in += first[i] ? exp2_((zi[i] - st.m) * p.c) : 0.f;
+      all = {st.m, wave_reduce<Sum>(in, 0.f) + rest.s * exp2_((rest.m - st.m) * p.c)};
     }
     float loss;
-    const float3 q = finish_row(t, zi, o, p.inv_t, nullptr, loss);
-    st = make_float4(q.x, q.y, q.z, 0.f);
+    st = finish_row<T, TAIL>(t, zi, all, rest, p.inv_t, nullptr, loss);
     if (lane == 0) {
       p.loss[r] = blank ? 0.f : loss;
-      if (!GRAD) *(float4*)(p.stats + r * LT_DISTILL_STATS) = st;
+      if (!GRAD) put_stats(p.stats, r, st);
     }
   }
   if (!GRAD) return;
-  const float w = weight_of(p, r), all = st.z * w;
+  const float w = weight_of(p, r), all = st.other * w;
   raw* const g = (raw*)p.grad.data + p.grad.at(r);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -520,14 +634,19 @@ __global__ __launch_bounds__(256) void lt_distill_wave(DistillParams p) {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    if (t.id[i] >= 0) g[t.id[i]] = T::put((exp2_((zi[i] - st.x) * p.c) * st.y - mass[i]) * w);
+    if (t.id[i] >= 0) g[t.id[i]] = T::put((exp2_((zi[i] - st.m) * p.c) * st.entry - mass[i]) * w);
 }
 
 // Rows of at most FEW logits: a thread a row, the row in LDS, its entries a
-// mask of 64 bits.  The gradient is made of the logits alone (no stats).  131072 x
+// mask of 64 bits.  The others' sum is taken with the row's, and again beside the
+// largest of their own where it is LITTLE beside that: there its exponents'
+// roundings cost more than 2^-18 of it, further down it vanishes.  The gradient is
+// made of the logits alone (no stats).  131072 x
 // 41 float32, 5 entries: loss 17 us, gradient 24, where reading the logits and
 // writing the gradient take 4 each: its instructions bound it, those in 64 bits
 // for every entry foremost.
+constexpr float LITTLE = 0x1p-24f;
+
 template <class T, bool LOSS, bool GRAD>
 __global__ __launch_bounds__(64) void lt_distill_few(DistillParams p) {
   using raw = typename T::raw;
@@ -570,45 +689,70 @@ __global__ __launch_bounds__(64) void lt_distill_few(DistillParams p) {
     sum = sum > 0 ? 1 : sum;               // (a NaN stays)
   }
   const bool blank = sum == 0 && rest == 0;
-  Sums o;
-  for (int i = 0; i < vocab; i += 4) o.m = max2(max3(o.m, z[i], z[i + 1]), max2(z[i + 2], z[i + 3]));
+  Sums all, others;
+  for (int i = 0; i < vocab; i += 4) all.m = max2(max3(all.m, z[i], z[i + 1]), max2(z[i + 2], z[i + 3]));
+  others.m = all.m;
   for (int i = 0; i < vocab; i += 4) {
     float e[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) e[j] = exp2_((z[i + j] - o.m) * p.c);
+    for (int j = 0; j < 4; ++j) e[j] = exp2_((z[i + j] - all.m) * p.c);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const bool entry = mask >> (i + j) & 1;
-      o.in += entry ? e[j] : 0.f;
-      o.out += entry ? 0.f : e[j];
+      all.s += entry ? e[j] : 0.f;
+      others.s += entry ? 0.f : e[j];
     }
   }
-  float qrest;
-  const float3 st = factors(o, sum, rest, p.inv_t, qrest);
+  all.s += others.s;
+  if (__builtin_expect(rest > 0 && others.s < LITTLE, 0)) {
+    others = Sums{};
+    for (int i = 0; i < vocab; i += 4) {
+      float f[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[j] = mask >> (i + j) & 1 ? -INFINITY : z[i + j];
+      others.m = max2(max3(others.m, f[0], f[1]), max2(f[2], f[3]));
+    }
+    for (int i = 0; i < vocab; i += 4) {
+      float f[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[j] = exp2_(((mask >> (i + j) & 1 ? -INFINITY : z[i + j]) - others.m) * p.c);
+      others.s += (f[0] + f[1]) + (f[2] + f[3]);
+    }
+  }
+  const double logs = log2_(all.s);
+  double log_rest;
+  const Factors st = factors<T, true>(all, others, sum, rest, p.inv_t, logs, log_rest);
   if (LOSS) {
     double loss = 0;
-    const double logs = log2_(o.in + o.out);
     for (int j = 0; j < n; ++j)
       if (entry(j, id, v)) {
         const double logp = v - ref - norm, pj = exp2_or_0(logp);
-        if (pj != 0) loss += pj * (logp - ((double)z[id] - o.m) * c + logs);
+        if (pj != 0) loss += pj * (logp - ((double)z[id] - all.m) * c + logs);
       }
-    if (rest > 0) loss += rest * (log2_((float)rest) - log2_(qrest));
+    if (rest > 0) loss += rest * (log2_((float)rest) - log_rest);
     if (lane < rows) {
       p.loss[r] = (float)(loss * LN2);
-      if (p.stats) *(float4*)(p.stats + r * LT_DISTILL_STATS) = make_float4(st.x, st.y, st.z, 0.f);
+      if (p.stats) put_stats(p.stats, r, st);
     }
   }
   if (GRAD) {
     const float w = weight_of(p, r);
     if (lane < rows) {
-      for (int i = 0; i < vocab; i += 4) {
-        float e[4];
+      // (two references in a row are rare: for a wave without, one less selection)
+      auto each = [&](auto two) {
+        for (int i = 0; i < vocab; i += 4) {
+          float e[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) e[j] = exp2_((z[i + j] - o.m) * p.c) * (mask >> (i + j) & 1 ? st.y : st.z) * w;
+          for (int j = 0; j < 4; ++j) {
+            const bool entry = mask >> (i + j) & 1;
+            e[j] = exp2_((z[i + j] - (decltype(two)::value && entry ? st.m : st.other_m)) * p.c) * (entry ? st.entry : st.other) * w;
+          }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) z[i + j] = blank ? 0.f : e[j];
-      }
+          for (int j = 0; j < 4; ++j) z[i + j] = blank ? 0.f : e[j];
+        }
+      };
+      if (__any(st.m != st.other_m)) each(std::true_type());
+      else each(std::false_type());
       for (int j = 0; j < n && !blank; ++j)
         if (entry(j, id, v)) z[id] -= (float)(exp2_or_0(v - ref - norm) * p.inv_t) * w;
     }
@@ -659,7 +803,8 @@ void split_grad(DistillParams& p, int dtype) {
   split_rows(p, step, n);
 }
 
-int64_t parts_bytes(const DistillParams& p) { return p.splits == 1 ? 0 : p.rows * p.splits * (int64_t)sizeof(float4); }
+// (whole 16 bytes: the statistics lie behind them)
+int64_t parts_bytes(const DistillParams& p) { return p.splits == 1 ? 0 : (p.rows * p.splits * (int64_t)sizeof(float2) + 15) / 16 * 16; }
 
 template <class T, int NT, int U, int WINDOW>
 lt_status launch_block(const DistillParams& p, Pass pass, void* stream, const char* what) {
@@ -715,7 +860,8 @@ lt_status launch_pass(const DistillParams& p, Pass pass, void* stream, const cha
   if (p.z.vocab <= 16384) return launch_block<T, 256, 4, 16384>(p, pass, stream, what);
   const lt_status st = launch_block<T, 512, 4, 1 << 18>(p, pass, stream, what);
   if (st != LT_OK || pass != SUMS || p.splits == 1) return st;
-  return launch(lt_distill_join<T>, p.rows, 256, p, stream, what);
+  return p.t.top_lse ? launch(lt_distill_join<T, true>, p.rows, 256, p, stream, what)
+                     : launch(lt_distill_join<T, false>, p.rows, 256, p, stream, what);
 }
 
 lt_status launch_pass(const DistillParams& p, int dtype, Pass pass, void* stream, const char* what) {
@@ -786,7 +932,7 @@ lt_status lt_distill_forward(const lt_rows* z, const lt_teacher* t, double tempe
   DistillParams p = distill_params(z, t, temperature);
   if (!workspace_ok(p, workspace, workspace_bytes))
     BAD("workspace: %lld bytes, 16 B aligned, are needed", (long long)lt_distill_workspace(z, t->entries));
-  p.part = (float4*)workspace;
+  p.part = (float2*)workspace;
   p.loss = loss;
   p.stats = stats;
   ON_DEVICE(z->device);
@@ -821,7 +967,7 @@ lt_status lt_distill_fused(const lt_rows* z, const lt_teacher* t, double tempera
   DistillParams p = distill_params(z, t, temperature);
   if (!workspace_ok(p, workspace, workspace_bytes))
     BAD("workspace: %lld bytes, 16 B aligned, are needed", (long long)lt_distill_workspace(z, t->entries));
-  p.part = (float4*)workspace;
+  p.part = (float2*)workspace;
   p.loss = loss;
   p.stats = p.splits > 1 ? (float*)((char*)workspace + parts_bytes(p)) : nullptr;
   p.scale = (float)scale;

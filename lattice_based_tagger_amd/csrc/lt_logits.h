@@ -25,16 +25,19 @@ struct Rows {
 };
 
 struct F32 {
+  static constexpr float lowest = -3.4028234663852886e38f;
   using raw = float;
   static __device__ __forceinline__ float get(raw v) { return v; }
   static __device__ __forceinline__ raw put(float v) { return v; }
 };
 struct F16 {
+  static constexpr float lowest = -65504.f;
   using raw = uint16_t;
   static __device__ __forceinline__ float get(raw v) { return (float)__builtin_bit_cast(_Float16, v); }
   static __device__ __forceinline__ raw put(float v) { return __builtin_bit_cast(raw, (_Float16)v); }
 };
 struct BF16 {
+  static constexpr float lowest = -3.3895313892515355e38f;
   using raw = uint16_t;
   static __device__ __forceinline__ float get(raw v) { return __builtin_bit_cast(float, (uint32_t)v << 16); }
   static __device__ __forceinline__ raw put(float v) { return __builtin_bit_cast(raw, (__bf16)v); }
@@ -89,6 +92,15 @@ struct Vec {
         if constexpr (E == 4) x[at + i] = __builtin_bit_cast(float, b.w[i]);
         else x[at + i] = (typename T::raw)(b.w[i >> 1] >> (i & 1) * 16);
       }
+  }
+  // -inf for the logits whose bits are set.
+  __device__ __forceinline__ void mask(uint32_t bits) {
+    auto all = [&](int i) { return (uint32_t)((int)(bits << (31 - i)) >> 31); };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t m = E == 4 ? all(i) : (all(2 * i) & 0xffffu) | (all(2 * i + 1) & 0xffff0000u);
+      b.w[i] = (b.w[i] & ~m) | (twice(T::put(-INFINITY)) & m);
+    }
   }
   // What is computed from the logits ahead of this is not kept for later.
   __device__ __forceinline__ void keep() { asm volatile("" : "+v"(b.w[0]), "+v"(b.w[1]), "+v"(b.w[2]), "+v"(b.w[3])); }
@@ -215,6 +227,7 @@ struct One {
   __device__ __forceinline__ void load(const typename T::raw* x, int at, int, int end, typename T::raw) {
     f = at < end ? T::get(x[at]) : -INFINITY;
   }
+  __device__ __forceinline__ void mask(uint32_t bits) { f = bits & 1 ? -INFINITY : f; }
   __device__ __forceinline__ float get(int) const { return f; }
   __device__ __forceinline__ void keep() {}
 };

@@ -326,7 +326,8 @@ def distill_loss(logits, top_ids, top_values, top_lse=None, temperature=1.0):
     * with ``top_lse`` ``[...]`` (the teacher's log-sum-exp at the same
       temperature): p = exp(top_values / temperature - top_lse), and all else
       of the vocabulary as one more place with what is left of 1 (left out
-      where the student's logits leave it nothing).
+      where the student's logits mask all of it: -inf, or the type's lowest
+      value, more than 745 temperatures below the row's largest).
 
     A row without entries -- padding: every id -1 -- has loss 0 and gradient 0,
     whatever its logits are.
