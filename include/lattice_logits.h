@@ -83,7 +83,8 @@ lt_status lt_top_logits(const lt_rows* x, int32_t k, double temperature, void* v
  *                    1/temperature * (P - p_rest / q_rest) q_v         else
  *     with P = sum p_j + p_rest
  * A row without entries has loss 0 and gradient 0, whatever its logits, top and
- * top_lse hold.  An id that a row repeats counts once for each time.  The teacher is a constant.
+ * top_lse hold.  One with entries whose logits hold a NaN or +inf, or are -inf
+ * throughout, has loss NaN and gradient NaN, all of it.  An id that a row repeats counts once for each time.  The teacher is a constant.
  * 1 <= K <= LT_MAX_TOP. */
 typedef struct {
   const void* ids;        /* [rows][entries] int32 or int64 */

@@ -278,12 +278,14 @@ __device__ __forceinline__ void put_stats(float* stats, int64_t r, Factors f) {
 //   q_v = q_rest r_v,  r_v = exp2((z - other_m) c) / others.s
 // the gradient (P - p_rest / q_rest) q_v is (P q_rest - p_rest) r_v, which neither
 // under- nor overflows.  log_s: the row's sum's, to the base 2 as all.
+// A sum that is not above 0 -- logits of NaN or +inf, or -inf throughout -- has no
+// softmax: all of the gradient is NaN, and the loss.
 constexpr double GONE = 745;               // exp(-745) is the least in 64 bits
 template <class T, bool TAIL>
 __device__ __forceinline__ Factors factors(Sums all, Sums others, double sum, double& rest, double inv_t, double log_s,
                                            double& log_rest) {
   if (!TAIL) {
-    const float entry = all.s > 0 ? (float)(sum * inv_t) * (1 / all.s) : 0.f;
+    const float entry = all.s > 0 ? (float)(sum * inv_t) * (1 / all.s) : NAN;
     return {all.m, entry, all.m, entry};
   }
   double t = 0;
@@ -295,7 +297,7 @@ __device__ __forceinline__ Factors factors(Sums all, Sums others, double sum, do
   if (!(others.s > 0) || (others.m <= T::lowest && -t > GONE * LOG2E)) rest = 0;
   log_rest = t + log2_(others.s) - log_s;
   const double whole = sum + rest;
-  if (!(all.s > 0)) return {others.m, 0.f, all.m, 0.f};
+  if (!(all.s > 0)) return {others.m, NAN, all.m, NAN};
   const float inv = 1 / all.s, entry = (float)(whole * inv_t) * inv;
   if (!(rest > 0)) return {others.m, entry * far, all.m, entry};
   const float qrest = others.s * inv * far;
@@ -315,7 +317,7 @@ __device__ __forceinline__ Factors finish_row(const Entries<NT, N>& t, const flo
   l = block_reduce<NT, Sum>(l, sh);
   const Factors f = factors<T, TAIL>(all, others, t.sum, rest, inv_t, logs, log_rest);
   if (TAIL && rest > 0) l += rest * (log2_((float)rest) - log_rest);
-  loss = (float)(l * LN2);
+  loss = all.s > 0 ? (float)(l * LN2) : t.blank() ? 0.f : NAN;
   return f;
 }
 
@@ -731,7 +733,7 @@ __global__ __launch_bounds__(64) void lt_distill_few(DistillParams p) {
       }
     if (rest > 0) loss += rest * (log2_((float)rest) - log_rest);
     if (lane < rows) {
-      p.loss[r] = (float)(loss * LN2);
+      p.loss[r] = all.s > 0 ? (float)(loss * LN2) : blank ? 0.f : NAN;
       if (p.stats) put_stats(p.stats, r, st);
     }
   }

@@ -330,7 +330,8 @@ def distill_loss(logits, top_ids, top_values, top_lse=None, temperature=1.0):
       value, more than 745 temperatures below the row's largest).
 
     A row without entries -- padding: every id -1 -- has loss 0 and gradient 0,
-    whatever its logits are.
+    whatever its logits are.  One with entries whose logits hold a NaN or +inf,
+    or are -inf throughout, has loss NaN and a gradient of NaN.
     No factor temperature^2 is applied, and no reduction.  The teacher is a
     constant: no gradient flows to it, and there is no second derivative."""
     _logits(logits, 'logits')
