@@ -202,6 +202,7 @@ template <class T, int NT, int U, int C, int CL>
 __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
   using raw = typename T::raw;
   constexpr int E = Vec<T>::E, W = NT / 64, STEP = NT * U * E, GROUPS = NT == 64 ? 4 : 1;
+  numbers_win();
   __shared__ __attribute__((aligned(16))) TopShared<NT, C, CL> shared[GROUPS];
   TopShared<NT, C, CL>& sh = shared[group_of<NT>()];
   uint64_t* const buf = sh.buf;
@@ -460,6 +461,7 @@ template <class T, int K>
 __global__ __launch_bounds__(64) void lt_top_few(TopParams p) {
   using raw = typename T::raw;
   extern __shared__ float few[];           // [64][few_pitch(vocab)], then [64][k] results
+  numbers_win();
   const int lane = threadIdx.x, vocab = p.x.vocab, pitch = few_pitch(vocab);
   const int64_t r0 = (p.block0 + blockIdx.x) * 64;
   const int rows = (int)min((int64_t)64, p.rows - r0);
@@ -535,6 +537,7 @@ template <class T, class V, int U>
 __global__ __launch_bounds__(256) void lt_top_wave(TopParams p) {
   using raw = typename T::raw;
   constexpr int E = V::E, C = 2 * MAXK;
+  numbers_win();
   __shared__ __attribute__((aligned(16))) uint64_t keys[4][C];
   uint64_t* const buf = keys[group_of<64>()];
   const int lane = threadIdx.x & 63, vocab = p.x.vocab, k = p.k;

@@ -135,6 +135,7 @@ __device__ __forceinline__ float2 sum_part(const typename T::raw* row, int lead,
   sum_thread<T, U, false>(row, lead, c0, v0, v1, c, m, s);
   float top = block_reduce<NT, Max>(m, shf), sum = block_reduce<NT, Sum>(s * exp2_((m - top) * c), shf);
   if (sum != sum) {                        // (for the block as a whole)
+    numbers_win();
     sum_thread<T, U, true>(row, lead, c0, v0, v1, c, m, s);
     top = block_reduce<NT, Max>(m, shf);
     sum = block_reduce<NT, Sum>(s * exp2_((m - top) * c), shf);
