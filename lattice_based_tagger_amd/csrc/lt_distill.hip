@@ -40,7 +40,7 @@ __device__ __forceinline__ float weight_of(const DistillParams& p, int64_t r) {
 // a bit for each logit of a window that says whether it is one.
 template <int NT, int WINDOW>
 struct DistillShared {
-  int id[MAXK];
+  alignas(16) int id[MAXK];                // (read four at a time)
   float mass[MAXK];
   uint32_t bits[WINDOW / 32];
   double sh[NT / 64];
@@ -396,7 +396,7 @@ __device__ __forceinline__ void grad_row(const typename T::raw* row, typename T:
 
 // A block's row, and the part of it that is the block's.
 #define BLOCK_HEAD                                                                                        \
-  __shared__ __attribute__((aligned(16))) DistillShared<NT, WINDOW> sh;                                   \
+  __shared__ DistillShared<NT, WINDOW> sh;                                                                \
   const int64_t blk = p.block0 + blockIdx.x, r = p.splits == 1 ? blk : blk / p.splits;                    \
   const typename T::raw* z = (const typename T::raw*)p.z.data + p.z.at(r);                                \
   const int lead = lead_of<T>(z), c0 = p.splits == 1 ? 0 : (int)(blk % p.splits) * p.chunk;               \
@@ -449,7 +449,7 @@ __global__ __launch_bounds__(NT) void lt_distill_sums(DistillParams p) {
 template <class T, bool TAIL>
 __global__ __launch_bounds__(256) void lt_distill_join(DistillParams p) {
   constexpr int NT = 256;
-  __shared__ __attribute__((aligned(16))) DistillShared<NT, 32> sh;
+  __shared__ DistillShared<NT, 32> sh;
   const int64_t r = p.block0 + blockIdx.x;
   Entries<NT> t;
   load_entries(p.t, r, p.z.vocab, p.inv_t, t, sh.sh);

@@ -1,6 +1,7 @@
 // lt_top.hip -- the k best logits of a row with its log-sum-exp
 // (include/lattice_logits.h lt_top_logits).
 #include <dlfcn.h>
+#include <stddef.h>
 
 #include "lt_logits.h"
 
@@ -117,7 +118,7 @@ __device__ __forceinline__ void sort_keys(uint64_t* buf, int n, int k) {
 // Keeps the k largest of the keys buf[0 .. n), k < n <= C, in any order, and
 // returns a key that they reach and the others do not: the k-th is found eight
 // bits at a time, from the leading bit in which the keys differ, by counting the
-// keys of every value of the eight.  hist: 256 counts,
+// keys of every value of the eight.  hist: 256 counts, 16 B aligned,
 // cnt: one more, sh: NT / 64 keys.
 template <int NT, int C>
 __device__ __forceinline__ uint64_t cut_keys(uint64_t* buf, int n, int k, int* hist, int* cnt, uint64_t* sh) {
@@ -190,7 +191,7 @@ template <int NT, int C, int CL>
 struct TopShared {
   uint64_t buf[C];
   uint64_t sh64[NT / 64];
-  int hist[256];
+  alignas(16) int hist[256];               // (read four at a time)
   uint32_t list[CL];
   float shf[NT / 64];
   uint32_t th[NT / 64];
@@ -203,8 +204,10 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
   using raw = typename T::raw;
   constexpr int E = Vec<T>::E, W = NT / 64, STEP = NT * U * E, GROUPS = NT == 64 ? 4 : 1;
   numbers_win();
-  __shared__ __attribute__((aligned(16))) TopShared<NT, C, CL> shared[GROUPS];
-  TopShared<NT, C, CL>& sh = shared[group_of<NT>()];
+  using Shared = TopShared<NT, C, CL>;
+  static_assert(offsetof(Shared, hist) % 16 == 0 && sizeof(Shared) % 16 == 0, "each wave's counts at 16 B");
+  __shared__ Shared shared[GROUPS];
+  Shared& sh = shared[group_of<NT>()];
   uint64_t* const buf = sh.buf;
   const int tid = thread_of<NT>(), lane = tid & 63, wave = tid >> 6;
   const int64_t blk = (p.block0 + blockIdx.x) * GROUPS + group_of<NT>();
@@ -427,7 +430,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void lt_top_k(TopParams p) {
 template <class T>
 __global__ __launch_bounds__(256) void lt_top_join(TopParams p) {
   constexpr int NT = 256, C = JOIN;
-  __shared__ __attribute__((aligned(16))) TopShared<NT, C, 1> sh;
+  __shared__ TopShared<NT, C, 1> sh;
   const int tid = threadIdx.x;
   const int64_t r = p.block0 + blockIdx.x;
   const int n = p.splits * p.k;
