@@ -3,7 +3,7 @@
 //
 // A drafted token is accepted by comparing two probabilities with a random
 // number: from sums in 32 bits, unless the two are within these sums' error
-// (some 2e-5) of each other; then the rows are summed again in 64 bits.  A token
+// (some 3e-5) of each other; then the rows are summed again in 64 bits.  A token
 // is drawn where a running sum over the vocabulary crosses a
 // line, so a relative error e of the sums moves it with a probability of about
 // e times the number of tokens that the line may fall beside, 131072 e: the
@@ -603,10 +603,17 @@ void plan(VerifyParams& p, int dtype) {
   int64_t n = p.rounds ? chunks(numbers, step, p.batch * kinds, 4096) : chunks(numbers, step, p.batch * kinds * (p.drafts + 1), 8192);
   p.chunk = (int32_t)((numbers + n * step - 1) / (n * step) * step);
   p.splits = (int32_t)((numbers + p.chunk - 1) / p.chunk);
-  // of each sum: a thread's additions one after another (16 of a step, the
-  // steps), 30 to join them, 3 roundings of an exponent of 12 and one of its
-  // power of 2; twice that for two
-  p.margin = 2 * (16 + p.chunk / step + 30 + p.splits + 3 * 12 + 2) * 0x1p-24;
+  // A bound of a sum's relative error, in roundings of 2^-24: a thread's additions
+  // one after another (18 of a step, the steps), 9 to join the block's; its powers
+  // of 2 (each within 2) of the term, once where the reference moves and to join,
+  // and the two products of these: 8.  An exponent's three roundings (difference,
+  // constant, product) are each up to its size times ln 2: the term's and those that
+  // carry it to the block's reference add up to at most its depth below the row's
+  // largest logit, of a mean of log2(vocab) at most, and 64, as a reference may lag
+  // by 32.  (The chunks are joined in 64 bits.)  Twice that for the two that are
+  // compared, and a thousandth for the products of errors.
+  const double sum = 18 + p.chunk / step + 9 + 8 + 3 * LN2 * (64 + log2((double)p.target.vocab));
+  p.margin = 2.002 * sum * 0x1p-24;
   n = chunks(numbers, vectors, p.batch, 1024);
   p.weigh_chunk = (int32_t)((numbers + n * vectors - 1) / (n * vectors) * vectors);
   p.weigh_splits = (int32_t)((numbers + p.weigh_chunk - 1) / p.weigh_chunk);

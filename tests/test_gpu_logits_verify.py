@@ -110,3 +110,38 @@ def test_a_row_of_nan(certain):
     got = check(dict(target=target, draft_ids=ids, accept_u=torch.full((4, 1), 0.001).cuda(),
                      sample_u=torch.rand(4, generator=torch.Generator().manual_seed(2)).cuda(), draft=draft))
     assert got.tokens[0].tolist() == [-1, -1] and got.tokens[1, 1] == -1
+
+
+@pytest.mark.parametrize('certain', [False, True])
+@pytest.mark.parametrize('vocab, seed', [(9000, 1), (40000, 2), (131072, 3)])
+def test_close_to_the_line(certain, vocab, seed):
+    """Random numbers within a few steps of 32 bits of p / q on either side, of rows
+    whose every thread begins 2^31 below its largest: decided as by 64 bits."""
+    g = torch.Generator().manual_seed(seed)
+    batch, temperature = 64, 0.7317
+    def rows():
+        x = torch.rand(batch, 2, vocab, generator=g) * 0.3
+        # a block's first steps of every chunk it may begin at
+        x[:, :, (torch.arange(vocab) // 4096) % 2 == 0] -= 31 * math.log(2) * temperature
+        return x
+    target = rows()
+    ids = torch.randint(4096, 8192, (batch, 1), generator=g)
+    target[torch.arange(batch), 0, ids[:, 0]] += 11.0
+    draft = None
+    p = torch.softmax(target[:, 0].double() / temperature, -1).gather(1, ids)[:, 0]
+    q = torch.ones_like(p)
+    if not certain:
+        draft = rows()[:, :1]
+        draft[torch.arange(batch), 0, ids[:, 0]] += 11.5
+        q = torch.softmax(draft[:, 0].double() / temperature, -1).gather(1, ids)[:, 0]
+    u = (p / q).clamp(max=1 - 2.0 ** -23).float()
+    for step in range(-3, 4):
+        near = u.clone()
+        for _ in range(abs(step)):
+            near = torch.nextafter(near, torch.tensor(2.0 if step > 0 else -1.0)).clamp(max=1 - 2.0 ** -24)
+        a = dict(target=target.cuda(), draft_ids=ids.cuda(), accept_u=near[:, None].cuda(),
+                 sample_u=torch.rand(batch, generator=g).cuda(), draft=None if certain else draft.cuda())
+        got = logits.verify_draft(temperature=temperature, **a)
+        # (64-bit sums decide: p of the plain form is within 1e-12 of the kernel's)
+        clear = (near.double() * q - p).abs() > 1e-10 * p
+        assert torch.equal(got.accepted.cpu()[clear], (near.double() * q < p)[clear].long())
