@@ -145,3 +145,44 @@ def test_close_to_the_line(certain, vocab, seed):
         # (64-bit sums decide: p of the plain form is within 1e-12 of the kernel's)
         clear = (near.double() * q - p).abs() > 1e-10 * p
         assert torch.equal(got.accepted.cpu()[clear], (near.double() * q < p)[clear].long())
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('certain', [False, True])
+@pytest.mark.parametrize('drafts', [255, 256])
+def test_the_most_drafts(dtype, certain, drafts):
+    """As many as a call takes, a place more than a block has threads: none, some and
+    all of them accepted, with and without lengths."""
+    g = torch.Generator().manual_seed(drafts)
+    batch, vocab = 6, 70
+    target = torch.randn(batch, drafts + 1, vocab, generator=g).to(dtype).cuda()
+    ids = target[:, :drafts].float().argmax(-1)
+    target.scatter_add_(2, ids[..., None], torch.full(ids[..., None].shape, 12, dtype=dtype, device='cuda'))
+    draft = None if certain else target[:, :drafts].clone()
+    u = torch.full((batch, drafts), 0.5)
+    if not certain:
+        draft[1, drafts - 1, ids[1, drafts - 1]] += 30     # (surer than the target: still accepted, p is near 1)
+    ids[2, 0] = vocab                                      # none
+    ids[3, drafts - 1] = vocab                             # all but the last
+    ids[4, drafts // 2] = -1
+    a = dict(target=target, draft_ids=ids, accept_u=u.cuda(), sample_u=torch.rand(batch, generator=g).cuda(), draft=draft)
+    got = check(a)
+    assert got.accepted.tolist() == [drafts, drafts, 0, drafts - 1, drafts // 2, drafts]
+    n = torch.tensor([drafts, drafts - 1, 5, drafts, 0, 200], dtype=torch.int32)
+    tokens, accepted = plain.verify(target, ids, u, a['sample_u'], draft, n)
+    got = logits.verify_draft(lengths=n.cuda(), **a)
+    assert torch.equal(got.accepted.cpu(), accepted) and torch.equal(got.tokens.cpu(), tokens)
+
+
+def test_lengths_beyond_their_ends():
+    """Lengths are taken as within [0, drafts]."""
+    g = torch.Generator().manual_seed(9)
+    target = torch.randn(5, 4, 100, generator=g).cuda()
+    ids = target[:, :3].argmax(-1)
+    target.scatter_add_(2, ids[..., None], torch.full((5, 3, 1), 9.0, device='cuda'))
+    u, s = torch.full((5, 3), 0.01).cuda(), torch.rand(5, generator=g).cuda()
+    n = torch.tensor([-1, -2 ** 31, 4, 2 ** 31 - 1, 2], dtype=torch.int32)
+    got = logits.verify_draft(target, ids, u, s, lengths=n.cuda())
+    tokens, accepted = plain.verify(target, ids, u, s, None, n.clamp(0, 3))
+    assert torch.equal(got.accepted.cpu(), accepted) and torch.equal(got.tokens.cpu(), tokens)
+    assert got.accepted.tolist() == [0, 0, 3, 3, 2]
