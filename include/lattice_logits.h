@@ -126,8 +126,8 @@ lt_status lt_distill_fused(const lt_rows* z, const lt_teacher* t, double tempera
  *           else the last with w_v > 0; -1 if p_a is empty (a row of -inf)
  *   tokens[b] = x_0 .. x_{a-1}, token, -1 ...  [drafts + 1];  accepted[b] = a
  * Logits are finite or -inf (a NaN counts as -inf); a probability below 2^-1000 of
- * its row's largest counts as 0.  Rows past lengths[b] are
- * not read; lengths are taken as within [0, drafts].
+ * its row's largest counts as 0.  Rows past lengths[b] are not read; lengths are
+ * taken as within [0, drafts].
  * Sums that decide the token are held in 64 bits. */
 typedef struct {
   const lt_rows* target;

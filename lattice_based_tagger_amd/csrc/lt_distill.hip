@@ -214,6 +214,25 @@ __device__ __forceinline__ Sums sum_row(const typename T::raw* row, int lead, in
   return o;
 }
 
+// 2^t, t <= 0.
+__device__ __forceinline__ float exp2_of(double t) {
+  if (t < -160) return 0.f;
+  const double n = rint(t);
+  return ldexpf(exp2_((float)(t - n)), (int)n);
+}
+
+// How far the others' reference lies below the row's, to the base 2, and 2 to that
+// (from 64 bits: an error here is all of the others').
+struct Apart {
+  double t;
+  float far;
+};
+__device__ __forceinline__ Apart apart(float other_m, float m, double inv_t) {
+  if (other_m == m) return {0, 1.f};
+  const double t = ((double)other_m - m) * (inv_t * LOG2E);
+  return {t, exp2_of(t)};
+}
+
 // Two at once: a thread's sum and, of the entries beside it, the row's.
 struct Two {
   float a, b;
@@ -237,7 +256,7 @@ __device__ __forceinline__ Sums join(Sums o, float c, double* sh) {
 // (`first` tells) however often the row repeats it, of the row.
 template <int NT>
 __device__ __forceinline__ Sums join(Sums o, const float (&zi)[Entries<NT>::N], const bool (&first)[Entries<NT>::N], float c,
-                                     double* sh, Sums& all) {
+                                     double inv_t, double* sh, Sums& all, Apart& ap) {
   float in = -INFINITY;
 #pragma unroll
   for (int i = 0; i < Entries<NT>::N; ++i) in = first[i] ? max2(in, zi[i]) : in;
@@ -246,15 +265,9 @@ __device__ __forceinline__ Sums join(Sums o, const float (&zi)[Entries<NT>::N], 
 #pragma unroll
   for (int i = 0; i < Entries<NT>::N; ++i) in += first[i] ? exp2_((zi[i] - m.b) * c) : 0.f;
   const Two s = block_reduce<NT, Sum2>(Two{o.s * exp2_((o.m - m.a) * c), in}, (Two*)sh);
-  all = {m.b, s.b + s.a * exp2_((m.a - m.b) * c)};
+  ap = apart(m.a, m.b, inv_t);
+  all = {m.b, s.b + s.a * ap.far};
   return {m.a, s.a};
-}
-
-// 2^t, t <= 0.
-__device__ __forceinline__ float exp2_of(double t) {
-  if (t < -160) return 0.f;
-  const double n = rint(t);
-  return ldexpf(exp2_((float)(t - n)), (int)n);
 }
 
 // What the gradient of a row is made of: an entry's is exp2((z - m) entry) less
@@ -274,40 +287,32 @@ __device__ __forceinline__ void put_stats(float* stats, int64_t r, Factors f) {
 // the row's).  p_rest becomes 0 where these have nothing: all of them are -inf, or
 // all the type's lowest value -- a mask -- and so far below the largest logit that
 // 64 bits hold nothing of them.  Else q_rest may lie as far below as logits can:
-// log_rest is its logarithm, and with
+// log_rest is its logarithm to the base 2, and with
 //   q_v = q_rest r_v,  r_v = exp2((z - other_m) c) / others.s
 // the gradient (P - p_rest / q_rest) q_v is (P q_rest - p_rest) r_v, which neither
-// under- nor overflows.  log_s: the row's sum's, to the base 2 as all.
+// under- nor overflows.
 // A sum that is not above 0 -- logits of NaN or +inf, or -inf throughout -- has no
 // softmax: all of the gradient is NaN, and the loss.
 constexpr double GONE = 745;               // exp(-745) is the least in 64 bits
 template <class T, bool TAIL>
-__device__ __forceinline__ Factors factors(Sums all, Sums others, double sum, double& rest, double inv_t, double log_s,
-                                           double& log_rest) {
+__device__ __forceinline__ Factors factors(Sums all, Sums others, Apart ap, double sum, double& rest, double inv_t, double& log_rest) {
   if (!TAIL) {
     const float entry = all.s > 0 ? (float)(sum * inv_t) * (1 / all.s) : NAN;
     return {all.m, entry, all.m, entry};
   }
-  double t = 0;
-  float far = 1;
-  if (others.m != all.m) {
-    t = ((double)others.m - all.m) * (inv_t * LOG2E);
-    far = exp2_of(t);
-  }
-  if (!(others.s > 0) || (others.m <= T::lowest && -t > GONE * LOG2E)) rest = 0;
-  log_rest = t + log2_(others.s) - log_s;
+  if (!(others.s > 0) || (others.m <= T::lowest && -ap.t > GONE * LOG2E)) rest = 0;
   const double whole = sum + rest;
   if (!(all.s > 0)) return {others.m, NAN, all.m, NAN};
-  const float inv = 1 / all.s, entry = (float)(whole * inv_t) * inv;
-  if (!(rest > 0)) return {others.m, entry * far, all.m, entry};
-  const float qrest = others.s * inv * far;
-  return {others.m, (float)((whole * qrest - rest) * inv_t) / others.s, all.m, entry};
+  const float inv = 1 / all.s, entry = (float)(whole * inv_t) * inv, share = others.s * inv;
+  log_rest = ap.t + log2_(share);             // (one logarithm: each is off by 2^-23)
+  if (!(rest > 0)) return {others.m, entry * ap.far, all.m, entry};
+  return {others.m, (float)((whole * (share * ap.far) - rest) * inv_t) / others.s, all.m, entry};
 }
 
 // Loss and the gradient's factors of a row from its sums (zi: the logits of the
 // entries).
 template <class T, bool TAIL, int NT, int N>
-__device__ __forceinline__ Factors finish_row(const Entries<NT, N>& t, const float (&zi)[N], Sums all, Sums others, double inv_t,
+__device__ __forceinline__ Factors finish_row(const Entries<NT, N>& t, const float (&zi)[N], Sums all, Sums others, Apart ap, double inv_t,
                                               double* sh, float& loss) {
   const double logs = log2_(all.s), c = inv_t * LOG2E;
   double l = 0, rest = t.rest, log_rest;
@@ -315,7 +320,7 @@ __device__ __forceinline__ Factors finish_row(const Entries<NT, N>& t, const flo
   for (int i = 0; i < N; ++i)
     if (t.id[i] >= 0 && t.p[i] != 0) l += t.p[i] * (t.logp[i] - ((double)zi[i] - all.m) * c + logs);
   l = block_reduce<NT, Sum>(l, sh);
-  const Factors f = factors<T, TAIL>(all, others, t.sum, rest, inv_t, logs, log_rest);
+  const Factors f = factors<T, TAIL>(all, others, ap, t.sum, rest, inv_t, log_rest);
   if (TAIL && rest > 0) l += rest * (log2_((float)rest) - log_rest);
   loss = all.s > 0 ? (float)(l * LN2) : t.blank() ? 0.f : NAN;
   return f;
@@ -411,6 +416,7 @@ __device__ __forceinline__ void grad_row(const typename T::raw* row, typename T:
   bool first[Entries<NT>::N] = {};                                                                        \
   load_zi<T>(t, z, zi);                                                                                   \
   Sums o, all;                                                                                            \
+  Apart ap{0, 1.f};                                                                                       \
   if (threadIdx.x == 0) sh.again = 0;                                                                     \
   if (!t.blank()) {                                                                                       \
     o = sum_row<T, NT, U, WINDOW, TAIL>(z, lead, c0, v0, v1, p.c, t, sh, first);                          \
@@ -420,7 +426,7 @@ __device__ __forceinline__ void grad_row(const typename T::raw* row, typename T:
         __syncthreads();                                                                                  \
         only_first<NT>(t, sh.id, p.t.entries, first);                                                     \
       }                                                                                                   \
-      o = join<NT>(o, zi, first, p.c, sh.sh, all);                                                        \
+      o = join<NT>(o, zi, first, p.c, p.inv_t, sh.sh, all, ap);                                           \
     } else {                                                                                              \
       all = o = join<NT>(o, p.c, sh.sh);                                                                  \
     }                                                                                                     \
@@ -438,7 +444,7 @@ __global__ __launch_bounds__(NT) void lt_distill_sums(DistillParams p) {
     return;
   }
   float loss;
-  const Factors st = finish_row<T, TAIL>(t, zi, all, o, p.inv_t, sh.sh, loss);
+  const Factors st = finish_row<T, TAIL>(t, zi, all, o, ap, p.inv_t, sh.sh, loss);
   if (threadIdx.x == 0) {
     p.loss[r] = loss;
     put_stats(p.stats, r, st);
@@ -464,16 +470,17 @@ __global__ __launch_bounds__(256) void lt_distill_join(DistillParams p) {
   float zi[Entries<NT>::N];
   load_zi<T>(t, (const typename T::raw*)p.z.data + p.z.at(r), zi);
   Sums all;
+  Apart ap{0, 1.f};
   if (TAIL) {
     bool first[1] = {t.id[0] >= 0};
     sh.id[threadIdx.x] = t.id[0];
     if (__syncthreads_or(again)) only_first<NT>(t, sh.id, p.t.entries, first);
-    o = join<NT>(o, zi, first, p.c, sh.sh, all);
+    o = join<NT>(o, zi, first, p.c, p.inv_t, sh.sh, all, ap);
   } else {
     all = o = join<NT>(o, p.c, sh.sh);
   }
   float loss;
-  const Factors st = finish_row<T, TAIL>(t, zi, all, o, p.inv_t, sh.sh, loss);
+  const Factors st = finish_row<T, TAIL>(t, zi, all, o, ap, p.inv_t, sh.sh, loss);
   if (threadIdx.x == 0) {
     p.loss[r] = loss;
     put_stats(p.stats, r, st);
@@ -497,7 +504,7 @@ __global__ __launch_bounds__(NT, 8) void lt_distill_both(DistillParams p) {
   BLOCK_HEAD;
   PASS;
   float loss;
-  const Factors st = finish_row<T, TAIL>(t, zi, all, o, p.inv_t, sh.sh, loss);
+  const Factors st = finish_row<T, TAIL>(t, zi, all, o, ap, p.inv_t, sh.sh, loss);
   if (threadIdx.x == 0) p.loss[r] = loss;
   grad_row<T, NT, U, WINDOW, true>(z, (typename T::raw*)p.grad.data + p.grad.at(r), lead, c0, v0, v1, p.c, st,
                                    weight_of(p, r), p.inv_t, t, sh, p.t.entries, p.past);
@@ -550,7 +557,12 @@ __global__ __launch_bounds__(256, (TAIL && N > 1 && U == 4 && V::E == 8 ? 6 : 1)
   sync<64>();
   Factors st{0.f, 0.f, 0.f, 0.f};
   if (LOSS) {
-    float m = -INFINITY;
+    float m = -INFINITY, in = -INFINITY;
+    if (TAIL) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) in = first[i] ? max2(in, zi[i]) : in;
+      in = wave_reduce<Max>(in, -INFINITY);
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (TAIL) {
@@ -560,15 +572,8 @@ __global__ __launch_bounds__(256, (TAIL && N > 1 && U == 4 && V::E == 8 ? 6 : 1)
       m = max2(m, max_of(v[u]));
       v[u].keep();
     }
-    st.m = st.other_m = max2(wave_reduce<Max>(m, -INFINITY), LOWEST);
-    if (TAIL) {
-      // (the entries' sum too beside the others' largest, unless that lies so far
-      // below that the roundings of their exponents would count)
-      float in = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < N; ++i) in = first[i] ? max2(in, zi[i]) : in;
-      if (__any((in - st.m) * p.c > 16.f)) st.m = max2(st.m, wave_reduce<Max>(in, -INFINITY));
-    }
+    st.other_m = max2(wave_reduce<Max>(m, -INFINITY), LOWEST);
+    st.m = TAIL ? max2(st.other_m, in) : st.other_m;
   } else {
     st = of_stats(p.stats, r);
   }
@@ -582,14 +587,16 @@ __global__ __launch_bounds__(256, (TAIL && N > 1 && U == 4 && V::E == 8 ? 6 : 1)
     }
   if (LOSS) {
     Sums rest{st.other_m, wave_reduce<Sum>(out[0] + out[1], 0.f)}, all = rest;
+    Apart ap{0, 1.f};
     if (TAIL) {
       float in = 0.f;
 #pragma unroll
       for (int i = 0; i < N; ++i) in += first[i] ? exp2_((zi[i] - st.m) * p.c) : 0.f;
-      all = {st.m, wave_reduce<Sum>(in, 0.f) + rest.s * exp2_((rest.m - st.m) * p.c)};
+      ap = apart(rest.m, st.m, p.inv_t);
+      all = {st.m, wave_reduce<Sum>(in, 0.f) + rest.s * ap.far};
     }
     float loss;
-    st = finish_row<T, TAIL>(t, zi, all, rest, p.inv_t, nullptr, loss);
+    st = finish_row<T, TAIL>(t, zi, all, rest, ap, p.inv_t, nullptr, loss);
     if (lane == 0) {
       p.loss[r] = blank ? 0.f : loss;
       if (!GRAD) put_stats(p.stats, r, st);
@@ -721,11 +728,11 @@ __global__ __launch_bounds__(64) void lt_distill_few(DistillParams p) {
       others.s += (f[0] + f[1]) + (f[2] + f[3]);
     }
   }
-  const double logs = log2_(all.s);
   double log_rest;
-  const Factors st = factors<T, true>(all, others, sum, rest, p.inv_t, logs, log_rest);
+  const Factors st = factors<T, true>(all, others, apart(others.m, all.m, p.inv_t), sum, rest, p.inv_t, log_rest);
   if (LOSS) {
     double loss = 0;
+    const double logs = log2_(all.s);
     for (int j = 0; j < n; ++j)
       if (entry(j, id, v)) {
         const double logp = v - ref - norm, pj = exp2_or_0(logp);

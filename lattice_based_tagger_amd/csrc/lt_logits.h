@@ -286,6 +286,7 @@ __device__ __forceinline__ int64_t any_id(const void* p, int64_t i, int bytes) {
 struct Max {
   template <class T>
   static __device__ __forceinline__ T of(T a, T b) { return a > b ? a : b; }
+  static __device__ __forceinline__ float of(float a, float b) { return max2(a, b); }
 };
 struct Sum {
   template <class T>
