@@ -433,7 +433,7 @@ __device__ __forceinline__ void grad_row(const typename T::raw* row, typename T:
   }
 
 // Loss and statistics, or the gradient from them: one pass each, bound by memory
-// (2039 x 50261 bf16, 32 entries with the tail: 49 us, 4.2 TB/s, and 65 us, 6.3
+// (2039 x 50261 bf16, 32 entries with the tail: 50 us, 4.1 TB/s, and 66 us, 6.2
 // TB/s with what of the logits is still in the last cache).
 template <class T, int NT, int U, int WINDOW, bool TAIL>
 __global__ __launch_bounds__(NT) void lt_distill_sums(DistillParams p) {
@@ -498,7 +498,7 @@ __global__ __launch_bounds__(NT) void lt_distill_grad(DistillParams p) {
 // the gradient is written past them: kept, they push out the rows that other
 // blocks are about to read again (4096 x 131072 bf16: 570 us; with the stores
 // past the caches 500, with the loads too 467, 4.6 TB/s; 32768 x 16000: 518 and
-// 461).
+// 464).
 template <class T, int NT, int U, int WINDOW, bool TAIL>
 __global__ __launch_bounds__(NT, 8) void lt_distill_both(DistillParams p) {
   BLOCK_HEAD;
@@ -651,9 +651,9 @@ __global__ __launch_bounds__(256, (TAIL && N > 1 && U == 4 && V::E == 8 ? 6 : 1)
 // largest of their own where it is LITTLE beside that: there its exponents'
 // roundings cost more than 2^-18 of it, further down it vanishes.  The gradient is
 // made of the logits alone (no stats).  131072 x
-// 41 float32, 5 entries: loss 17 us, gradient 24, where reading the logits and
-// writing the gradient take 4 each: its instructions bound it, those in 64 bits
-// for every entry foremost.
+// 41 float32, 5 entries: loss 20 us, gradient 26, where reading the logits and
+// writing the gradient take 4 each: two waves a SIMD, 7 and 10 us of instructions
+// and the rest waiting, for the entries' loads foremost.
 constexpr float LITTLE = 0x1p-24f;
 
 template <class T, bool LOSS, bool GRAD>
@@ -787,7 +787,7 @@ void split_rows(DistillParams& p, int step, int64_t n) {
 // For the sums: one where the rows fill the card or a row is a few steps --
 // chunks have to be joined, in a launch of its own.  (Loss and gradient of 8 x
 // 32000 bf16 in one launch 11 us, in three 16 and the gaps between them; of 64 x
-// 131072 in three 24 us.)
+// 131072 in three 25 us, in one 28; of 200 42 and 39.)
 void split_sums(DistillParams& p, int dtype) {
   const int step = 512 * 4 * (dtype == LT_F32 ? 4 : 8);
   int64_t n = 1;
@@ -800,8 +800,8 @@ void split_sums(DistillParams& p, int dtype) {
 }
 
 // For the gradient, which needs no joining: blocks enough for the card.  (Loss and
-// gradient of 64 x 131072 bf16 26 us, with a block a row's gradient 32; of 200 42
-// and 45.)
+// gradient of 64 x 131072 bf16 25 us, with a block a row's gradient 31; of 200 42
+// and 43.)
 void split_grad(DistillParams& p, int dtype) {
   const int step = 512 * 4 * (dtype == LT_F32 ? 4 : 8);
   int64_t n = 1;
@@ -834,7 +834,7 @@ lt_status launch_wave(const DistillParams& p, Pass pass, void* stream, const cha
                         : launch(lt_distill_wave<T, V, U, N, TAIL, true, true>, blocks, 256, p, stream, what);
 }
 
-// (Room for 64 entries or 256: 65536 x 200 bf16, 8 entries 46 us and 52.)
+// (Room for 64 entries or 256: 65536 x 200 bf16, 8 entries 48 us and 53.)
 template <class T, class V, int U>
 lt_status launch_wave(const DistillParams& p, Pass pass, void* stream, const char* what) {
   if (p.t.entries <= 64)
@@ -846,8 +846,8 @@ template <class T>
 lt_status launch_pass(const DistillParams& p, Pass pass, void* stream, const char* what) {
   // Rows of few logits, and enough of them: a thread a row, which goes through
   // its entries one after another.  (Loss and gradient of float32, us, a wave a
-  // row the second: 131072 x 41, 3 entries 23, 60; 12 entries 41, 60; 16384 x 41,
-  // 12 entries 25, 17.)
+  // row the second: 131072 x 41, 3 entries 24, 70; 12 entries 44, 68; 16384 x 41,
+  // 12 entries 28, 17.)
   if (p.z.vocab <= FEW && p.rows >= 65536 && p.t.entries <= 16) {
     const int64_t blocks = (p.rows + 63) / 64;
     const int lds = 64 * few_pitch(p.z.vocab) * 4;
@@ -855,9 +855,9 @@ lt_status launch_pass(const DistillParams& p, Pass pass, void* stream, const cha
            : pass == GRAD ? launch(lt_distill_few<T, false, true>, blocks, 64, p, stream, what, lds)
                           : launch(lt_distill_few<T, true, true>, blocks, 64, p, stream, what, lds);
   }
-  // Rows that fit a wave's registers.  (65536 x 2000 bf16, 32 entries: 123 us, 4.3
-  // TB/s; 65536 x 200, 8 entries: 47, by its instructions; a wave that reads the
-  // row twice 190 and 82.  16384 x 4000: 68 us, a block of 256 threads 100.)
+  // Rows that fit a wave's registers.  (65536 x 2000 bf16, 32 entries: 120 us, 4.5
+  // TB/s; 65536 x 200, 8 entries: 48, by its instructions; a wave that reads the
+  // row twice 190 and 82.  16384 x 4000: 55 us, a block of 256 threads 105.)
   using W = Vec<T>;
   if (p.z.vocab <= 128) return launch_wave<T, One<T>, 2>(p, pass, stream, what);
   if (p.z.vocab <= 256) return launch_wave<T, One<T>, 4>(p, pass, stream, what);
@@ -865,7 +865,7 @@ lt_status launch_pass(const DistillParams& p, Pass pass, void* stream, const cha
   if (p.z.vocab <= 128 * W::E) return launch_wave<T, W, 2>(p, pass, stream, what);
   if (p.z.vocab <= 256 * W::E) return launch_wave<T, W, 4>(p, pass, stream, what);
   if (p.z.vocab <= 512 * W::E) return launch_wave<T, W, 8>(p, pass, stream, what);
-  // (4096 x 8000 bf16: 40 us by 256 threads, 57 by 512; 4096 x 131072: 508 and 468.)
+  // (4096 x 8000 bf16: 39 us by 256 threads, 56 by 512; 4096 x 131072: 504 and 467.)
   if (p.z.vocab <= 16384) return launch_block<T, 256, 4, 16384>(p, pass, stream, what);
   const lt_status st = launch_block<T, 512, 4, 1 << 18>(p, pass, stream, what);
   if (st != LT_OK || pass != SUMS || p.splits == 1) return st;

@@ -184,7 +184,7 @@ __device__ __forceinline__ uint64_t cut_keys(uint64_t* buf, int n, int k, int* h
 //   they are full.
 // (keep() has the logits unpacked anew for each use: held as floats between
 // the uses they took 118 registers and half the waves.)
-// 4096 x 131072 bf16, k 64: 211 us, 5.1 TB/s, which is the memory's; 509 x 50261
+// 4096 x 131072 bf16, k 64: 213 us, 5.1 TB/s, which is the memory's; 509 x 50261
 // float16, k 256: 32 us, where reading takes 11: two blocks a CU, whose steps and
 // sorts wait for each other.
 template <int NT, int C, int CL>
@@ -459,7 +459,8 @@ __global__ __launch_bounds__(256) void lt_top_join(TopParams p) {
 // Rows of at most FEW logits and k <= K: a thread keeps its row's k best in
 // registers, inserting each logit (64 rows of 41 logits, k 5: about 40
 // instructions of a wave a row, where a wave a row takes 240; 131072 x 41
-// float32: 16 us, 1.9 TB/s, bound by the insertions).
+// float32: 16 us, 1.9 TB/s: two waves a SIMD, 9 us of instructions, the insertions
+// foremost, and the rest waiting).
 template <class T, int K>
 __global__ __launch_bounds__(64) void lt_top_few(TopParams p) {
   using raw = typename T::raw;
@@ -529,13 +530,13 @@ __device__ __forceinline__ int renewed(int v) {
 // largest logits, of the vectors' or of all logits, the fewest that are at least
 // twice as many as k -- k logits reach what is found, and not many more.  Those
 // become keys in LDS, which are sorted.  Its instructions bound it, but for long
-// rows and a small k: 65536 x 2000 bf16, k 5: 61 us (4.4 TB/s), k 100: 138;
+// rows and a small k: 65536 x 2000 bf16, k 5: 60 us (4.4 TB/s), k 100: 138;
 // 65536 x 200, k 5: 32 (a wave that sorts all of the row 108).
 // Rows where more than C logits reach it (equal ones, mostly) or where it is
 // -inf, and rows with a NaN: the bound is raised to the largest logit if k equal
 // it, else by a search among all logits, which ends when few enough reach it or at
 // the k-th itself; then only those above it become keys, and the first of those
-// that equal it (65536 x 2000 bf16, k 5: 61 us, constant rows 172).
+// that equal it (65536 x 2000 bf16, k 5: 60 us, constant rows 172).
 template <class T, class V, int U>
 __global__ __launch_bounds__(256) void lt_top_wave(TopParams p) {
   using raw = typename T::raw;
@@ -726,7 +727,7 @@ int64_t top_workspace(const TopParams& p) {
 }
 
 // (65536 rows of 100 logits, k 5: 28 us by single logits, 68 by vectors; of 300:
-// 35 by a vector a lane, 39 by two.  16384 rows of 4000, k 100: 66 us, lt_top_k
+// 35 by a vector a lane, 39 by two.  16384 rows of 4000, k 100: 60 us, lt_top_k
 // of 256 threads 105.)
 template <class T>
 auto wave_kernel(int vocab) -> void (*)(TopParams) {
@@ -753,7 +754,8 @@ lt_status launch_top(TopParams& p, void* stream) {
   const int64_t fours = (p.rows + 3) / 4;
   // Rows that fit a wave's registers; few of them with many wanted are sorted
   // sooner by a block.  (bf16, us, 256 threads the second: 256 x 2000, k 60 13, 13;
-  // k 200 18, 13; 2000 x 2000, k 200 20, 26; 256 x 1000, k 200 14, 14.)
+  // k 200 18, 13; 2000 x 2000, k 200 20, 26; 256 x 1000, k 200 14, 14.  float32: 256 x
+  // 2000, k 200 17, 13; 400 x 1100, k 150 16, 13; 500 x 2000, k 110 13, 13.)
   const bool few_rows = p.rows < 512 && p.k > 100 && p.k <= 252 && p.x.vocab > 1024;
   if (p.x.vocab <= 512 * Vec<T>::E && !few_rows)
     return launch(wave_kernel<T>(p.x.vocab), fours, 256, p, stream, "lt_top_logits");
@@ -765,8 +767,11 @@ lt_status launch_top(TopParams& p, void* stream) {
   // other less, more find enough to do in few rows and hold a k of their size.
   // (bf16, us: 16384 x 6000, k 5: 48, 96, -; k 32: 96, 97, -; 2048 x 6000, k 32:
   // 27, 18, -; 4096 x 16000, k 60: 76, 42, 61; k 200: -, 97, 68; 16384 x 8000, k
-  // 200: -, 187, 241; 256 x 50000, k 60: 83, 24, 17.)  Beyond k 252 the first
-  // bound of 256 threads would need more of a wave's threads than it has.
+  // 200: -, 187, 241; 256 x 50000, k 60: 83, 24, 17.  float32: 16384 x 6000, k 5: 79,
+  // 118, 183; k 32: 105, 123, 193; 2048 x 6000, k 32: 25, 20, 26; 4096 x 16000, k 60:
+  // -, 66, 65; k 200: -, 95, 85; 16384 x 8000, k 200: -, 246, 223; 256 x 50000, k 60:
+  // -, 27, 21.)  Beyond k 252 the first bound of 256 threads would need more of a
+  // wave's threads than it has.
   if (p.k <= 32 && p.x.vocab <= 8192 && p.rows >= 2048)
     return launch(lt_top_k<T, 64, 4, 256, 128>, fours, 256, p, stream, "lt_top_logits");
   if (p.k > 252 || (p.k > 192 && p.x.vocab > 8192) || (p.rows < 512 && p.x.vocab > 8192))

@@ -12,8 +12,8 @@
 // operation takes two), where memory allows 14; the sums in 32 bits take 9.
 //
 // Three launches: sums, weigh, draw.  64 sequences of up to 5 drafts of 131072
-// bf16: 22 us (4.6 TB/s), 27 and 8; one of 4 drafts of 32000: 4, 9 and 6, which are
-// latencies.  (The draw by a sequence's last block to weigh, which saves a launch,
+// bf16: 22 us (4.6 TB/s), 27 and 8, half of it instructions; one of 4 drafts of
+// 32000: 4, 9 and 6, which are latencies.  (The draw by a sequence's last block to weigh, which saves a launch,
 // took 25 us longer with a fence of the whole card in every block.)
 #include <type_traits>
 
